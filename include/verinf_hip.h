@@ -373,6 +373,44 @@ size_t vi_lookup_histogram_workspace_bytes(int64_t n_x, int64_t n_table, int tab
 int vi_lookup_histogram(const uint64_t *x, int64_t n_x, const uint64_t *table, int64_t n_table, int table_is_range, int accumulate,
                         uint64_t *mult, void *ws, size_t ws_bytes, void *stream);
 
+/* ---- the forward pass a proof is about, in 8-bit integers (no counterpart in the reference) -------------------------
+ * Matrices are row-major with unit column stride; rows are ld* elements apart (>= their length) and start at any address
+ * that their type may have.  Types of numbers: */
+#define VI_F32 0
+#define VI_BF16 1
+#define VI_F16 2
+#define VI_I32 3     /* int8_matmul: the exact sums                        */
+#define VI_FIELD 4   /* int8_matmul: the exact sums as residues mod p      */
+
+/* q[i][j] = rint(x[i][j] * (127 / A_i)), half to even, scale[i] = A_i / 127, A_i = max_j |x[i][j]|, each operation rounded to 32
+ * bits.  A row with A_i < 127 * 2^-126 is zero (scale 0); one with a NaN or an infinity has integers of zero and a scale of NaN. */
+int vi_quantize_rows(int dtype, const void *x, int64_t m, int64_t k, int64_t ldx, int8_t *q, int64_t ldq, float *scale, void *stream);
+
+/* S = a b^T, a (m, k), b (n, k), k <= 131071.  dtype VI_I32: out = S; VI_FIELD: out = S mod p (the scales and bias are not
+ * read); VI_F32, VI_BF16, VI_F16: out[i][j] = (S[i][j] a_scale[i]) b_scale[j] + bias[j] in 32 bits, rounded once (bias NULL: none).
+ * ws: vi_int8_matmul_workspace_bytes() bytes of device scratch. */
+size_t vi_int8_matmul_workspace_bytes(int64_t m, int64_t k, int64_t n);
+int vi_int8_matmul(const int8_t *a, int64_t lda, const int8_t *b, int64_t ldb, int64_t m, int64_t k, int64_t n, const float *a_scale,
+                   const float *b_scale, const float *bias, int dtype, void *out, int64_t ldo, void *ws, size_t ws_bytes, void *stream);
+
+/* out = act(G) U with G = (a gate^T a_scale) gate_scale and U = (a up^T a_scale) up_scale, both weights (n, k): a gated
+ * feed-forward block up to its last projection.  activation: VI_SILU x / (1 + e^-x), VI_GELU x Phi(x).  dtype VI_F32, VI_BF16 or VI_F16. */
+#define VI_SILU 0
+#define VI_GELU 1
+size_t vi_int8_gated_workspace_bytes(int64_t m, int64_t k, int64_t n);
+int vi_int8_gated(const int8_t *a, int64_t lda, const int8_t *gate, int64_t ldg, const int8_t *up, int64_t ldu, int64_t m, int64_t k, int64_t n,
+                  const float *a_scale, const float *gate_scale, const float *up_scale, int activation, int dtype, void *out, int64_t ldo,
+                  void *ws, size_t ws_bytes, void *stream);
+
+/* For each of m rows of v logits (1 <= v <= 2^24) divided by the temperature (1e-3 to 1e3): logprob[i] = the log probability of
+ * tokens[i] (0 for a token of -1, NaN for another one outside [0, v)), entropy[i] in nats, and the `top` <= 64 largest logits as
+ * top_tokens[i][.] with their log probabilities top_logprobs[i][.], in falling order, of equal logits the lowest index first.
+ * Logits of -inf have log probability -inf and add nothing; a row of nothing else has entropy 0.  A row with a NaN or +inf has NaN
+ * everywhere but in top_tokens, which has NaN first, then +inf.  ws: vi_token_logprobs_workspace_bytes() bytes of device scratch. */
+size_t vi_token_logprobs_workspace_bytes(int dtype, int64_t m, int64_t v, int top);
+int vi_token_logprobs(int dtype, const void *logits, int64_t m, int64_t v, int64_t ld, const int64_t *tokens, float temperature, int top,
+                      float *logprob, float *entropy, float *top_logprobs, int64_t *top_tokens, void *ws, size_t ws_bytes, void *stream);
+
 /* ---------------------------------------------------------------------------------------------
  * Measurement hook (no counterpart in the reference): the issue rate of the integer VALU instructions the field
  * arithmetic and the hashing consist of, which is the bound their kernels are put against.

@@ -11,7 +11,7 @@ import ctypes
 import functools
 import os
 import threading
-from ctypes import POINTER, c_char_p, c_double, c_int, c_int64, c_size_t, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
 
 import numpy as np
 import torch  # noqa: F401  (must precede the CDLL below)
@@ -39,6 +39,8 @@ EXPORTS = [
     "vi_eq_vector", "vi_mle_eval_workspace_bytes", "vi_mle_eval",
     "vi_challenge", "vi_gl_spmv", "vi_lookup_multiplicities",
     "vi_lookup_histogram_workspace_bytes", "vi_lookup_histogram",
+    "vi_quantize_rows", "vi_int8_matmul_workspace_bytes", "vi_int8_matmul", "vi_int8_gated_workspace_bytes", "vi_int8_gated",
+    "vi_token_logprobs_workspace_bytes", "vi_token_logprobs",
     "vi_valu_probe_count", "vi_valu_probe_name", "vi_wall_clock_khz", "vi_valu_probe",
 ]
 
@@ -137,6 +139,20 @@ def lib():
     L.vi_mle_eval_workspace_bytes.restype = sz
     L.vi_mle_eval_workspace_bytes.argtypes = [i64]
     L.vi_mle_eval.argtypes = [vp, i64, i64, POINTER(u64), c_int, vp, vp, sz, vp]
+    L.vi_quantize_rows.argtypes = [c_int, vp, i64, i64, i64, vp, i64, vp, vp]
+    L.vi_quantize_rows.restype = c_int
+    L.vi_int8_matmul_workspace_bytes.restype = sz
+    L.vi_int8_matmul_workspace_bytes.argtypes = [i64, i64, i64]
+    L.vi_int8_matmul.argtypes = [vp, i64, vp, i64, i64, i64, i64, vp, vp, vp, c_int, vp, i64, vp, sz, vp]
+    L.vi_int8_matmul.restype = c_int
+    L.vi_int8_gated_workspace_bytes.restype = sz
+    L.vi_int8_gated_workspace_bytes.argtypes = [i64, i64, i64]
+    L.vi_int8_gated.argtypes = [vp, i64, vp, i64, vp, i64, i64, i64, i64, vp, vp, vp, c_int, c_int, vp, i64, vp, sz, vp]
+    L.vi_int8_gated.restype = c_int
+    L.vi_token_logprobs_workspace_bytes.restype = sz
+    L.vi_token_logprobs_workspace_bytes.argtypes = [c_int, i64, i64, c_int]
+    L.vi_token_logprobs.argtypes = [c_int, vp, i64, i64, i64, vp, c_float, c_int, vp, vp, vp, vp, vp, sz, vp]
+    L.vi_token_logprobs.restype = c_int
     L.vi_valu_probe_name.restype = c_char_p
     L.vi_valu_probe_name.argtypes = [c_int]
     L.vi_valu_probe.argtypes = [c_int, c_int, c_int, vp, vp, POINTER(i64), vp]

@@ -1,0 +1,141 @@
+// What the kernels of the 8-bit products share: the job, what becomes of a sum (finish), the loads of ragged rows.
+#pragma once
+
+#include "number_types.hpp"
+
+namespace i8 {
+
+using namespace num;
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+typedef int v16i __attribute__((ext_vector_type(16)));
+
+constexpr int BLOCK = 256;
+constexpr int VEC = 8;                         // neighbouring outputs that a thread finishes at once
+
+struct Job {
+    const signed char *a, *b, *b2;             // b2: the second weights of the gated form
+    i64 lda, ldb, ldb2;
+    i64 m, k, n;
+    const float *a_scale, *b_scale, *b2_scale, *bias;
+    int dtype, act;
+    void *out;
+    i64 ldo;
+    int *partial;                              // [slices][1 or 2][m][n] sums, for more than one slice of the inner dimension
+    int slices, steps_per_slice, steps;
+    int mt, nt;                                // tiles down and across
+};
+
+// 16 bytes of a row of which `left` are there (any number, also none or fewer); zero behind them
+__device__ __forceinline__ v4i load_part(const signed char *p, i64 left) {
+    if (left >= 16) return load_any<v4i>(p);
+    v4i v = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 15; ++e)
+        if (e < left) v[e / 4] |= (int)((u32)(unsigned char)p[e] << (8 * (e & 3)));
+    return v;
+}
+
+// x / (1 + e^-x), with e^-|x| so that nothing overflows, and a step of Newton's behind the reciprocal (one unit off as it comes)
+__device__ __forceinline__ float silu(float x) {
+    const float t = __builtin_amdgcn_exp2f(fabsf(x) * -1.44269504f), y = 1.0f + t, r = __builtin_amdgcn_rcpf(y);
+    return (x < 0.0f ? x * t : x) * fmaf(fmaf(-y, r, 1.0f), r, r);
+}
+
+__device__ __forceinline__ void activate(float (&v)[VEC], int act) {
+    if (act == VI_GELU) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = 0.5f * v[e] * (1.0f + erff(v[e] * 0.70710678f));
+        return;
+    }
+    float least = v[0];
+#pragma unroll
+    for (int e = 1; e < VEC; ++e) least = fminf(least, v[e]);
+    if (least > -80.0f) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = silu(v[e]);
+    } else {
+        // v_exp_f32 has no results below 2^-126; there the sum is one
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = v[e] <= -80.0f ? v[e] * expf(v[e]) : silu(v[e]);
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void store_floats(void *out, i64 at, const float (&v)[VEC], int count) {
+    typedef typename type<DT>::t T;
+    T *o = (T *)out + at;
+    T r[VEC];
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) r[e] = (T)v[e];
+    if (count == VEC) {
+        store_any(o, r);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (e < count) o[e] = r[e];
+    }
+}
+
+// The sums of row `row`, columns col .. col + count - 1, as they go out: s of the first weights, t of the second.  Integers leave
+// as they are (or as residues mod p); otherwise (s a_scale) b_scale in 32 bits, a sum of more than 24 bits rounded by the conversion,
+// and one rounding to the type of the output.
+template <bool GATED>
+__device__ __forceinline__ void finish(const Job &J, i64 row, i64 col, int count, const int (&s)[VEC], const int (&t)[VEC]) {
+    const i64 at = row * J.ldo + col;
+    if (!GATED && J.dtype == VI_I32) {
+        int *o = (int *)J.out + at;
+        if (count == VEC) {
+            store_any(o, s);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (e < count) o[e] = s[e];
+        }
+        return;
+    }
+    if (!GATED && J.dtype == VI_FIELD) {
+        u64 *o = (u64 *)J.out + at;
+        u64 r[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) r[e] = (u64)(i64)s[e] - (s[e] < 0 ? 0xFFFFFFFFull : 0);       // p - |s| below zero
+        if (count == VEC) {
+            store_any(o, r);
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (e < count) o[e] = r[e];
+        }
+        return;
+    }
+    const float as = J.a_scale[row];
+    float bs[VEC], v[VEC];
+    auto scales = [&](const float *p) {
+        if (count == VEC) {
+            __builtin_memcpy(bs, p + col, sizeof(bs));
+        } else {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) bs[e] = e < count ? p[col + e] : 0.0f;
+        }
+    };
+    scales(J.b_scale);
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (float)s[e] * as * bs[e];
+    if (GATED) {
+        scales(J.b2_scale);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) bs[e] = (float)t[e] * as * bs[e];
+        activate(v, J.act);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] *= bs[e];
+    } else if (J.bias) {
+        scales(J.bias);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] += bs[e];
+    }
+    if (J.dtype == VI_F32) store_floats<VI_F32>(J.out, at, v, count);
+    if (J.dtype == VI_BF16) store_floats<VI_BF16>(J.out, at, v, count);
+    if (J.dtype == VI_F16) store_floats<VI_F16>(J.out, at, v, count);
+}
+
+}  // namespace i8
