@@ -388,16 +388,19 @@ int vi_quantize_rows(int dtype, const void *x, int64_t m, int64_t k, int64_t ldx
 
 /* S = a b^T, a (m, k), b (n, k), k <= 131071.  dtype VI_I32: out = S; VI_FIELD: out = S mod p (the scales and bias are not
  * read); VI_F32, VI_BF16, VI_F16: out[i][j] = (S[i][j] a_scale[i]) b_scale[j] + bias[j] in 32 bits, rounded once (bias NULL: none).
- * ws: vi_int8_matmul_workspace_bytes() bytes of device scratch. */
+ * ws: vi_int8_matmul_workspace_bytes() bytes of device scratch; operands that do not start at a multiple of 16 bytes, or have rows that
+ * are not a multiple of 16 or 2^23 bytes or more apart, are copied first where that pays and vi_int8_matmul_best_workspace_bytes() are there. */
 size_t vi_int8_matmul_workspace_bytes(int64_t m, int64_t k, int64_t n);
+size_t vi_int8_matmul_best_workspace_bytes(int64_t m, int64_t k, int64_t n);
 int vi_int8_matmul(const int8_t *a, int64_t lda, const int8_t *b, int64_t ldb, int64_t m, int64_t k, int64_t n, const float *a_scale,
                    const float *b_scale, const float *bias, int dtype, void *out, int64_t ldo, void *ws, size_t ws_bytes, void *stream);
 
 /* out = act(G) U with G = (a gate^T a_scale) gate_scale and U = (a up^T a_scale) up_scale, both weights (n, k): a gated
- * feed-forward block up to its last projection.  activation: VI_SILU x / (1 + e^-x), VI_GELU x Phi(x).  dtype VI_F32, VI_BF16 or VI_F16. */
+ * feed-forward block up to its last projection.  activation: VI_SILU x / (1 + e^-x), VI_GELU x Phi(x).  dtype VI_F32, VI_BF16 or VI_F16. ws as above. */
 #define VI_SILU 0
 #define VI_GELU 1
 size_t vi_int8_gated_workspace_bytes(int64_t m, int64_t k, int64_t n);
+size_t vi_int8_gated_best_workspace_bytes(int64_t m, int64_t k, int64_t n);
 int vi_int8_gated(const int8_t *a, int64_t lda, const int8_t *gate, int64_t ldg, const int8_t *up, int64_t ldu, int64_t m, int64_t k, int64_t n,
                   const float *a_scale, const float *gate_scale, const float *up_scale, int activation, int dtype, void *out, int64_t ldo,
                   void *ws, size_t ws_bytes, void *stream);

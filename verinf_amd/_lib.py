@@ -39,7 +39,9 @@ EXPORTS = [
     "vi_eq_vector", "vi_mle_eval_workspace_bytes", "vi_mle_eval",
     "vi_challenge", "vi_gl_spmv", "vi_lookup_multiplicities",
     "vi_lookup_histogram_workspace_bytes", "vi_lookup_histogram",
-    "vi_quantize_rows", "vi_int8_matmul_workspace_bytes", "vi_int8_matmul", "vi_int8_gated_workspace_bytes", "vi_int8_gated",
+    "vi_quantize_rows",
+    "vi_int8_matmul_workspace_bytes", "vi_int8_matmul_best_workspace_bytes", "vi_int8_matmul",
+    "vi_int8_gated_workspace_bytes", "vi_int8_gated_best_workspace_bytes", "vi_int8_gated",
     "vi_token_logprobs_workspace_bytes", "vi_token_logprobs",
     "vi_valu_probe_count", "vi_valu_probe_name", "vi_wall_clock_khz", "vi_valu_probe",
 ]
@@ -143,10 +145,14 @@ def lib():
     L.vi_quantize_rows.restype = c_int
     L.vi_int8_matmul_workspace_bytes.restype = sz
     L.vi_int8_matmul_workspace_bytes.argtypes = [i64, i64, i64]
+    L.vi_int8_matmul_best_workspace_bytes.restype = sz
+    L.vi_int8_matmul_best_workspace_bytes.argtypes = [i64, i64, i64]
     L.vi_int8_matmul.argtypes = [vp, i64, vp, i64, i64, i64, i64, vp, vp, vp, c_int, vp, i64, vp, sz, vp]
     L.vi_int8_matmul.restype = c_int
     L.vi_int8_gated_workspace_bytes.restype = sz
     L.vi_int8_gated_workspace_bytes.argtypes = [i64, i64, i64]
+    L.vi_int8_gated_best_workspace_bytes.restype = sz
+    L.vi_int8_gated_best_workspace_bytes.argtypes = [i64, i64, i64]
     L.vi_int8_gated.argtypes = [vp, i64, vp, i64, vp, i64, i64, i64, i64, vp, vp, vp, c_int, c_int, vp, i64, vp, sz, vp]
     L.vi_int8_gated.restype = c_int
     L.vi_token_logprobs_workspace_bytes.restype = sz

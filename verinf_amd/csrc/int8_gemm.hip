@@ -5,6 +5,8 @@
 //
 // Both operands have their inner dimension along the rows, so a wavefront's operands of a matrix instruction are 16 contiguous bytes a
 // lane.  Sums are exact: |S| <= 2^14 k fits 32 bits up to MAX_K.
+#include <type_traits>
+
 #include "int8_gemm.hpp"
 
 namespace {
@@ -12,110 +14,59 @@ namespace {
 using namespace i8;
 
 constexpr int MAX_K = 131071;
-constexpr int STEP = 64;                       // inner indices of a step
-constexpr int UNITS = STEP / 16;
 
-// units of a row are stored in another order, by the row, so that lanes that read one unit of neighbouring rows meet different banks
-__device__ __forceinline__ int slot(int row, int unit) { return row * UNITS + (unit ^ ((row >> 1) & 3)); }
+// Where unit `unit` of row `row` is in a stage, in units: those of a row are in another order by the row, so that the sixteen lanes that LDS
+// serves at a time, one unit of as many neighbouring rows, meet all 64 banks.
+template <int U>
+__device__ __forceinline__ int order(int row) { return U == 4 ? (row >> 2) & 3 : (row >> 1) & 7; }
 
-// column c of a tile's 64 WN virtual columns -> its row of B, or of the second B where *second: a wavefront's first half of the
-// columns are the gate's, its other half the same channels' of the up projection, so that both sums of an output are in one lane
+// Column c of a tile's 64 WN virtual columns -> its row of B behind the tile's first, or of the second B where *second: a wavefront's
+// first half of the columns are the gate's, its other half the same channels' of the up projection, so that both sums of an output
+// are in one lane.
 template <int WN, bool GATED>
-__device__ __forceinline__ i64 channel(int tn, int c, bool *second) {
-    if (!GATED) {
-        *second = false;
-        return (i64)tn * (64 * WN) + c;
-    }
-    const int wc = c / (32 * WN), in = c % (32 * WN), half = in / (16 * WN);
-    *second = half;
-    return (i64)tn * (32 * WN) + wc * (16 * WN) + in % (16 * WN);
+__device__ __forceinline__ i64 channel(int c, bool *second) {
+    if (!GATED) return c;
+    const int wc = c / (32 * WN), in = c % (32 * WN);
+    *second = in >= 16 * WN;
+    return wc * (16 * WN) + in % (16 * WN);
 }
 
-template <int WM, int WN>
-struct Lds {
-    v4i a[64 * WM * UNITS], b[64 * WN * UNITS];
-};
+// Words between the rows of a wavefront's sums in LDS: sixteen lanes' 16 bytes in neighbouring rows meet different banks.
+constexpr int pitch(int wn) { return 32 * wn + 4; }
 
-// A tile of 64 WM rows and 64 WN (virtual) columns by four wavefronts in a square.
+// a wavefront's own LDS accesses are in order for all its lanes
+__device__ __forceinline__ void meet_wave() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A wavefront's sums acc[j][i]: columns 32 j, rows 32 i.  The weights are the first operand of the matrix instruction, so register r of a
+// lane is column 8 (r / 4) + 4 half + r % 4 of row lane % 32: four neighbouring columns in neighbouring registers.
+//
+// This way out goes through LDS, 32 rows at a time in the wavefront's own part (after a barrier), with any number of columns.
 template <int WM, int WN, bool GATED>
-__global__ __launch_bounds__(BLOCK) void k_tile(Job J) {
-    constexpr int TM = 64 * WM, TN = 64 * WN, PITCH = 32 * WN + 8;
-    __shared__ union {
-        Lds<WM, WN> in;
-        int out[4][32 * PITCH];
-    } lds;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int total = J.mt * J.nt;
-    const int slice = blockIdx.x / total, id = blockIdx.x % total, tm = id % J.mt, tn = id / J.mt;
-    const int s0 = slice * J.steps_per_slice, s1 = min(s0 + J.steps_per_slice, J.steps);
-
-    const signed char *src[WM + WN];
-#pragma unroll
-    for (int j = 0; j < WM + WN; ++j) {
-        const int row = (j < WM ? j : j - WM) * 64 + (tid >> 2);
-        if (j < WM) {
-            src[j] = J.a + min((i64)tm * TM + row, J.m - 1) * J.lda;
-        } else {
-            bool second;
-            const i64 c = min(channel<WN, GATED>(tn, row, &second), J.n - 1);
-            src[j] = second ? J.b2 + c * J.ldb2 : J.b + c * J.ldb;
-        }
-        src[j] += (tid & 3) * 16;
-    }
-    v16i acc[WM][WN];
-#pragma unroll
-    for (int i = 0; i < WM; ++i)
-#pragma unroll
-        for (int j = 0; j < WN; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
-    const int row0 = (wave >> 1) * (32 * WM) + (lane & 31), col0 = (wave & 1) * (32 * WN) + (lane & 31), half = lane >> 5;
-    for (int s = s0; s < s1; ++s) {
-        const i64 at = (i64)s * STEP;
-        v4i in[WM + WN];
-#pragma unroll
-        for (int j = 0; j < WM + WN; ++j) in[j] = load_part(src[j] + at, J.k - at - (tid & 3) * 16);
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < WM + WN; ++j) {
-            const int row = (j < WM ? j : j - WM) * 64 + (tid >> 2);
-            (j < WM ? lds.in.a : lds.in.b)[slot(row, tid & 3)] = in[j];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < UNITS / 2; ++t) {
-            v4i x[WM], y[WN];
-#pragma unroll
-            for (int i = 0; i < WM; ++i) x[i] = lds.in.a[slot(row0 + 32 * i, 2 * t + half)];
-#pragma unroll
-            for (int j = 0; j < WN; ++j) y[j] = lds.in.b[slot(col0 + 32 * j, 2 * t + half)];
-#pragma unroll
-            for (int i = 0; i < WM; ++i)
-#pragma unroll
-                for (int j = 0; j < WN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(x[i], y[j], acc[i][j], 0, 0, 0);
-        }
-    }
-
-    // 32 rows at a time through the wavefront's own part of LDS, so that a lane has neighbouring columns: register r of a
-    // tile is row 8 (r / 4) + 4 half + r % 4, column lane % 32
-    __syncthreads();
-    int *buf = lds.out[wave];
-    constexpr int WIDE = GATED ? 16 * WN : 32 * WN, VECS = WIDE / VEC;
+__device__ __forceinline__ void put_ragged(const Job &J, int *buf, const v16i (&acc)[WN][WM], i64 row0, i64 col0, int slice, int lane) {
+    constexpr int WIDE = GATED ? 16 * WN : 32 * WN, VECS = WIDE / VEC, PITCH = pitch(WN);
+    const int half = lane >> 5;
 #pragma unroll
     for (int i = 0; i < WM; ++i) {
 #pragma unroll
         for (int j = 0; j < WN; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) buf[(8 * (r / 4) + 4 * half + r % 4) * PITCH + 32 * j + (lane & 31)] = acc[i][j][r];
-        __syncthreads();
+            for (int g = 0; g < 4; ++g) {
+                const v4i v = {acc[j][i][4 * g], acc[j][i][4 * g + 1], acc[j][i][4 * g + 2], acc[j][i][4 * g + 3]};
+                *(v4i *)(buf + (lane & 31) * PITCH + 32 * j + 8 * g + 4 * half) = v;
+            }
+        meet_wave();
+#pragma unroll 1
         for (int it = 0; it < 32 * VECS / 64; ++it) {
             const int p = it * 64 + lane, lrow = p / VECS, lcol = p % VECS * VEC;
-            const i64 row = (i64)tm * TM + (wave >> 1) * (32 * WM) + 32 * i + lrow, col = (i64)tn * (GATED ? TN / 2 : TN) + (wave & 1) * WIDE + lcol;
+            const i64 row = row0 + 32 * i + lrow, col = col0 + lcol;
             const int count = (int)min(J.n - col, (i64)VEC);
             if (row >= J.m || count <= 0) continue;
             int v[VEC], w[VEC];
-            __builtin_memcpy(v, buf + lrow * PITCH + lcol, sizeof(v));
-            if (GATED) __builtin_memcpy(w, buf + lrow * PITCH + WIDE + lcol, sizeof(w));
+            __builtin_memcpy(v, __builtin_assume_aligned(buf + lrow * PITCH + lcol, 16), sizeof(v));
+            if (GATED) __builtin_memcpy(w, __builtin_assume_aligned(buf + lrow * PITCH + WIDE + lcol, 16), sizeof(w));
             if (J.slices == 1) {
                 finish<GATED>(J, row, col, count, v, w);
             } else {
@@ -128,7 +79,452 @@ __global__ __launch_bounds__(BLOCK) void k_tile(Job J) {
                 }
             }
         }
+        meet_wave();
+    }
+}
+
+// The lower lanes get the eight columns of group 2 p of their row, the upper ones those of 2 p + 1: w[0] and w[1] are a lane's own four
+// columns of either group.
+__device__ __forceinline__ void swap_halves(u32 &a, u32 &b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+}
+
+// A sum as it is needed, here: without it the compiler converts all of a wavefront's sums in front of the branches that ask for their
+// type, and has to put them into scratch memory.
+__device__ __forceinline__ int here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// The way out for tiles whose columns all exist: from the registers, 32 neighbouring bytes or more of each of 32 rows in a store.
+// Scaled sums; the type of the output is looked at eight values at a time.
+template <int WM, int WN, bool GATED>
+__device__ __forceinline__ void put_scaled(const Job &J, const v16i (&acc)[WN][WM], i64 row0, i64 col0, int lane) {
+    const int half = lane >> 5;
+    float as[WM];
+#pragma unroll
+    for (int i = 0; i < WM; ++i) as[i] = J.a_scale[min(row0 + 32 * i + (lane & 31), J.m - 1)];
+#pragma unroll
+    for (int q = 0; q < (GATED ? WN : 2 * WN); ++q) {                  // 16 columns at a time: half a tile of the matrix instruction
+        float bs[VEC], us[VEC];
+        auto scales = [&](float (&to)[VEC], const float *from) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) __builtin_memcpy(to + 4 * g, from + col0 + 16 * q + 8 * g + 4 * half, 16);
+        };
+        scales(bs, J.b_scale);
+        if (GATED) scales(us, J.b2_scale);
+        else if (J.bias) scales(us, J.bias);
+#pragma unroll
+        for (int i = 0; i < WM; ++i) {
+            const i64 row = row0 + 32 * i + (lane & 31);
+            float v[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = (float)here(acc[q / 2][i][8 * (q % 2) + e]) * as[i] * bs[e];
+            if constexpr (GATED) {
+                activate(v, J.act);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] *= (float)here(acc[(WN + q) / 2][i][8 * ((WN + q) % 2) + e]) * as[i] * us[e];
+            } else if (J.bias) {
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[e] += us[e];
+            }
+            const i64 at = row * J.ldo + col0 + 16 * q;
+            if (J.dtype == VI_F32) {
+                if (row < J.m) {
+                    store_any((float *)J.out + at + 4 * half, *(const float (*)[4])v);
+                    store_any((float *)J.out + at + 8 + 4 * half, *(const float (*)[4])(v + 4));
+                }
+            } else {
+                u32 w[4];
+                if (J.dtype == VI_BF16) {
+                    __bf16 r[VEC];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) r[e] = (__bf16)v[e];
+                    __builtin_memcpy(w, r, sizeof(w));
+                } else {
+                    _Float16 r[VEC];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) r[e] = (_Float16)v[e];
+                    __builtin_memcpy(w, r, sizeof(w));
+                }
+                swap_halves(w[0], w[2]);
+                swap_halves(w[1], w[3]);
+                if (row < J.m) store_any((unsigned short *)J.out + at + 8 * half, w);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+}
+
+// the same for the sums themselves, as 32-bit integers or as residues; those of the second weights `second` behind the first's
+template <int DT, int WM, int WN, bool GATED>
+__device__ __forceinline__ void put_sums(const v16i (&acc)[WN][WM], void *out, i64 ldo, i64 m, i64 second, i64 row0, i64 col0, int lane) {
+    const int half = lane >> 5;
+#pragma unroll
+    for (int q = 0; q < 2 * WN; ++q)
+#pragma unroll
+        for (int i = 0; i < WM; ++i) {
+            const i64 row = row0 + 32 * i + (lane & 31);
+            const bool up = GATED && q >= WN;
+            if (row < m) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const i64 at = row * ldo + col0 + 16 * (up ? q - WN : q) + 8 * g + 4 * half + (up ? second : 0);
+                    const int r = 8 * (q % 2) + 4 * g;
+                    if constexpr (DT == VI_I32) {
+                        const v4i v = {acc[q / 2][i][r], acc[q / 2][i][r + 1], acc[q / 2][i][r + 2], acc[q / 2][i][r + 3]};
+                        store_any((int *)out + at, v);
+                    } else {
+                        u64 v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int s = here(acc[q / 2][i][r + e]);
+                            v[e] = (u64)(i64)s - (s < 0 ? 0xFFFFFFFFull : 0);
+                        }
+                        store_any((u64 *)out + at, v);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+}
+
+template <int WM, int WN, bool GATED>
+__device__ __forceinline__ void put(const Job &J, int *buf, const v16i (&acc)[WN][WM], int tm, int tn, int slice, int wave, int lane) {
+    constexpr int WIDE = GATED ? 16 * WN : 32 * WN;
+    const i64 row0 = (i64)tm * (64 * WM) + (wave >> 1) * (32 * WM), col0 = (i64)tn * (2 * WIDE) + (wave & 1) * WIDE;
+    if (col0 + WIDE > J.n) {
+        put_ragged<WM, WN, GATED>(J, buf, acc, row0, col0, slice, lane);
+    } else if (J.slices > 1) {
+        put_sums<VI_I32, WM, WN, GATED>(acc, J.partial + (i64)slice * (GATED ? 2 : 1) * J.m * J.n, J.n, J.m, J.m * J.n, row0, col0, lane);
+    } else if (!GATED && J.dtype == VI_I32) {
+        put_sums<VI_I32, WM, WN, false>(acc, J.out, J.ldo, J.m, 0, row0, col0, lane);
+    } else if (!GATED && J.dtype == VI_FIELD) {
+        put_sums<VI_FIELD, WM, WN, false>(acc, J.out, J.ldo, J.m, 0, row0, col0, lane);
+    } else {
+        put_scaled<WM, WN, GATED>(J, acc, row0, col0, lane);
+    }
+}
+
+// Which tile a workgroup takes.  Workgroups go to the eight XCDs in turn: those of one XCD (id % 8) take neighbouring tiles, GROUP
+// tiles down and as many across as there are, so that what they read at a time is in its L2.
+constexpr int GROUP = 8;
+__device__ __forceinline__ void place(const Job &J, int id, int *tm, int *tn) {
+    const int total = J.mt * J.nt, xcd = id & 7, each = total >> 3, more = total & 7;
+    id = xcd * each + min(xcd, more) + (id >> 3);
+    const int strip = id / (GROUP * J.nt), first = strip * GROUP, rows = min(GROUP, J.mt - first), in = id - first * J.nt;
+    *tm = first + in % rows;
+    *tn = in / rows;
+}
+
+// ---- tiles --------------------------------------------------------------------------------------------------------
+// 64 lanes' 16 bytes at base + off into 1 KiB of LDS at byte `at`, without a register in between; base and at are the same for the
+// wavefront.  As an instruction of its own the compiler does not wait for it before the next LDS read, as it does for its builtin: the
+// waits are wait_and_meet's.  M0, which it takes its LDS address from, has its value back afterwards: the compiler does not accept it in
+// a list of clobbered registers.
+__device__ __forceinline__ void fetch_to_lds(const signed char *base, u32 off, u32 at) {
+    u32 m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "s"(at), "v"(off), "s"(base) : "memory");
+}
+// all but the wavefront's last `n` loads have arrived and its LDS accesses are done, then the workgroup's barrier
+template <int N>
+__device__ __forceinline__ void wait_and_meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(N) : "memory");
+}
+
+// the same with all the loads, where there are any; the compiler waits for those to registers
+template <bool LOADS>
+__device__ __forceinline__ void meet() {
+    if constexpr (LOADS) wait_and_meet<0>();
+    else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
+}
+
+template <int WM, int WN, int U, int ST>
+union alignas(16) Lds {
+    char in[ST * 64 * (WM + WN) * U * 16];
+    int out[4][32 * pitch(WN)];
+};
+
+// A tile of 64 WM rows and 64 WN (virtual) columns by four wavefronts in a square, in steps of U units of 16 inner indices.  ST stages of LDS,
+// PER_CU workgroups to a CU.  The operands of the next 32 inner indices are read from LDS, and loads requested, between the products
+// of these, so that the matrix cores have work throughout: they stop only where the workgroup meets, once a step.  The ragged end of
+// the rows goes first, through registers.
+// DIRECT: operands at 16-byte boundaries go straight into LDS, ST - 1 steps ahead.  Others go through registers: loads of one step are
+// under way while the next stage but one is written.
+template <int WM, int WN, int U, int ST, int PER_CU, bool GATED, bool DIRECT>
+__global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
+    constexpr int TM = 64 * WM, STEP = 16 * U, AHEAD = DIRECT ? ST - 1 : 2, N = WM * WN, T = U / 2;
+    constexpr int CHUNK_ROWS = 64 / U, NL = (WM + WN) * U / 4, A_LOADS = WM * U / 4, READS = WM + WN;
+    constexpr u32 STAGE = 64 * (WM + WN) * U * 16;
+    static_assert(DIRECT || ST == 3, "");
+    __shared__ Lds<WM, WN, U, ST> lds;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int total = J.mt * J.nt;
+    const int slice = blockIdx.x / total;
+    int tm, tn;
+    place(J, blockIdx.x % total, &tm, &tn);
+    const int s0 = slice * J.steps_per_slice, s1 = min(s0 + J.steps_per_slice, J.steps), steps = s1 - s0;
+
+    // Load j of the wavefront is chunk 4 j + wave of a stage, 1 KiB: CHUNK_ROWS rows of A or B.  Rows that do not exist are the last
+    // one again.  DIRECT: rows less than 2^23 apart, a tile's distances fit 32 bits.
+    typedef typename std::conditional<DIRECT, u32, i64>::type Off;
+    Off off[NL];
+    bool other[NL];                            // of the second B
+    const int in_row = lane / U, unit = ((lane % U) ^ order<U>(wave * CHUNK_ROWS + in_row)) * 16;
+    static_assert(U == 4 || CHUNK_ROWS * 4 % 16 == 0, "");
+    const i64 a_first = (i64)tm * TM, b_first = (i64)tn * (GATED ? 32 : 64) * WN;
+    const signed char *pa = J.a + a_first * J.lda, *pb = J.b + b_first * J.ldb, *pb2 = GATED ? J.b2 + b_first * J.ldb2 : nullptr;
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+        other[j] = false;
+        if (j < A_LOADS) {
+            const i64 row = min((i64)((j * 4 + wave) * CHUNK_ROWS + in_row), J.m - 1 - a_first);
+            off[j] = (Off)row * (Off)J.lda + unit;
+        } else {
+            const int c = ((j - A_LOADS) * 4 + wave) * CHUNK_ROWS;
+            const i64 row = min(channel<WN, GATED>(c, &other[j]) + in_row, J.n - 1 - b_first);
+            off[j] = (Off)row * (Off)(other[j] ? J.ldb2 : J.ldb) + unit;
+        }
+    }
+    // position 0 is the ragged end, where this slice has it; position p else the step s0 + p - ragged
+    const int ragged = s1 == J.steps && J.k % STEP ? 1 : 0;
+    pa += (i64)s0 * STEP;
+    pb += (i64)s0 * STEP;
+    if (GATED) pb2 += (i64)s0 * STEP;
+    auto source = [&](int j) { return j < A_LOADS ? pa : other[j] ? pb2 : pb; };
+    const u32 lds0 = (u32)(uintptr_t)(__attribute__((address_space(3))) char *)lds.in;
+    u32 put_at = ragged * STAGE;               // the stage that the next step is fetched to
+    v4i in[NL];                                // !DIRECT: that step, on its way
+    auto load = [&](int j) { in[j] = load_any<v4i>(source(j) + off[j]); };
+    auto store = [&](int j) { *(v4i *)(lds.in + put_at + (j * 4 + wave) * 1024 + lane * 16) = in[j]; };
+    auto advance = [&]() {
+        pa += STEP;
+        pb += STEP;
+        if (GATED) pb2 += STEP;
+    };
+    auto next_stage = [](u32 s) { return s == (ST - 1) * STAGE ? 0 : s + STAGE; };
+    auto fetch = [&](int j) {
+        if constexpr (DIRECT) {
+            fetch_to_lds(source(j), off[j], lds0 + put_at + (j * 4 + wave) * 1024);
+        } else {
+            store(j);
+            load(j);
+        }
+        if (j == NL - 1) {
+            advance();
+            put_at = next_stage(put_at);
+        }
+    };
+
+    v16i acc[WN][WM];
+#pragma unroll
+    for (int i = 0; i < WM; ++i)
+#pragma unroll
+        for (int j = 0; j < WN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[j][i][r] = 0;
+    const int half = lane >> 5, row0 = (wave >> 1) * (32 * WM) + (lane & 31), col0 = TM + (wave & 1) * (32 * WN) + (lane & 31);
+    u32 x_at[T], y_at[T];
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+        x_at[t] = (row0 * U + ((2 * t + half) ^ order<U>(row0))) * 16;
+        y_at[t] = (col0 * U + ((2 * t + half) ^ order<U>(col0))) * 16;
+    }
+    v4i x[2][WM], y[2][WN];
+    // operand q of the 32 inner indices t of the stage at byte `from`, in the order in which the products take them
+    auto read = [&](u32 from, int t, int q) {
+        const char *xs = lds.in + from + x_at[t], *ys = lds.in + from + y_at[t];
+        constexpr int APART = 32 * U * 16;
+        if (q == 0) x[t & 1][0] = *(const v4i *)xs;
+        else if (q <= WN) y[t & 1][q - 1] = *(const v4i *)(ys + APART * (q - 1));
+        else x[t & 1][q - WN] = *(const v4i *)(xs + APART * (q - WN));
+    };
+    // the products of part t, `between(c)` behind the c-th
+    auto multiply = [&](int t, auto between) {
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+            const int i = c / WN, j = c % WN;
+            acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(y[t & 1][j], x[t & 1][i], acc[j][i], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            between(c);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    u32 take = 0;                              // the stage that is multiplied
+    // All parts of a step but the last, the next part's reads and the loads of a step to come (LOADS) among them; then, behind `wait`, the
+    // last with the reads of the next step's first.
+    auto step = [&](auto loads, auto last, auto wait) {
+        constexpr bool LOADS = decltype(loads)::value, LAST = decltype(last)::value;
+#pragma unroll
+        for (int t = 0; t < T - 1; ++t)
+            multiply(t, [&](int c) {
+                const int from = t * NL / (T - 1), ops = READS + (LOADS ? (t + 1) * NL / (T - 1) - from : 0);
+#pragma unroll
+                for (int q = c * ops / N; q < (c + 1) * ops / N; ++q) {
+                    if (q < READS) read(take, t + 1, q);
+                    else fetch(from + q - READS);
+                }
+            });
+        wait();
+        take = next_stage(take);
+        multiply(T - 1, [&](int c) {
+            if constexpr (!LAST) {
+                constexpr int EACH = (READS + N - 1) / N;
+#pragma unroll
+                for (int q = c * EACH; q < (c + 1) * EACH && q < READS; ++q) read(take, 0, q);
+            }
+        });
+    };
+
+    if (steps > 0) {
+        if (ragged) {
+            const i64 at = (i64)(J.steps - 1 - s0) * STEP;
+#pragma unroll
+            for (int j = 0; j < NL; ++j)
+                *(v4i *)(lds.in + (j * 4 + wave) * 1024 + lane * 16) = load_part(source(j) + at + off[j], J.k - (i64)(J.steps - 1) * STEP - unit);
+        }
+        if constexpr (DIRECT) {
+#pragma unroll
+            for (int p = 0; p < AHEAD; ++p)
+                if (p < steps && p >= ragged) {
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) fetch(j);
+                }
+        } else if (steps > ragged) {
+#pragma unroll
+            for (int j = 0; j < NL; ++j) load(j);
+            advance();
+#pragma unroll
+            for (int p = 0; p < AHEAD; ++p)
+                if (p < steps && p >= ragged) {
+                    if (p + 1 < steps) {
+#pragma unroll
+                        for (int j = 0; j < NL; ++j) fetch(j);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < NL; ++j) store(j);
+                    }
+                }
+        }
+        if (DIRECT && steps >= AHEAD) wait_and_meet<(AHEAD - 1) * NL>();
+        else meet<DIRECT>();
+#pragma unroll
+        for (int q = 0; q < READS; ++q) read(take, 0, q);
+        int p = 0;
+        // the last load of !DIRECT would be one step too many
+        for (; p + AHEAD + (DIRECT ? 0 : 1) < steps; ++p)
+            step(std::true_type(), std::false_type(), [] {
+                if constexpr (DIRECT) wait_and_meet<(AHEAD - 1) * NL>();
+                else meet<false>();
+            });
+        if constexpr (!DIRECT) {
+            if (p + AHEAD < steps) {
+#pragma unroll
+                for (int j = 0; j < NL; ++j) store(j);
+            }
+        }
+        for (; p + 1 < steps; ++p) step(std::false_type(), std::false_type(), [] { meet<DIRECT>(); });
+        step(std::false_type(), std::true_type(), [] {});
         __syncthreads();
+    }
+    put<WM, WN, GATED>(J, lds.out[wave], acc, tm, tn, slice, wave, lane);
+}
+
+// ---- rows at any address, to 16-byte boundaries -------------------------------------------------------------------
+// Up to three matrices in one launch, 16 bytes a thread, zero behind the last of a row.
+struct Pack {
+    const signed char *from[3];
+    v4i *to[3];
+    i64 ld[3], rows[3];                        // rows: up to and with this matrix
+    i64 k, units;                              // units of a row
+};
+
+__global__ __launch_bounds__(BLOCK) void k_pack(Pack P) {
+    const i64 total = P.rows[2] * P.units;
+    for (i64 p = (i64)blockIdx.x * BLOCK + threadIdx.x; p < total; p += (i64)gridDim.x * BLOCK) {
+        i64 row = p / P.units;
+        const i64 at = p - row * P.units;
+        const int which = row < P.rows[0] ? 0 : row < P.rows[1] ? 1 : 2;
+        if (which) row -= P.rows[which - 1];
+        P.to[which][row * P.units + at] = load_part(P.from[which] + row * P.ld[which] + at * 16, P.k - at * 16);
+    }
+}
+
+// ---- few rows -----------------------------------------------------------------------------------------------------
+// Up to 16 MT rows: the weights are read once and hardly used, so they go from memory to the matrix instruction without LDS.  A workgroup
+// takes 16 channels (of both weights), its W wavefronts parts of the inner dimension: a lane has channel lane % 16, 16 inner indices of
+// each 64 by lane / 16, FEW_BLOCKS loads of either operand under way at once.  The parts meet in LDS.
+constexpr int FEW_BLOCKS = 8;
+
+template <int MT, int W, bool GATED>
+__global__ __launch_bounds__(64 * W) void k_few(Job J) {
+    constexpr int NT = GATED ? 2 : 1;
+    __shared__ int parts[W][NT * MT * 256];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const i64 first = (i64)blockIdx.x * 16, ch = min(first + (lane & 15), J.n - 1);
+    const signed char *w[NT], *x[MT];
+    w[0] = J.b + ch * J.ldb + (lane >> 4) * 16;
+    if (GATED) w[NT - 1] = J.b2 + ch * J.ldb2 + (lane >> 4) * 16;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) x[i] = J.a + min((i64)(16 * i + (lane & 15)), J.m - 1) * J.lda + (lane >> 4) * 16;
+    v4i acc[NT][MT];
+#pragma unroll
+    for (int h = 0; h < NT; ++h)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) acc[h][i] = v4i{0, 0, 0, 0};
+    const int blocks = (int)(J.k / 64);
+    int b = (int)((i64)blocks * wave / W);
+    const int end = (int)((i64)blocks * (wave + 1) / W);
+    auto some = [&](auto count) {
+        constexpr int C = decltype(count)::value;
+        v4i wv[C][NT], xv[C][MT];
+#pragma unroll
+        for (int u = 0; u < C; ++u) {
+#pragma unroll
+            for (int h = 0; h < NT; ++h) wv[u][h] = load_any<v4i>(w[h] + (i64)(b + u) * 64);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) xv[u][i] = load_any<v4i>(x[i] + (i64)(b + u) * 64);
+        }
+#pragma unroll
+        for (int u = 0; u < C; ++u)
+#pragma unroll
+            for (int h = 0; h < NT; ++h)
+#pragma unroll
+                for (int i = 0; i < MT; ++i) acc[h][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[u][h], xv[u][i], acc[h][i], 0, 0, 0);
+        b += C;
+    };
+    while (b + FEW_BLOCKS <= end) some(std::integral_constant<int, FEW_BLOCKS>());
+    if (b + 4 <= end) some(std::integral_constant<int, 4>());
+    if (b + 2 <= end) some(std::integral_constant<int, 2>());
+    if (b + 1 <= end) some(std::integral_constant<int, 1>());
+    if (wave == W - 1 && J.k % 64) {
+        const i64 at = (i64)blocks * 64, left = J.k - at - (lane >> 4) * 16;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const v4i xv = load_part(x[i] + at, left);
+#pragma unroll
+            for (int h = 0; h < NT; ++h) acc[h][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(load_part(w[h] + at, left), xv, acc[h][i], 0, 0, 0);
+        }
+    }
+    // register r of a lane is channel 4 (lane / 16) + r of row lane % 16
+#pragma unroll
+    for (int h = 0; h < NT; ++h)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) *(v4i *)&parts[wave][(h * MT + i) * 256 + (lane & 15) * 16 + (lane >> 4) * 4] = acc[h][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < MT * 256; e += 64 * W) {
+        const i64 row = e / 16, col = first + e % 16;
+        if (row >= J.m || col >= J.n) continue;
+        int s = 0, t = 0;
+#pragma unroll
+        for (int v = 0; v < W; ++v) {
+            s += parts[v][e];
+            if (GATED) t += parts[v][MT * 256 + e];
+        }
+        finish_one<GATED>(J, row, col, s, t);
     }
 }
 
@@ -140,37 +536,105 @@ __global__ __launch_bounds__(BLOCK) void k_join(Job J) {
         const i64 row = p / per_row, col = (p - row * per_row) * VEC;
         const int count = (int)min(J.n - col, (i64)VEC);
         int v[VEC] = {0}, w[VEC] = {0};
-        for (int q = 0; q < J.slices; ++q)
+        const int *s = J.partial + row * J.n + col;
+        if (count == VEC) {
+#pragma unroll 4
+            for (int q = 0; q < J.slices; ++q)
 #pragma unroll
-            for (int h = 0; h < (GATED ? 2 : 1); ++h) {
-                const int *s = J.partial + ((i64)q * (GATED ? 2 : 1) + h) * mn + row * J.n + col;
+                for (int h = 0; h < (GATED ? 2 : 1); ++h, s += mn) {
+                    int part[VEC];
+                    __builtin_memcpy(part, s, sizeof(part));
 #pragma unroll
-                for (int e = 0; e < VEC; ++e)
-                    if (e < count) (h ? w : v)[e] += s[e];
-            }
+                    for (int e = 0; e < VEC; ++e) (h ? w : v)[e] += part[e];
+                }
+        } else {
+            for (int q = 0; q < J.slices; ++q)
+#pragma unroll
+                for (int h = 0; h < (GATED ? 2 : 1); ++h, s += mn)
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e)
+                        if (e < count) (h ? w : v)[e] += s[e];
+        }
         finish<GATED>(J, row, col, count, v, w);
     }
 }
 
+// What a call is done with: the cheapest of these by their times in us, measured on this chip.
+//
+// Tiles, in units of 64 rows and 64 (virtual) columns: a step of one workgroup alone on its CU and of two that share it (0: there is
+// room for one), all CUs busy; what a tile takes beside its steps (first loads, scaling, stores); the same step with operands through
+// registers.  Larger tiles read less a product (a CU's path to LDS takes 64 bytes a cycle, which 128 x 128 tiles would use up) and waste
+// more where the last round of tiles is not full.
+struct Tile {
+    int wm, wn, units;
+    double alone, shared, rest, staged;
+};
+constexpr Tile TILES[] = {{4, 4, 4, 0.875, 0, 8, 1.5},           // 8192 x 8192 x 8192 502 us; 128 x 128: 582
+                          {4, 3, 4, 0.67, 0, 8, 1.2},            // 1000 x 4096 x 11008 54 us, 256 x 256: 55
+                          {4, 2, 4, 0.5, 1.015, 6, 0.95},        // gated 1000 x 4096 x 11008 111 us, 256 x 256: 128
+                          {2, 2, 8, 0.56, 1.06, 4, 1.3},         // 1000 x 4096 x 4096 24.7 us, 256 x 128: 36, 64 x 128: 29
+                          {1, 2, 8, 0.42, 0.6, 3, 0.75}};        // 128 x 4096 x 11008 13.3 us, 128 x 128: 16.5
+constexpr int N_TILES = sizeof(TILES) / sizeof(TILES[0]), CUS = 256;
+constexpr int FEW = N_TILES;                   // k_few, up to FEW_ROWS rows
+constexpr i64 FEW_ROWS = 32;
+
 struct Plan {
-    int slices, steps_per_slice, steps, mt, nt;
-    size_t ws_bytes;
+    int tile, slices, steps_per_slice, steps, mt, nt;
+    bool pack;
+    size_t pack_bytes, ws_bytes;
 };
 
-Plan make_plan(i64 m, i64 k, i64 n, bool gated) {
-    Plan L;
-    const i64 cols = gated ? 64 : 128, mt = (m + 127) / 128, nt = (n + cols - 1) / cols;
-    L.mt = (int)mt;
-    L.nt = (int)nt;
-    L.steps = (int)((k + STEP - 1) / STEP);
-    // slices of the inner dimension until there are two tiles for every CU, of at least 8 steps
-    i64 slices = 1;
-    while (mt * nt * slices * 2 <= 512 && L.steps / (slices * 2) >= 8) slices *= 2;
-    L.steps_per_slice = (int)((L.steps + slices - 1) / slices);
-    L.slices = L.steps ? (L.steps + L.steps_per_slice - 1) / L.steps_per_slice : 1;
-    L.ws_bytes = L.slices > 1 ? (size_t)4 * L.slices * (gated ? 2 : 1) * m * n + vi::WS_SLACK : 0;
-    return L;
+// aligned: all operands' rows at 16-byte boundaries; may_pack: others may be copied
+Plan make_plan(i64 m, i64 k, i64 n, bool gated, bool aligned, bool may_pack) {
+    const double two = gated ? 2 : 1, weights = two * (double)n * k;
+    Plan best = {};
+    double least = 1e30;
+    if (m <= FEW_ROWS) {
+        // weights from memory, rows of A once for each 16 channels from the L2s: 1 x 4096 x 11008 11.8 us (64 x 128 tiles in two
+        // slices 14.4), 16 rows 16.1 (14.9), 32 rows of 4096 x 4096 8.3 (10.1)
+        least = weights / 5.0e6 + (double)n * k * m / 16 / 9.5e6 + (double)k / 16384 * 6;
+        best.tile = FEW;
+        best.slices = 1;
+    }
+    // copying unaligned operands: two passes over them and a launch
+    const double pack_cost = aligned ? 0 : 4 + 2 * ((double)m * k + weights) / 4e6;
+    for (int t = 0; t < N_TILES; ++t) {
+        const Tile &T = TILES[t];
+        const i64 rows = 64 * T.wm, cols = (gated ? 32 : 64) * T.wn, mt = (m + rows - 1) / rows, nt = (n + cols - 1) / cols, per_step = 16 * T.units;
+        const int steps = (int)((k + per_step - 1) / per_step);
+        for (int slices = 1; slices <= 16 && (slices == 1 || (steps / slices >= 4 && (double)mt * nt * slices <= 4 * CUS)); slices *= 2) {
+            const int each = (steps + slices - 1) / slices, used = each ? (steps + each - 1) / each : 1;
+            const double groups = (double)mt * nt * used;
+            const double join = used > 1 ? 3 + (double)used * m * n * two * 8 / 3.5e6 : 0;
+            for (int pack = 0; pack < (may_pack && !aligned ? 2 : 1); ++pack) {
+                const bool staged = !aligned && !pack;
+                // rounds of all CUs, with as many workgroups as share one, then a last that may leave them alone
+                const int share = !staged && T.shared ? 2 : 1;
+                const double alone = staged ? T.staged : T.alone, full = share == 2 ? T.shared : alone;
+                const double rounds = (double)(i64)(groups / (CUS * share)), rest = groups - rounds * CUS * share;
+                const double cost = join + (pack ? pack_cost : 0) + rounds * (each * full + T.rest) + (rest > CUS ? each * full + T.rest : rest > 0 ? each * alone + T.rest : 0);
+                if (cost < least) {
+                    least = cost;
+                    best = {t, used, each, steps, (int)mt, (int)nt, pack != 0, 0, 0};
+                }
+            }
+        }
+    }
+    if (best.pack) best.pack_bytes = (size_t)((k + 15) / 16 * 16) * (m + (gated ? 2 : 1) * n);
+    best.ws_bytes = best.pack_bytes + (best.slices > 1 ? (size_t)4 * best.slices * (gated ? 2 : 1) * m * n : 0);
+    if (best.ws_bytes) best.ws_bytes += vi::WS_SLACK;
+    return best;
 }
+
+// for operands wherever they are; may_pack: with copies of those that are not aligned
+size_t workspace_bytes(i64 m, i64 k, i64 n, bool gated, bool may_pack) {
+    if (m <= 0 || k < 0 || n <= 0 || k > MAX_K) return 0;
+    const size_t a = make_plan(m, k, n, gated, true, false).ws_bytes, b = make_plan(m, k, n, gated, false, false).ws_bytes;
+    const size_t c = may_pack ? make_plan(m, k, n, gated, false, true).ws_bytes : 0;
+    return a > b ? (a > c ? a : c) : (b > c ? b : c);
+}
+
+bool aligned_rows(const void *p, i64 ld) { return ((uintptr_t)p & 15) == 0 && (ld & 15) == 0 && ld < (i64)1 << 23; }
 
 // what is the same to check of both entries
 int check(const char *who, const Job &J, bool gated) {
@@ -185,18 +649,80 @@ int check(const char *who, const Job &J, bool gated) {
     return VI_OK;
 }
 
+template <bool GATED, bool DIRECT>
+void launch_tile(const Plan &L, const Job &J, hipStream_t s) {
+    const int groups = L.mt * L.nt * L.slices;
+    const dim3 grid((unsigned)groups);
+    const bool few = groups <= CUS;            // deeper prefetch where no CU has two
+#define GO(WM, WN, U, ST, CU) hipLaunchKernelGGL((k_tile<WM, WN, U, ST, CU, GATED, DIRECT>), grid, dim3(BLOCK), 0, s, J)
+    if constexpr (DIRECT) {
+        if (L.tile == 0) GO(4, 4, 4, 5, 1);
+        if (L.tile == 1) GO(4, 3, 4, 5, 1);
+        if (L.tile == 2 && few) GO(4, 2, 4, 6, 1);
+        if (L.tile == 2 && !few) GO(4, 2, 4, 3, 2);
+        if (L.tile == 3 && few) GO(2, 2, 8, 4, 1);
+        if (L.tile == 3 && !few) GO(2, 2, 8, 2, 2);
+        if (L.tile == 4 && few) GO(1, 2, 8, 6, 1);
+        if (L.tile == 4 && !few) GO(1, 2, 8, 3, 2);
+    } else {
+        if (L.tile == 0) GO(4, 4, 4, 3, 1);
+        if (L.tile == 1) GO(4, 3, 4, 3, 1);
+        if (L.tile == 2) GO(4, 2, 4, 3, 2);
+        if (L.tile == 3) GO(2, 2, 8, 3, 1);
+        if (L.tile == 4) GO(1, 2, 8, 3, 2);
+    }
+#undef GO
+}
+
 template <bool GATED>
 int launch(const char *who, Job J, void *ws, size_t ws_bytes, hipStream_t s) {
-    const Plan L = make_plan(J.m, J.k, J.n, GATED);
+    const bool aligned = aligned_rows(J.a, J.lda) && aligned_rows(J.b, J.ldb) && (!GATED || aligned_rows(J.b2, J.ldb2));
+    Plan L = make_plan(J.m, J.k, J.n, GATED, aligned, true);
+    if (L.pack && (!ws || ws_bytes < L.ws_bytes)) L = make_plan(J.m, J.k, J.n, GATED, aligned, false);
     if (ws_bytes < L.ws_bytes || (L.ws_bytes && !ws)) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, L.ws_bytes);
-    if ((i64)L.mt * L.nt * L.slices > 0x7FFFFFFF) return vi::fail(VI_EINVAL, "%s: %lld x %lld outputs", who, (long long)J.m, (long long)J.n);
-    J.partial = (int *)vi::align16(ws);
+    if (L.tile == FEW) {
+        const dim3 grid((unsigned)((J.n + 15) / 16));
+        // wavefronts for 512 inner indices each, four to sixteen of them
+        const int waves = J.k <= 2048 ? 4 : 8;
+#define GO(MT, W) hipLaunchKernelGGL((k_few<MT, W, GATED>), grid, dim3(64 * W), 0, s, J)
+        if (J.m <= 16 && waves == 4) GO(1, 4);
+        if (J.m <= 16 && waves == 8) GO(1, 8);
+        if (J.m > 16 && waves == 4) GO(2, 4);
+        if (J.m > 16 && waves == 8) GO(2, 8);
+#undef GO
+        VI_LAUNCH_CHECK(who);
+        return VI_OK;
+    }
+    if ((double)L.mt * L.nt * L.slices > 0x7FFFFFFF) return vi::fail(VI_EINVAL, "%s: %lld x %lld outputs", who, (long long)J.m, (long long)J.n);
+    char *at = (char *)vi::align16(ws);
+    J.partial = (int *)(at + L.pack_bytes);
     J.slices = L.slices;
     J.steps_per_slice = L.steps_per_slice;
     J.steps = L.steps;
     J.mt = L.mt;
     J.nt = L.nt;
-    hipLaunchKernelGGL((k_tile<2, 2, GATED>), dim3((unsigned)(L.mt * L.nt * L.slices)), dim3(BLOCK), 0, s, J);
+    if (L.pack) {
+        Pack P = {};
+        P.k = J.k;
+        P.units = (J.k + 15) / 16;
+        const signed char **from[3] = {&J.a, &J.b, &J.b2};
+        i64 *ld[3] = {&J.lda, &J.ldb, &J.ldb2}, rows = 0;
+        for (int i = 0; i < 3; ++i) {
+            const i64 here = i == 0 ? J.m : i == 1 || GATED ? J.n : 0;
+            P.from[i] = *from[i];
+            P.ld[i] = *ld[i];
+            P.to[i] = (v4i *)at;
+            P.rows[i] = rows += here;
+            *from[i] = (const signed char *)at;
+            *ld[i] = P.units * 16;
+            at += here * P.units * 16;
+        }
+        const i64 blocks = (rows * P.units + BLOCK - 1) / BLOCK;
+        hipLaunchKernelGGL(k_pack, dim3((unsigned)(blocks < 16 * CUS ? blocks : 16 * CUS)), dim3(BLOCK), 0, s, P);
+        VI_LAUNCH_CHECK(who);
+    }
+    if (aligned || L.pack) launch_tile<GATED, true>(L, J, s);
+    else launch_tile<GATED, false>(L, J, s);
     VI_LAUNCH_CHECK(who);
     if (L.slices > 1) {
         const i64 blocks = ((J.n + VEC - 1) / VEC * J.m + BLOCK - 1) / BLOCK;
@@ -208,13 +734,10 @@ int launch(const char *who, Job J, void *ws, size_t ws_bytes, hipStream_t s) {
 
 }  // namespace
 
-extern "C" size_t vi_int8_matmul_workspace_bytes(int64_t m, int64_t k, int64_t n) {
-    return m > 0 && k >= 0 && n > 0 && k <= MAX_K ? make_plan(m, k, n, false).ws_bytes : 0;
-}
-
-extern "C" size_t vi_int8_gated_workspace_bytes(int64_t m, int64_t k, int64_t n) {
-    return m > 0 && k >= 0 && n > 0 && k <= MAX_K ? make_plan(m, k, n, true).ws_bytes : 0;
-}
+extern "C" size_t vi_int8_matmul_workspace_bytes(int64_t m, int64_t k, int64_t n) { return workspace_bytes(m, k, n, false, false); }
+extern "C" size_t vi_int8_matmul_best_workspace_bytes(int64_t m, int64_t k, int64_t n) { return workspace_bytes(m, k, n, false, true); }
+extern "C" size_t vi_int8_gated_workspace_bytes(int64_t m, int64_t k, int64_t n) { return workspace_bytes(m, k, n, true, false); }
+extern "C" size_t vi_int8_gated_best_workspace_bytes(int64_t m, int64_t k, int64_t n) { return workspace_bytes(m, k, n, true, true); }
 
 extern "C" int vi_int8_matmul(const int8_t *a, int64_t lda, const int8_t *b, int64_t ldb, int64_t m, int64_t k, int64_t n,
                               const float *a_scale, const float *b_scale, const float *bias, int dtype, void *out, int64_t ldo, void *ws,

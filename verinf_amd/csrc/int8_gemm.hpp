@@ -42,10 +42,12 @@ __device__ __forceinline__ float silu(float x) {
     return (x < 0.0f ? x * t : x) * fmaf(fmaf(-y, r, 1.0f), r, r);
 }
 
+__device__ __forceinline__ float gelu(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678f)); }
+
 __device__ __forceinline__ void activate(float (&v)[VEC], int act) {
     if (act == VI_GELU) {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = 0.5f * v[e] * (1.0f + erff(v[e] * 0.70710678f));
+        for (int e = 0; e < VEC; ++e) v[e] = gelu(v[e]);
         return;
     }
     float least = v[0];
@@ -136,6 +138,32 @@ __device__ __forceinline__ void finish(const Job &J, i64 row, i64 col, int count
     if (J.dtype == VI_F32) store_floats<VI_F32>(J.out, at, v, count);
     if (J.dtype == VI_BF16) store_floats<VI_BF16>(J.out, at, v, count);
     if (J.dtype == VI_F16) store_floats<VI_F16>(J.out, at, v, count);
+}
+
+// the same of one output
+template <bool GATED>
+__device__ __forceinline__ void finish_one(const Job &J, i64 row, i64 col, int s, int t) {
+    const i64 at = row * J.ldo + col;
+    if (!GATED && J.dtype == VI_I32) {
+        ((int *)J.out)[at] = s;
+        return;
+    }
+    if (!GATED && J.dtype == VI_FIELD) {
+        ((u64 *)J.out)[at] = (u64)(i64)s - (s < 0 ? 0xFFFFFFFFull : 0);
+        return;
+    }
+    const float as = J.a_scale[row];
+    float v = (float)s * as * J.b_scale[col];
+    if (GATED) {
+        if (J.act == VI_GELU) v = gelu(v);
+        else v = v <= -80.0f ? v * expf(v) : silu(v);
+        v *= (float)t * as * J.b2_scale[col];
+    } else if (J.bias) {
+        v += J.bias[col];
+    }
+    if (J.dtype == VI_F32) ((float *)J.out)[at] = v;
+    if (J.dtype == VI_BF16) ((__bf16 *)J.out)[at] = (__bf16)v;
+    if (J.dtype == VI_F16) ((_Float16 *)J.out)[at] = (_Float16)v;
 }
 
 }  // namespace i8

@@ -93,6 +93,10 @@ def _operands(who, a, weights):
     return m, k, n, lds
 
 
+def _aligned(t, ld):
+    return not (t.data_ptr() | ld) & 15
+
+
 def int8_matmul(a, b, a_scale=None, b_scale=None, bias=None, dtype=None):
     """a (m, k) int8 times the transpose of b (n, k) int8.
 
@@ -126,7 +130,7 @@ def int8_matmul(a, b, a_scale=None, b_scale=None, bias=None, dtype=None):
     L = _lib.lib()
     with _lib.on_device(dev):
         sp = _lib.stream_ptr()
-        need = _lib.workspace_bytes("int8_matmul", m, k, n)
+        need = _lib.workspace_bytes("int8_matmul" if _aligned(a, lda) and _aligned(b, ldb) else "int8_matmul_best", m, k, n)
         args = (a.data_ptr(), lda, b.data_ptr(), ldb, m, k, n, sa, sb, sbias, kind, out.data_ptr(), n)
         if not need:
             _lib.check(L.vi_int8_matmul(*args, None, 0, sp))
@@ -157,7 +161,7 @@ def int8_gated(a, gate, up, a_scale, gate_scale, up_scale, activation="silu", dt
     L = _lib.lib()
     with _lib.on_device(dev):
         sp = _lib.stream_ptr()
-        need = _lib.workspace_bytes("int8_gated", m, k, n)
+        need = _lib.workspace_bytes("int8_gated" if _aligned(a, lda) and _aligned(gate, ldg) and _aligned(up, ldu) else "int8_gated_best", m, k, n)
         args = (a.data_ptr(), lda, gate.data_ptr(), ldg, up.data_ptr(), ldu, m, k, n, sa, sg, su, _ACTIVATIONS[activation], _FLOATS[dtype],
                 out.data_ptr(), n)
         if not need:
