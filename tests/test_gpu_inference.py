@@ -423,3 +423,14 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("m,k,pad,shift", [(1024, 128, 0, 0), (2000, 250, 0, 0), (1500, 256, 3, 1), (2048, 257, 0, 0), (3001, 333, 0, 0), (2500, 1030, 6, 0),
+                                           (2049, 2048, 0, 0), (2048, 2049, 0, 0), (1200, 9, 0, 0), (40, 12300, 0, 0)])
+def test_many_short_rows_are_quantized_as_defined(dtype, m, k, pad, shift):
+    x = torch.randn(m, k, generator=torch.Generator().manual_seed(m + 3 * k)) * 5
+    x[m // 2] = 0
+    x[m - 1, k - 1] = math.nan
+    x[m - 2, 0] = -math.inf
+    check_quantized(rows(x.to(dtype), pad, shift))

@@ -31,7 +31,7 @@ __device__ __forceinline__ void store_any(P *p, const V &v) {
 
 // element e of 16 loaded bytes as a float
 template <int DT>
-__device__ __forceinline__ float element(const u32 (&w)[4], int e) {
+__device__ __forceinline__ float element(const u32 *w, int e) {
     if constexpr (DT == VI_F32) return __uint_as_float(w[e]);
     if constexpr (DT == VI_BF16) return __uint_as_float(e & 1 ? w[e / 2] & 0xFFFF0000u : w[e / 2] << 16);
     const unsigned short h = (unsigned short)(e & 1 ? w[e / 2] >> 16 : w[e / 2]);
