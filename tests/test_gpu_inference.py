@@ -434,3 +434,14 @@ def test_many_short_rows_are_quantized_as_defined(dtype, m, k, pad, shift):
     x[m - 1, k - 1] = math.nan
     x[m - 2, 0] = -math.inf
     check_quantized(rows(x.to(dtype), pad, shift))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("m,v,pad,shift,top", [(2, 32768, 0, 0, 9), (2, 32769, 1, 0, 9), (2, 65536, 0, 0, 64), (1, 65537, 0, 1, 7), (256, 4096, 0, 0, 2), (257, 4100, 0, 0, 2), (520, 70000, 0, 0, 5),
+                                               (1030, 16390, 0, 0, 64), (3, 131072, 8, 0, 33), (1025, 1024, 0, 0, 1)])
+def test_logprobs_where_rows_are_cut_otherwise(dtype, m, v, pad, shift, top):
+    gen = torch.Generator(device="cuda").manual_seed(m + v)
+    flat = (torch.randn(m, v + pad + shift, generator=gen, device="cuda") * 4).to(dtype)
+    flat[m // 2, : v // 3] = -math.inf
+    x = flat[:, shift:shift + v]
+    check_logprobs(x, torch.randint(0, v, (m,), generator=gen, device="cuda"), top)

@@ -17,11 +17,13 @@ MAX_TOP = 64
 MAX_K = 131071
 
 _FLOATS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_INT8 = (torch.int8,)
 _SUMS = {torch.int32: 3, torch.uint64: 4}
 _ACTIVATIONS = {"silu": 0, "gelu": 1}
 
 
-def _check(t, name, dtypes, dims, device=None):
+def _refuse(t, name, dtypes, dims, device):
+    """Says what is wrong with an argument that _matrix or _vector did not take at once; nothing may be."""
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a torch.Tensor")
     if not t.is_cuda:
@@ -36,20 +38,26 @@ def _check(t, name, dtypes, dims, device=None):
         raise RuntimeError(f"{name} requires a gradient: these operators have none (detach it, or call them under torch.no_grad())")
 
 
-def _rows(t, name):
-    """How many elements the rows of a matrix are apart."""
+def _matrix(t, name, dtypes, device=None):
+    """Rows, columns and how many elements the rows are apart.  The checks are a call's host time, so the usual case is one line."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.dim() == 2 and not t.requires_grad
+            and (device is None or t.device == device)):
+        _refuse(t, name, dtypes, 2, device)
     m, k = t.shape
-    if k > 1 and t.stride(1) != 1:
+    ld, apart = t.stride()
+    if k > 1 and apart != 1:
         raise RuntimeError(f"{name} must have unit column stride")
-    if m <= 1:
-        return max(k, 1)
-    if t.stride(0) < k:
+    if m > 1 and ld >= k and ld > 0:
+        return m, k, ld
+    if m > 1 and k > 0:
         raise RuntimeError(f"{name} has rows that overlap")
-    return max(t.stride(0), 1)
+    return m, k, (k + 15) & ~15 or 16          # a single row: any distance, one that keeps it aligned
 
 
-def _vector(t, name, length, dtypes, device):
-    _check(t, name, dtypes, 1, device)
+def _vector(t, name, length, dtype, device):
+    """The address of a contiguous vector."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.dim() == 1 and not t.requires_grad and t.device == device):
+        _refuse(t, name, (dtype,), 1, device)
     if t.shape[0] != length:
         raise RuntimeError(f"{name} has {t.shape[0]} elements, not {length}")
     if not t.is_contiguous():
@@ -63,34 +71,24 @@ def quantize_rows(x):
     scale = max |x[i]| / 127, q = x[i] * (127 / max |x[i]|) to the nearest integer, half to even, in 32 bits.  A row of zeros
     (or of nothing above 2^-119) has scale 0; one with a NaN or an infinity has scale NaN and integers of zero.  The rows of q are
     a multiple of 16 bytes apart, as the products read them fastest."""
-    _check(x, "x", _FLOATS, 2)
-    ldx = _rows(x, "x")
-    m, k = x.shape
-    q = torch.empty((m, -(-k // 16) * 16), dtype=torch.int8, device=x.device)[:, :k]
-    scale = torch.empty((m,), dtype=torch.float32, device=x.device)
-    with _lib.on_device(x.device):
-        _lib.check(_lib.lib().vi_quantize_rows(_FLOATS[x.dtype], x.data_ptr(), m, k, ldx, q.data_ptr(), _rows(q, "q"), scale.data_ptr(),
-                                               _lib.stream_ptr()))
+    m, k, ldx = _matrix(x, "x", _FLOATS)
+    dev = x.device
+    ldq = (k + 15) & ~15 or 16
+    q = torch.empty_strided((m, k), (ldq, 1), dtype=torch.int8, device=dev)
+    scale = torch.empty(m, dtype=torch.float32, device=dev)
+    with _lib.on_device(dev):
+        _lib.check(_lib.lib().vi_quantize_rows(_FLOATS[x.dtype], x.data_ptr(), m, k, ldx, q.data_ptr(), ldq, scale.data_ptr(), _lib.stream_ptr()))
     return q, scale
 
 
-def _operands(who, a, weights):
-    """Shapes and row distances of a product's operands."""
-    _check(a, "a", (torch.int8,), 2)
-    m, k = a.shape
-    n = None
-    lds = [_rows(a, "a")]
-    for name, w in weights:
-        _check(w, name, (torch.int8,), 2, a.device)
-        if w.shape[1] != k:
-            raise RuntimeError(f"{who}: a has rows of {k}, {name} of {w.shape[1]}")
-        if n is not None and w.shape[0] != n:
-            raise RuntimeError(f"{who}: the weights have {n} and {w.shape[0]} channels")
-        n = w.shape[0]
-        lds.append(_rows(w, name))
+def _weights(who, w, name, k, device):
+    """Channels of a weight matrix and how far apart they are."""
+    n, kw, ld = _matrix(w, name, _INT8, device)
+    if kw != k:
+        raise RuntimeError(f"{who}: a has rows of {k}, {name} of {kw}")
     if k > MAX_K:
         raise RuntimeError(f"{who}: an inner dimension of {k}: the 32-bit sums hold {MAX_K}")
-    return m, k, n, lds
+    return n, ld
 
 
 def _aligned(t, ld):
@@ -103,27 +101,28 @@ def int8_matmul(a, b, a_scale=None, b_scale=None, bias=None, dtype=None):
     Without scales the exact sums: int32 (the default), or with dtype=torch.uint64 the same as field elements, p - |s| below
     zero: what gl_matmul gives for the lifted operands.  With a_scale (m,) and b_scale (n,) float32: (s * a_scale) * b_scale
     (+ bias (n,) float32) in 32 bits, rounded once to dtype: bfloat16 (the default), float16 or float32."""
-    m, k, n, (lda, ldb) = _operands("int8_matmul", a, [("b", b)])
+    m, k, lda = _matrix(a, "a", _INT8)
+    dev = a.device
+    n, ldb = _weights("int8_matmul", b, "b", k, dev)
     scaled = a_scale is not None or b_scale is not None
     if dtype is None:
         dtype = torch.bfloat16 if scaled else torch.int32
-    dev = a.device
     sa = sb = sbias = None
     if scaled:
         if a_scale is None or b_scale is None:
             raise RuntimeError("int8_matmul: both scales or none")
         if dtype not in _FLOATS:
             raise RuntimeError(f"int8_matmul: scaled sums are no {dtype}")
-        sa = _vector(a_scale, "a_scale", m, (torch.float32,), dev)
-        sb = _vector(b_scale, "b_scale", n, (torch.float32,), dev)
+        sa = _vector(a_scale, "a_scale", m, torch.float32, dev)
+        sb = _vector(b_scale, "b_scale", n, torch.float32, dev)
         if bias is not None:
-            sbias = _vector(bias, "bias", n, (torch.float32,), dev)
+            sbias = _vector(bias, "bias", n, torch.float32, dev)
     else:
         if bias is not None:
             raise RuntimeError("int8_matmul: a bias needs scales")
         if dtype not in _SUMS:
             raise RuntimeError(f"int8_matmul: without scales the sums are int32 or uint64, not {dtype}")
-    out = torch.empty((m, n), dtype=dtype, device=dev)
+    out = torch.empty(m, n, dtype=dtype, device=dev)
     if m == 0 or n == 0:
         return out
     kind = _FLOATS[dtype] if scaled else _SUMS[dtype]
@@ -146,16 +145,20 @@ def int8_gated(a, gate, up, a_scale, gate_scale, up_scale, activation="silu", dt
     a gated feed-forward block up to its last projection, (m, n), rounded once to dtype (bfloat16, float16 or float32).
 
     activation: "silu" x / (1 + e^-x), or "gelu" x Phi(x)."""
-    m, k, n, (lda, ldg, ldu) = _operands("int8_gated", a, [("gate", gate), ("up", up)])
+    m, k, lda = _matrix(a, "a", _INT8)
+    dev = a.device
+    n, ldg = _weights("int8_gated", gate, "gate", k, dev)
+    nu, ldu = _weights("int8_gated", up, "up", k, dev)
+    if nu != n:
+        raise RuntimeError(f"int8_gated: gate has {n} channels, up {nu}")
     if activation not in _ACTIVATIONS:
         raise RuntimeError(f"int8_gated: no activation {activation!r}")
     if dtype not in _FLOATS:
         raise RuntimeError(f"int8_gated: no outputs of {dtype}")
-    dev = a.device
-    sa = _vector(a_scale, "a_scale", m, (torch.float32,), dev)
-    sg = _vector(gate_scale, "gate_scale", n, (torch.float32,), dev)
-    su = _vector(up_scale, "up_scale", n, (torch.float32,), dev)
-    out = torch.empty((m, n), dtype=dtype, device=dev)
+    sa = _vector(a_scale, "a_scale", m, torch.float32, dev)
+    sg = _vector(gate_scale, "gate_scale", n, torch.float32, dev)
+    su = _vector(up_scale, "up_scale", n, torch.float32, dev)
+    out = torch.empty(m, n, dtype=dtype, device=dev)
     if m == 0 or n == 0:
         return out
     L = _lib.lib()
@@ -180,17 +183,16 @@ def token_logprobs(logits, tokens, top=0, temperature=1.0):
     largest entries of each row in falling order, equal logits by the lowest index.  A token of -1 is not scored (logprob 0), another
     one outside [0, v) gives NaN.  Logits of -inf have log probability -inf and add nothing; a row of nothing else has entropy 0.
     A NaN or +inf makes its row NaN, except for top_tokens (NaN first, then +inf)."""
-    _check(logits, "logits", _FLOATS, 2)
-    ld = _rows(logits, "logits")
-    m, v = logits.shape
+    m, v, ld = _matrix(logits, "logits", _FLOATS)
     dev = logits.device
-    t = _vector(tokens, "tokens", m, (torch.int64,), dev)
+    t = _vector(tokens, "tokens", m, torch.int64, dev)
     top, temperature = int(top), float(temperature)
     if not 0 <= top <= MAX_TOP or top > v:
         raise RuntimeError(f"token_logprobs: the {top} largest of {v} ({MAX_TOP} at most)")
-    logprob, entropy = torch.empty((2, m), dtype=torch.float32, device=dev).unbind(0)
-    top_logprobs = torch.empty((m, top), dtype=torch.float32, device=dev)
-    top_tokens = torch.empty((m, top), dtype=torch.int64, device=dev)
+    logprob = torch.empty(m, dtype=torch.float32, device=dev)
+    entropy = torch.empty(m, dtype=torch.float32, device=dev)
+    top_logprobs = torch.empty(m, top, dtype=torch.float32, device=dev)
+    top_tokens = torch.empty(m, top, dtype=torch.int64, device=dev)
     kind = _FLOATS[logits.dtype]
     L = _lib.lib()
     with _lib.on_device(dev):
