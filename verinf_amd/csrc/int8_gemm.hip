@@ -98,69 +98,103 @@ __device__ __forceinline__ int here(int v) {
     return v;
 }
 
-// The way out for tiles whose columns all exist: from the registers, 32 neighbouring bytes or more of each of 32 rows in a store.
-// Scaled sums; the type of the output is looked at eight values at a time.
-template <int WM, int WN, bool GATED>
-__device__ __forceinline__ void put_scaled(const Job &J, const v16i (&acc)[WN][WM], i64 row0, i64 col0, int lane) {
+// two values as the 16-bit type, the first in the lower half
+template <int DT>
+__device__ __forceinline__ u32 pack(float a, float b) {
+    typedef float v2f __attribute__((ext_vector_type(2)));
+    typedef typename type<DT>::t v2t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(u32, __builtin_convertvector((v2f{a, b}), v2t));
+}
+
+// a sum as a residue mod p = 2^64 - 2^32 + 1, in words: s, or 2^64 + s - (2^32 - 1) below zero
+__device__ __forceinline__ int residue_low(int s) { return s < 0 ? s + 1 : s; }
+__device__ __forceinline__ int residue_high(int s) { return s < 0 && s + 1 != 0 ? -2 : s < 0 ? -1 : 0; }
+
+// The way out for tiles whose columns all exist: 16 columns at a time (half a tile of the matrix instruction; the next ones' scales are on
+// their way meanwhile), 32 rows through the wavefront's part of LDS as they go out, so that a store writes whole lines: 8192 x 1024 x 8192
+// 103 us, 120 with 32 bytes of each of 32 rows in a store straight from the registers.
+template <int DT, int WM, int WN, bool GATED>
+__device__ __forceinline__ void put_rows(const Job &J, char *buf, const v16i (&acc)[WN][WM], i64 row0, i64 col0, int lane) {
+    constexpr int Q = GATED ? WN : 2 * WN, SIZE = size_of(DT), ROW = Q * 16 * SIZE, PITCH = ROW + 16, UNITS = ROW / 16;     // bytes
     const int half = lane >> 5;
-    float as[WM];
-#pragma unroll
-    for (int i = 0; i < WM; ++i) as[i] = J.a_scale[min(row0 + 32 * i + (lane & 31), J.m - 1)];
-#pragma unroll
-    for (int q = 0; q < (GATED ? WN : 2 * WN); ++q) {                  // 16 columns at a time: half a tile of the matrix instruction
-        float bs[VEC], us[VEC];
-        auto scales = [&](float (&to)[VEC], const float *from) {
+    float as[WM], bs[2][VEC], us[2][VEC];
+    auto scales = [&](int q) {
+        if (!is_float(DT)) return;
+        auto some = [&](float (&to)[VEC], const float *from) {
 #pragma unroll
             for (int g = 0; g < 2; ++g) __builtin_memcpy(to + 4 * g, from + col0 + 16 * q + 8 * g + 4 * half, 16);
         };
-        scales(bs, J.b_scale);
-        if (GATED) scales(us, J.b2_scale);
-        else if (J.bias) scales(us, J.bias);
+        some(bs[q & 1], J.b_scale);
+        if (GATED) some(us[q & 1], J.b2_scale);
+        else if (J.bias) some(us[q & 1], J.bias);
+    };
+    if (is_float(DT))
 #pragma unroll
-        for (int i = 0; i < WM; ++i) {
-            const i64 row = row0 + 32 * i + (lane & 31);
+        for (int i = 0; i < WM; ++i) as[i] = J.a_scale[min(row0 + 32 * i + (lane & 31), J.m - 1)];
+#pragma unroll
+    for (int i = 0; i < WM; ++i) {
+        char *mine = buf + (lane & 31) * PITCH;
+        scales(0);
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+            if (q + 1 < Q) scales(q + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (!is_float(DT)) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    int s[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[e] = here(acc[q / 2][i][8 * (q % 2) + 4 * g + e]);
+                    char *to = mine + (16 * q + 8 * g + 4 * half) * SIZE;
+                    if constexpr (DT == VI_I32) {
+                        *(v4i *)to = v4i{s[0], s[1], s[2], s[3]};
+                    } else {
+                        // p - |s| below zero: the upper word is 2^32 - 1 either way, the lower one more
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            *(v4i *)(to + 16 * e) = v4i{residue_low(s[2 * e]), residue_high(s[2 * e]), residue_low(s[2 * e + 1]), residue_high(s[2 * e + 1])};
+                    }
+                }
+                continue;
+            }
+            const float(&b)[VEC] = bs[q & 1], (&u)[VEC] = us[q & 1];
             float v[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = (float)here(acc[q / 2][i][8 * (q % 2) + e]) * as[i] * bs[e];
+            for (int e = 0; e < VEC; ++e) v[e] = (float)here(acc[q / 2][i][8 * (q % 2) + e]) * as[i] * b[e];
             if constexpr (GATED) {
                 activate(v, J.act);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] *= (float)here(acc[(WN + q) / 2][i][8 * ((WN + q) % 2) + e]) * as[i] * us[e];
+                for (int e = 0; e < VEC; ++e) v[e] *= (float)here(acc[(WN + q) / 2][i][8 * ((WN + q) % 2) + e]) * as[i] * u[e];
             } else if (J.bias) {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) v[e] += us[e];
+                for (int e = 0; e < VEC; ++e) v[e] += u[e];
             }
-            const i64 at = row * J.ldo + col0 + 16 * q;
-            if (J.dtype == VI_F32) {
-                if (row < J.m) {
-                    store_any((float *)J.out + at + 4 * half, *(const float (*)[4])v);
-                    store_any((float *)J.out + at + 8 + 4 * half, *(const float (*)[4])(v + 4));
-                }
-            } else {
+            if constexpr (DT == VI_F32) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) *(v4i *)(mine + 64 * q + 32 * g + 16 * half) = __builtin_bit_cast(v4i, *(const float (*)[4])(v + 4 * g));
+            } else if constexpr (is_float(DT)) {
                 u32 w[4];
-                if (J.dtype == VI_BF16) {
-                    __bf16 r[VEC];
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) r[e] = (__bf16)v[e];
-                    __builtin_memcpy(w, r, sizeof(w));
-                } else {
-                    _Float16 r[VEC];
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) r[e] = (_Float16)v[e];
-                    __builtin_memcpy(w, r, sizeof(w));
-                }
+                for (int e = 0; e < 4; ++e) w[e] = pack<DT>(v[2 * e], v[2 * e + 1]);
                 swap_halves(w[0], w[2]);
                 swap_halves(w[1], w[3]);
-                if (row < J.m) store_any((unsigned short *)J.out + at + 8 * half, w);
+                *(v4i *)(mine + 32 * q + 16 * half) = v4i{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
             }
-            __builtin_amdgcn_sched_barrier(0);
         }
+        meet_wave();
+#pragma unroll
+        for (int p = 0; p < 32 * UNITS / 64; ++p) {
+            const int at = p * 64 + lane, row = at / UNITS, unit = at % UNITS;
+            const v4i w = *(const v4i *)(buf + row * PITCH + unit * 16);
+            if (row0 + 32 * i + row < J.m) store_any((char *)J.out + ((row0 + 32 * i + row) * J.ldo + col0) * (i64)SIZE + unit * 16, w);
+        }
+        meet_wave();
     }
 }
 
-// the same for the sums themselves, as 32-bit integers or as residues; those of the second weights `second` behind the first's
-template <int DT, int WM, int WN, bool GATED>
-__device__ __forceinline__ void put_sums(const v16i (&acc)[WN][WM], void *out, i64 ldo, i64 m, i64 second, i64 row0, i64 col0, int lane) {
+// The sums of a slice to its part of the scratch; those of the second weights `second` behind the first's.
+template <int WM, int WN, bool GATED>
+__device__ __forceinline__ void put_sums(const v16i (&acc)[WN][WM], int *out, i64 ld, i64 m, i64 second, i64 row0, i64 col0, int lane) {
     const int half = lane >> 5;
 #pragma unroll
     for (int q = 0; q < 2 * WN; ++q)
@@ -171,20 +205,9 @@ __device__ __forceinline__ void put_sums(const v16i (&acc)[WN][WM], void *out, i
             if (row < m) {
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
-                    const i64 at = row * ldo + col0 + 16 * (up ? q - WN : q) + 8 * g + 4 * half + (up ? second : 0);
                     const int r = 8 * (q % 2) + 4 * g;
-                    if constexpr (DT == VI_I32) {
-                        const v4i v = {acc[q / 2][i][r], acc[q / 2][i][r + 1], acc[q / 2][i][r + 2], acc[q / 2][i][r + 3]};
-                        store_any((int *)out + at, v);
-                    } else {
-                        u64 v[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int s = here(acc[q / 2][i][r + e]);
-                            v[e] = (u64)(i64)s - (s < 0 ? 0xFFFFFFFFull : 0);
-                        }
-                        store_any((u64 *)out + at, v);
-                    }
+                    const v4i v = {acc[q / 2][i][r], acc[q / 2][i][r + 1], acc[q / 2][i][r + 2], acc[q / 2][i][r + 3]};
+                    store_any(out + row * ld + col0 + 16 * (up ? q - WN : q) + 8 * g + 4 * half + (up ? second : 0), v);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -198,13 +221,17 @@ __device__ __forceinline__ void put(const Job &J, int *buf, const v16i (&acc)[WN
     if (col0 + WIDE > J.n) {
         put_ragged<WM, WN, GATED>(J, buf, acc, row0, col0, slice, lane);
     } else if (J.slices > 1) {
-        put_sums<VI_I32, WM, WN, GATED>(acc, J.partial + (i64)slice * (GATED ? 2 : 1) * J.m * J.n, J.n, J.m, J.m * J.n, row0, col0, lane);
+        put_sums<WM, WN, GATED>(acc, J.partial + (i64)slice * (GATED ? 2 : 1) * J.m * J.n, J.n, J.m, J.m * J.n, row0, col0, lane);
     } else if (!GATED && J.dtype == VI_I32) {
-        put_sums<VI_I32, WM, WN, false>(acc, J.out, J.ldo, J.m, 0, row0, col0, lane);
+        put_rows<VI_I32, WM, WN, false>(J, (char *)buf, acc, row0, col0, lane);
     } else if (!GATED && J.dtype == VI_FIELD) {
-        put_sums<VI_FIELD, WM, WN, false>(acc, J.out, J.ldo, J.m, 0, row0, col0, lane);
+        put_rows<VI_FIELD, WM, WN, false>(J, (char *)buf, acc, row0, col0, lane);
+    } else if (J.dtype == VI_BF16) {
+        put_rows<VI_BF16, WM, WN, GATED>(J, (char *)buf, acc, row0, col0, lane);
+    } else if (J.dtype == VI_F16) {
+        put_rows<VI_F16, WM, WN, GATED>(J, (char *)buf, acc, row0, col0, lane);
     } else {
-        put_scaled<WM, WN, GATED>(J, acc, row0, col0, lane);
+        put_rows<VI_F32, WM, WN, GATED>(J, (char *)buf, acc, row0, col0, lane);
     }
 }
 
@@ -220,14 +247,16 @@ __device__ __forceinline__ void place(const Job &J, int id, int *tm, int *tn) {
 }
 
 // ---- tiles --------------------------------------------------------------------------------------------------------
-// 64 lanes' 16 bytes at base + off into 1 KiB of LDS at byte `at`, without a register in between; base and at are the same for the
-// wavefront.  As an instruction of its own the compiler does not wait for it before the next LDS read, as it does for its builtin: the
-// waits are wait_and_meet's.  M0, which it takes its LDS address from, has its value back afterwards: the compiler does not accept it in
-// a list of clobbered registers.
-__device__ __forceinline__ void fetch_to_lds(const signed char *base, u32 off, u32 at) {
-    u32 m0;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
-                 : "=&s"(m0) : "s"(at), "v"(off), "s"(base) : "memory");
+// 64 lanes' 16 bytes at base + off into 1 KiB of LDS, without a register in between, where fetch_from_here() says and 4 KiB on for each
+// call; base is the same for the wavefront.  As instructions of their own the compiler does not wait for them before the next LDS read, as
+// it does for its builtin: the waits are wait_and_meet's.  The place is in M0, a register that the compiler keeps nothing in: it sets it
+// in front of instructions that read it, of which it makes none here.
+// Wait states, which inside an asm block nothing inserts: one between a write of M0 and the load, five between a vector instruction's write
+// of a scalar register (readfirstlane, where the compiler has kept the base in vector registers) and a load that reads it.
+__device__ __forceinline__ void fetch_from_here(u32 at) { asm volatile("s_mov_b32 m0, %0" : : "s"(at) : "memory"); }
+__device__ __forceinline__ void fetch_to_lds(const signed char *base, u32 off) {
+    const u64 b = (u64)__builtin_amdgcn_readfirstlane((u32)((u64)base >> 32)) << 32 | (u32)__builtin_amdgcn_readfirstlane((u32)(u64)base);
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1\n\ts_add_u32 m0, m0, 0x1000" : : "v"(off), "s"(b) : "memory", "scc");
 }
 // all but the wavefront's last `n` loads have arrived and its LDS accesses are done, then the workgroup's barrier
 template <int N>
@@ -245,7 +274,7 @@ __device__ __forceinline__ void meet() {
 template <int WM, int WN, int U, int ST>
 union alignas(16) Lds {
     char in[ST * 64 * (WM + WN) * U * 16];
-    int out[4][32 * pitch(WN)];
+    int out[4][2 * 32 * pitch(WN)];            // 32 rows of a wavefront's sums or outputs, which may have 64 bits
 };
 
 // A tile of 64 WM rows and 64 WN (virtual) columns by four wavefronts in a square, in steps of U units of 16 inner indices.  ST stages of LDS,
@@ -263,9 +292,11 @@ __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
     __shared__ Lds<WM, WN, U, ST> lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int total = J.mt * J.nt;
-    const int slice = blockIdx.x / total;
+    const int slice = __builtin_amdgcn_readfirstlane(blockIdx.x / total);
     int tm, tn;
     place(J, blockIdx.x % total, &tm, &tn);
+    tm = __builtin_amdgcn_readfirstlane(tm);   // the divisions are vector instructions: what follows from them stays scalar this way
+    tn = __builtin_amdgcn_readfirstlane(tn);
     const int s0 = slice * J.steps_per_slice, s1 = min(s0 + J.steps_per_slice, J.steps), steps = s1 - s0;
 
     // Load j of the wavefront is chunk 4 j + wave of a stage, 1 KiB: CHUNK_ROWS rows of A or B.  Rows that do not exist are the last
@@ -308,7 +339,8 @@ __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
     auto next_stage = [](u32 s) { return s == (ST - 1) * STAGE ? 0 : s + STAGE; };
     auto fetch = [&](int j) {
         if constexpr (DIRECT) {
-            fetch_to_lds(source(j), off[j], lds0 + put_at + (j * 4 + wave) * 1024);
+            if (j == 0) fetch_from_here(lds0 + put_at + wave * 1024);
+            fetch_to_lds(source(j), off[j]);
         } else {
             store(j);
             load(j);
