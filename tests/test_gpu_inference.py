@@ -445,3 +445,17 @@ def test_logprobs_where_rows_are_cut_otherwise(dtype, m, v, pad, shift, top):
     flat[m // 2, : v // 3] = -math.inf
     x = flat[:, shift:shift + v]
     check_logprobs(x, torch.randint(0, v, (m,), generator=gen, device="cuda"), top)
+
+
+def test_more_rows_than_a_launch_has_workgroups_for():
+    # 2^23 rows at a time: the last ones are as they would be alone
+    m, some = (1 << 23) + 300, 1000
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn((m, 3), generator=gen, device="cuda").to(torch.bfloat16)
+    t = torch.randint(0, 3, (m,), generator=gen, device="cuda")
+    got, lp = inf.quantize_rows(x), inf.token_logprobs(x, t, top=2)
+    for part in (slice(0, some), slice(m - some, m)):
+        check_quantized(x[part])
+        check_logprobs(x[part], t[part], 2)
+        for a, b in zip(got + lp, inf.quantize_rows(x[part]) + inf.token_logprobs(x[part], t[part], top=2)):
+            assert torch.equal(a[part], b)

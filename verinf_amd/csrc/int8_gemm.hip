@@ -281,11 +281,17 @@ union alignas(16) Lds {
 // PER_CU workgroups to a CU.  The operands of the next 32 inner indices are read from LDS, and loads requested, between the products
 // of these, so that the matrix cores have work throughout: they stop only where the workgroup meets, once a step.  The ragged end of
 // the rows goes first, through registers.
+// Whole lines: a step of four units is half a line of each row, and 64 KiB of lines do not stay in a CU's 32 KiB cache until the next step
+// comes for the other half, so that the L2s would be asked for twice the operands (8192 x 8192 x 8192 in tiles of 256 x 128: 585 us, 509 in
+// steps of eight units).  The large tiles, of whose steps of eight units LDS holds two, load two of four at a time (PAIR): five stages, two
+// steps requested together, half a line behind the other, in every other step.
 // DIRECT: operands at 16-byte boundaries go straight into LDS, ST - 1 steps ahead.  Others go through registers: loads of one step are
 // under way while the next stage but one is written.
 template <int WM, int WN, int U, int ST, int PER_CU, bool GATED, bool DIRECT>
 __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
     constexpr int TM = 64 * WM, STEP = 16 * U, AHEAD = DIRECT ? ST - 1 : 2, N = WM * WN, T = U / 2;
+    constexpr bool PAIR = DIRECT && U == 4;
+    static_assert(!PAIR || ST == 5, "");
     constexpr int CHUNK_ROWS = 64 / U, NL = (WM + WN) * U / 4, A_LOADS = WM * U / 4, READS = WM + WN;
     constexpr u32 STAGE = 64 * (WM + WN) * U * 16;
     static_assert(DIRECT || ST == 3, "");
@@ -337,6 +343,19 @@ __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
         if (GATED) pb2 += STEP;
     };
     auto next_stage = [](u32 s) { return s == (ST - 1) * STAGE ? 0 : s + STAGE; };
+    // PAIR: of the next two steps at once
+    auto fetch_two = [&](int j) {
+        const u32 chunk = lds0 + wave * 1024 + j * 4096;
+        fetch_from_here(chunk + put_at);
+        fetch_to_lds(source(j), off[j]);
+        fetch_from_here(chunk + next_stage(put_at));
+        fetch_to_lds(source(j) + STEP, off[j]);
+        if (j == NL - 1) {
+            advance();
+            advance();
+            put_at = next_stage(next_stage(put_at));
+        }
+    };
     auto fetch = [&](int j) {
         if constexpr (DIRECT) {
             if (j == 0) fetch_from_here(lds0 + put_at + wave * 1024);
@@ -387,29 +406,40 @@ __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
     };
     u32 take = 0;                              // the stage that is multiplied
     // All parts of a step but the last, the next part's reads and the loads of a step to come (LOADS) among them; then, behind `wait`, the
-    // last with the reads of the next step's first.
+    // last with the reads of the next step's first.  PAIR: half of two steps' loads in each of the two parts.
+    constexpr int FIRST = PAIR ? NL / 2 : NL;
     auto step = [&](auto loads, auto last, auto wait) {
         constexpr bool LOADS = decltype(loads)::value, LAST = decltype(last)::value;
 #pragma unroll
         for (int t = 0; t < T - 1; ++t)
             multiply(t, [&](int c) {
-                const int from = t * NL / (T - 1), ops = READS + (LOADS ? (t + 1) * NL / (T - 1) - from : 0);
+                const int from = t * FIRST / (T - 1), ops = READS + (LOADS ? (t + 1) * FIRST / (T - 1) - from : 0);
 #pragma unroll
                 for (int q = c * ops / N; q < (c + 1) * ops / N; ++q) {
                     if (q < READS) read(take, t + 1, q);
+                    else if constexpr (PAIR) fetch_two(from + q - READS);
                     else fetch(from + q - READS);
                 }
             });
         wait();
         take = next_stage(take);
         multiply(T - 1, [&](int c) {
-            if constexpr (!LAST) {
+            if constexpr (PAIR && LOADS) {
+                constexpr int OPS = READS + NL - FIRST;
+#pragma unroll
+                for (int q = c * OPS / N; q < (c + 1) * OPS / N; ++q) {
+                    if (q < READS) read(take, 0, q);
+                    else fetch_two(FIRST + q - READS);
+                }
+            } else if constexpr (!LAST) {
                 constexpr int EACH = (READS + N - 1) / N;
 #pragma unroll
                 for (int q = c * EACH; q < (c + 1) * EACH && q < READS; ++q) read(take, 0, q);
             }
         });
     };
+    const auto yes = std::true_type();
+    const auto no = std::false_type();
 
     if (steps > 0) {
         if (ragged) {
@@ -418,48 +448,84 @@ __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
             for (int j = 0; j < NL; ++j)
                 *(v4i *)(lds.in + (j * 4 + wave) * 1024 + lane * 16) = load_part(source(j) + at + off[j], J.k - (i64)(J.steps - 1) * STEP - unit);
         }
-        if constexpr (DIRECT) {
+        // how far the loads go in front of the loop, and the first position there
+        if constexpr (PAIR) {
+            // two steps, then two more, or one: positions from `ragged` on
+            const int pairs = ragged ? 1 : 2, left = steps - ragged;
+            for (int i = 0; i < pairs && 2 * i < left; ++i) {
+                if (2 * i + 1 < left) {
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) fetch_two(j);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) fetch(j);
+                }
+            }
+            if (left >= 2 * pairs) wait_and_meet<2 * NL>();            // all but the last pair
+            else wait_and_meet<0>();
+        } else if constexpr (DIRECT) {
 #pragma unroll
             for (int p = 0; p < AHEAD; ++p)
                 if (p < steps && p >= ragged) {
 #pragma unroll
                     for (int j = 0; j < NL; ++j) fetch(j);
                 }
-        } else if (steps > ragged) {
+            if (steps >= AHEAD) wait_and_meet<(AHEAD - 1) * NL>();
+            else wait_and_meet<0>();
+        } else {
+            if (steps > ragged) {
 #pragma unroll
-            for (int j = 0; j < NL; ++j) load(j);
-            advance();
+                for (int j = 0; j < NL; ++j) load(j);
+                advance();
 #pragma unroll
-            for (int p = 0; p < AHEAD; ++p)
-                if (p < steps && p >= ragged) {
-                    if (p + 1 < steps) {
+                for (int p = 0; p < AHEAD; ++p)
+                    if (p < steps && p >= ragged) {
+                        if (p + 1 < steps) {
 #pragma unroll
-                        for (int j = 0; j < NL; ++j) fetch(j);
-                    } else {
+                            for (int j = 0; j < NL; ++j) fetch(j);
+                        } else {
 #pragma unroll
-                        for (int j = 0; j < NL; ++j) store(j);
+                            for (int j = 0; j < NL; ++j) store(j);
+                        }
                     }
-                }
+            }
+            meet<false>();
         }
-        if (DIRECT && steps >= AHEAD) wait_and_meet<(AHEAD - 1) * NL>();
-        else meet<DIRECT>();
 #pragma unroll
         for (int q = 0; q < READS; ++q) read(take, 0, q);
         int p = 0;
-        // the last load of !DIRECT would be one step too many
-        for (; p + AHEAD + (DIRECT ? 0 : 1) < steps; ++p)
-            step(std::true_type(), std::false_type(), [] {
-                if constexpr (DIRECT) wait_and_meet<(AHEAD - 1) * NL>();
-                else meet<false>();
-            });
-        if constexpr (!DIRECT) {
-            if (p + AHEAD < steps) {
+        if constexpr (PAIR) {
+            // At a step with loads the three positions from its own on are in LDS or on their way, and the next two are requested; those
+            // of the step before the last one with loads have arrived behind it.
+            if (!ragged && steps > 1) {
+                step(no, no, [] { wait_and_meet<2 * NL>(); });
+                p = 1;
+            }
+            while (p + 4 < steps) {
+                step(yes, no, [] { wait_and_meet<2 * FIRST>(); });
+                step(no, no, [] { wait_and_meet<2 * NL>(); });
+                p += 2;
+            }
+            if (p + 3 < steps) {
 #pragma unroll
-                for (int j = 0; j < NL; ++j) store(j);
+                for (int j = 0; j < NL; ++j) fetch(j);
+            }
+        } else {
+            // the last load of !DIRECT would be one step too many
+            for (; p + AHEAD + (DIRECT ? 0 : 1) < steps; ++p)
+                step(yes, no, [] {
+                    if constexpr (DIRECT) wait_and_meet<(AHEAD - 1) * NL>();
+                    else meet<false>();
+                });
+            if constexpr (!DIRECT) {
+                if (p + AHEAD < steps) {
+#pragma unroll
+                    for (int j = 0; j < NL; ++j) store(j);
+                }
             }
         }
-        for (; p + 1 < steps; ++p) step(std::false_type(), std::false_type(), [] { meet<DIRECT>(); });
-        step(std::false_type(), std::true_type(), [] {});
+        for (; p + 1 < steps; ++p) step(no, no, [] { meet<DIRECT>(); });
+        step(no, yes, [] {});
         __syncthreads();
     }
     put<WM, WN, GATED>(J, lds.out[wave], acc, tm, tn, slice, wave, lane);
@@ -490,6 +556,8 @@ __global__ __launch_bounds__(BLOCK) void k_pack(Pack P) {
 // takes 16 channels (of both weights), its W wavefronts parts of the inner dimension: a lane has channel lane % 16, 16 inner indices of
 // each 64 by lane / 16, FEW_BLOCKS loads of either operand under way at once.  The parts meet in LDS.
 constexpr int FEW_BLOCKS = 8;
+// wavefronts of a workgroup
+constexpr int few_waves(i64 k) { return k <= 2048 ? 4 : 8; }
 
 template <int MT, int W, bool GATED>
 __global__ __launch_bounds__(64 * W) void k_few(Job J) {
@@ -594,21 +662,22 @@ __global__ __launch_bounds__(BLOCK) void k_join(Job J) {
 // What a call is done with: the cheapest of these by their times in us, measured on this chip.
 //
 // Tiles, in units of 64 rows and 64 (virtual) columns: a step of one workgroup alone on its CU and of two that share it (0: there is
-// room for one), all CUs busy; what a tile takes beside its steps (first loads, scaling, stores); the same step with operands through
-// registers.  Larger tiles read less a product (a CU's path to LDS takes 64 bytes a cycle, which 128 x 128 tiles would use up) and waste
-// more where the last round of tiles is not full.
+// room for one), all CUs busy; what a tile takes beside its steps (first loads, scaling, stores), and what of that shows where two share a
+// CU; a step with operands through registers, and of two such.  Larger tiles read less a product (a CU's path to LDS takes 64 bytes a
+// cycle, which 128 x 128 tiles would use up) and waste more where the last round of tiles is not full.
 struct Tile {
     int wm, wn, units;
-    double alone, shared, rest, staged;
+    double alone, shared, rest, between, staged, staged_shared;
 };
-constexpr Tile TILES[] = {{4, 4, 4, 0.875, 0, 8, 1.5},           // 8192 x 8192 x 8192 502 us; 128 x 128: 582
-                          {4, 3, 4, 0.67, 0, 8, 1.2},            // 1000 x 4096 x 11008 54 us, 256 x 256: 55
-                          {4, 2, 4, 0.5, 1.015, 6, 0.95},        // gated 1000 x 4096 x 11008 111 us, 256 x 256: 128
-                          {2, 2, 8, 0.56, 1.06, 4, 1.3},         // 1000 x 4096 x 4096 24.7 us, 256 x 128: 36, 64 x 128: 29
-                          {1, 2, 8, 0.42, 0.6, 3, 0.75}};        // 128 x 4096 x 11008 13.3 us, 128 x 128: 16.5
+constexpr Tile TILES[] = {{4, 4, 4, 0.85, 0, 7, 0, 1.45, 0},          // 8192 x 8192 x 8192 464 us; 256 x 192 tiles 521, 256 x 128 495, 128 x 128 551
+                          {4, 3, 4, 0.6, 0, 9, 0, 1.2, 0},            // 1000 x 4096 x 11008 57 us; 256 x 256: 58, 256 x 128: 64
+                          {4, 2, 8, 0.9, 0, 6.5, 0, 1.3, 0},          // 2000 x 4096 x 4096 36 us; 256 x 256: 51, gated 1000 x 4096 x 11008 101, 256 x 192: 103
+                          {2, 2, 8, 0.48, 1.0, 4.5, 1.3, 1.2, 0},     // 1000 x 4096 x 4096 21 us; 256 x 128: 42, 64 x 128: 26
+                          {1, 2, 8, 0.27, 0.62, 3, 0.5, 0.75, 1.25}};  // 128 x 4096 x 4096 12 us; 128 x 128: 15
 constexpr int N_TILES = sizeof(TILES) / sizeof(TILES[0]), CUS = 256;
 constexpr int FEW = N_TILES;                   // k_few, up to FEW_ROWS rows
 constexpr i64 FEW_ROWS = 32;
+constexpr i64 MAX_GROUPS = (1 << 24) - 1;     // a launch has less than 2^32 threads: of 256, and half as many workgroups of 512
 
 struct Plan {
     int tile, slices, steps_per_slice, steps, mt, nt;
@@ -621,10 +690,12 @@ Plan make_plan(i64 m, i64 k, i64 n, bool gated, bool aligned, bool may_pack) {
     const double two = gated ? 2 : 1, weights = two * (double)n * k;
     Plan best = {};
     double least = 1e30;
-    if (m <= FEW_ROWS) {
-        // weights from memory, rows of A once for each 16 channels from the L2s: 1 x 4096 x 11008 11.8 us (64 x 128 tiles in two
-        // slices 14.4), 16 rows 16.1 (14.9), 32 rows of 4096 x 4096 8.3 (10.1)
-        least = weights / 5.0e6 + (double)n * k * m / 16 / 9.5e6 + (double)k / 16384 * 6;
+    if (m <= FEW_ROWS && (n + 15) / 16 <= MAX_GROUPS / 2) {
+        // weights from memory, rows of A once for each 16 channels from the L2s, and a wavefront's blocks of loads one after the other: 1 x 4096 x
+        // 11008 11.8 us (64 x 128 tiles in two slices 14.4), 16 rows 16.1 (14.9), 32 rows of 4096 x 4096 8.3 (10.1); gated 1 x 12288 x 1280
+        // unaligned 34 (13.5 in eight slices)
+        const double blocks = k / 64.0 / few_waves(k) / FEW_BLOCKS;
+        least = weights / (aligned ? 5.0e6 : 3.9e6) + (double)n * k * m / 16 / (m > 16 ? 7.5e6 : 9.5e6) + blocks * (aligned ? 1 : 5) * (gated ? 1.5 : 1);
         best.tile = FEW;
         best.slices = 1;
     }
@@ -635,16 +706,20 @@ Plan make_plan(i64 m, i64 k, i64 n, bool gated, bool aligned, bool may_pack) {
         const i64 rows = 64 * T.wm, cols = (gated ? 32 : 64) * T.wn, mt = (m + rows - 1) / rows, nt = (n + cols - 1) / cols, per_step = 16 * T.units;
         const int steps = (int)((k + per_step - 1) / per_step);
         for (int slices = 1; slices <= 16 && (slices == 1 || (steps / slices >= 4 && (double)mt * nt * slices <= 4 * CUS)); slices *= 2) {
-            const int each = (steps + slices - 1) / slices, used = each ? (steps + each - 1) / each : 1;
+            int each = (steps + slices - 1) / slices;
+            if (T.units == 4) each += each & 1;         // whole lines
+            const int used = each ? (steps + each - 1) / each : 1;
             const double groups = (double)mt * nt * used;
-            const double join = used > 1 ? 3 + (double)used * m * n * two * 8 / 3.5e6 : 0;
+            if (groups > MAX_GROUPS) continue;
+            const double join = used > 1 ? 4.5 + (double)used * m * n * two * 8 / 3.5e6 : 0;
             for (int pack = 0; pack < (may_pack && !aligned ? 2 : 1); ++pack) {
                 const bool staged = !aligned && !pack;
                 // rounds of all CUs, with as many workgroups as share one, then a last that may leave them alone
-                const int share = !staged && T.shared ? 2 : 1;
-                const double alone = staged ? T.staged : T.alone, full = share == 2 ? T.shared : alone;
-                const double rounds = (double)(i64)(groups / (CUS * share)), rest = groups - rounds * CUS * share;
-                const double cost = join + (pack ? pack_cost : 0) + rounds * (each * full + T.rest) + (rest > CUS ? each * full + T.rest : rest > 0 ? each * alone + T.rest : 0);
+                const double alone = staged ? T.staged : T.alone, two_share = staged ? T.staged_shared : T.shared, rest = T.rest * (gated ? 1.5 : 1);
+                const int share = two_share > 0 ? 2 : 1;
+                const double full = each * (share == 2 ? two_share : alone), rounds = (double)(i64)(groups / (CUS * share)), left = groups - rounds * CUS * share;
+                const double cost = join + (pack ? pack_cost : 0) + rounds * (full + (share == 2 ? T.between : rest)) +
+                                    (left > CUS ? full + rest : left > 0 ? each * alone + rest : share == 2 ? rest : 0);
                 if (cost < least) {
                     least = cost;
                     best = {t, used, each, steps, (int)mt, (int)nt, pack != 0, 0, 0};
@@ -690,8 +765,7 @@ void launch_tile(const Plan &L, const Job &J, hipStream_t s) {
     if constexpr (DIRECT) {
         if (L.tile == 0) GO(4, 4, 4, 5, 1);
         if (L.tile == 1) GO(4, 3, 4, 5, 1);
-        if (L.tile == 2 && few) GO(4, 2, 4, 6, 1);
-        if (L.tile == 2 && !few) GO(4, 2, 4, 3, 2);
+        if (L.tile == 2) GO(4, 2, 8, 3, 1);
         if (L.tile == 3 && few) GO(2, 2, 8, 4, 1);
         if (L.tile == 3 && !few) GO(2, 2, 8, 2, 2);
         if (L.tile == 4 && few) GO(1, 2, 8, 6, 1);
@@ -699,7 +773,7 @@ void launch_tile(const Plan &L, const Job &J, hipStream_t s) {
     } else {
         if (L.tile == 0) GO(4, 4, 4, 3, 1);
         if (L.tile == 1) GO(4, 3, 4, 3, 1);
-        if (L.tile == 2) GO(4, 2, 4, 3, 2);
+        if (L.tile == 2) GO(4, 2, 8, 3, 1);
         if (L.tile == 3) GO(2, 2, 8, 3, 1);
         if (L.tile == 4) GO(1, 2, 8, 3, 2);
     }
@@ -709,13 +783,19 @@ void launch_tile(const Plan &L, const Job &J, hipStream_t s) {
 template <bool GATED>
 int launch(const char *who, Job J, void *ws, size_t ws_bytes, hipStream_t s) {
     const bool aligned = aligned_rows(J.a, J.lda) && aligned_rows(J.b, J.ldb) && (!GATED || aligned_rows(J.b2, J.ldb2));
-    Plan L = make_plan(J.m, J.k, J.n, GATED, aligned, true);
+    // the sizes of a call are often those of the thread's last one, and the plan is a good half of a microsecond
+    static thread_local struct {
+        i64 m, k, n;
+        bool aligned;
+        Plan plan;
+    } last = {};
+    if (last.m != J.m || last.k != J.k || last.n != J.n || last.aligned != aligned) last = {J.m, J.k, J.n, aligned, make_plan(J.m, J.k, J.n, GATED, aligned, true)};
+    Plan L = last.plan;
     if (L.pack && (!ws || ws_bytes < L.ws_bytes)) L = make_plan(J.m, J.k, J.n, GATED, aligned, false);
     if (ws_bytes < L.ws_bytes || (L.ws_bytes && !ws)) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, L.ws_bytes);
     if (L.tile == FEW) {
         const dim3 grid((unsigned)((J.n + 15) / 16));
-        // wavefronts for 512 inner indices each, four to sixteen of them
-        const int waves = J.k <= 2048 ? 4 : 8;
+        const int waves = few_waves(J.k);
 #define GO(MT, W) hipLaunchKernelGGL((k_few<MT, W, GATED>), grid, dim3(64 * W), 0, s, J)
         if (J.m <= 16 && waves == 4) GO(1, 4);
         if (J.m <= 16 && waves == 8) GO(1, 8);
@@ -725,7 +805,7 @@ int launch(const char *who, Job J, void *ws, size_t ws_bytes, hipStream_t s) {
         VI_LAUNCH_CHECK(who);
         return VI_OK;
     }
-    if ((double)L.mt * L.nt * L.slices > 0x7FFFFFFF) return vi::fail(VI_EINVAL, "%s: %lld x %lld outputs", who, (long long)J.m, (long long)J.n);
+    if (!L.mt) return vi::fail(VI_EINVAL, "%s: %lld x %lld outputs", who, (long long)J.m, (long long)J.n);
     char *at = (char *)vi::align16(ws);
     J.partial = (int *)(at + L.pack_bytes);
     J.slices = L.slices;

@@ -32,6 +32,7 @@ constexpr int MAX_TOP = 64;                    // a lane of a wavefront for each
 constexpr int KEEP = 512, KEEP_VECTORS = 128;  // collected entries, and 16 bytes of them
 constexpr i64 MAX_V = (i64)1 << 24;
 constexpr int CUS = 256;
+constexpr i64 MAX_ROWS = 1 << 23;              // of a launch, and slices of rows: it has less than 2^32 threads
 constexpr int MAX_R = 16, MAX_WIDE_R = 8;      // 16-byte loads a thread
 
 // a value as a number whose order is that of the values
@@ -562,16 +563,21 @@ extern "C" int vi_token_logprobs(int dtype, const void *logits, int64_t m, int64
     if (m == 0) return VI_OK;
     if (!logits || !tokens || !logprob || !entropy || (top && (!top_logprobs || !top_tokens))) return vi::fail(VI_EINVAL, "%s: null pointer", who);
     const Plan L = make_plan(m, v, dtype, top);
-    if (m > 0x7FFFFFFF / L.slices) return vi::fail(VI_EINVAL, "%s: %lld rows of %lld logits", who, (long long)m, (long long)v);
+    if (m > (L.slices > 1 ? MAX_ROWS / L.slices : 0x7FFFFFFF)) return vi::fail(VI_EINVAL, "%s: %lld rows of %lld logits", who, (long long)m, (long long)v);
     if (ws_bytes < L.ws_bytes || (L.ws_bytes && !ws)) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, L.ws_bytes);
-    Args A = {};
-    A.x = logits, A.v = v, A.ld = ld, A.tokens = tokens, A.c = 1.44269504f / temperature, A.per_t = 1.0f / temperature, A.top = top, A.slices = L.slices, A.per_slice = L.per_slice;
-    A.logprob = logprob, A.entropy = entropy, A.top_logprobs = top_logprobs, A.top_tokens = top_tokens;
-    A.parts = (Part *)vi::align16(ws);
-    A.keys = (u64 *)(A.parts + m * L.slices);
-    if (dtype == VI_F32) launch<VI_F32>(L, A, m, (hipStream_t)stream);
-    if (dtype == VI_BF16) launch<VI_BF16>(L, A, m, (hipStream_t)stream);
-    if (dtype == VI_F16) launch<VI_F16>(L, A, m, (hipStream_t)stream);
-    VI_LAUNCH_CHECK(who);
+    for (i64 first = 0; first < m; first += MAX_ROWS) {
+        const i64 rows = m - first < MAX_ROWS ? m - first : MAX_ROWS;
+        Args A = {};
+        A.x = (const char *)logits + first * ld * size_of(dtype), A.v = v, A.ld = ld, A.tokens = tokens + first;
+        A.c = 1.44269504f / temperature, A.per_t = 1.0f / temperature, A.top = top, A.slices = L.slices, A.per_slice = L.per_slice;
+        A.logprob = logprob + first, A.entropy = entropy + first;
+        A.top_logprobs = top ? top_logprobs + first * top : nullptr, A.top_tokens = top ? top_tokens + first * top : nullptr;
+        A.parts = (Part *)vi::align16(ws);
+        A.keys = (u64 *)(A.parts + m * L.slices);
+        if (dtype == VI_F32) launch<VI_F32>(L, A, rows, (hipStream_t)stream);
+        if (dtype == VI_BF16) launch<VI_BF16>(L, A, rows, (hipStream_t)stream);
+        if (dtype == VI_F16) launch<VI_F16>(L, A, rows, (hipStream_t)stream);
+        VI_LAUNCH_CHECK(who);
+    }
     return VI_OK;
 }

@@ -13,6 +13,7 @@ using namespace num;
 
 constexpr int BLOCK = 256;
 constexpr int CHUNK = 8;                       // neighbouring entries of a thread: 16 or 32 bytes in, 8 out
+constexpr i64 MAX_ROWS = 1 << 23;              // of a launch, which has less than 2^32 threads
 constexpr int MAX_CHUNKS = 8;                  // of a thread, in registers between the two looks at them
 
 // Eight entries as they come, in four words (16-bit types) or eight.
@@ -201,9 +202,13 @@ extern "C" int vi_quantize_rows(int dtype, const void *x, int64_t m, int64_t k, 
     if (m == 0) return VI_OK;
     if (!scale || (k && (!x || !q))) return vi::fail(VI_EINVAL, "vi_quantize_rows: null pointer");
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == VI_F32) launch<VI_F32>(x, m, k, ldx, q, ldq, scale, s);
-    if (dtype == VI_BF16) launch<VI_BF16>(x, m, k, ldx, q, ldq, scale, s);
-    if (dtype == VI_F16) launch<VI_F16>(x, m, k, ldx, q, ldq, scale, s);
-    VI_LAUNCH_CHECK("quantize_rows");
+    for (i64 first = 0; first < m; first += MAX_ROWS) {
+        const void *from = (const char *)x + first * ldx * size_of(dtype);
+        const i64 rows = m - first < MAX_ROWS ? m - first : MAX_ROWS;
+        if (dtype == VI_F32) launch<VI_F32>(from, rows, k, ldx, q + first * ldq, ldq, scale + first, s);
+        if (dtype == VI_BF16) launch<VI_BF16>(from, rows, k, ldx, q + first * ldq, ldq, scale + first, s);
+        if (dtype == VI_F16) launch<VI_F16>(from, rows, k, ldx, q + first * ldq, ldq, scale + first, s);
+        VI_LAUNCH_CHECK("quantize_rows");
+    }
     return VI_OK;
 }
