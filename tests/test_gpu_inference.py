@@ -459,3 +459,17 @@ def test_more_rows_than_a_launch_has_workgroups_for():
         check_logprobs(x[part], t[part], 2)
         for a, b in zip(got + lp, inf.quantize_rows(x[part]) + inf.token_logprobs(x[part], t[part], top=2)):
             assert torch.equal(a[part], b)
+
+
+@pytest.mark.parametrize("m,k,n", [(1500, 4097, 2500), (2000, 1634, 4096), (700, 2111, 9000), (1241, 8200, 1632)])
+def test_unaligned_rows_that_are_copied_first(m, k, n):
+    # the same integers at 16-byte boundaries are read in place; sums are exact either way
+    gen = torch.Generator().manual_seed(k)
+    a, b, c = eighths(m, k, gen), eighths(n, k, gen), eighths(n, k, gen)
+    sa, sb = torch.rand(m, generator=gen).cuda(), torch.rand(n, generator=gen).cuda() * 1e-4
+    even = -k % 16
+    got = inf.int8_matmul(rows(a, 1), rows(b, 3))
+    assert torch.equal(got, inf.int8_matmul(rows(a, even), rows(b, even)))
+    some = torch.arange(0, m, 97)
+    assert torch.equal(got[some.cuda()].cpu(), (a[some].double() @ b.double().T).to(torch.int32))
+    assert torch.equal(inf.int8_gated(rows(a, 0, 1), rows(b, 3), rows(c, 0, 2), sa, sb, sb), inf.int8_gated(rows(a, even), rows(b, even), rows(c, even), sa, sb, sb))

@@ -5,6 +5,10 @@
 //
 // Both operands have their inner dimension along the rows, so a wavefront's operands of a matrix instruction are 16 contiguous bytes a
 // lane.  Sums are exact: |S| <= 2^14 k fits 32 bits up to MAX_K.
+//
+// What bounds them, by rows of A: up to some 32 the weights' way from memory (1 x 4096 x 11008 11 us, 4.1 TB/s); hundreds of rows, where a
+// CU has one small tile, its loads from the L2s (1000 x 4096 x 4096 23 us, 1.5 POP/s at 13 TB/s into LDS); more the matrix cores at the clock
+// that the power limit leaves them (4096 x 4096 x 11008 177 us, 2.1 POP/s; 8192 x 8192 x 8192 464 us, 2.4; gated 1000 x 4096 x 11008 97 us, 1.9).
 #include <type_traits>
 
 #include "int8_gemm.hpp"
@@ -442,12 +446,19 @@ __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
     const auto no = std::false_type();
 
     if (steps > 0) {
+        v4i end[NL];
         if (ragged) {
             const i64 at = (i64)(J.steps - 1 - s0) * STEP;
 #pragma unroll
-            for (int j = 0; j < NL; ++j)
-                *(v4i *)(lds.in + (j * 4 + wave) * 1024 + lane * 16) = load_part(source(j) + at + off[j], J.k - (i64)(J.steps - 1) * STEP - unit);
+            for (int j = 0; j < NL; ++j) end[j] = load_end(source(j) + at + off[j], J.k - (i64)(J.steps - 1) * STEP - unit, J.k);
         }
+        // behind the other loads' requests
+        auto store_end = [&]() {
+            if (ragged) {
+#pragma unroll
+                for (int j = 0; j < NL; ++j) *(v4i *)(lds.in + (j * 4 + wave) * 1024 + lane * 16) = end[j];
+            }
+        };
         // how far the loads go in front of the loop, and the first position there
         if constexpr (PAIR) {
             // two steps, then two more, or one: positions from `ragged` on
@@ -461,6 +472,7 @@ __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
                     for (int j = 0; j < NL; ++j) fetch(j);
                 }
             }
+            store_end();
             if (left >= 2 * pairs) wait_and_meet<2 * NL>();            // all but the last pair
             else wait_and_meet<0>();
         } else if constexpr (DIRECT) {
@@ -470,6 +482,7 @@ __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
 #pragma unroll
                     for (int j = 0; j < NL; ++j) fetch(j);
                 }
+            store_end();
             if (steps >= AHEAD) wait_and_meet<(AHEAD - 1) * NL>();
             else wait_and_meet<0>();
         } else {
@@ -489,6 +502,7 @@ __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
                         }
                     }
             }
+            store_end();
             meet<false>();
         }
 #pragma unroll
@@ -532,7 +546,11 @@ __global__ __launch_bounds__(BLOCK, PER_CU) void k_tile(Job J) {
 }
 
 // ---- rows at any address, to 16-byte boundaries -------------------------------------------------------------------
-// Up to three matrices in one launch, 16 bytes a thread, zero behind the last of a row.
+// Up to three matrices in one launch, 16 bytes a thread, zero behind the last of a row: whole lines, and whole steps of any tile, so that no
+// row has a ragged end any more.
+constexpr i64 LINE = 128;
+i64 whole_lines(i64 k) { return (k + LINE - 1) / LINE * LINE; }
+
 struct Pack {
     const signed char *from[3];
     v4i *to[3];
@@ -547,20 +565,19 @@ __global__ __launch_bounds__(BLOCK) void k_pack(Pack P) {
         const i64 at = p - row * P.units;
         const int which = row < P.rows[0] ? 0 : row < P.rows[1] ? 1 : 2;
         if (which) row -= P.rows[which - 1];
-        P.to[which][row * P.units + at] = load_part(P.from[which] + row * P.ld[which] + at * 16, P.k - at * 16);
+        P.to[which][row * P.units + at] = load_end(P.from[which] + row * P.ld[which] + at * 16, P.k - at * 16, P.k);
     }
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------
 // Up to 16 MT rows: the weights are read once and hardly used, so they go from memory to the matrix instruction without LDS.  A workgroup
-// takes 16 channels (of both weights), its W wavefronts parts of the inner dimension: a lane has channel lane % 16, 16 inner indices of
+// takes 16 channels (of both weights), its eight wavefronts parts of the inner dimension: a lane has channel lane % 16, 16 inner indices of
 // each 64 by lane / 16, FEW_BLOCKS loads of either operand under way at once.  The parts meet in LDS.
-constexpr int FEW_BLOCKS = 8;
-// wavefronts of a workgroup
-constexpr int few_waves(i64 k) { return k <= 2048 ? 4 : 8; }
+constexpr int FEW_BLOCKS = 8, FEW_WAVES = 8;
 
-template <int MT, int W, bool GATED>
-__global__ __launch_bounds__(64 * W) void k_few(Job J) {
+template <int MT, bool GATED>
+__global__ __launch_bounds__(64 * FEW_WAVES) void k_few(Job J) {
+    constexpr int W = FEW_WAVES;
     constexpr int NT = GATED ? 2 : 1;
     __shared__ int parts[W][NT * MT * 256];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -604,9 +621,9 @@ __global__ __launch_bounds__(64 * W) void k_few(Job J) {
         const i64 at = (i64)blocks * 64, left = J.k - at - (lane >> 4) * 16;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-            const v4i xv = load_part(x[i] + at, left);
+            const v4i xv = load_end(x[i] + at, left, J.k);
 #pragma unroll
-            for (int h = 0; h < NT; ++h) acc[h][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(load_part(w[h] + at, left), xv, acc[h][i], 0, 0, 0);
+            for (int h = 0; h < NT; ++h) acc[h][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(load_end(w[h] + at, left, J.k), xv, acc[h][i], 0, 0, 0);
         }
     }
     // register r of a lane is channel 4 (lane / 16) + r of row lane % 16
@@ -671,7 +688,7 @@ struct Tile {
 };
 constexpr Tile TILES[] = {{4, 4, 4, 0.85, 0, 7, 0, 1.45, 0},          // 8192 x 8192 x 8192 464 us; 256 x 192 tiles 521, 256 x 128 495, 128 x 128 551
                           {4, 3, 4, 0.6, 0, 9, 0, 1.2, 0},            // 1000 x 4096 x 11008 57 us; 256 x 256: 58, 256 x 128: 64
-                          {4, 2, 8, 0.9, 0, 6.5, 0, 1.3, 0},          // 2000 x 4096 x 4096 36 us; 256 x 256: 51, gated 1000 x 4096 x 11008 101, 256 x 192: 103
+                          {4, 2, 8, 0.9, 0, 6.5, 0, 1.5, 0},          // 2000 x 4096 x 4096 36 us; 256 x 256: 51, gated 1000 x 4096 x 11008 101, 256 x 192: 103
                           {2, 2, 8, 0.48, 1.0, 4.5, 1.3, 1.2, 0},     // 1000 x 4096 x 4096 21 us; 256 x 128: 42, 64 x 128: 26
                           {1, 2, 8, 0.27, 0.62, 3, 0.5, 0.75, 1.25}};  // 128 x 4096 x 4096 12 us; 128 x 128: 15
 constexpr int N_TILES = sizeof(TILES) / sizeof(TILES[0]), CUS = 256;
@@ -694,7 +711,7 @@ Plan make_plan(i64 m, i64 k, i64 n, bool gated, bool aligned, bool may_pack) {
         // weights from memory, rows of A once for each 16 channels from the L2s, and a wavefront's blocks of loads one after the other: 1 x 4096 x
         // 11008 11.8 us (64 x 128 tiles in two slices 14.4), 16 rows 16.1 (14.9), 32 rows of 4096 x 4096 8.3 (10.1); gated 1 x 12288 x 1280
         // unaligned 34 (13.5 in eight slices)
-        const double blocks = k / 64.0 / few_waves(k) / FEW_BLOCKS;
+        const double blocks = k / 64.0 / FEW_WAVES / FEW_BLOCKS;
         least = weights / (aligned ? 5.0e6 : 3.9e6) + (double)n * k * m / 16 / (m > 16 ? 7.5e6 : 9.5e6) + blocks * (aligned ? 1 : 5) * (gated ? 1.5 : 1);
         best.tile = FEW;
         best.slices = 1;
@@ -727,7 +744,7 @@ Plan make_plan(i64 m, i64 k, i64 n, bool gated, bool aligned, bool may_pack) {
             }
         }
     }
-    if (best.pack) best.pack_bytes = (size_t)((k + 15) / 16 * 16) * (m + (gated ? 2 : 1) * n);
+    if (best.pack) best.pack_bytes = (size_t)whole_lines(k) * (m + (gated ? 2 : 1) * n);
     best.ws_bytes = best.pack_bytes + (best.slices > 1 ? (size_t)4 * best.slices * (gated ? 2 : 1) * m * n : 0);
     if (best.ws_bytes) best.ws_bytes += vi::WS_SLACK;
     return best;
@@ -760,7 +777,7 @@ template <bool GATED, bool DIRECT>
 void launch_tile(const Plan &L, const Job &J, hipStream_t s) {
     const int groups = L.mt * L.nt * L.slices;
     const dim3 grid((unsigned)groups);
-    const bool few = groups <= CUS;            // deeper prefetch where no CU has two
+    const bool few = groups <= CUS;            // deeper prefetch where no CU has two: 1000 x 4096 x 4096 23 us, 29 without; 128 x 4096 x 4096 11.7, 12.7
 #define GO(WM, WN, U, ST, CU) hipLaunchKernelGGL((k_tile<WM, WN, U, ST, CU, GATED, DIRECT>), grid, dim3(BLOCK), 0, s, J)
     if constexpr (DIRECT) {
         if (L.tile == 0) GO(4, 4, 4, 5, 1);
@@ -795,13 +812,8 @@ int launch(const char *who, Job J, void *ws, size_t ws_bytes, hipStream_t s) {
     if (ws_bytes < L.ws_bytes || (L.ws_bytes && !ws)) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, L.ws_bytes);
     if (L.tile == FEW) {
         const dim3 grid((unsigned)((J.n + 15) / 16));
-        const int waves = few_waves(J.k);
-#define GO(MT, W) hipLaunchKernelGGL((k_few<MT, W, GATED>), grid, dim3(64 * W), 0, s, J)
-        if (J.m <= 16 && waves == 4) GO(1, 4);
-        if (J.m <= 16 && waves == 8) GO(1, 8);
-        if (J.m > 16 && waves == 4) GO(2, 4);
-        if (J.m > 16 && waves == 8) GO(2, 8);
-#undef GO
+        if (J.m <= 16) hipLaunchKernelGGL((k_few<1, GATED>), grid, dim3(64 * FEW_WAVES), 0, s, J);
+        else hipLaunchKernelGGL((k_few<2, GATED>), grid, dim3(64 * FEW_WAVES), 0, s, J);
         VI_LAUNCH_CHECK(who);
         return VI_OK;
     }
@@ -816,7 +828,8 @@ int launch(const char *who, Job J, void *ws, size_t ws_bytes, hipStream_t s) {
     if (L.pack) {
         Pack P = {};
         P.k = J.k;
-        P.units = (J.k + 15) / 16;
+        P.units = whole_lines(J.k) / 16;
+        J.k = J.steps * (16 * TILES[L.tile].units);
         const signed char **from[3] = {&J.a, &J.b, &J.b2};
         i64 *ld[3] = {&J.lda, &J.ldb, &J.ldb2}, rows = 0;
         for (int i = 0; i < 3; ++i) {

@@ -13,7 +13,7 @@
 // are taken, and each counts how many are above it.  Where more reach the bound than LDS holds (equal values), another is found by a
 // bisection over the keys, all entries counted in each step, until few enough reach it: at the latest with the exact one.
 //
-// 1000 x 32000 bfloat16, 5 largest: 22 us, 2.9 TB/s; 4096 rows 61 us, 4.3 TB/s.  A wave's 128 entries a lane are some 11 operations and an
+// 1000 x 32000 bfloat16, 5 largest: 21 us, 3.0 TB/s; 4096 rows 61 us, 4.3 TB/s.  A wave's 128 entries a lane are some 11 operations and an
 // exponential each, 10 us of the CUs' time for 1000 rows, which comes behind the loads where all rows are there at once, and under them where
 // there are more.  Sums taken as the loads arrive, relative to an entry of each thread, were no faster (23.5 us, 64).
 //
