@@ -473,3 +473,27 @@ def test_unaligned_rows_that_are_copied_first(m, k, n):
     some = torch.arange(0, m, 97)
     assert torch.equal(got[some.cuda()].cpu(), (a[some].double() @ b.double().T).to(torch.int32))
     assert torch.equal(inf.int8_gated(rows(a, 0, 1), rows(b, 3), rows(c, 0, 2), sa, sb, sb), inf.int8_gated(rows(a, even), rows(b, even), rows(c, even), sa, sb, sb))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("v", [70, 1000, 3000, 9001, 32000, 70001, 200003])
+@pytest.mark.parametrize("top", [1, 3, 20, 64])
+def test_logprobs_of_negative_zeros(dtype, v, top):
+    """-0.0 is equal to 0.0, and goes with it by the lowest index"""
+    gen = torch.Generator().manual_seed(v)
+    x = (-torch.randn(8, v, generator=gen).abs() - 1).to(dtype)
+    x[0] = -0.0
+    x[1] = -0.0
+    x[1, v // 2] = 5.0                         # one positive entry
+    x[2, :16] = -0.0                           # in front of 0.0
+    x[2, 64:70] = 0.0
+    x[3, 3::64] = -0.0                         # far apart, among negative ones
+    x[4] = -0.0
+    x[4, v - 1] = 0.0
+    x[5] = -math.inf
+    x[5, 5:60:7] = -0.0
+    x[6, v - 20:] = -0.0
+    x[7] = (torch.randn(v, generator=gen).abs() * 1e-9).neg().to(dtype)     # float16: underflows to -0.0
+    check_logprobs(x.cuda(), torch.tensor([0, 1, 2, 3, 4, 5, v - 1, 7], device="cuda"), top)
+    many = x[:1].expand(300, v).contiguous().cuda()                         # one workgroup of 256 threads a row, or slices of it
+    check_logprobs(many, torch.arange(300, device="cuda") % v, top)

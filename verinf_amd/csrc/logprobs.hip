@@ -326,7 +326,7 @@ __global__ __launch_bounds__(B, 4) void k_slice(Args A) {
     const float most = value_of((u64)all << 32), m = centre(most);
     // -inf does not reach it; where none are asked for only +inf does, which does no harm
     const float bound = A.top ? value_of((u64)max(reach, ordered(-FLT_MAX)) << 32) : INFINITY;
-    const Largest<DT> least(bound);
+    const Largest<DT> least(bound == 0.0f ? -0.0f : bound);        // 0.0 reaches -0.0 as well, but not the other way round: bits are compared
     float z = 0, w = 0;
     again(raw);
 #pragma unroll
