@@ -124,6 +124,22 @@ def zeros(so):
                 L.check(x, kind, tokens, top)
 
 
+def few(so):
+    """Rows with fewer allowed entries than are asked for: the rest is filled up, no entries are counted for it.  A workgroup comes to as many
+    barriers in every type."""
+    L = Logprobs(so)
+    for v in (300, 1000, 9001, 30000):
+        for allowed in (0, 1, 2, 5):
+            print("few", v, allowed, flush=True)
+            x = np.full((1, v), -np.inf, np.float32)
+            x[0, np.random.default_rng(v).choice(v, allowed, replace=False)] = np.arange(allowed) - 2
+            met = []
+            for kind in FLOATS:
+                L.check(x, kind, np.array([v // 2]), 8)
+                met.append(L.met)
+            assert met[0] == met[1] == met[2], (v, allowed, met)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[1]](sys.argv[2])
     print("OK")

@@ -70,3 +70,7 @@ def check(built, unit, what, **switches):
 
 def test_log_probabilities_of_negative_zeros(built):
     check(built, "logprobs", "zeros")
+
+
+def test_log_probabilities_of_few_allowed_entries(built):
+    check(built, "logprobs", "few")

@@ -18,7 +18,7 @@
 // there are more.  Sums taken as the loads arrive, relative to an entry of each thread, were no faster (23.5 us, 64).
 //
 // -inf is no value: such entries are not in the sums nor collected.  Where there are fewer than `top` others the lowest indexes of -inf
-// fill up, which are among the first `top` entries.  NaN or +inf make Z NaN, and with it everything but the order.
+// fill up, which are among the first `top` entries (1000 x 50257 float16, 8 largest: 39 us with 5 entries allowed, 35 with 500).  NaN or +inf make Z NaN, and with it everything but the order.
 #include <cfloat>
 
 #include "number_types.hpp"
@@ -324,8 +324,9 @@ __global__ __launch_bounds__(B, 4) void k_slice(Args A) {
     u32 all, reach;
     look_at_all(sh, ordered(top.value()), A.top, &all, &reach);
     const float most = value_of((u64)all << 32), m = centre(most);
-    // -inf does not reach it; where none are asked for only +inf does, which does no harm
-    const float bound = A.top ? value_of((u64)max(reach, ordered(-FLT_MAX)) << 32) : INFINITY;
+    // -inf does not reach it, nor once it is a number of the type; where none are asked for only +inf does, which does no harm
+    constexpr float LOWEST = DT == VI_F32 ? -FLT_MAX : DT == VI_BF16 ? -0x1.FEp127f : -65504.0f;
+    const float bound = A.top ? value_of((u64)max(reach, ordered(LOWEST)) << 32) : INFINITY;
     const Largest<DT> least(bound == 0.0f ? -0.0f : bound);        // 0.0 reaches -0.0 as well, but not the other way round: bits are compared
     float z = 0, w = 0;
     again(raw);
