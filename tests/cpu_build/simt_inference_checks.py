@@ -140,6 +140,34 @@ def few(so):
             assert met[0] == met[1] == met[2], (v, allowed, met)
 
 
+def rows(so):
+    """Every form of the launch: threads to a row, loads to a thread, one slice and several; ragged ends, rows apart; what is no number."""
+    L = Logprobs(so)
+    for kind in FLOATS:
+        unit = 1024 if kind == 0 else 2048                     # entries that 256 threads load at once
+        for m, v, pad, top in ((1, 1, 0, 1), (3, 2, 1, 2), (2, 63, 0, 63), (2, unit, 3, 64), (2, unit + 1, 0, 5), (1, 4 * unit + 1, 0, 5), (1, 9 * unit, 0, 64),
+                               (1, 32 * unit, 0, 8), (1, 32 * unit + 1, 1, 8), (2, 35 * unit, 0, 20), (257, unit + 1, 0, 2), (257, 2 * unit + 3, 0, 2),
+                               (300, 4 * unit - 5, 0, 3), (300, 8 * unit + 1, 0, 2)) + (((520, 6 * unit + 1, 0, 1), (520, 9 * unit, 0, 2)) if kind == 1 else ()):
+            print("rows", FLOATS[kind], m, v, pad, top, flush=True)
+            rng = np.random.default_rng(m + v)
+            x = (rng.standard_normal((m, v)) * 4).astype(np.float32)
+            if v > 2:
+                x[m // 2, : v // 3] = -np.inf
+            L.check(x, kind, rng.integers(-1, v, m), top, 0.7 if pad else 1.0, pad)
+        for v in (70, 3 * unit, 33 * unit):
+            print("no numbers", FLOATS[kind], v, flush=True)
+            x = np.random.default_rng(v).standard_normal((8, v)).astype(np.float32)
+            x[0] = -np.inf
+            x[1] = LOWEST[kind]
+            x[2] = 1.5
+            x[3, 5] = np.nan
+            x[4, [3, 60]], x[4, 61] = np.inf, np.nan
+            x[5] = np.arange(v) % 3
+            x[6], x[6, 9] = -np.inf, np.nan
+            x[7, :40], x[7, 40:] = -np.inf, LOWEST[kind]
+            L.check(x, kind, np.array([0, 1, v, -2, 3, -1, 6, 50]), 20)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[1]](sys.argv[2])
     print("OK")

@@ -573,8 +573,10 @@ extern "C" int vi_token_logprobs(int dtype, const void *logits, int64_t m, int64
         A.c = 1.44269504f / temperature, A.per_t = 1.0f / temperature, A.top = top, A.slices = L.slices, A.per_slice = L.per_slice;
         A.logprob = logprob + first, A.entropy = entropy + first;
         A.top_logprobs = top ? top_logprobs + first * top : nullptr, A.top_tokens = top ? top_tokens + first * top : nullptr;
-        A.parts = (Part *)vi::align16(ws);
-        A.keys = (u64 *)(A.parts + m * L.slices);
+        if (L.slices > 1) {
+            A.parts = (Part *)vi::align16(ws);
+            A.keys = (u64 *)(A.parts + m * L.slices);
+        }
         if (dtype == VI_F32) launch<VI_F32>(L, A, rows, (hipStream_t)stream);
         if (dtype == VI_BF16) launch<VI_BF16>(L, A, rows, (hipStream_t)stream);
         if (dtype == VI_F16) launch<VI_F16>(L, A, rows, (hipStream_t)stream);
