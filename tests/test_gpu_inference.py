@@ -497,3 +497,20 @@ def test_logprobs_of_negative_zeros(dtype, v, top):
     check_logprobs(x.cuda(), torch.tensor([0, 1, 2, 3, 4, 5, v - 1, 7], device="cuda"), top)
     many = x[:1].expand(300, v).contiguous().cuda()                         # one workgroup of 256 threads a row, or slices of it
     check_logprobs(many, torch.arange(300, device="cuda") % v, top)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("m,n", [(1, 256), (20, 256), (33, 256), (200, 256), (200, 253)])
+def test_gelu_of_negative_numbers(dtype, m, n):
+    """x Phi(x) far below zero has all its digits: G = 0, -0.1, -0.2 ... -12.8 in the first row, U = 0.1."""
+    g = torch.arange(n, dtype=torch.int64).sub(255).div(2, rounding_mode="floor").to(torch.int8)[:, None].cuda()
+    one = torch.ones((m, 1), dtype=torch.int8, device="cuda")
+    sa = 0.1 / torch.arange(1, m + 1, device="cuda").float()
+    sn = torch.ones((n,), device="cuda")
+    out = inf.int8_gated(one, g, torch.ones_like(g), sa, sn, sn, activation="gelu", dtype=dtype)
+    G = (g[:, 0].float()[None, :] * sa[:, None]).double().cpu()                       # as it is in 32 bits
+    want = 0.5 * G * torch.special.erfc(-G * 0.5 ** 0.5) * sa.double().cpu()[:, None]
+    # the argument's rounding and that of the constant: 1.5 units of 2^-24, times the 2 t^2 = x^2 by which erfc grows; 16 units of 2^-23 of erfc itself; four products
+    rel = 2.0 ** -24 * (1.5 * (1 + G ** 2) + 32 + 4)
+    most = want.abs() * (rel + ROUND[dtype] * 1.0001) + LEAST[dtype]
+    assert ((out.cpu().double() - want).abs() <= most).all()

@@ -56,7 +56,20 @@ __device__ __forceinline__ float silu(float x) {
     return (x < 0.0f ? x * t : x) * fmaf(fmaf(-y, r, 1.0f), r, r);
 }
 
-__device__ __forceinline__ float gelu(float x) { return 0.5f * x * (1.0f + erff(x * 0.70710678f)); }
+// x Phi(x), with all digits below zero too, where 0.5 (1 + erf(x / sqrt 2)) cancels (4 % off at -5, 0 from -5.5 on):
+// Phi(-u) = e^(-u^2 / 2) h(u), and h, which falls slowly from 1/2, is q P(q) with q = 1 / (1 + 0.27 u), P of degree 8 fitted to it over
+// Chebyshev's nodes of q (2.4e-8 of h off for u up to 14.5, where the exponential has ended).  Some 7 + x^2 units of 2^-24 off, the second
+// from the exponent's roundings.  Gated 1000 x 4096 x 11008 100 us, 1000 x 512 x 11008 31.5; 112 and 31.6 with erff, 111 and 36 with erfcf.
+__device__ __forceinline__ float gelu(float x) {
+    constexpr float P[] = {0.107720658f, 0.107542865f, 0.101810686f, 0.0720492899f, 0.107826404f,
+                           -0.0692119151f, 0.169787183f, -0.126486361f, 0.0289612059f};
+    const float q = __builtin_amdgcn_rcpf(fmaf(fabsf(x), 0.27f, 1.0f));
+    float p = P[8];
+#pragma unroll
+    for (int i = 7; i >= 0; --i) p = fmaf(p, q, P[i]);
+    const float tail = p * q * __builtin_amdgcn_exp2f(x * (x * -0.72134752f));
+    return x < 0.0f ? x * tail : fmaf(-x, tail, x);
+}
 
 __device__ __forceinline__ void activate(float (&v)[VEC], int act) {
     if (act == VI_GELU) {
