@@ -111,21 +111,39 @@ T lane_value(T v, int from) {
     return v;
 }
 
-typedef int v4i __attribute__((ext_vector_type(4)));
-// 16 x 16 x 64 on signed bytes: lane l holds row (column) l % 16 of A (B), the sixteen inner indices from 16 (l / 16); register r of the
-// result is row 4 (l / 16) + r of column l % 16
-inline v4i mfma_16x16x64(const v4i &a, const v4i &b, v4i c) {
+// Matrix instructions on signed bytes, 16 * PARTS inner indices: lane l holds row (column) l % N of A (B), the sixteen inner indices from
+// 16 (l / N); at(r) is the row of the result's register r, whose column is l % N.
+template <int N, int REGS, class At>
+__attribute__((no_sanitize("address", "undefined"))) void multiply(const int8_t (*a)[16], const int8_t (*b)[16], int32_t *c, int lane, At at) {
+    for (int r = 0; r < REGS; ++r)
+        for (int part = 0; part < 64; part += N) {
+            const int8_t *x = a[at(r) + part], *y = b[lane % N + part];
+            int sum = 0;
+            for (int i = 0; i < 16; ++i) sum += x[i] * y[i];
+            c[r] += sum;
+        }
+}
+inline int8_t bytes_a[16][64][16], bytes_b[16][64][16];
+template <int N, int REGS, class V, class C, class At>
+void mfma(const V &a, const V &b, C &c, At at) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int i = 0; i < 4; ++i) {
-        wave_a[wave][lane][i] = a[i];
-        wave_b[wave][lane][i] = b[i];
-    }
+    memcpy(bytes_a[wave][lane], &a, 16);
+    memcpy(bytes_b[wave][lane], &b, 16);
     __builtin_amdgcn_wave_barrier();
-    for (int r = 0; r < 4; ++r)
-        for (int part = 0; part < 4; ++part)
-            for (int i = 0; i < 4; ++i)
-                c[r] = __builtin_amdgcn_sdot4(wave_a[wave][4 * (lane / 16) + r + 16 * part][i], wave_b[wave][lane % 16 + 16 * part][i], c[r], false);
+    int32_t sums[REGS];
+    memcpy(sums, &c, sizeof(sums));
+    multiply<N, REGS>(bytes_a[wave], bytes_b[wave], sums, lane, at);
+    memcpy(&c, sums, sizeof(sums));
     __builtin_amdgcn_wave_barrier();
+}
+template <class V, class C>
+C mfma_32x32x32(const V &a, const V &b, C c) {
+    mfma<32, 16>(a, b, c, [half = (int)(threadIdx.x & 63) / 32](int r) { return 8 * (r / 4) + 4 * half + r % 4; });
+    return c;
+}
+template <class V, class C>
+C mfma_16x16x64(const V &a, const V &b, C c) {
+    mfma<16, 4>(a, b, c, [part = (int)(threadIdx.x & 63) / 16](int r) { return 4 * part + r; });
     return c;
 }
 
@@ -144,7 +162,7 @@ inline Two swap_halves(uint32_t a, uint32_t b) {
 
 template <class T>
 T __shfl_xor(T v, int mask) { return simt::lane_value(v, (int)(threadIdx.x & 63) ^ mask); }
-inline uint64_t __ballot(bool v) {                                    // where all lanes are
+__attribute__((no_sanitize("address", "undefined"))) inline uint64_t __ballot(bool v) {                                    // where all lanes are
     const uint64_t *lanes = simt::all_say(v);
     uint64_t all = 0;
     for (int i = 0; i < 64; ++i) all |= lanes[i] << i;
@@ -157,6 +175,8 @@ inline void simt_meet() {
 #define __syncthreads() simt_meet()
 #define __builtin_amdgcn_sched_barrier(x) ((void)0)
 #define __builtin_amdgcn_permlane32_swap(a, b, x, y) simt::swap_halves(a, b)
+#undef __builtin_amdgcn_mfma_i32_32x32x32_i8
+#define __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, c, x, y, z) simt::mfma_32x32x32(a, b, c)
 #define __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, x, y, z) simt::mfma_16x16x64(a, b, c)
 // results below the least normal number are zero
 inline float simt_exp2(float x) {

@@ -1,6 +1,9 @@
 """The kernels of the forward pass in 8-bit integers on the CPU (simt_inference.hpp), against 64-bit results, as a program of its own: the
 test runs it under AddressSanitizer, where every numpy array is a heap block of exactly its size."""
 import ctypes
+import json
+import math
+import os
 import sys
 
 import numpy as np
@@ -35,7 +38,14 @@ def decode(a, kind):
 def strided(a, pad, shift=0):
     """The rows of a with `pad` elements of something else behind each, nothing behind the last; a view and how far they are apart."""
     m, k = a.shape
-    flat = np.full(shift + (m - 1) * (k + pad) + k, 77, dtype=a.dtype)
+    n = shift + (m - 1) * (k + pad) + k
+    others = []
+    for lead in (0, 8) * 50:                                   # bytes: the first element is at a multiple of 16 bytes, but for the shift
+        flat = np.full(n + lead // a.itemsize, 77, dtype=a.dtype)
+        others.append(flat)
+        if (flat.ctypes.data + lead) % 16 == 0:
+            break
+    flat = flat[lead // a.itemsize:]
     view = np.lib.stride_tricks.as_strided(flat[shift:], (m, k), ((k + pad) * a.itemsize, a.itemsize))
     view[:] = a
     return view, k + pad
@@ -120,7 +130,7 @@ def zeros(so):
             x[5, 5:60:7] = -0.0
             x[6, v - 20:] = -0.0
             tokens = np.array([0, 1, 2, 3, 4, 5, v - 1])
-            for top in (1, 3, 20, 64) if v < 10000 else (5, 64):
+            for top in (1, 3, 20, 64) if v < 3000 else (5, 64) if v < 10000 else (5,):
                 L.check(x, kind, tokens, top)
 
 
@@ -146,8 +156,8 @@ def rows(so):
     for kind in FLOATS:
         unit = 1024 if kind == 0 else 2048                     # entries that 256 threads load at once
         for m, v, pad, top in ((1, 1, 0, 1), (3, 2, 1, 2), (2, 63, 0, 63), (2, unit, 3, 64), (2, unit + 1, 0, 5), (1, 4 * unit + 1, 0, 5), (1, 9 * unit, 0, 64),
-                               (1, 32 * unit, 0, 8), (1, 32 * unit + 1, 1, 8), (2, 35 * unit, 0, 20), (257, unit + 1, 0, 2), (257, 2 * unit + 3, 0, 2),
-                               (300, 4 * unit - 5, 0, 3), (300, 8 * unit + 1, 0, 2)) + (((520, 6 * unit + 1, 0, 1), (520, 9 * unit, 0, 2)) if kind == 1 else ()):
+                               (1, 32 * unit, 0, 8), (1, 32 * unit + 1, 1, 8), (2, 35 * unit, 0, 20), (257, unit + 1, 0, 2)) + \
+                (((257, 2 * unit + 3, 0, 2), (300, 4 * unit - 5, 0, 3), (300, 8 * unit + 1, 0, 2), (520, 6 * unit + 1, 0, 1), (520, 9 * unit, 0, 2)) if kind == 1 else ()):
             print("rows", FLOATS[kind], m, v, pad, top, flush=True)
             rng = np.random.default_rng(m + v)
             x = (rng.standard_normal((m, v)) * 4).astype(np.float32)
@@ -166,6 +176,143 @@ def rows(so):
             x[6], x[6, 9] = -np.inf, np.nan
             x[7, :40], x[7, 40:] = -np.inf, LOWEST[kind]
             L.check(x, kind, np.array([0, 1, v, -2, 3, -1, 6, 50]), 20)
+
+
+# ---- products -----------------------------------------------------------------------------------------------------
+I32, FIELD, SILU, GELU = 3, 4, 0, 1
+P = (1 << 64) - (1 << 32) + 1
+ROUND = {0: 2.0 ** -24, 1: 2.0 ** -8, 2: 2.0 ** -11}          # half a unit in the last place, relative
+LEAST = {0: 2.0 ** -126, 1: 2.0 ** -126, 2: 2.0 ** -24}
+OUT = {0: np.float32, 1: np.uint16, 2: np.float16, I32: np.int32, FIELD: np.uint64}
+
+
+class Products:
+    def __init__(self, so):
+        self.L = L = ctypes.CDLL(so)
+        L.simt_workspace.restype, L.simt_workspace.argtypes = SZ, [INT, INT, INT, INT, I64, I64, I64]
+        L.simt_product.argtypes = [INT] * 4 + [VP, I64] * 3 + [I64] * 3 + [VP] * 4 + [INT, INT, VP, VP]
+        L.simt_error.restype = ctypes.c_char_p
+        self.tiles = L.simt_tiles()
+
+    def check(self, gated, tile, m, k, n, kind, slices=1, pack=0, pad=None, shift=0, bias=False, act=SILU):
+        """One product; pad: bytes behind each row, to 16-byte boundaries where there is none given."""
+        rng = np.random.default_rng(m * 131 + k * 17 + n + tile)
+        a, b, u = (rng.integers(-128, 128, (r, k)).astype(np.int8) for r in (m, n, n))
+        pad = -k % 16 if pad is None else pad
+        (ga, lda), (gb, ldb), (gu, ldu) = (strided(t, pad, shift) for t in (a, b, u))
+        assert not k or all(t.ctypes.data % 16 == shift for t in (ga, gb, gu))
+        sa, sb, su = (((rng.random(r) * 0.01 + 0.0001) * 9 / math.sqrt(k + 1) ** p).astype(np.float32) for r, p in ((m, 0), (n, 1), (n, 1)))
+        add = rng.standard_normal(n).astype(np.float32) if bias else None
+        out = np.empty((m, n), OUT[kind])
+        ws = scratch(self.L.simt_workspace(gated, tile, slices, pack, m, k, n)) if tile < self.tiles else None
+        rc = self.L.simt_product(gated, tile, slices, pack, ga.ctypes.data, lda, gb.ctypes.data, ldb, gu.ctypes.data if gated else None, ldu, m, k, n, ptr(sa), ptr(sb), ptr(su), ptr(add), act, kind, ptr(out), ptr(ws))
+        what = ("gated" if gated else "plain", "tile", tile, m, k, n, "type", kind, "slices", slices, "copy", pack, "pad", pad, "shift", shift, "bias", bias, "act", act)
+        assert rc == 0, (what, self.L.simt_error())
+        S = a.astype(np.int64) @ b.astype(np.int64).T
+        if kind == I32:
+            assert np.array_equal(out, S), what
+            return
+        if kind == FIELD:
+            assert np.array_equal(out, np.where(S < 0, S.astype(np.uint64) + np.uint64(P), S.astype(np.uint64))), what
+            return
+        got = decode(out, kind).astype(np.float64)
+        G = S * sa.astype(np.float64)[:, None] * sb.astype(np.float64)
+        if not gated:
+            # the sum's conversion, two products and an addition in 32 bits, then one rounding to the type
+            want = G if add is None else G + add
+            most = np.abs(want) * (ROUND[kind] * 1.0001) + 2.0 ** -24 * 4 * (np.abs(G) + (0 if add is None else np.abs(add))) + LEAST[kind]
+        else:
+            U = (a.astype(np.int64) @ u.astype(np.int64).T) * sa.astype(np.float64)[:, None] * su.astype(np.float64)
+            acted = G / (1 + np.exp(-G)) if act == SILU else G * 0.5 * np.vectorize(math.erfc)(-G * math.sqrt(0.5))
+            want = acted * U
+            # three roundings of 2^-24 in G and in U; silu's argument, exponential and reciprocal; gelu's relative derivative is below 1 + x^2, and its
+            # exponential has no results below 2^-126, which U multiplies
+            rel = 2.0 ** -24 * (8 + 8 * np.abs(G)) if act == SILU else 2.0 ** -24 * (16 + 8 * np.abs(G) ** 2)
+            most = np.abs(want) * (ROUND[kind] * 1.0001 + rel) + LEAST[kind] + 2.0 ** -126 * np.abs(U)
+        assert (np.abs(got - want) <= most).all(), (what, np.max(np.abs(got - want) - most))
+
+
+SIZES = [(256, 256), (256, 192), (256, 128), (128, 128), (64, 128)]    # of the tiles; half as many channels gated
+STEPS = [64, 64, 128, 128, 128]
+
+
+def tiles(so, pick):
+    """Every tile over one to nine steps, with and without a ragged end: operands straight into LDS, through registers, copied first; all types."""
+    L = Products(so)
+    assert L.tiles == len(SIZES)
+    for tile in range(L.tiles):
+        rows, cols = SIZES[tile]
+        for gated in (0, 1):
+            wide = cols // 2 if gated else cols
+            kinds = (0, 1, 2) if gated else (0, 1, 2, I32, FIELD)
+            at = 0
+            for steps in range(1, 10):
+                for end in (0, 1, 16, 37):
+                    k = steps * STEPS[tile] - (STEPS[tile] - end if end else 0)
+                    # whole tiles; a ragged one; a little more than one
+                    m, n = ((rows, wide), (rows - 7, wide - 5), (33, wide), (1, 1))[(steps + end) % 4]
+                    at += 1
+                    kind = kinds[at % len(kinds)]
+                    print(pick, gated, tile, m, k, n, kind, flush=True)
+                    opts = {"bias": at % 2 == 0 and not gated, "act": at // 3 % 2}
+                    if pick == "direct":
+                        L.check(gated, tile, m, k, n, kind, **opts)
+                    elif pick == "staged":
+                        L.check(gated, tile, m, k, n, kind, pad=1 + at % 3, shift=at % 2, **opts)
+                    elif pick == "copied" and steps % 2:
+                        L.check(gated, tile, m, k, n, kind, pack=1, pad=1 + at % 3, shift=at % 2, **opts)
+                    elif pick == "sliced" and steps > 2:
+                        L.check(gated, tile, m, k, n, kind, slices=2 + at % 3, pad=at % 2 or None, pack=at % 2 * (at // 2 % 2), **opts)
+            # several tiles, each way out to the end of a row
+            for kind in kinds:
+                print(pick, gated, tile, "several", kind, flush=True)
+                more = {"pad": 3} if pick in ("staged", "copied") else {}
+                L.check(gated, tile, rows + 1, 200, 2 * wide + 3, kind, slices=2 if pick == "sliced" else 1, pack=int(pick == "copied"), act=kind % 2, **more)
+                L.check(gated, tile, rows + 40, 100, 2 * wide, kind, slices=2 if pick == "sliced" else 1, pack=int(pick == "copied"), act=kind % 2, bias=not gated, **more)
+
+
+def direct(so):
+    tiles(so, "direct")
+
+
+def staged(so):
+    tiles(so, "staged")
+
+
+def copied(so):
+    tiles(so, "copied")
+
+
+def sliced(so):
+    tiles(so, "sliced")
+
+
+def few_rows(so):
+    """Up to 32 rows: lengths about a block of 64 and the workgroup's eight parts, no channels or rows behind the last."""
+    L = Products(so)
+    for gated in (0, 1):
+        for at, (m, k, n) in enumerate([(1, 1, 1), (1, 15, 3), (2, 16, 16), (3, 0, 5), (1, 63, 17), (16, 64, 33), (17, 65, 16), (5, 500, 40), (32, 513, 18),
+                                        (31, 4200, 16), (1, 9000, 5), (16, 4096, 20)]):
+            for kind in (0, 1, 2) if gated else (0, 1, 2, I32, FIELD):
+                print("few rows", gated, m, k, n, kind, flush=True)
+                L.check(gated, L.tiles, m, k, n, kind, pad=(None, 0, 1)[at % 3], shift=at % 2, bias=not gated and kind != 1, act=at % 2)
+
+
+def plans(so):
+    """The sizes of the tests on the GPU, which are in SHAPES: what they reach."""
+    L = ctypes.CDLL(so)
+    L.simt_plan.argtypes = [I64, I64, I64, INT, INT, VP]
+    for gated, shapes in enumerate(json.loads(os.environ["SHAPES"])):
+        reached = set()
+        for m, k, n, aligned in shapes:
+            plan = np.zeros(3, np.int32)
+            L.simt_plan(m, k, n, gated, aligned, ptr(plan))
+            tile, slices, copied = plan
+            print("plan", gated, m, k, n, aligned, *plan, flush=True)
+            reached |= {("tile", tile)} if aligned else {("copied" if copied else "through registers", "slices" if slices > 1 else "one slice")}
+            reached |= {"slices"} if aligned and slices > 1 else set()
+        want = {("tile", t) for t in range(L.simt_tiles())} | {(how, s) for how in ("copied", "through registers") for s in ("slices", "one slice")} | {"slices"}
+        assert reached == want, want - reached
 
 
 if __name__ == "__main__":

@@ -3,6 +3,7 @@ cpu_build/simt (workgroups as fibers), run through their own entry points under 
 
 Their inline assembly is replaced in a copy of the source, statement by statement: a load straight into LDS, its place, the waits and the
 barriers by what they do (simt_inference.hpp), an empty one by nothing.  One that is not known here is an error."""
+import json
 import os
 import re
 import subprocess
@@ -48,7 +49,7 @@ def _build(unit, folder):
         with open(os.path.join(folder, name), "w") as f:
             f.write(text.replace('"../../include/verinf_hip.h"', f'"{os.path.join(os.path.dirname(HERE), "include", "verinf_hip.h")}"'))
     so = os.path.join(folder, f"simt_{unit}.so")
-    subprocess.check_call([CLANG, "-O1", "-g", "-std=c++17", "-fPIC", "-shared", "-rtlib=compiler-rt", "-ffp-contract=off", "-Wno-unknown-attributes", "-Wno-unused-value",
+    subprocess.check_call([CLANG, "-O2", "-g", "-std=c++17", "-fPIC", "-shared", "-rtlib=compiler-rt", "-ffp-contract=off", "-Wno-unknown-attributes", "-Wno-unused-value", "-Wno-psabi",
                            "-fsanitize=address,undefined", "-fno-sanitize=function,vptr", "-fno-sanitize-recover=undefined", "-shared-libasan", "-I", folder,
                            "-I", DIR, "-I", os.path.join(DIR, "simt"), "-o", so, os.path.join(DIR, f"simt_{unit}.cpp")])
     return so
@@ -78,3 +79,22 @@ def test_log_probabilities_of_few_allowed_entries(built):
 
 def test_log_probabilities_over_their_forms(built):
     check(built, "logprobs", "rows")
+
+
+@pytest.mark.parametrize("how", ["direct", "staged", "copied", "sliced"])
+def test_products_of_every_tile(built, how):
+    check(built, "int8_gemm", how)
+
+
+@pytest.mark.parametrize("how", ["direct", "copied", "sliced"])
+def test_products_whose_loads_arrive_late(built, how):
+    check(built, "int8_gemm", how, SIMT_LATE="1")
+
+
+def test_products_of_few_rows(built):
+    check(built, "int8_gemm", "few_rows")
+
+
+def test_the_sizes_of_the_gpu_tests_take_every_tile(built):
+    import test_gpu_inference as gpu
+    check(built, "int8_gemm", "plans", SHAPES=json.dumps([gpu.LARGE, gpu.LARGE_GATED]))

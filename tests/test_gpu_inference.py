@@ -514,3 +514,58 @@ def test_gelu_of_negative_numbers(dtype, m, n):
     rel = 2.0 ** -24 * (1.5 * (1 + G ** 2) + 32 + 4)
     most = want.abs() * (rel + ROUND[dtype] * 1.0001) + LEAST[dtype]
     assert ((out.cpu().double() - want).abs() <= most).all()
+
+
+# m, k, n, rows at 16-byte boundaries: sizes that between them take every tile, plain and gated (which the CPU build asserts of them), with whole and
+# ragged tiles and inner dimensions; unaligned ones read through registers or copied, in one slice and in several
+LARGE = [(5000, 448, 3000, True), (3001, 500, 5003, True), (8191, 300, 2000, True), (1025, 4100, 11009, True), (2500, 1411, 4099, True), (2000, 4096, 4099, True),
+         (1025, 4096, 8000, True), (4095, 1000, 2000, True), (2049, 4096, 3000, True), (2049, 1411, 1000, True), (4095, 400, 3000, True), (300, 4096, 400, True),
+         (1537, 130, 8000, False), (2060, 257, 3000, False), (130, 8200, 3000, False), (4100, 1411, 400, False), (1030, 8200, 400, False)]
+LARGE_GATED = [(4095, 1000, 2000, True), (2049, 1411, 3000, True), (4100, 2048, 1500, True), (777, 4100, 5003, True), (2049, 4096, 2000, True), (1300, 4096, 2305, True),
+               (2049, 4100, 1500, True), (1300, 1000, 2305, True), (2049, 1000, 1500, True), (300, 4096, 200, True),
+               (1000, 257, 8000, False), (333, 1411, 11008, False), (130, 8200, 3000, False), (1537, 1024, 2000, False), (200, 8200, 1030, False)]
+
+
+def large_operands(m, k, n, aligned, weights):
+    gen = torch.Generator(device="cuda").manual_seed(m * 131 + k * 17 + n)
+    pads = [-k % 16] * 3 if aligned else [1 + (-k % 16), 3, 5]
+    mats = [rows(torch.randint(-128, 128, (r, k), generator=gen, device="cuda", dtype=torch.int8), pad, 0 if aligned else 1) for r, pad in zip([m] + [n] * weights, pads)]
+    # rows of every tile, the first and the last among them; sums of them in 64 bits
+    some = torch.unique(torch.cat([torch.arange(0, m, max(1, m // 61)), torch.tensor([0, m - 1])])).cuda()
+    return mats, [mats[0][some].double() @ w.double().T for w in mats[1:]], some, gen
+
+
+@pytest.mark.parametrize("m,k,n,aligned", LARGE)
+def test_matmul_of_large_tiles(m, k, n, aligned):
+    (a, b), (S,), some, gen = large_operands(m, k, n, aligned, 1)
+    assert torch.equal(inf.int8_matmul(a, b)[some], S.to(torch.int32))
+    s = S.to(torch.int64)
+    assert torch.equal(inf.int8_matmul(a, b, dtype=torch.uint64).view(torch.int64)[some], torch.where(s < 0, s - ((1 << 32) - 1), s))
+    sa = torch.rand((m,), generator=gen, device="cuda") * 0.1 + 0.001
+    sb = torch.rand((n,), generator=gen, device="cuda") * 0.01 + 0.0001
+    s = S * sa.double()[some, None] * sb.double()
+    for dtype in FLOATS:
+        for bias in (None, torch.randn((n,), generator=gen, device="cuda")):
+            out = inf.int8_matmul(a, b, sa, sb, bias=bias, dtype=dtype)
+            want = s if bias is None else s + bias.double()
+            # as of the small ones: the sum's conversion, two products and an addition in 32 bits, then one rounding to the type
+            most = want.abs() * (ROUND[dtype] * 1.0001) + 2.0 ** -24 * 4 * (s.abs() + (0 if bias is None else bias.double().abs())) + LEAST[dtype]
+            assert ((out[some].double() - want).abs() <= most).all()
+
+
+@pytest.mark.parametrize("m,k,n,aligned", LARGE_GATED)
+def test_gated_of_large_tiles(m, k, n, aligned):
+    (a, g, u), (S, T), some, gen = large_operands(m, k, n, aligned, 2)
+    sa = torch.rand((m,), generator=gen, device="cuda") * 0.02 + 0.001
+    sg, su = ((torch.rand((n,), generator=gen, device="cuda") * 0.01 + 0.0001) * 40 / math.sqrt(k + 1) for _ in range(2))
+    G, U = S * sa.double()[some, None] * sg.double(), T * sa.double()[some, None] * su.double()
+    for act in ("silu", "gelu"):
+        acted = G * torch.sigmoid(G) if act == "silu" else 0.5 * G * torch.special.erfc(-G * 0.5 ** 0.5)
+        want = acted * U
+        # three roundings of 2^-24 in G and in U; silu's argument, exponential and reciprocal; gelu's relative derivative is below 1 + x^2, and its
+        # exponential has no results below 2^-126, which U multiplies
+        rel = 2.0 ** -24 * (8 + 8 * G.abs() if act == "silu" else 16 + 8 * G ** 2)
+        for dtype in FLOATS:
+            out = inf.int8_gated(a, g, u, sa, sg, su, activation=act, dtype=dtype)
+            most = want.abs() * (ROUND[dtype] * 1.0001 + rel) + LEAST[dtype] + 2.0 ** -126 * U.abs()
+            assert ((out[some].double() - want).abs() <= most).all()

@@ -797,19 +797,9 @@ void launch_tile(const Plan &L, const Job &J, hipStream_t s) {
 #undef GO
 }
 
+// a call as planned; ws is large enough
 template <bool GATED>
-int launch(const char *who, Job J, void *ws, size_t ws_bytes, hipStream_t s) {
-    const bool aligned = aligned_rows(J.a, J.lda) && aligned_rows(J.b, J.ldb) && (!GATED || aligned_rows(J.b2, J.ldb2));
-    // the sizes of a call are often those of the thread's last one, and the plan is a good half of a microsecond
-    static thread_local struct {
-        i64 m, k, n;
-        bool aligned;
-        Plan plan;
-    } last = {};
-    if (last.m != J.m || last.k != J.k || last.n != J.n || last.aligned != aligned) last = {J.m, J.k, J.n, aligned, make_plan(J.m, J.k, J.n, GATED, aligned, true)};
-    Plan L = last.plan;
-    if (L.pack && (!ws || ws_bytes < L.ws_bytes)) L = make_plan(J.m, J.k, J.n, GATED, aligned, false);
-    if (ws_bytes < L.ws_bytes || (L.ws_bytes && !ws)) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, L.ws_bytes);
+int run(const char *who, const Plan &L, Job J, bool aligned, void *ws, hipStream_t s) {
     if (L.tile == FEW) {
         const dim3 grid((unsigned)((J.n + 15) / 16));
         if (J.m <= 16) hipLaunchKernelGGL((k_few<1, GATED>), grid, dim3(64 * FEW_WAVES), 0, s, J);
@@ -817,7 +807,6 @@ int launch(const char *who, Job J, void *ws, size_t ws_bytes, hipStream_t s) {
         VI_LAUNCH_CHECK(who);
         return VI_OK;
     }
-    if (!L.mt) return vi::fail(VI_EINVAL, "%s: %lld x %lld outputs", who, (long long)J.m, (long long)J.n);
     char *at = (char *)vi::align16(ws);
     J.partial = (int *)(at + L.pack_bytes);
     J.slices = L.slices;
@@ -855,6 +844,23 @@ int launch(const char *who, Job J, void *ws, size_t ws_bytes, hipStream_t s) {
         VI_LAUNCH_CHECK(who);
     }
     return VI_OK;
+}
+
+template <bool GATED>
+int launch(const char *who, const Job &J, void *ws, size_t ws_bytes, hipStream_t s) {
+    const bool aligned = aligned_rows(J.a, J.lda) && aligned_rows(J.b, J.ldb) && (!GATED || aligned_rows(J.b2, J.ldb2));
+    // the sizes of a call are often those of the thread's last one, and the plan is a good half of a microsecond
+    static thread_local struct {
+        i64 m, k, n;
+        bool aligned;
+        Plan plan;
+    } last = {};
+    if (last.m != J.m || last.k != J.k || last.n != J.n || last.aligned != aligned) last = {J.m, J.k, J.n, aligned, make_plan(J.m, J.k, J.n, GATED, aligned, true)};
+    Plan L = last.plan;
+    if (L.pack && (!ws || ws_bytes < L.ws_bytes)) L = make_plan(J.m, J.k, J.n, GATED, aligned, false);
+    if (ws_bytes < L.ws_bytes || (L.ws_bytes && !ws)) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, L.ws_bytes);
+    if (L.tile != FEW && !L.mt) return vi::fail(VI_EINVAL, "%s: %lld x %lld outputs", who, (long long)J.m, (long long)J.n);
+    return run<GATED>(who, L, J, aligned, ws, s);
 }
 
 }  // namespace
