@@ -56,6 +56,37 @@ def scratch(nbytes):
     return np.full(nbytes + 8, 0xA5, dtype=np.uint8)[8:]
 
 
+# ---- quantize_rows ------------------------------------------------------------------------------------------------
+def quantize(so):
+    """Rows in 16 lanes, a wavefront and a workgroup, in one to eight chunks a thread and read twice; ends of one to seven entries; the definition's
+    operations one by one in 32 bits."""
+    L = ctypes.CDLL(so)
+    L.vi_quantize_rows.argtypes = [INT, VP, I64, I64, I64, VP, I64, VP, VP]
+    for kind in FLOATS:
+        for m, k, pad, shift in ((1, 1, 0, 0), (3, 0, 2, 0), (3, 7, 1, 0), (2, 8, 0, 0), (5, 1000, 3, 0), (2, 2049, 0, 4), (2, 4100, 0, 0), (1, 8191, 0, 0), (2, 11008, 0, 0),
+                                 (2, 12289, 1, 0), (1, 16384, 0, 0), (2, 16385, 3, 0), (1, 40001, 0, 4), (1025, 100, 0, 0), (1030, 130, 1, 0), (1024, 256, 0, 4), (2050, 300, 0, 0),
+                                 (2048, 1000, 1, 0), (2049, 2047, 0, 0)):
+            print("quantize", FLOATS[kind], m, k, pad, shift, flush=True)
+            x = (np.random.default_rng(m + k).standard_normal((m, k)) * 5).astype(np.float32)
+            if k > 6 and m > 4:
+                x[0], x[1], x[2, 3], x[3, k - 1] = 0, -0.0, np.nan, -np.inf
+                x[4] = 2.0 ** -118 if kind != 2 else 2.0 ** -24
+            a, ldx = strided(encode(x, kind), pad, shift if kind else 0)
+            f = decode(a, kind)
+            q, scale = np.full((m - 1) * (k + pad) + max(k, 1), 99, np.int8), np.empty(m, np.float32)
+            assert L.vi_quantize_rows(kind, a.ctypes.data, m, k, ldx, q.ctypes.data, k + pad, ptr(scale), None) == 0
+            with np.errstate(all="ignore"):
+                top, finite = np.abs(f).max(axis=1, initial=0), np.isfinite(f).all(axis=1)
+                fine = finite & (top >= np.float32(127) * np.float32(2.0 ** -126))
+                step = np.where(fine, np.float32(127) / top, np.float32(0)).astype(np.float32)
+                want = np.where(fine[:, None], np.rint(f * step[:, None]), 0).astype(np.int8)
+                want_scale = np.where(fine, top / np.float32(127), np.where(finite, np.float32(0), np.float32(np.nan)))
+            got = np.lib.stride_tricks.as_strided(q, (m, k), (k + pad, 1))
+            assert np.array_equal(got, want) and np.array_equal(scale, want_scale.astype(np.float32), equal_nan=True), (FLOATS[kind], m, k)
+            for r in range(m - 1):
+                assert (q[r * (k + pad) + k:(r + 1) * (k + pad)] == 99).all()
+
+
 # ---- token_logprobs -----------------------------------------------------------------------------------------------
 class Logprobs:
     def __init__(self, so):

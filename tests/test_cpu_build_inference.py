@@ -98,3 +98,7 @@ def test_products_of_few_rows(built):
 def test_the_sizes_of_the_gpu_tests_take_every_tile(built):
     import test_gpu_inference as gpu
     check(built, "int8_gemm", "plans", SHAPES=json.dumps([gpu.LARGE, gpu.LARGE_GATED]))
+
+
+def test_rows_to_8_bits(built):
+    check(built, "quantize", "quantize")
