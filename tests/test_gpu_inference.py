@@ -569,3 +569,22 @@ def test_gated_of_large_tiles(m, k, n, aligned):
             out = inf.int8_gated(a, g, u, sa, sg, su, activation=act, dtype=dtype)
             most = want.abs() * (ROUND[dtype] * 1.0001 + rel) + LEAST[dtype] + 2.0 ** -126 * U.abs()
             assert ((out[some].double() - want).abs() <= most).all()
+
+
+def test_tensors_with_a_tangent_are_refused():
+    from torch.autograd import forward_ad
+    x, s, ws = torch.randn((4, 64), device="cuda"), torch.ones((4,), device="cuda"), torch.ones((6,), device="cuda")
+    q, w, t = torch.zeros((4, 64), dtype=torch.int8, device="cuda"), torch.zeros((6, 64), dtype=torch.int8, device="cuda"), torch.zeros((4,), dtype=torch.int64, device="cuda")
+    with forward_ad.dual_level():
+        dx, ds, dws = (forward_ad.make_dual(v, torch.ones_like(v)) for v in (x, s, ws))
+        for call in (lambda: inf.quantize_rows(dx), lambda: inf.token_logprobs(dx, t), lambda: inf.int8_matmul(q, w, ds, ws), lambda: inf.int8_matmul(q, w, s, ws, bias=dws),
+                     lambda: inf.int8_gated(q, w, w, s, dws, ws), lambda: inf.quantize_rows(dx[:, :7])):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="tangent"):
+                call()
+        # others are taken there as anywhere
+        assert torch.equal(inf.quantize_rows(x)[0], inf.quantize_rows(forward_ad.unpack_dual(dx).primal)[0])
+        inf.int8_gated(q, w, w, s, ws, ws)
+        inf.token_logprobs(x, t, top=2)
+    for call in (inf.quantize_rows, lambda v: inf.token_logprobs(v, t)[0]):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (x,), (x,))
