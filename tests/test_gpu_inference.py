@@ -588,3 +588,18 @@ def test_tensors_with_a_tangent_are_refused():
     for call in (inf.quantize_rows, lambda v: inf.token_logprobs(v, t)[0]):
         with pytest.raises(RuntimeError):
             torch.func.jvp(call, (x,), (x,))
+
+
+def test_negative_views_are_refused():
+    """the imaginary part of a conjugate is a view of numbers of the other sign"""
+    x = torch.complex(torch.zeros((4, 1), device="cuda"), torch.randn((4, 1), device="cuda")).conj().imag
+    assert x.is_neg()
+    q, w, t = torch.ones((4, 8), dtype=torch.int8, device="cuda"), torch.ones((6, 8), dtype=torch.int8, device="cuda"), torch.zeros((4,), dtype=torch.int64, device="cuda")
+    s, ws = torch.ones((4,), device="cuda"), torch.ones((6,), device="cuda")
+    minus, minus_ws = torch._neg_view(s), torch._neg_view(ws)
+    for call in (lambda: inf.quantize_rows(x), lambda: inf.token_logprobs(x, t), lambda: inf.int8_matmul(q, w, minus, ws), lambda: inf.int8_matmul(q, w, s, ws, bias=minus_ws),
+                 lambda: inf.int8_gated(q, w, w, s, ws, minus_ws), lambda: inf.int8_matmul(torch._neg_view(q), w)):
+        with pytest.raises(RuntimeError, match="resolve_neg"):
+            call()
+    got, scale = inf.quantize_rows(x.resolve_neg())
+    assert torch.equal(got[:, 0].float().sign(), x[:, 0].sign()) and (scale > 0).all()

@@ -35,6 +35,8 @@ def _refuse(t, name, dtypes, dims, device):
         raise RuntimeError(f"{name} dtype must be {' or '.join(str(d)[6:] for d in dtypes)}")
     if t.dim() != dims:
         raise RuntimeError(f"{name} must have {dims} dimensions")
+    if t.is_neg():
+        raise RuntimeError(f"{name} is the negative of what its memory holds (take its resolve_neg())")
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{name} requires a gradient: these operators have none (detach it, or call them under torch.no_grad())")
     if forward_ad._current_level >= 0 and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
@@ -44,7 +46,7 @@ def _refuse(t, name, dtypes, dims, device):
 def _matrix(t, name, dtypes, device=None):
     """Rows, columns and how many elements the rows are apart.  The checks are a call's host time, so the usual case is one line."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in dtypes and t.dim() == 2 and not t.requires_grad
-            and forward_ad._current_level < 0 and (device is None or t.device == device)):
+            and not t.is_neg() and forward_ad._current_level < 0 and (device is None or t.device == device)):
         _refuse(t, name, dtypes, 2, device)
     m, k = t.shape
     ld, apart = t.stride()
@@ -60,7 +62,7 @@ def _matrix(t, name, dtypes, device=None):
 def _vector(t, name, length, dtype, device):
     """The address of a contiguous vector."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dtype == dtype and t.dim() == 1 and not t.requires_grad
-            and forward_ad._current_level < 0 and t.device == device):
+            and not t.is_neg() and forward_ad._current_level < 0 and t.device == device):
         _refuse(t, name, (dtype,), 1, device)
     if t.shape[0] != length:
         raise RuntimeError(f"{name} has {t.shape[0]} elements, not {length}")
