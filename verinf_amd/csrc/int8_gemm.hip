@@ -6,9 +6,11 @@
 // Both operands have their inner dimension along the rows, so a wavefront's operands of a matrix instruction are 16 contiguous bytes a
 // lane.  Sums are exact: |S| <= 2^14 k fits 32 bits up to MAX_K.
 //
-// What bounds them, by rows of A: up to some 32 the weights' way from memory (1 x 4096 x 11008 11 us, 4.1 TB/s); hundreds of rows, where a
-// CU has one small tile, its loads from the L2s (1000 x 4096 x 4096 23 us, 1.5 POP/s at 13 TB/s into LDS); more the matrix cores at the clock
-// that the power limit leaves them (4096 x 4096 x 11008 177 us, 2.1 POP/s; 8192 x 8192 x 8192 464 us, 2.4; gated 1000 x 4096 x 11008 97 us, 1.9).
+// What bounds them, by rows of A: up to some 32 the weights' way from memory (1 x 4096 x 11008 11-12 us, 4 TB/s).  Hundreds of rows, where a
+// CU has one small tile and a SIMD one wavefront, what that wavefront waits for: 1000 x 4096 x 4096 takes 23 us, 1.45 POP/s (as field elements
+// 27); its wavefronts are at a wait or barrier for 51 % of their cycles, the matrix cores work in 43 %, LDS is read in 23 %, and 27 bytes a cycle
+// come from the L2s of 64 that the path takes.  More rows, the matrix cores at the clock that the power limit leaves them (4096 x 4096 x 11008
+// 177-188 us by the card, 2.0 POP/s; 8192 x 8192 x 8192 462-480, 2.3; gated 1000 x 4096 x 11008 97-106, 1.8).
 #include <type_traits>
 
 #include "int8_gemm.hpp"
@@ -153,7 +155,6 @@ __device__ __forceinline__ void put_rows(const Job &J, char *buf, const v16i (&a
                     if constexpr (DT == VI_I32) {
                         *(v4i *)to = v4i{s[0], s[1], s[2], s[3]};
                     } else {
-                        // p - |s| below zero: the upper word is 2^32 - 1 either way, the lower one more
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
                             *(v4i *)(to + 16 * e) = v4i{residue_low(s[2 * e]), residue_high(s[2 * e]), residue_low(s[2 * e + 1]), residue_high(s[2 * e + 1])};
@@ -686,11 +687,11 @@ struct Tile {
     int wm, wn, units;
     double alone, shared, rest, between, staged, staged_shared;
 };
-constexpr Tile TILES[] = {{4, 4, 4, 0.85, 0, 7, 0, 1.45, 0},          // 8192 x 8192 x 8192 464 us; 256 x 192 tiles 521, 256 x 128 495, 128 x 128 551
-                          {4, 3, 4, 0.6, 0, 9, 0, 1.2, 0},            // 1000 x 4096 x 11008 57 us; 256 x 256: 58, 256 x 128: 64
-                          {4, 2, 8, 0.9, 0, 6.5, 0, 1.5, 0},          // 2000 x 4096 x 4096 36 us; 256 x 256: 51, gated 1000 x 4096 x 11008 101, 256 x 192: 103
-                          {2, 2, 8, 0.48, 1.0, 4.5, 1.3, 1.2, 0},     // 1000 x 4096 x 4096 21 us; 256 x 128: 42, 64 x 128: 26
-                          {1, 2, 8, 0.27, 0.62, 3, 0.5, 0.75, 1.25}};  // 128 x 4096 x 4096 12 us; 128 x 128: 15
+constexpr Tile TILES[] = {{4, 4, 4, 0.85, 0, 7, 0, 1.45, 0},          // 8192 x 8192 x 8192 462 us; 256 x 192 tiles 524, 256 x 128 494, 128 x 128 588
+                          {4, 3, 4, 0.6, 0, 9, 0, 1.2, 0},            // 1000 x 4096 x 11008 58 us; 256 x 256: 58, 256 x 128: 65, 128 x 128: 74
+                          {4, 2, 8, 0.9, 0, 6.5, 0, 1.5, 0},          // 2000 x 4096 x 4096 37 us; 256 x 256: 51, 128 x 128: 41; gated 1000 x 4096 x 11008 103, 256 x 192: 106
+                          {2, 2, 8, 0.48, 1.0, 4.5, 1.3, 1.2, 0},     // 1000 x 4096 x 4096 23 us; 256 x 128: 26, 64 x 128: 24
+                          {1, 2, 8, 0.27, 0.62, 3, 0.5, 0.75, 1.25}};  // 128 x 4096 x 4096 12 us; 128 x 128: 16
 constexpr int N_TILES = sizeof(TILES) / sizeof(TILES[0]), CUS = 256;
 constexpr int FEW = N_TILES;                   // k_few, up to FEW_ROWS rows
 constexpr i64 FEW_ROWS = 32;
@@ -709,7 +710,7 @@ Plan make_plan(i64 m, i64 k, i64 n, bool gated, bool aligned, bool may_pack) {
     double least = 1e30;
     if (m <= FEW_ROWS && (n + 15) / 16 <= MAX_GROUPS / 2) {
         // weights from memory, rows of A once for each 16 channels from the L2s, and a wavefront's blocks of loads one after the other: 1 x 4096 x
-        // 11008 11.8 us (64 x 128 tiles in two slices 14.4), 16 rows 16.1 (14.9), 32 rows of 4096 x 4096 8.3 (10.1); gated 1 x 12288 x 1280
+        // 11008 12.0 us (64 x 128 tiles in slices 14.6), 16 rows 16.6 (15.7), 32 rows of 4096 x 4096 8.3 (10.2); gated 1 x 12288 x 1280
         // unaligned 34 (13.5 in eight slices)
         const double blocks = k / 64.0 / FEW_WAVES / FEW_BLOCKS;
         least = weights / (aligned ? 5.0e6 : 3.9e6) + (double)n * k * m / 16 / (m > 16 ? 7.5e6 : 9.5e6) + blocks * (aligned ? 1 : 5) * (gated ? 1.5 : 1);
@@ -777,7 +778,7 @@ template <bool GATED, bool DIRECT>
 void launch_tile(const Plan &L, const Job &J, hipStream_t s) {
     const int groups = L.mt * L.nt * L.slices;
     const dim3 grid((unsigned)groups);
-    const bool few = groups <= CUS;            // deeper prefetch where no CU has two: 1000 x 4096 x 4096 23 us, 29 without; 128 x 4096 x 4096 11.7, 12.7
+    const bool few = groups <= CUS;            // deeper prefetch where no CU has two: 1000 x 4096 x 4096 23 us, 30 without; 128 x 4096 x 4096 12.1, 12.8
 #define GO(WM, WN, U, ST, CU) hipLaunchKernelGGL((k_tile<WM, WN, U, ST, CU, GATED, DIRECT>), grid, dim3(BLOCK), 0, s, J)
     if constexpr (DIRECT) {
         if (L.tile == 0) GO(4, 4, 4, 5, 1);

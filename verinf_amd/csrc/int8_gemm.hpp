@@ -37,7 +37,7 @@ __device__ __forceinline__ v4i load_part(const signed char *p, i64 left) {
 }
 
 // The same of a row of k: one load, of a long row's last 16 bytes at the latest, moved down where they begin before p.  (In single
-// bytes, one behind the other, 3000 x 250 x 3000 took 27 us, 18 so, 12.7 with 256.)
+// bytes, one behind the other, 3000 x 250 x 3000 took 27 us, 17-18 so, 12.3 with 256.)
 __device__ __forceinline__ v4i load_end(const signed char *p, i64 left, i64 k) {
     if (k < 16) return load_part(p, left);
     const int here = (int)max((i64)0, min(left, (i64)16)), bits = (16 - here) * 8 & 63;
@@ -59,7 +59,8 @@ __device__ __forceinline__ float silu(float x) {
 // x Phi(x), with all digits below zero too, where 0.5 (1 + erf(x / sqrt 2)) cancels (4 % off at -5, 0 from -5.5 on):
 // Phi(-u) = e^(-u^2 / 2) h(u), and h, which falls slowly from 1/2, is q P(q) with q = 1 / (1 + 0.27 u), P of degree 8 fitted to it over
 // Chebyshev's nodes of q (2.4e-8 of h off for u up to 14.5, where the exponential has ended).  Some 7 + x^2 units of 2^-24 off, the second
-// from the exponent's roundings.  Gated 1000 x 4096 x 11008 100 us, 1000 x 512 x 11008 31.5; 112 and 31.6 with erff, 111 and 36 with erfcf.
+// from the exponent's roundings.  Gated 1000 x 4096 x 11008 100 us, 1000 x 512 x 11008 31.5 (silu 98 and 28);
+// 112 and 31.6 with erff, 111 and 36 with erfcf.
 __device__ __forceinline__ float gelu(float x) {
     constexpr float P[] = {0.107720658f, 0.107542865f, 0.101810686f, 0.0720492899f, 0.107826404f,
                            -0.0692119151f, 0.169787183f, -0.126486361f, 0.0289612059f};

@@ -4,21 +4,24 @@
 //
 // One pass over the logits: a workgroup keeps its slice of a row in registers, 16-byte loads all requested before the first is
 // looked at, and goes over them twice, for M and for the sums.  A row is cut into slices where there are few rows; a second
-// launch joins the slices' (M, Z, sum, largest) and finishes.  All sums are in 32 bits, in the base of v_exp_f32: e^d = 2^((x - M) c), c = log2(e) / T.
+// launch joins the slices' (M, Z, sum, largest) and finishes.  All sums are in 32 bits, in the base of v_exp_f32: e^d = 2^((x - M) c), c = log2(e) / T,
+// c and the product rounded to 32 bits and the exponential by the hardware, about 1e-7 of a log probability in all (0.5e-7 with expf).
 //
 // The largest entries.  Entries are ordered by a 64-bit key, above the value's bits as an ordered number (NaN above infinity, -0 as 0),
 // below the complement of the index, so that keys differ and equal values go by the lowest index.  Each thread's largest value is known
 // after the first pass; the top-th largest of them (or a little less: bisection with ballots, ended once few enough reach it) is a
 // bound below which no entry of the result is, and hardly more than `top` entries reach it: they are collected in LDS while the sums
 // are taken, and each counts how many are above it.  Where more reach the bound than LDS holds (equal values), another is found by a
-// bisection over the keys, all entries counted in each step, until few enough reach it: at the latest with the exact one.
+// bisection over the keys, all entries counted in each step, until few enough reach it: at the latest with the exact one.  (That branch alone
+// has registers in scratch memory, 23 to 55 of them with 16 loads a thread.)
 //
-// 1000 x 32000 bfloat16, 5 largest: 21 us, 3.0 TB/s; 4096 rows 61 us, 4.3 TB/s.  A wave's 128 entries a lane are some 11 operations and an
+// 1000 x 32000 bfloat16, 5 largest: 21-23 us, 2.9 TB/s; 4096 rows 60 us, 4.3 TB/s.  A wave's 128 entries a lane are some 11 operations and an
 // exponential each, 10 us of the CUs' time for 1000 rows, which comes behind the loads where all rows are there at once, and under them where
 // there are more.  Sums taken as the loads arrive, relative to an entry of each thread, were no faster (23.5 us, 64).
 //
 // -inf is no value: such entries are not in the sums nor collected.  Where there are fewer than `top` others the lowest indexes of -inf
-// fill up, which are among the first `top` entries (1000 x 50257 float16, 8 largest: 39 us with 5 entries allowed, 35 with 500).  NaN or +inf make Z NaN, and with it everything but the order.
+// fill up, which are among the first `top` entries (1000 x 50257 float16, 8 largest: 39 us with 5 entries allowed, 35 with 500).  NaN or +inf
+// make Z NaN, and with it everything but the order.
 #include <cfloat>
 
 #include "number_types.hpp"

@@ -7,7 +7,8 @@
 // row's scale NaN and its integers zero, so that it shows in every product with them.
 //
 // Memory bounds it: a row stays in registers between the two looks at it, so it is read once.  32000 x 4096 float32 132 us, 5.0 TB/s in and
-// out, which a large copy reaches too; 1000 x 11008 bfloat16 9.1 us, 3.6 TB/s (one round of workgroups); one row of 4096 2.0 us.
+// out, which a large copy reaches too (116 us over the same two inputs again and again, part of which stays in the last-level cache);
+// 1000 x 11008 bfloat16 9.4 us, 3.5 TB/s (one round of workgroups); one row of 4096 2.1 us.
 #include "number_types.hpp"
 
 namespace {
