@@ -1,11 +1,11 @@
-"""How likely was the answer?  The end of a forward pass in 8-bit integers, and the words of it that a proof is about.
+"""How likely was the answer?  The end of a forward pass in 8-bit integers, and the exact sums of a projection in the field.
 
     python examples/score_answer.py [--tokens 1000] [--hidden 4096] [--ffn 11008] [--vocab 32000] [--top 5]
 
 Random weights and activations of a layer's sizes go through a gated feed-forward block and the projection to the vocabulary, all
 products in 8-bit integers with a scale for each token and channel (`verinf_amd.prover.inference`); the logits then say how likely given
-tokens were, how uncertain the model was, and what it would rather have said.  The sums of a projection are also taken as field elements
-and compared with the field product of the lifted operands: they are the words that a prover commits to.
+tokens were, how uncertain the model was, and what it would rather have said.  The sums of the block's first projection are also taken as
+field elements and compared with the field product of the lifted operands; nothing is committed to or proved here.
 """
 import argparse
 import os
@@ -81,9 +81,9 @@ def main():
           f"{100 * s['agreed']:.1f} % were the likeliest token, {start.elapsed_time(end):.3f} ms")
     some = min(a.tokens, 64)
     q, _ = inf.quantize_rows(x[:some])
-    w = weights["down"][0][:256, :a.hidden].contiguous()
+    w = weights["gate"][0][:256]
     same = torch.equal(words(q, w).view(torch.int64), cp.gl_matmul(lift(q), lift(w.T)).view(torch.int64))
-    print(f"sums of a projection as field elements {'equal' if same else 'DIFFER FROM'} the field product of the lifted operands")
+    print(f"sums of the first projection as field elements {'equal' if same else 'DIFFER FROM'} the field product of the lifted operands")
     return 0 if same else 1
 
 

@@ -373,7 +373,7 @@ size_t vi_lookup_histogram_workspace_bytes(int64_t n_x, int64_t n_table, int tab
 int vi_lookup_histogram(const uint64_t *x, int64_t n_x, const uint64_t *table, int64_t n_table, int table_is_range, int accumulate,
                         uint64_t *mult, void *ws, size_t ws_bytes, void *stream);
 
-/* ---- the forward pass a proof is about, in 8-bit integers (no counterpart in the reference) -------------------------
+/* ---- a forward pass in 8-bit integers, beside the proof (no counterpart in the reference) ---------------------------
  * Matrices are row-major with unit column stride; rows are ld* elements apart (>= their length) and start at any address
  * that their type may have.  Types of numbers: */
 #define VI_F32 0

@@ -692,7 +692,7 @@ constexpr Tile TILES[] = {{4, 4, 4, 0.85, 0, 7, 0, 1.45, 0},          // 8192 x 
                           {4, 2, 8, 0.9, 0, 6.5, 0, 1.5, 0},          // 2000 x 4096 x 4096 37 us; 256 x 256: 51, 128 x 128: 41; gated 1000 x 4096 x 11008 103, 256 x 192: 106
                           {2, 2, 8, 0.48, 1.0, 4.5, 1.3, 1.2, 0},     // 1000 x 4096 x 4096 23 us; 256 x 128: 26, 64 x 128: 24
                           {1, 2, 8, 0.27, 0.62, 3, 0.5, 0.75, 1.25}};  // 128 x 4096 x 4096 12 us; 128 x 128: 16
-constexpr int N_TILES = sizeof(TILES) / sizeof(TILES[0]), CUS = 256;
+constexpr int N_TILES = sizeof(TILES) / sizeof(TILES[0]), CUS = 256;                    // of a whole card; on a part of one the choices cost time, nothing else
 constexpr int FEW = N_TILES;                   // k_few, up to FEW_ROWS rows
 constexpr i64 FEW_ROWS = 32;
 constexpr i64 MAX_GROUPS = (1 << 24) - 1;     // a launch has less than 2^32 threads: of 256, and half as many workgroups of 512

@@ -34,7 +34,7 @@ constexpr int BLOCK = 256, WIDE = 1024;         // threads
 constexpr int MAX_TOP = 64;                    // a lane of a wavefront for each
 constexpr int KEEP = 512, KEEP_VECTORS = 128;  // collected entries, and 16 bytes of them
 constexpr i64 MAX_V = (i64)1 << 24;
-constexpr int CUS = 256;
+constexpr int CUS = 256;                       // of a whole card; on a part of one the choice of slices costs time, nothing else
 constexpr i64 MAX_ROWS = 1 << 23;              // of a launch, and slices of rows: it has less than 2^32 threads
 constexpr int MAX_R = 16, MAX_WIDE_R = 8;      // 16-byte loads a thread
 

@@ -1,7 +1,8 @@
-"""The forward pass that a proof is about, in 8-bit integers, and what it says of an answer (no counterpart in the reference).
+"""A forward pass in 8-bit integers, and what it says of an answer: a tool beside the proof, which nothing in it calls (no counterpart in the
+reference; a layer that is proved has 16-bit activations of its own).
 
     quantize_rows(x)                       rows of floats -> 8-bit integers with a scale each
-    int8_matmul(a, b, ...)                 a b^T: exact sums (int32, or field elements as the proof takes them), or scaled
+    int8_matmul(a, b, ...)                 a b^T: exact sums (int32, or field elements, as gl_matmul has them), or scaled
     int8_gated(a, gate, up, ...)           act(a gate^T) * (a up^T), both projections and the activation in one kernel
     token_logprobs(logits, tokens, ...)    log probabilities of given tokens, entropies, the likeliest alternatives
 
