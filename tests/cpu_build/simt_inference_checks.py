@@ -294,6 +294,8 @@ def tiles(so, pick):
                         L.check(gated, tile, m, k, n, kind, pack=1, pad=1 + at % 3, shift=at % 2, **opts)
                     elif pick == "sliced" and steps > 2:
                         L.check(gated, tile, m, k, n, kind, slices=2 + at % 3, pad=at % 2 or None, pack=at % 2 * (at // 2 % 2), **opts)
+            if pick in ("direct", "staged"):                   # no inner dimension: nothing is read
+                L.check(gated, tile, rows + 1, 0, wide + 3, kinds[tile % len(kinds)], pad=0 if pick == "direct" else 3, bias=not gated)
             # several tiles, each way out to the end of a row
             for kind in kinds:
                 print(pick, gated, tile, "several", kind, flush=True)

@@ -603,3 +603,12 @@ def test_negative_views_are_refused():
             call()
     got, scale = inf.quantize_rows(x.resolve_neg())
     assert torch.equal(got[:, 0].float().sign(), x[:, 0].sign()) and (scale > 0).all()
+
+
+@pytest.mark.parametrize("m,n", [(1, 5), (70, 33), (300, 200)])
+def test_products_of_no_inner_dimension(m, n):
+    a, b = torch.empty((m, 0), dtype=torch.int8, device="cuda"), torch.empty((n, 0), dtype=torch.int8, device="cuda")
+    one_m, one_n, bias = torch.ones((m,), device="cuda"), torch.ones((n,), device="cuda"), torch.arange(n, device="cuda").float()
+    assert (inf.int8_matmul(a, b) == 0).all() and (inf.int8_matmul(a, b, dtype=torch.uint64).view(torch.int64) == 0).all()
+    assert torch.equal(inf.int8_matmul(a, b, one_m, one_n, bias=bias, dtype=torch.float32), bias.expand(m, n))
+    assert (inf.int8_gated(a, b, b, one_m, one_n, one_n, dtype=torch.float32) == 0).all()

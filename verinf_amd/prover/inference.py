@@ -76,7 +76,7 @@ def quantize_rows(x):
     """(m, k) float32 / bfloat16 / float16 -> (q, scale): q (m, k) int8 in [-127, 127], scale (m,) float32, x[i] ~ q[i] * scale[i].
 
     scale = max |x[i]| / 127, q = x[i] * (127 / max |x[i]|) to the nearest integer, half to even, in 32 bits.  A row of zeros
-    (or of nothing above 2^-119) has scale 0; one with a NaN or an infinity has scale NaN and integers of zero.  The rows of q are
+    (or of nothing as large as 127 * 2^-126) has scale 0; one with a NaN or an infinity has scale NaN and integers of zero.  The rows of q are
     a multiple of 16 bytes apart, as the products read them fastest."""
     m, k, ldx = _matrix(x, "x", _FLOATS)
     dev = x.device
