@@ -165,6 +165,19 @@ def zeros(so):
                 L.check(x, kind, tokens, top)
 
 
+def far(so):
+    """Logits further apart than 32 bits hold, which a temperature brings together."""
+    L = Logprobs(so)
+    for kind in FLOATS:
+        for v in widths(kind):
+            print("far", FLOATS[kind], v, flush=True)
+            x = np.full((3, v), LOWEST[kind], np.float32)
+            x[0, v // 2] = x[1, :5] = -LOWEST[kind]
+            x[2, v // 2], x[2, 0] = -LOWEST[kind], 1.0
+            for temperature in (2.5, 50.0, 1000.0) if v < 2000 else (50.0,):
+                L.check(x, kind, np.array([1, v - 1, 0]), 3, temperature)
+
+
 def few(so):
     """Rows with fewer allowed entries than are asked for: the rest is filled up, no entries are counted for it.  A workgroup comes to as many
     barriers in every type."""

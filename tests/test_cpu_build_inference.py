@@ -102,3 +102,7 @@ def test_the_sizes_of_the_gpu_tests_take_every_tile(built):
 
 def test_rows_to_8_bits(built):
     check(built, "quantize", "quantize")
+
+
+def test_log_probabilities_of_logits_far_apart(built):
+    check(built, "logprobs", "far")

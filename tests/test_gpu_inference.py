@@ -612,3 +612,15 @@ def test_products_of_no_inner_dimension(m, n):
     assert (inf.int8_matmul(a, b) == 0).all() and (inf.int8_matmul(a, b, dtype=torch.uint64).view(torch.int64) == 0).all()
     assert torch.equal(inf.int8_matmul(a, b, one_m, one_n, bias=bias, dtype=torch.float32), bias.expand(m, n))
     assert (inf.int8_gated(a, b, b, one_m, one_n, one_n, dtype=torch.float32) == 0).all()
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("v", [70, 3000, 9001, 70001])
+def test_logprobs_of_logits_far_apart(dtype, v):
+    """further than 32 bits hold, which a temperature brings together"""
+    x = torch.full((3, v), torch.finfo(dtype).min, dtype=dtype)
+    x[0, v // 2] = torch.finfo(dtype).max
+    x[1, :5] = torch.finfo(dtype).max
+    x[2, v // 2], x[2, 0] = torch.finfo(dtype).max, 1.0
+    for temperature in (2.5, 50.0, 1000.0):
+        check_logprobs(x.cuda(), torch.tensor([1, v - 1, 0], device="cuda"), 3, temperature)

@@ -191,8 +191,9 @@ __device__ __forceinline__ Asked ask(const Args &A, i64 row) {
 
 __device__ void finish(const Args &A, i64 row, float most, float z, float w, const u64 *best, const Asked &asked) {
     const float m = centre(most), logz = log2f(z) * LN2;
-    // in nats from the start: (x - M) c would overflow for a mask of the type's lowest value, (x - M) / 1 does not
-    auto lp_of = [&](float x) { return z != z ? z : x == -INFINITY ? x : (x - m) * A.per_t - logz; };
+    // in nats from the start: (x - M) c would overflow for a mask of the type's lowest value, (x - M) / 1 does not; and by halves, since x - M
+    // may be twice what 32 bits hold
+    auto lp_of = [&](float x) { return z != z ? z : x == -INFINITY ? x : (0.5f * x - 0.5f * m) * (2.0f * A.per_t) - logz; };
     if (threadIdx.x < A.top) {
         const u64 key = best[threadIdx.x];
         A.top_logprobs[row * A.top + threadIdx.x] = lp_of(value_of(key));
