@@ -344,6 +344,26 @@ def few_rows(so):
                 L.check(gated, L.tiles, m, k, n, kind, pad=(None, 0, 1)[at % 3], shift=at % 2, bias=not gated and kind != 1, act=at % 2)
 
 
+def overflow(so):
+    """Products that overflow before the activation: +inf stays, -inf gives 0, a NaN shows."""
+    L = Products(so)
+    for tile in range(L.tiles + 1):
+        for act in (SILU, GELU):
+            for kind in (0, 1, 2):
+                print("overflow", tile, act, kind, flush=True)
+                m, n = (20, 37) if tile == L.tiles else (40, 128)
+                a, g, u = np.ones((m, 16), np.int8), np.ones((n, 16), np.int8), np.ones((n, 16), np.int8)
+                g[1::3] = -1
+                sm, sn, su = np.full(m, 1e30, np.float32), np.full(n, 1e30, np.float32), np.full(n, 1e-30, np.float32)
+                sn[2::3] = np.nan
+                (a, _), (g, _), (u, _) = strided(a, 0), strided(g, 0), strided(u, 0)
+                out = np.empty((m, n), OUT[kind])
+                ws = scratch(L.L.simt_workspace(1, tile, 1, 0, m, 16, n))
+                assert L.L.simt_product(1, tile, 1, 0, a.ctypes.data, 16, g.ctypes.data, 16, u.ctypes.data, 16, m, 16, n, ptr(sm), ptr(sn), ptr(su), None, act, kind, ptr(out), ptr(ws)) == 0
+                out = decode(out, kind)
+                assert (out[:, 0::3] == np.inf).all() and (out[:, 1::3] == 0).all() and np.isnan(out[:, 2::3]).all(), (tile, act, kind)
+
+
 def plans(so):
     """The sizes of the tests on the GPU, which are in SHAPES: what they reach."""
     L = ctypes.CDLL(so)

@@ -95,6 +95,10 @@ def test_products_of_few_rows(built):
     check(built, "int8_gemm", "few_rows")
 
 
+def test_gated_products_that_overflow(built):
+    check(built, "int8_gemm", "overflow")
+
+
 def test_the_sizes_of_the_gpu_tests_take_every_tile(built):
     import test_gpu_inference as gpu
     check(built, "int8_gemm", "plans", SHAPES=json.dumps([gpu.LARGE, gpu.LARGE_GATED]))

@@ -624,3 +624,18 @@ def test_logprobs_of_logits_far_apart(dtype, v):
     x[2, v // 2], x[2, 0] = torch.finfo(dtype).max, 1.0
     for temperature in (2.5, 50.0, 1000.0):
         check_logprobs(x.cuda(), torch.tensor([1, v - 1, 0], device="cuda"), 3, temperature)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("m,n", [(1, 128), (20, 128), (40, 128), (40, 125), (300, 256)])
+def test_gated_products_that_overflow(act, m, n):
+    """G of +inf stays, G of -inf gives 0, a NaN shows"""
+    one = torch.ones((m, 16), dtype=torch.int8, device="cuda")
+    g = torch.ones((n, 16), dtype=torch.int8, device="cuda")
+    g[1::3] = -1
+    sm, sn = torch.full((m,), 1e30, device="cuda"), torch.full((n,), 1e30, device="cuda")
+    sn[2::3] = math.nan
+    su = torch.full((n,), 1e-30, device="cuda")                        # U = 16
+    for dtype in FLOATS:
+        out = inf.int8_gated(one, g, torch.ones_like(g), sm, sn, su, activation=act, dtype=dtype)
+        assert (out[:, 0::3] == math.inf).all() and (out[:, 1::3] == 0).all() and out[:, 2::3].isnan().all()

@@ -51,10 +51,13 @@ __device__ __forceinline__ v4i load_end(const signed char *p, i64 left, i64 k) {
 }
 
 // x / (1 + e^-x), with e^-|x| so that nothing overflows, and a step of Newton's behind the reciprocal (one unit off as it comes)
+// (for x > -80: v_exp_f32 has no results below 2^-126)
 __device__ __forceinline__ float silu(float x) {
     const float t = __builtin_amdgcn_exp2f(fabsf(x) * -1.44269504f), y = 1.0f + t, r = __builtin_amdgcn_rcpf(y);
     return (x < 0.0f ? x * t : x) * fmaf(fmaf(-y, r, 1.0f), r, r);
 }
+// the same below, where the sum is one; 0 for products that have overflowed to -inf
+__device__ __forceinline__ float silu_far(float x) { return fmaxf(x, -200.0f) * expf(x); }
 
 // x Phi(x), with all digits below zero too, where 0.5 (1 + erf(x / sqrt 2)) cancels (4 % off at -5, 0 from -5.5 on):
 // Phi(-u) = e^(-u^2 / 2) h(u), and h, which falls slowly from 1/2, is q P(q) with q = 1 / (1 + 0.27 u), P of degree 8 fitted to it over
@@ -69,7 +72,8 @@ __device__ __forceinline__ float gelu(float x) {
 #pragma unroll
     for (int i = 7; i >= 0; --i) p = fmaf(p, q, P[i]);
     const float tail = p * q * __builtin_amdgcn_exp2f(x * (x * -0.72134752f));
-    return x < 0.0f ? x * tail : fmaf(-x, tail, x);
+    const float near = fminf(fmaxf(x, -100.0f), 100.0f);           // the tail is 0 there, which infinities would make a NaN of
+    return x < 0.0f ? near * tail : fmaf(-near, tail, x);
 }
 
 __device__ __forceinline__ void activate(float (&v)[VEC], int act) {
@@ -85,9 +89,8 @@ __device__ __forceinline__ void activate(float (&v)[VEC], int act) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = silu(v[e]);
     } else {
-        // v_exp_f32 has no results below 2^-126; there the sum is one
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = v[e] <= -80.0f ? v[e] * expf(v[e]) : silu(v[e]);
+        for (int e = 0; e < VEC; ++e) v[e] = v[e] <= -80.0f ? silu_far(v[e]) : silu(v[e]);
     }
 }
 
@@ -184,7 +187,7 @@ __device__ __forceinline__ void finish_one(const Job &J, i64 row, i64 col, int s
     float v = (float)s * as * J.b_scale[col];
     if (GATED) {
         if (J.act == VI_GELU) v = gelu(v);
-        else v = v <= -80.0f ? v * expf(v) : silu(v);
+        else v = v <= -80.0f ? silu_far(v) : silu(v);
         v *= (float)t * as * J.b2_scale[col];
     } else if (J.bias) {
         v += J.bias[col];
