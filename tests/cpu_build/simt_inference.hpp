@@ -1,8 +1,8 @@
 // What the kernels of the forward pass in 8-bit integers use beside the rest of cpu_build/simt, for clang: their 16-bit number types,
 // vectors of them and element-wise operations are that compiler's own.  LDS is static here, so that AddressSanitizer sees its ends.
 //
-// Loads straight into LDS.  A lane's load arrives either at once or when a wait for it is reached and not before (SIMT_LATE=1): a wait that
-// is missing shows in the one, a place that is overwritten while it is still read in the other.
+// Loads straight into LDS.  A lane's load arrives at once, which shows a place that is overwritten while it is still read, or (SIMT_LATE=1) when a
+// wait for it is reached and not before, which shows a wait that is missing.
 //
 // Fibers change places by a switch of their own: AddressSanitizer clears the whole stack's shadow at every swapcontext, and these kernels
 // meet at every vote of the lanes.
