@@ -161,7 +161,7 @@ def zeros(so):
             x[5, 5:60:7] = -0.0
             x[6, v - 20:] = -0.0
             tokens = np.array([0, 1, 2, 3, 4, 5, v - 1])
-            for top in (1, 3, 20, 64) if v < 3000 else (5, 64) if v < 10000 else (5,):
+            for top in (1, 3, 20, 64) if v < 3000 else (5,):
                 L.check(x, kind, tokens, top)
 
 
@@ -201,7 +201,7 @@ def rows(so):
         unit = 1024 if kind == 0 else 2048                     # entries that 256 threads load at once
         for m, v, pad, top in ((1, 1, 0, 1), (3, 2, 1, 2), (2, 63, 0, 63), (2, unit, 3, 64), (2, unit + 1, 0, 5), (1, 4 * unit + 1, 0, 5), (1, 9 * unit, 0, 64),
                                (1, 32 * unit, 0, 8), (1, 32 * unit + 1, 1, 8), (2, 35 * unit, 0, 20), (257, unit + 1, 0, 2)) + \
-                (((257, 2 * unit + 3, 0, 2), (300, 4 * unit - 5, 0, 3), (300, 8 * unit + 1, 0, 2), (520, 6 * unit + 1, 0, 1), (520, 9 * unit, 0, 2)) if kind == 1 else ()):
+                (((257, 2 * unit + 3, 0, 2), (300, 4 * unit - 5, 0, 3), (520, 6 * unit + 1, 0, 1), (520, 9 * unit, 0, 2)) if kind == 1 else ()):
             print("rows", FLOATS[kind], m, v, pad, top, flush=True)
             rng = np.random.default_rng(m + v)
             x = (rng.standard_normal((m, v)) * 4).astype(np.float32)
@@ -291,7 +291,7 @@ def tiles(so, pick):
             kinds = (0, 1, 2) if gated else (0, 1, 2, I32, FIELD)
             at = 0
             for steps in range(1, 10):
-                for end in (0, 1, 16, 37):
+                for end in (0, 1, 16, 37) if pick in ("direct", "staged") and not os.environ.get("SIMT_LATE") else (0, 37):
                     k = steps * STEPS[tile] - (STEPS[tile] - end if end else 0)
                     # whole tiles; a ragged one; a little more than one
                     m, n = ((rows, wide), (rows - 7, wide - 5), (33, wide), (1, 1))[(steps + end) % 4]
