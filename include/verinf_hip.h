@@ -414,6 +414,69 @@ size_t vi_token_logprobs_workspace_bytes(int dtype, int64_t m, int64_t v, int to
 int vi_token_logprobs(int dtype, const void *logits, int64_t m, int64_t v, int64_t ld, const int64_t *tokens, float temperature, int top,
                       float *logprob, float *entropy, float *top_logprobs, int64_t *top_tokens, void *ws, size_t ws_bytes, void *stream);
 
+/* ---- answering with a cache and drafted tokens (no counterpart in the reference) -------------------------------------
+ * A paged cache of keys and values: entry (page, head, row) is `dim` neighbouring numbers of type VI_BF16, VI_F16, or VI_I8 with a
+ * float32 scale each; strides are in elements, between pages, heads and rows (those of the scales: pages and heads, rows adjacent).
+ * dim is a multiple of 16 up to 256, page_size a power of two from 16 to 1024, entries start at multiples of 16 bytes. */
+#define VI_I8 5
+typedef struct vi_cache {
+    void *keys, *values;
+    float *key_scales, *value_scales;
+    int64_t key_strides[3], value_strides[3], key_scale_strides[2], value_scale_strides[2];
+    int64_t pages, heads, page_size, dim;
+    int64_t dtype;
+} vi_cache;
+
+/* What is in it and what is new: sequence b has the rows starts[b] .. starts[b + 1] - 1 of the new tokens' tensors (starts rises; rows
+ * of no sequence are left alone), and with them lengths[b] entries, of which number j lies in row j % page_size of page pages[b][j / page_size]; the
+ * new tokens' are the last.  Pages outside the cache hold nothing: they are not written, and what they should hold is masked.  All on the device. */
+typedef struct vi_batch {
+    const int32_t *starts, *lengths, *pages;
+    int64_t sequences, width, stride;
+} vi_batch;
+
+/* Rotary positions.  The first `rotated` columns of each head are pairs (x, y) - (i, i + rotated / 2), or interleaved (2 i, 2 i + 1) - that
+ * become ((x cos a - y sin a) A, (x sin a + y cos a) A), A the amplitude, a = positions[t] steps[i] / 2^64 turns (mod 2^64: exact, however
+ * far); the others stay.  x, out (n, heads, dim) of one type, columns adjacent, the others *_token and *_head elements apart; out may be x.  dim even, up to 256. */
+int vi_rotate_heads(int dtype, const void *x, int64_t n, int64_t heads, int64_t dim, int64_t x_token, int64_t x_head, const int64_t *positions,
+                    const uint64_t *steps, int64_t rotated, int interleaved, double amplitude, void *out, int64_t out_token, int64_t out_head, void *stream);
+
+/* The new tokens' keys, turned where steps is given, and values (n, heads, dim), float32, bfloat16 or float16, into the cache.  A
+ * token's position is positions[t], or its entry's number where positions is NULL.  VI_I8: rows to integers with a scale as
+ * vi_quantize_rows makes them, of the keys turned in 64 bits and rounded to 32. */
+int vi_append_tokens(const vi_cache *cache, const vi_batch *batch, int dtype, const void *k, int64_t k_token, int64_t k_head, const void *v,
+                     int64_t v_token, int64_t v_head, int64_t n, const int64_t *positions, const uint64_t *steps, int64_t rotated, int interleaved,
+                     double amplitude, void *stream);
+
+/* out = softmax(scale q k^T) v over the cache's entries, for q (n, heads, dim): heads / cache->heads heads of q share one of the cache's.  New token i of
+ * a sequence attends to all entries before the new ones' and, of those, to 0 .. i (parents NULL), or to itself and its ancestors: parents[row] is its parent's
+ * number in its sequence, lower than its own, anything else makes it a root.  A sequence of more than 256 new tokens is taken for a chain.  A token that
+ * attends to nothing gets zeros.  dtype VI_BF16 or VI_F16 as the cache's; VI_BF16 for a cache of VI_I8.  clear: rows of no sequence become zero.  longest:
+ * no sequence is longer (a hint: how the work is cut).  ws: vi_attend_cache_workspace_bytes() bytes of device scratch. */
+size_t vi_attend_cache_workspace_bytes(int cache_dtype, int64_t dim, int64_t cache_heads, int64_t n, int64_t heads, int64_t sequences, int64_t longest);
+int vi_attend_cache(const vi_cache *cache, const vi_batch *batch, int dtype, const void *q, int64_t n, int64_t heads, int64_t q_token, int64_t q_head,
+                    const int32_t *parents, float scale, int64_t longest, int clear, void *out, int64_t out_token, int64_t out_head, void *ws,
+                    size_t ws_bytes, void *stream);
+
+/* Drafted tokens against the target's probabilities p = softmax(logits / temperature), in 64 bits.  Sequence b has the nodes starts[b] ..
+ * starts[b + 1] - 1: a root and drafts, in an order in which parents[node], a number in the sequence, is lower than the node's own; row `node` of
+ * logits (n, v), v <= 2^20, is what the target says behind it.  From the root on, a node's children are tried in their order: with R = p, child c is accepted
+ * where uniforms[c] q(tokens[c]) sum(R) < R(tokens[c]), q = softmax(draft / temperature) of the node's row; behind a refused one R = max(R / sum(R) - q, 0).  Without
+ * draft logits q = 1 and R loses the entry.  A sequence's first 1024 nodes are tried.  Once none is accepted, or `depth` <= 256 are, the token behind the path is the smallest j with R(0) + ... + R(j) >
+ * uniforms[root] sum(R); where nothing is left of R, R = p; -1 where a row has a NaN or +inf or only -inf (no draft below it is accepted).
+ * counts (sequences): accepted drafts; nodes (sequences, depth): their numbers, -1 behind; out (sequences, depth + 1): their tokens, the one behind, -1.
+ * ws: vi_verify_drafts_workspace_bytes() bytes of device scratch. */
+size_t vi_verify_drafts_workspace_bytes(int dtype, int64_t n, int64_t v, int drafted);
+int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_t v, int64_t ld, const void *draft, int64_t ld_draft, const int64_t *tokens,
+                     const int32_t *starts, int64_t sequences, const int32_t *parents, const double *uniforms, double temperature, int64_t depth,
+                     int64_t *counts, int64_t *nodes, int64_t *out, void *ws, size_t ws_bytes, void *stream);
+
+/* The cache behind such a path: of each sequence's new entries (batch), node nodes[b][d]'s becomes number d + 1 behind the root's, d <
+ * counts[b] <= depth <= 256.  Numbers rise along a path: it ends in front of one that does not, or that is none of the sequence's.  lengths[b] (not
+ * batch->lengths itself): the entries there are then, up to the path's end. */
+int vi_keep_drafts(const vi_cache *cache, const vi_batch *batch, const int64_t *nodes, int64_t depth, const int64_t *counts, int32_t *lengths,
+                   void *stream);
+
 /* ---------------------------------------------------------------------------------------------
  * Measurement hook (no counterpart in the reference): the issue rate of the integer VALU instructions the field
  * arithmetic and the hashing consist of, which is the bound their kernels are put against.

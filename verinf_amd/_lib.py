@@ -43,10 +43,25 @@ EXPORTS = [
     "vi_int8_matmul_workspace_bytes", "vi_int8_matmul_best_workspace_bytes", "vi_int8_matmul",
     "vi_int8_gated_workspace_bytes", "vi_int8_gated_best_workspace_bytes", "vi_int8_gated",
     "vi_token_logprobs_workspace_bytes", "vi_token_logprobs",
+    "vi_rotate_heads", "vi_append_tokens", "vi_attend_cache_workspace_bytes", "vi_attend_cache",
+    "vi_verify_drafts_workspace_bytes", "vi_verify_drafts", "vi_keep_drafts",
     "vi_valu_probe_count", "vi_valu_probe_name", "vi_wall_clock_khz", "vi_valu_probe",
 ]
 
 COIN_FN = ctypes.CFUNCTYPE(c_int, c_int, POINTER(c_uint64), c_int, POINTER(c_uint64), c_void_p)
+
+
+
+class CacheArgs(ctypes.Structure):              # vi_cache
+    _fields_ = [("keys", c_void_p), ("values", c_void_p), ("key_scales", c_void_p), ("value_scales", c_void_p),
+                ("key_strides", c_int64 * 3), ("value_strides", c_int64 * 3), ("key_scale_strides", c_int64 * 2),
+                ("value_scale_strides", c_int64 * 2), ("pages", c_int64), ("heads", c_int64), ("page_size", c_int64), ("dim", c_int64),
+                ("dtype", c_int64)]
+
+
+class BatchArgs(ctypes.Structure):              # vi_batch
+    _fields_ = [("starts", c_void_p), ("lengths", c_void_p), ("pages", c_void_p), ("sequences", c_int64), ("width", c_int64), ("stride", c_int64)]
+
 
 _lib = None
 
@@ -159,6 +174,18 @@ def lib():
     L.vi_token_logprobs_workspace_bytes.argtypes = [c_int, i64, i64, c_int]
     L.vi_token_logprobs.argtypes = [c_int, vp, i64, i64, i64, vp, c_float, c_int, vp, vp, vp, vp, vp, sz, vp]
     L.vi_token_logprobs.restype = c_int
+    cache, batch = POINTER(CacheArgs), POINTER(BatchArgs)
+    L.vi_rotate_heads.argtypes = [c_int, vp, i64, i64, i64, i64, i64, vp, vp, i64, c_int, c_double, vp, i64, i64, vp]
+    L.vi_append_tokens.argtypes = [cache, batch, c_int, vp, i64, i64, vp, i64, i64, i64, vp, vp, i64, c_int, c_double, vp]
+    L.vi_attend_cache_workspace_bytes.restype = sz
+    L.vi_attend_cache_workspace_bytes.argtypes = [c_int, i64, i64, i64, i64, i64, i64]
+    L.vi_attend_cache.argtypes = [cache, batch, c_int, vp, i64, i64, i64, i64, vp, c_float, i64, c_int, vp, i64, i64, vp, sz, vp]
+    L.vi_verify_drafts_workspace_bytes.restype = sz
+    L.vi_verify_drafts_workspace_bytes.argtypes = [c_int, i64, i64, c_int]
+    L.vi_verify_drafts.argtypes = [c_int, vp, i64, i64, i64, vp, i64, vp, vp, i64, vp, vp, c_double, i64, vp, vp, vp, vp, sz, vp]
+    L.vi_keep_drafts.argtypes = [cache, batch, vp, i64, vp, vp, vp]
+    for name in ("vi_rotate_heads", "vi_append_tokens", "vi_attend_cache", "vi_verify_drafts", "vi_keep_drafts"):
+        getattr(L, name).restype = c_int
     L.vi_valu_probe_name.restype = c_char_p
     L.vi_valu_probe_name.argtypes = [c_int]
     L.vi_valu_probe.argtypes = [c_int, c_int, c_int, vp, vp, POINTER(i64), vp]

@@ -1,0 +1,520 @@
+// Drafted tokens held against the target's probabilities, and the accepted ones' cache entries moved to the front.
+//
+// A node's children are tried in their order, which is that of the nodes, so that one walk over a sequence's nodes tries them all.  With
+// p and q the target's and the draft model's probabilities behind the node, R = p at first, child c with token x is accepted where
+// u_c q(x) sum(R) < R(x), and behind a refused one R = max(R / sum(R) - q, 0).  Up to a factor that is
+//
+//     R = max(p - a q, 0)        a = 0 at first, a <- a + sum(R) at each refusal, sum(R) with the p and q that sum to one
+//
+// since max(max(p - a q, 0) - W q, 0) = max(p - (a + W) q, 0): nothing is stored of it but a.  Without the draft's probabilities R loses
+// the refused tokens and is otherwise p.
+//
+// Whole numbers come of it, decided by comparisons next to borders, of which the last token's have as many as there are tokens: all in 64
+// bits, exponentials too (the series of 2^f to the 12th power, 2e-16).
+//
+// Two launches: largest entry and sum of every row, in slices (k_stats), then a workgroup a sequence for the walk (k_walk).  What bounds them: reading the
+// logits, and 17 operations in 64 bits an exponential beside it.
+#include "cache.hpp"
+
+namespace {
+
+using namespace kv;
+
+constexpr int BLOCK = 256, WALK = 1024;        // threads
+constexpr i64 MAX_V = 1 << 20;
+constexpr i64 MAX_BLOCKS = 1 << 23;            // of a launch, which has less than 2^32 threads
+constexpr int MAX_NODES = 1024, MAX_DEPTH = 256;
+constexpr int EIGHT = 8;                       // neighbouring entries of a thread
+constexpr int MAX_SEGMENTS = (int)(MAX_V / (64 * EIGHT));               // of a row: a wavefront's entries
+
+struct Part {                                  // of a slice: its largest entry (NaN: it has a NaN or +inf), sum of 2^((x - most) c)
+    double z;
+    float most, pad;
+};
+struct Row {                                   // of a row: the most c that its sum is relative to; 1 / sum, 0 where it has none
+    double mc, per_z;
+};
+
+// 2^t, 0 from -1100 on
+__device__ __forceinline__ double exp2_64(double t) {
+    t = fmax(t, -1100.0);
+    const double n = rint(t), f = t - n;
+    constexpr double C[] = {2.5678435993488206e-11, 4.4455382718708116e-10, 7.0549116208011233e-9,  1.0178086009239700e-7, 1.3215486790144310e-6,
+                            1.5252733804059841e-5,  1.5403530393381610e-4,  1.3333558146428443e-3, 9.6181291076284772e-3, 5.5504108664821580e-2,
+                            2.4022650695910071e-1,  6.9314718055994531e-1,  1.0};
+    double p = C[0];
+#pragma unroll
+    for (int i = 1; i < 13; ++i) p = fma(p, f, C[i]);
+    return ldexp(p, (int)n);
+}
+
+template <int DT>
+struct Entries {                               // as they come
+    u32 w[DT == VI_F32 ? 8 : 4];
+};
+template <int DT>
+__device__ __forceinline__ float entry(const Entries<DT> &v, int e) {
+    if constexpr (DT == VI_F32) return __uint_as_float(v.w[e]);
+    else return element<DT>(v.w, e);
+}
+// the eight entries from `at` on; -inf behind the row's end
+template <int DT>
+__device__ __forceinline__ Entries<DT> eight(const typename type<DT>::t *x, i64 at, i64 v) {
+    if (at + EIGHT <= v) return load_any<Entries<DT>>(x + at);
+    typename type<DT>::t e[EIGHT];
+#pragma unroll
+    for (int i = 0; i < EIGHT; ++i) e[i] = at + i < v ? x[at + i] : (typename type<DT>::t)-INFINITY;
+    Entries<DT> r;
+    __builtin_memcpy(&r, e, sizeof(r));
+    return r;
+}
+
+struct Stats {
+    const void *x[2];                          // the target's logits, the draft's
+    i64 ld[2], n, v;
+    int slices;
+    double c;                                  // log2(e) / temperature
+    Part *parts;                               // [2 n][slices]
+};
+
+// R times eight entries a thread
+template <int DT, int R>
+__global__ __launch_bounds__(BLOCK) void k_stats(Stats A) {
+    typedef typename type<DT>::t T;
+    __shared__ float most_of[BLOCK / 64];
+    __shared__ double sum_of[BLOCK / 64];
+    const i64 row = blockIdx.x / A.slices;
+    const int slice = (int)(blockIdx.x % A.slices), which = row >= A.n, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    const T *x = (const T *)A.x[which] + (row - (which ? A.n : 0)) * A.ld[which];
+    const i64 first = (i64)slice * (BLOCK * EIGHT * R);
+    Entries<DT> v[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = eight<DT>(x, first + (r * BLOCK + (int)threadIdx.x) * EIGHT, A.v);
+    float most = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < EIGHT; ++e) {
+            const float f = entry<DT>(v[r], e);
+            most = fmaxf(most, f);
+            bad |= !(f < INFINITY);
+        }
+    if (bad) most = INFINITY;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    if (lane == 0) most_of[wave] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(most_of[0], most_of[1]), fmaxf(most_of[2], most_of[3]));
+    double z = 0;
+    if (most > -INFINITY && most < INFINITY) {
+        const double mc = (double)most * A.c;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < EIGHT; ++e) z += exp2_64(fma((double)entry<DT>(v[r], e), A.c, -mc));
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) z += __shfl_xor(z, d);
+    if (lane == 0) sum_of[wave] = z;
+    __syncthreads();
+    if (threadIdx.x == 0) A.parts[blockIdx.x] = {(sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]), most == INFINITY ? __uint_as_float(0x7FC00000u) : most, 0.0f};
+}
+
+struct Walk {
+    const void *x[2];
+    i64 ld[2], n, v;
+    int slices, sequences, depth, drafted;
+    double c;
+    const Part *parts;
+    Row *rows;                                 // [2 n]
+    const i64 *tokens;
+    const int *starts, *parents;
+    const double *uniforms;
+    i64 *counts, *nodes, *out;
+};
+
+struct Shared {
+    double have[MAX_NODES], said[MAX_NODES], u[MAX_NODES];             // p and q of a node's token behind its parent
+    int parent[MAX_NODES], token[MAX_NODES];                           // -1: none
+    double segment[MAX_SEGMENTS];
+    double total, rest;
+    int found;
+};
+
+// the sum of the wavefront's values up to this lane's
+__device__ __forceinline__ double sum_up_to(double v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double o = __shfl(v, max(lane - d, 0));
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+// the first lane whose sum is above the threshold, the last with anything where none is; -1: nothing anywhere
+__device__ __forceinline__ int first_above(double sum, double own, double threshold) {
+    const u64 above = __ballot(sum > threshold && own > 0), any = __ballot(own > 0);
+    return above ? __ffsll((unsigned long long)above) - 1 : any ? 63 - __clzll((long long)any) : -1;
+}
+
+// What is left of a row: R(j) = max(p - a q, 0), or p without the tokens of the refused children of `cur`
+template <int DT>
+struct Left {
+    const typename type<DT>::t *x, *y;
+    Row p, q;
+    double a, c;
+    i64 v;
+    const Shared *sh;
+    int nodes, cur;                            // the refused are the children of cur (-1: none are)
+
+    __device__ __forceinline__ void eight_at(i64 at, double (&r)[EIGHT]) const {
+        const Entries<DT> e = eight<DT>(x, at, v);
+#pragma unroll
+        for (int i = 0; i < EIGHT; ++i) r[i] = exp2_64(fma((double)entry<DT>(e, i), c, -p.mc)) * p.per_z;
+        if (a > 0) {
+            const Entries<DT> f = eight<DT>(y, at, v);
+            const double per = a * q.per_z;
+#pragma unroll
+            for (int i = 0; i < EIGHT; ++i) r[i] = fmax(r[i] - exp2_64(fma((double)entry<DT>(f, i), c, -q.mc)) * per, 0.0);
+        }
+        if (cur >= 0) {
+            for (int j = 1; j < nodes; ++j) {
+                const i64 place = sh->token[j] - at;
+                if (sh->parent[j] == cur && place >= 0 && place < EIGHT) {
+#pragma unroll
+                    for (int i = 0; i < EIGHT; ++i)
+                        if (place == i) r[i] = 0;
+                }
+            }
+        }
+    }
+};
+
+// the sum of what is left, and of each segment of 64 times eight entries; for all threads
+template <int DT>
+__device__ double sum_left(Shared &sh, const Left<DT> &left) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, segments = (int)((left.v + 64 * EIGHT - 1) / (64 * EIGHT));
+    __syncthreads();
+    for (int s = wave; s < segments; s += WALK / 64) {
+        double r[EIGHT], sum = 0;
+        left.eight_at((i64)(s * 64 + lane) * EIGHT, r);
+#pragma unroll
+        for (int i = 0; i < EIGHT; ++i) sum += r[i];
+#pragma unroll
+        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+        if (lane == 0) sh.segment[s] = sum;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        double sum = 0;
+        const int each = (segments + 63) / 64;
+        for (int s = lane * each; s < min(segments, (lane + 1) * each); ++s) sum += sh.segment[s];
+#pragma unroll
+        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+        if (lane == 0) sh.total = sum;
+    }
+    __syncthreads();
+    return sh.total;
+}
+
+// the smallest j with R(0) + ... + R(j) > threshold, behind sum_left; by the first wavefront
+template <int DT>
+__device__ int find_left(const Shared &sh, const Left<DT> &left, double threshold) {
+    const int lane = threadIdx.x & 63, segments = (int)((left.v + 64 * EIGHT - 1) / (64 * EIGHT)), each = (segments + 63) / 64;
+    double own = 0;
+    for (int s = lane * each; s < min(segments, (lane + 1) * each); ++s) own += sh.segment[s];
+    double sum = sum_up_to(own);
+    int at = first_above(sum, own, threshold);
+    if (at < 0) return -1;
+    double before = __shfl(sum, max(at - 1, 0));
+    if (at == 0) before = 0;
+    int segment = -1;
+    double base = 0;                           // what lies in front of the segment
+    for (int s = at * each; s < min(segments, (at + 1) * each); ++s) {               // the same for all lanes
+        if (sh.segment[s] > 0) {
+            segment = s, base = before;
+            if (before + sh.segment[s] > threshold) break;
+        }
+        before += sh.segment[s];
+    }
+    if (segment < 0) return -1;
+    double r[EIGHT];
+    own = 0;
+    left.eight_at((i64)(segment * 64 + lane) * EIGHT, r);
+#pragma unroll
+    for (int i = 0; i < EIGHT; ++i) own += r[i];
+    sum = base + sum_up_to(own);
+    at = first_above(sum, own, threshold);
+    if (at < 0) return -1;
+    double here = __shfl(sum, max(at - 1, 0));
+    if (at == 0) here = base;
+    int j = -1;
+    bool done = false;
+#pragma unroll
+    for (int i = 0; i < EIGHT; ++i) {
+        if (!done && r[i] > 0) j = i;
+        here += r[i];
+        done |= r[i] > 0 && here > threshold;
+    }
+    return __shfl(j < 0 ? -1 : (segment * 64 + lane) * EIGHT + j, at);
+}
+
+// The largest entry and the sum of a row of its slices', by a wavefront
+__device__ __forceinline__ Row join(const Part *parts, int slices, double c) {
+    const int lane = threadIdx.x & 63;
+    Part p = {0.0, -INFINITY, 0.0f};
+    if (lane < slices) p = parts[lane];
+    const bool bad = __ballot(!(p.most == p.most)) != 0;
+    float most = p.most;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    if (bad || !(most > -INFINITY)) return {0.0, 0.0};
+    const double mc = (double)most * c;
+    double z = p.most > -INFINITY ? p.z * exp2_64((double)p.most * c - mc) : 0.0;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) z += __shfl_xor(z, d);
+    return {mc, 1.0 / z};
+}
+
+template <int DT>
+__global__ __launch_bounds__(WALK) void k_walk(Walk A) {
+    typedef typename type<DT>::t T;
+    __shared__ Shared sh;
+    const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t / 64;
+    const i64 s0 = max((i64)0, min((i64)A.starts[b], A.n)), s1 = max(s0, min((i64)A.starts[b + 1], A.n));
+    const int nodes = (int)min(s1 - s0, (i64)MAX_NODES);
+    for (int d = t; d < A.depth; d += WALK) A.nodes[(i64)b * A.depth + d] = -1;
+    for (int d = t; d <= A.depth; d += WALK) A.out[(i64)b * (A.depth + 1) + d] = -1;
+    for (int r = wave; r < nodes * (A.drafted ? 2 : 1); r += WALK / 64) {
+        const i64 row = r < nodes ? s0 + r : A.n + s0 + r - nodes;
+        const Row joined = join(A.parts + row * A.slices, A.slices, A.c);
+        if (lane == 0) A.rows[row] = joined;
+    }
+    __syncthreads();
+    for (int i = t; i < nodes; i += WALK) {
+        const int parent = i ? A.parents ? A.parents[s0 + i] : i - 1 : -1;
+        const i64 token = A.tokens[s0 + i];
+        const bool fine = parent >= 0 && parent < i && token >= 0 && token < A.v;
+        sh.parent[i] = fine ? parent : -1;
+        sh.token[i] = fine ? (int)token : -1;
+        sh.u[i] = A.uniforms[s0 + i];
+        sh.have[i] = sh.said[i] = 0;
+        if (fine) {
+            auto of = [&](int which) {
+                const Row r = A.rows[(which ? A.n : 0) + s0 + parent];
+                return r.per_z == 0 ? 0.0 : exp2_64(fma((double)(float)((const T *)A.x[which])[(s0 + parent) * A.ld[which] + token], A.c, -r.mc)) * r.per_z;
+            };
+            sh.have[i] = of(0);
+            sh.said[i] = A.drafted ? of(1) : 1.0;
+        }
+    }
+    __syncthreads();
+    // from here on all threads do the same
+    Left<DT> left = {};
+    left.c = A.c, left.v = A.v, left.sh = &sh, left.nodes = nodes;
+    int cur = 0, count = 0;
+    auto stand_at = [&](int node) {
+        cur = node, left.a = 0, left.cur = -1;
+        if (node < nodes) {
+            left.x = (const T *)A.x[0] + (s0 + node) * A.ld[0], left.p = A.rows[s0 + node];
+            if (A.drafted) left.y = (const T *)A.x[1] + (s0 + node) * A.ld[1], left.q = A.rows[A.n + s0 + node];
+        }
+    };
+    stand_at(0);
+    double w = 1;                              // the sum of what is left; below zero: not known
+    for (int i = 1; i < nodes; ++i) {
+        if (sh.parent[i] != cur || count == A.depth || left.p.per_z == 0 || (A.drafted && left.q.per_z == 0)) continue;
+        double have = sh.have[i];
+        if (!A.drafted) {
+            for (int j = 1; j < i; ++j)
+                if (sh.parent[j] == cur && sh.token[j] == sh.token[i]) have = 0;       // refused before
+        } else if (left.a > 0) {
+            if (w < 0) w = sum_left(sh, left);
+            have = fmax(have - left.a * sh.said[i], 0.0);
+        }
+        if (sh.u[i] * sh.said[i] * w < have) {
+            if (t == 0) {
+                A.nodes[(i64)b * A.depth + count] = i;
+                A.out[(i64)b * (A.depth + 1) + count] = sh.token[i];
+            }
+            ++count;
+            stand_at(i);
+            w = 1;
+        } else if (A.drafted) {
+            left.a += w;
+            w = -1;
+        } else {
+            w -= have;
+            left.cur = cur;
+        }
+    }
+    int last = -1;
+    if (nodes > 0 && left.p.per_z != 0) {
+        double sum = sum_left(sh, left);
+        if (!(sum > 0)) {
+            left.a = 0, left.cur = -1;
+            sum = sum_left(sh, left);
+        }
+        if (wave == 0) last = find_left(sh, left, sh.u[0] * sum);
+    }
+    if (t == 0) {
+        A.counts[b] = count;
+        A.out[(i64)b * (A.depth + 1) + count] = last;
+    }
+}
+
+// eight entries a thread once where there are few, up to four times
+int rounds(int64_t v, int64_t rows) {
+    for (int r = 1; r < 8; r *= 2) {
+        const i64 slices = (v + BLOCK * EIGHT * r - 1) / (BLOCK * EIGHT * r);
+        if (slices <= 64 && slices * rows <= 4096) return r;
+    }
+    return 8;
+}
+i64 slices_of(int64_t v, int r) { return (v + BLOCK * EIGHT * r - 1) / (BLOCK * EIGHT * r); }
+// the largest rows that eight times eight entries a thread and 64 slices hold
+static_assert(MAX_V <= (i64)BLOCK * EIGHT * 8 * 64, "rows of too many slices");
+
+// ---- the path's entries -------------------------------------------------------------------------------------------
+struct Keep {
+    Cache cache;
+    Batch batch;
+    const i64 *nodes, *counts;
+    int depth;
+    int *lengths;
+};
+
+__global__ __launch_bounds__(BLOCK) void k_keep(Keep A) {
+    struct Move {
+        i64 from_page, to_page;
+        int from_row, to_row, fine;
+    };
+    __shared__ int node[MAX_DEPTH];
+    __shared__ Move moves[MAX_DEPTH];
+    __shared__ int path;
+    const int b = blockIdx.x, t = threadIdx.x, heads = (int)A.cache.heads;
+    const int nodes = max(A.batch.starts[b + 1] - A.batch.starts[b], 0);
+    const i64 length = A.batch.lengths[b], first = length - nodes;
+    const int count = (int)max((i64)0, min(A.counts[b], (i64)A.depth));
+    for (int d = t; d < count; d += BLOCK) node[d] = (int)max((i64)0, min(A.nodes[(i64)b * A.depth + d], (i64)0x7FFFFFFF));
+    __syncthreads();
+    if (t == 0) {
+        int d = 0;
+        for (int before = 0; d < count && node[d] > before && node[d] < nodes; ++d) before = node[d];
+        path = d;
+        if (blockIdx.y == 0) A.lengths[b] = (int)max((i64)0, nodes ? first + 1 + d : length);
+    }
+    __syncthreads();
+    const int n = path;
+    for (int d = t; d < n; d += BLOCK) {
+        Move m = {0, 0, 0, 0, 0};
+        m.fine = node[d] != d + 1 && find_entry(A.cache, A.batch, b, first + node[d], &m.from_page, &m.from_row) &&
+                 find_entry(A.cache, A.batch, b, first + d + 1, &m.to_page, &m.to_row);
+        moves[d] = m;
+    }
+    __syncthreads();
+    // A thread has one place in all entries of the path: 16 bytes of a head's, or a scale.  Numbers rise, so that an entry never comes from where an
+    // earlier one went: eight are read before the first is written.
+    const int units = A.cache.dim * A.cache.size / 16, all = heads * 2 * units;
+    const int item = (int)blockIdx.y * BLOCK + t;
+    if (item < all) {
+        typedef u32 v4u __attribute__((ext_vector_type(4)));
+        const Half &h = A.cache.half[item / (heads * units)];
+        const int head = item / units % heads;
+        char *at = h.at + head * h.head + item % units * 16;
+        for (int d = 0; d < n; d += 8) {
+            v4u v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (d + i < n && moves[d + i].fine) v[i] = *(const v4u *)(at + moves[d + i].from_page * h.page + moves[d + i].from_row * h.row);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (d + i < n && moves[d + i].fine) *(v4u *)(at + moves[d + i].to_page * h.page + moves[d + i].to_row * h.row) = v[i];
+        }
+    } else if (A.cache.dtype == VI_I8 && item < all + 2 * heads) {
+        const Half &h = A.cache.half[(item - all) / heads];
+        float *at = h.scales + (item - all) % heads * h.scale_head;
+        for (int d = 0; d < n; d += 8) {
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (d + i < n && moves[d + i].fine) v[i] = at[moves[d + i].from_page * h.scale_page + moves[d + i].from_row];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (d + i < n && moves[d + i].fine) at[moves[d + i].to_page * h.scale_page + moves[d + i].to_row] = v[i];
+        }
+    }
+}
+
+}  // namespace
+
+extern "C" size_t vi_verify_drafts_workspace_bytes(int dtype, int64_t n, int64_t v, int drafted) {
+    if (!is_float(dtype) || n <= 0 || n > MAX_BLOCKS || v <= 0 || v > MAX_V) return 0;
+    const i64 rows = drafted ? 2 * n : n;
+    return (size_t)(2 * n) * sizeof(Row) + (size_t)(rows * slices_of(v, rounds(v, rows))) * sizeof(Part) + vi::WS_SLACK;
+}
+
+extern "C" int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_t v, int64_t ld, const void *draft, int64_t ld_draft, const int64_t *tokens,
+                                const int32_t *starts, int64_t sequences, const int32_t *parents, const double *uniforms, double temperature, int64_t depth,
+                                int64_t *counts, int64_t *nodes, int64_t *out, void *ws, size_t ws_bytes, void *stream) {
+    const char *who = "vi_verify_drafts";
+    if (!is_float(dtype)) return vi::fail(VI_EINVAL, "%s: dtype %d is none of VI_F32, VI_BF16, VI_F16", who, dtype);
+    if (n < 0 || n > MAX_BLOCKS || v < 1 || v > MAX_V) return vi::fail(VI_EINVAL, "%s: %lld rows of %lld logits (1 to %lld)", who, (long long)n, (long long)v, (long long)MAX_V);
+    if (ld < v || (draft && ld_draft < v)) return vi::fail(VI_EINVAL, "%s: rows of %lld logits %lld apart", who, (long long)v, (long long)(ld < v ? ld : ld_draft));
+    if (sequences < 0 || sequences > 0xFFFFFF) return vi::fail(VI_EINVAL, "%s: %lld sequences", who, (long long)sequences);
+    if (depth < 0 || depth > MAX_DEPTH) return vi::fail(VI_EINVAL, "%s: a depth of %lld (%d at most)", who, (long long)depth, MAX_DEPTH);
+    if (!(temperature >= 1e-3 && temperature <= 1e3)) return vi::fail(VI_EINVAL, "%s: temperature %g", who, temperature);
+    if (sequences == 0) return VI_OK;
+    if (!starts || !counts || !out || (depth && !nodes) || (n && (!logits || !tokens || !uniforms))) return vi::fail(VI_EINVAL, "%s: null pointer", who);
+    const size_t need = vi_verify_drafts_workspace_bytes(dtype, n, v, draft != nullptr);
+    if (ws_bytes < need || (need && !ws)) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, need);
+    const i64 rows = draft ? 2 * n : n;
+    const int r = rounds(v, rows);
+    if (rows * slices_of(v, r) > MAX_BLOCKS) return vi::fail(VI_EINVAL, "%s: %lld rows of %lld logits", who, (long long)n, (long long)v);
+    const hipStream_t s = (hipStream_t)stream;
+    Walk W = {};
+    W.rows = (Row *)vi::align16(ws);
+    Part *parts = (Part *)(W.rows + 2 * n);
+    W.x[0] = logits, W.x[1] = draft, W.ld[0] = ld, W.ld[1] = ld_draft, W.n = n, W.v = v, W.slices = (int)slices_of(v, r), W.sequences = (int)sequences;
+    W.depth = (int)depth, W.drafted = draft != nullptr, W.c = 1.4426950408889634 / temperature, W.parts = parts, W.tokens = tokens, W.starts = starts;
+    W.parents = parents, W.uniforms = uniforms, W.counts = counts, W.nodes = nodes, W.out = out;
+    const Stats A = {{logits, draft}, {ld, ld_draft}, n, v, W.slices, W.c, parts};
+    const dim3 grid((unsigned)(rows * W.slices));
+#define STATS(DT, R) hipLaunchKernelGGL((k_stats<DT, R>), grid, dim3(BLOCK), 0, s, A)
+#define GO(DT)                                                                                      \
+    do {                                                                                            \
+        if (n) {                                                                                    \
+            if (r == 1) STATS(DT, 1);                                                               \
+            else if (r == 2) STATS(DT, 2);                                                          \
+            else if (r == 4) STATS(DT, 4);                                                          \
+            else STATS(DT, 8);                                                                      \
+            VI_LAUNCH_CHECK(who);                                                                   \
+        }                                                                                           \
+        hipLaunchKernelGGL(k_walk<DT>, dim3((unsigned)sequences), dim3(WALK), 0, s, W);             \
+    } while (0)
+    if (dtype == VI_F32) GO(VI_F32);
+    if (dtype == VI_BF16) GO(VI_BF16);
+    if (dtype == VI_F16) GO(VI_F16);
+#undef GO
+#undef STATS
+    VI_LAUNCH_CHECK(who);
+    return VI_OK;
+}
+
+extern "C" int vi_keep_drafts(const vi_cache *cache, const vi_batch *batch, const int64_t *nodes, int64_t depth, const int64_t *counts, int32_t *lengths,
+                              void *stream) {
+    const char *who = "vi_keep_drafts";
+    Keep A = {};
+    if (const int rc = take(who, cache, batch, &A.cache, &A.batch)) return rc;
+    if (depth < 0 || depth > MAX_DEPTH) return vi::fail(VI_EINVAL, "%s: a depth of %lld (%d at most)", who, (long long)depth, MAX_DEPTH);
+    if (batch->sequences == 0) return VI_OK;
+    if (!counts || !lengths || (depth && !nodes)) return vi::fail(VI_EINVAL, "%s: null pointer", who);
+    if (lengths == batch->lengths) return vi::fail(VI_EINVAL, "%s: the new lengths in the place of the old", who);
+    A.nodes = nodes, A.counts = counts, A.depth = (int)depth, A.lengths = lengths;
+    const i64 items = (i64)cache->heads * 2 * (cache->dim * A.cache.size / 16) + (cache->dtype == VI_I8 ? 2 * cache->heads : 0);
+    if (items / BLOCK >= 65535) return vi::fail(VI_EINVAL, "%s: %lld heads", who, (long long)cache->heads);
+    hipLaunchKernelGGL(k_keep, dim3((unsigned)batch->sequences, (unsigned)((items + BLOCK - 1) / BLOCK)), dim3(BLOCK), 0, (hipStream_t)stream, A);
+    VI_LAUNCH_CHECK(who);
+    return VI_OK;
+}
