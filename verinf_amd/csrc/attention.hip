@@ -27,26 +27,30 @@ typedef u32 v2u __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 
+#define INLINE __attribute__((always_inline))
+
 constexpr int MAX_NODES = 256;                 // of a tree
 constexpr int MASK_WORDS = MAX_NODES / 32 + 1;
 constexpr i64 MAX_BLOCKS = 1 << 22;            // of a launch, which has less than 2^32 threads
+constexpr i64 MAX_PARTS = 128;                 // of a sequence's keys
+constexpr int CLEARING = 64;                   // workgroups that look for rows of no sequence
 constexpr float LATE = 8.0f;                   // powers of two that scores may exceed what they are relative to
 
-// DT: of queries and outputs; I8: the cache has 8-bit integers; DP: columns, at least the cache's
-template <int DT_, bool I8_, int DP_, int NB_, int WM_, int WK_, int KBS_, int ST_, int OCC_>
+// DT: of queries and outputs; I8: the cache has 8-bit integers; DP: columns, at least the cache's; OCC: workgroups of a CU
+template <int DT_, bool I8_, int DP_, int WM_, int WK_, int OCC_>
 struct Form {
-    static constexpr int DT = DT_, DP = DP_, NB = NB_, WM = WM_, WK = WK_, KBS = KBS_, ST = ST_, OCC = OCC_;
-    static constexpr bool I8 = I8_;
-    static constexpr int WAVES = WM * WK, THREADS = 64 * WAVES, ROWS = 32 * NB * WM;
-    static constexpr int KEYS = 32 * KBS, GROUPS = 2 * KBS;            // of a stage; sixteen keys are of one page
-    static constexpr int ROW = DP * (I8 ? 1 : 2), UNITS = ROW / 16, PER_LOAD = 64 / UNITS, LOADS = 16 / PER_LOAD;        // bytes, units; rows of a load, loads of a group
-    static constexpr int HALF = KEYS * ROW, SCALES = I8 ? 2 * KEYS * 4 : 0, STAGE = 2 * HALF + SCALES;
-    static constexpr int MINE = 2 * GROUPS * LOADS / WM + (I8 ? KBS : 0);             // loads of a wavefront in a stage
+    static constexpr int DT = DT_, DP = DP_, WM = WM_, WK = WK_, ST = WM > 1 ? 2 : 1;
+    static constexpr bool I8 = I8_, WIDE = I8 && WM > 1;               // WIDE: 8-bit integers lie in LDS as 16-bit numbers
+    static constexpr int WAVES = WM * WK, THREADS = 64 * WAVES, ROWS = 32 * WM, OCC = OCC_ * WAVES / 4 > 0 ? OCC_ * WAVES / 4 : 1;           // wavefronts of a SIMD
+    static constexpr int KEYS = WM > 1 ? 64 : 32, GROUPS = KEYS / 16;  // of a stage; sixteen keys are of one page
+    static constexpr int ROW = DP * (I8 && !WIDE ? 1 : 2), UNITS = ROW / 16, PER_LOAD = 64 / UNITS, LOADS = 16 / PER_LOAD;       // bytes, units; rows of a load, loads of a group
+    static constexpr int SCALES = I8 ? KEYS * 4 : 0, HALF = KEYS * ROW + SCALES, STAGE = 2 * HALF;
+    static constexpr int MINE = GROUPS * LOADS / WM, KINDS = LOADS > WM ? LOADS / WM : 1;              // loads of a wavefront in half a stage, different ones of a group
     static constexpr int PITCH = 36;           // floats between rows of 32 on their way out
-    static constexpr int OUT = WAVES * NB * 32 * PITCH * 4 + WAVES * NB * 32 * 8 + ROWS * 8;
+    static constexpr int OUT = WAVES * 32 * PITCH * 4 + WAVES * 32 * 8 + ROWS * 8;
     static constexpr int LDS = WK * ST * STAGE > OUT ? WK * ST * STAGE : OUT;
     static constexpr int MASKS = ROWS < MAX_NODES ? ROWS : MAX_NODES;
-    static_assert(2 * GROUPS * LOADS % WM == 0, "loads of a stage");
+    static_assert(WIDE || (GROUPS * LOADS % WM == 0 && (LOADS % WM == 0 || WM % LOADS == 0)), "loads of a stage");
 };
 
 struct Args {
@@ -56,7 +60,7 @@ struct Args {
     void *out;
     i64 q_token, q_head, out_token, out_head, n;
     const int *parents;
-    int heads, group, tiles, splits, clear;
+    int heads, group, tiles, splits, per_split, clear;                 // per_split: keys
     float c;                                   // scale log2(e)
     float *part;                               // [tile][head][split][ROWS][DP] sums
     float *most;                               // [tile][head][split][ROWS][2] what they are relative to, sums of the exponentials
@@ -74,7 +78,8 @@ __device__ __forceinline__ int order(int row) {
 // the compiler does not wait for it before the next read of LDS: the waits are arrive()'s.  Inside an asm block nothing inserts wait states: one between the
 // write of M0 and the load, five between a vector instruction's write of a scalar register (readfirstlane) and a load that reads it.
 __device__ __forceinline__ void fetch_to_lds(u32 at, u32 off, const char *base) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(at), "v"(off), "s"(base) : "memory");
+    const u64 b = (u64)__builtin_amdgcn_readfirstlane((u32)((u64)base >> 32)) << 32 | (u32)__builtin_amdgcn_readfirstlane((u32)(u64)base);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(at), "v"(off), "s"(b) : "memory");
 }
 // the same of 4 bytes a lane, each at an address of its own
 __device__ __forceinline__ void fetch_words_to_lds(u32 at, const float *from) {
@@ -85,6 +90,8 @@ template <int N>
 __device__ __forceinline__ void arrive() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory");
 }
+// its LDS accesses are done
+__device__ __forceinline__ void read() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory"); }
 __device__ __forceinline__ void meet_wave() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -138,65 +145,176 @@ __device__ __forceinline__ int same(int v) { return (int)__builtin_amdgcn_readfi
 // Sequence b's tiles begin at starts[b] group / rows + b: apart by at least as many as it needs, and no sequence's start has to be known to count them.
 struct Tile {
     int b, n, first;                           // sequence, its new tokens, the tile's first row in it
-    i64 s0;
+    int s0, context, end;                      // its first row; entries before the new ones; the key behind the last that a row of the tile may attend to
 };
 template <int ROWS>
 __device__ __forceinline__ bool find_tile(const Args &A, int tile, Tile *t) {
-    auto start = [&](int b) { return max((i64)0, min((i64)A.batch.starts[b], A.n)); };
-    int count = 0;
+    int found = -1, s0 = 0, s1 = 0, length = 0;
     for (int first = 0; first < A.batch.sequences; first += 64) {
-        const int b = min(first + (int)(threadIdx.x & 63), A.batch.sequences);
-        count += __popcll(__ballot(b < A.batch.sequences && start(b) * A.group / ROWS + b <= tile));
+        const int b = min(first + (int)(threadIdx.x & 63), A.batch.sequences - 1);
+        const i64 here = max((i64)0, min((i64)A.batch.starts[b], A.n)), next = max((i64)0, min((i64)A.batch.starts[b + 1], A.n));
+        const int its = A.batch.lengths[b];
+        const int count = __popcll(__ballot(first + (int)(threadIdx.x & 63) < A.batch.sequences && here * A.group / ROWS + b <= tile));
+        if (count == 0) break;                 // starts rises
+        found = first + count - 1;
+        s0 = __shfl((int)here, count - 1), s1 = __shfl((int)next, count - 1), length = __shfl(its, count - 1);
     }
-    const int b = count - 1;
-    if (b < 0) return false;
-    const int s0 = same((int)start(b)), s1 = same((int)start(b + 1));
-    const i64 first = ((i64)tile - b - (i64)s0 * A.group / ROWS) * ROWS;
-    t->b = b, t->n = s1 - s0, t->s0 = s0, t->first = (int)first;
-    return first >= 0 && first < (i64)t->n * A.group;         // less than 0 where starts does not rise
+    if (found < 0) return false;
+    found = same(found), s0 = same(s0), s1 = same(s1), length = same(length);
+    const i64 first = ((i64)tile - found - (i64)s0 * A.group / ROWS) * ROWS;
+    t->b = found, t->n = s1 - s0, t->s0 = s0, t->first = (int)first, t->context = length - t->n;
+    if (first < 0 || first >= (i64)t->n * A.group) return false;       // less than 0 where starts does not rise
+    const int last = min(t->n - 1, (int)((u32)(t->first + ROWS - 1) / (u32)A.group));
+    t->end = (int)max((i64)0, min(min((i64)length, A.batch.most), (i64)t->context + last + 1));
+    return true;
 }
+
+// how many workgroups share a tile's keys: the last has what is left
+__device__ __forceinline__ int parts_of(const Args &A, int end) { return max(1, min(A.splits, (end + A.per_split - 1) / A.per_split)); }
 
 // ---- the pass over the keys ---------------------------------------------------------------------------------------
 template <class F>
 __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
-    constexpr int DT = F::DT, DP = F::DP, NB = F::NB, WM = F::WM, WK = F::WK, ROW = F::ROW, UNITS = F::UNITS;
+    constexpr int DT = F::DT, DP = F::DP, WM = F::WM, WK = F::WK, ROW = F::ROW, UNITS = F::UNITS;
+    constexpr bool NARROW = F::I8 && !F::WIDE;                         // 8-bit integers in LDS
     typedef typename type<DT>::t T;
     __shared__ alignas(16) char lds[F::LDS];
     __shared__ u32 masks[F::MASKS * MASK_WORDS];
     __shared__ int above[MAX_NODES];
-    const int lane = threadIdx.x & 63, half = lane >> 5, wave = same((int)threadIdx.x >> 6), wm = wave % WM, part = wave / WM;
+    const int lane = threadIdx.x & 63, half = lane >> 5, wave = same((int)threadIdx.x >> 6), wm = WM == 1 ? 0 : WK == 1 ? wave : wave % WM, part = WK == 1 ? 0 : WM == 1 ? wave : wave / WM;
     const int heads = (int)A.cache.heads, head = (int)blockIdx.x % heads, split = (int)blockIdx.x / heads % A.splits;
     const int tile = A.tiles - 1 - (int)blockIdx.x / heads / A.splits;         // the longest first, where a prompt's tiles differ
 
-    if (A.clear) {                             // rows of no sequence
+    if (A.clear && blockIdx.x < CLEARING) {    // rows of no sequence
         const i64 s0 = A.batch.sequences ? max((i64)0, min((i64)A.batch.starts[0], A.n)) : A.n, s1 = A.batch.sequences ? max(s0, min((i64)A.batch.starts[A.batch.sequences], A.n)) : A.n;
-        for (i64 r = blockIdx.x; r < s0 + A.n - s1; r += gridDim.x)
+        for (i64 r = blockIdx.x; r < s0 + A.n - s1; r += min(CLEARING, (int)gridDim.x))
             for (int i = threadIdx.x; i < A.heads * A.cache.dim; i += F::THREADS)
                 ((T *)A.out)[(r < s0 ? r : s1 + r - s0) * A.out_token + i / A.cache.dim * A.out_head + i % A.cache.dim] = (T)0.0f;
     }
     Tile t;
     if (!find_tile<F::ROWS>(A, tile, &t)) return;
-    const int length = same((int)max((i64)0, min((i64)A.batch.lengths[t.b], A.batch.most))), context = same(A.batch.lengths[t.b]) - t.n;
+    const int end = t.end, context = t.context;
     const bool tree = A.parents && t.n <= MAX_NODES;
-    // key j < limit: the tokens of the tile's, and the wavefront's, first and last row; keys below `free` are masked for none of the wavefront's
-    auto token = [&](int row) { return (int)((u32)row / (u32)A.group); };
-    const int last = min(t.n - 1, token(t.first + F::ROWS - 1)), end = max(0, min(length, context + last + 1));
-    const int row0 = t.first + wm * NB * 32, wave_first = token(row0), wave_last = min(t.n - 1, token(row0 + 32 * NB - 1));
-    const int wave_end = wave_first < t.n ? min(end, context + wave_last + 1) : 0, wave_free = tree ? context : context + wave_first + 1;
-    const int units = (end + F::KEYS * WK - 1) / (F::KEYS * WK);
-    const int from = (int)((i64)split * units / A.splits), to = (int)((i64)(split + 1) * units / A.splits);
+    auto token = [&](int row) INLINE { return (int)((u32)row / (u32)A.group); };
+    // a workgroup's part of the keys; where one has all of them it is done with that
+    const int first_key = split * A.per_split, parts = parts_of(A, end);
+    if (split >= parts) return;
+    const int stages = ((split == parts - 1 ? end - first_key : A.per_split) + F::KEYS * WK - 1) / (F::KEYS * WK);       // of each of the WK groups
     const i64 slot = ((i64)tile * heads + head) * A.splits + split;
-    if (A.splits > 1 && from == to) {
-        for (int r = threadIdx.x; r < F::ROWS; r += F::THREADS) A.most[(slot * F::ROWS + r) * 2] = -INFINITY, A.most[(slot * F::ROWS + r) * 2 + 1] = 0.0f;
-        return;
+    // the wavefront's rows attend to keys below wave_end, all of them to those below wave_free
+    const int row0 = t.first + wm * 32, wave_first = token(row0), wave_last = min(t.n - 1, token(row0 + 31));
+    const int wave_end = wave_first < t.n ? min(end, context + wave_last + 1) : 0, wave_free = tree ? context : context + wave_first + 1;
+
+    // queries: unit (of eight columns) `chunk` of a row for half and step
+    const int row = row0 + (lane & 31), tok = token(row);
+    const bool there = tok < t.n;
+    v4u q[DP / 16];
+    {
+        const T *x = (const T *)A.q + ((i64)t.s0 + (there ? tok : 0)) * A.q_token + (head * A.group + (there ? row - tok * A.group : 0)) * A.q_head;
+#pragma unroll
+        for (int st = 0; st < DP / 16; ++st) {
+            const int chunk = F::I8 && !F::WIDE ? 4 * (st / 2) + 2 * half + st % 2 : 2 * st + half;
+            q[st] = v4u{0, 0, 0, 0};
+            if (there && chunk * 8 < A.cache.dim) q[st] = load_any<v4u>(x + chunk * 8);
+        }
     }
+
+    // ---- stages
+    const u32 lds_at = (u32)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    const char *from[2];
+    const float *scales_from[2];
+    u32 page_apart[2], row_apart[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        from[h] = A.cache.half[h].at + head * A.cache.half[h].head, scales_from[h] = A.cache.half[h].scales + head * A.cache.half[h].scale_head;
+        page_apart[h] = (u32)A.cache.half[h].page, row_apart[h] = (u32)A.cache.half[h].row;
+    }
+    const int full_units = A.cache.dim * (F::I8 ? 1 : 2) / 16, row_mask = A.cache.mask;
+    const u32 n_pages = (u32)A.cache.pages;
+    const bool one_page = row_mask >= F::KEYS - 1;                     // a stage has entries of one page
+    typedef const __attribute__((address_space(4))) int *Table;        // constant while the kernel runs: read by the scalar cache
+    const Table pages = (Table)(A.batch.pages + t.b * A.batch.stride);
+    auto stage_key = [&](int it) INLINE { return first_key + (it * WK + part) * F::KEYS; };
+    struct Pages {
+        int number[F::GROUPS];                 // of sixteen keys each: only the first is looked at where a stage is in one page
+    };
+    auto look_up = [&](int it) INLINE {
+        const int j = stage_key(it);
+        Pages p;
+#pragma unroll
+        for (int g = 0; g < F::GROUPS; ++g) p.number[g] = pages[min(j + 16 * g, end - 1) >> A.cache.shift];
+        return p;
+    };
+    auto number_of = [&](const Pages &p, int g) INLINE {
+        const int first = p.number[0], own = p.number[g];
+        return one_page ? first : own;
+    };
+    // how many of the sixteen keys from j on there are
+    auto valid_of = [&](int number, int j) INLINE { return (u32)number < n_pages ? max(0, min(16, end - j)) : 0; };
+    // whether a stage has all its keys, and columns fill the units
+    auto whole = [&](const Pages &p, int j) INLINE {
+        bool all = full_units == UNITS && j + F::KEYS <= end && (u32)p.number[0] < n_pages;
+        if (!one_page) {
+#pragma unroll
+            for (int g = 1; g < F::GROUPS; ++g) all = all && (u32)p.number[g] < n_pages;
+        }
+        return all;
+    };
+    // A lane's unit of 16 bytes in a load: its row is lane / UNITS and a multiple of PER_LOAD behind, and rows differ in the order of their units.  A wavefront
+    // has KINDS different loads of sixteen keys.
+    const int lane_row = lane / UNITS, wave_load = F::LOADS >= WM ? wm : wm % F::LOADS;
+    u32 lane_unit[F::KINDS], lane_off[2];
+#pragma unroll
+    for (int k = 0; k < F::KINDS; ++k) lane_unit[k] = (u32)(lane % UNITS ^ order<UNITS>((k * WM + wave_load) * F::PER_LOAD + lane_row)) * 16;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) lane_off[h] = (u32)(wave_load * F::PER_LOAD + lane_row) * row_apart[h];
+    // The keys (h = 0) or values of a stage on their way to its slot: MINE loads, and one of scales, where it is whole (fewer, and zeros in the places of
+    // the others, elsewhere).
+    auto fetch = [&](int h, u32 place, int j, const Pages &p, bool all) INLINE {
+        const u32 wave_place = lds_at + place + (u32)(wave_load * 1024 + (F::LOADS >= WM ? 0 : wm / F::LOADS * 16 * ROW));
+        // sixteen keys after sixteen; where a group has fewer loads than there are wavefronts, these are at several groups at a time
+        constexpr int STEP = F::LOADS >= WM ? 1 : WM / F::LOADS;
+        const int mine = F::LOADS >= WM ? 0 : wm / F::LOADS;
+        if (all && one_page) {
+            const char *b = from[h] + (u64)(u32)p.number[0] * page_apart[h] + (u32)((j & row_mask) + 16 * mine) * row_apart[h];
+#pragma unroll
+            for (int l = 0; l < F::MINE; ++l) {
+                const int g = l / F::KINDS * STEP, k = l % F::KINDS;
+                fetch_to_lds(wave_place + (u32)(g * 16 * ROW + k * WM * 1024), lane_off[h] + lane_unit[k], b + (u32)(16 * g + k * WM * F::PER_LOAD) * row_apart[h]);
+            }
+        } else {
+#pragma unroll
+            for (int l = 0; l < F::MINE; ++l) {
+                const int g = l / F::KINDS * STEP, k = l % F::KINDS, jj = j + 16 * (g + mine);
+                int number = number_of(p, g);
+#pragma unroll
+                for (int o = 1; o < STEP; ++o) number = mine == o ? number_of(p, g + o) : number;
+                const u32 at = wave_place + (u32)(g * 16 * ROW + k * WM * 1024);
+                const char *b = from[h] + (u64)(u32)number * page_apart[h] + (u32)((jj & row_mask) + k * WM * F::PER_LOAD) * row_apart[h];
+                const int r = (k * WM + wave_load) * F::PER_LOAD + lane_row;
+                if (r < valid_of(number, jj) && (int)lane_unit[k] < full_units * 16) fetch_to_lds(at, lane_off[h] + lane_unit[k], b);
+                else *(v4u *)(lds + (at - lds_at) + lane * 16) = v4u{0, 0, 0, 0};
+            }
+        }
+        if constexpr (F::I8 && !F::WIDE) {
+            const int one = number_of(p, 0), two = number_of(p, 1), jj = j + (lane & 16), number = lane & 16 ? two : one;
+            const u32 at = place + F::KEYS * ROW;
+            if (lane < 32) {
+                if ((lane & 15) < valid_of(number, jj)) fetch_words_to_lds(lds_at + at, scales_from[h] + number * A.cache.half[h].scale_page + (jj & row_mask) + (lane & 15));
+                else *(float *)(lds + at + lane * 4) = 0.0f;
+            }
+        }
+    };
+    constexpr int LOADS_OF_HALF = F::MINE + (F::I8 ? 1 : 0);
+    auto place_of = [&](int h, int into) INLINE { return (u32)((part * F::ST + into) * F::STAGE + h * F::HALF); };
 
     // the rows' ancestors among the new tokens, a bit each
     if (tree) {
-        for (int i = threadIdx.x; i < t.n; i += F::THREADS) above[i] = A.parents[t.s0 + i];
+        const int first = token(t.first), last = min(t.n - 1, token(t.first + F::ROWS - 1));
+        for (int i = threadIdx.x; i < t.n; i += F::THREADS) above[i] = A.parents ? A.parents[t.s0 + i] : -1;
         __syncthreads();
-        for (int i = token(t.first) + (int)threadIdx.x; i <= last; i += F::THREADS) {
-            u32 *bits = masks + (i - token(t.first)) * MASK_WORDS;
+        for (int i = first + (int)threadIdx.x; i <= last; i += F::THREADS) {
+            u32 *bits = masks + (i - first) * MASK_WORDS;
 #pragma unroll
             for (int w = 0; w < MASK_WORDS; ++w) bits[w] = 0;
             for (int at = i;;) {
@@ -208,363 +326,399 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
         }
         __syncthreads();
     }
+    const u32 *mask = masks + (tree && there ? tok - token(t.first) : 0) * MASK_WORDS;
 
-    // queries: unit (of eight columns) `chunk` of a row for half and step
-    v4u q[NB][DP / 16];
-    int limit[NB];                             // of the lane's row: keys below it (a chain's), its mask's place (a tree's); -1: no row
+    v16f o[DP / 32];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const int row = row0 + 32 * nb + (lane & 31), tok = token(row), g = row - tok * A.group;
-        const bool fine = tok < t.n;
-        limit[nb] = !fine ? -1 : tree ? (tok - token(t.first)) * MASK_WORDS : max(0, context + tok + 1);
-        const T *x = (const T *)A.q + (t.s0 + (fine ? tok : 0)) * A.q_token + (head * A.group + (fine ? g : 0)) * A.q_head;
-#pragma unroll
-        for (int st = 0; st < DP / 16; ++st) {
-            const int chunk = F::I8 ? 4 * (st / 2) + 2 * half + st % 2 : 2 * st + half;
-            q[nb][st] = v4u{0, 0, 0, 0};
-            if (fine && chunk * 8 < A.cache.dim) q[nb][st] = load_any<v4u>(x + chunk * 8);
+    for (int db = 0; db < DP / 32; ++db) o[db] = v16f{};
+    float most = -INFINITY, relative = -INFINITY, sum = 0;             // largest score so far (or up to LATE behind), times c: what the sums are relative to
+
+    // which of the 32 keys from j on the lane's row attends to; the low and the high sixteen have so many
+    auto window_of = [&](int j, int low, int high) INLINE {
+        u32 w = ~0u;
+        if (there && !tree) {
+            const int left = context + tok + 1 - j;
+            w = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
+        } else if (there) {
+            const int node = j - context;
+            if (node >= MAX_NODES) w = 0;
+            else if (node >= 0) w = (u32)(((u64)mask[(node >> 5) + 1] << 32 | mask[node >> 5]) >> (node & 31));
+            else if (node > -32) w = mask[0] << -node | ((1u << -node) - 1);
         }
+        return w & ((low >= 16 ? 0xFFFFu : (1u << low) - 1) | (high >= 16 ? 0xFFFFu : (1u << high) - 1) << 16);
+    };
+    auto bit_of = [&](int r) INLINE { return 8 * (r / 4) + 4 * half + r % 4; };
+
+    // where a lane reads keys and values in a stage: kept in registers, the compiler would make them anew each time
+    u32 key_at[DP / 16], value_at[DP / 32][2];
+    {
+        const int r_ = lane & 31, in = lane & 15, right = lane >> 4 & 1;
+#pragma unroll
+        for (int st = 0; st < (NARROW ? DP / 32 : DP / 16); ++st) key_at[st] = (u32)(r_ * ROW + ((2 * st + half) ^ order<UNITS>(r_ & 15)) * 16);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int i = 0; i < (NARROW ? 1 : 2); ++i) {
+                const int row8 = (in >> 3) * 8 + 4 * half + (in >> 1 & 3), row16 = 8 * i + 4 * half + (in >> 2);
+                value_at[db][i] = NARROW ? (u32)(row8 * ROW + ((2 * db + right) ^ order<UNITS>(row8)) * 16 + (in & 1) * 8)
+                                         : (u32)(row16 * ROW + ((4 * db + 2 * right + (in >> 1 & 1)) ^ order<UNITS>(row16)) * 16 + (in & 1) * 8);
+            }
+#pragma unroll
+        for (int st = 0; st < (NARROW ? DP / 32 : DP / 16); ++st) asm volatile("" : "+v"(key_at[st]));
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int i = 0; i < (NARROW ? 1 : 2); ++i) asm volatile("" : "+v"(value_at[db][i]));
     }
 
-    // ---- stages
-    const u32 lds_at = (u32)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
-    const char *keys = A.cache.half[0].at + head * A.cache.half[0].head, *values = A.cache.half[1].at + head * A.cache.half[1].head;
-    const float *key_scales = A.cache.half[0].scales + head * A.cache.half[0].scale_head, *value_scales = A.cache.half[1].scales + head * A.cache.half[1].scale_head;
-    const int full_units = A.cache.dim * (F::I8 ? 1 : 2) / 16;
-    typedef const __attribute__((address_space(4))) int *Table;        // constant while the kernel runs: read by the scalar cache
-    const Table pages = (Table)(A.batch.pages + t.b * A.batch.stride);
-    const int stages = to - from;              // of each of the WK groups
-    auto stage_key = [&](int it) { return ((from + it) * WK + part) * F::KEYS; };
-    struct Page {
-        i64 page;
-        int row, valid;                        // row in the page of the first of sixteen keys; how many of them there are
-    };
-    auto page_of = [&](int j) {
-        Page p = {0, 0, 0};
-        if (j < end) {
-            const int n = pages[j >> A.cache.shift];
-            p.page = n, p.row = j & A.cache.mask;
-            p.valid = n >= 0 && n < A.cache.pages ? min(16, end - j) : 0;
-        }
-        return p;
-    };
-    u32 partial = 0;                           // a bit for each slot whose stage has fewer loads than MINE
-    auto fetch = [&](int it) {
-        const int j = stage_key(it), into = it % F::ST;
-        char *stage = lds + (part * F::ST + into) * F::STAGE;
-        const u32 at = lds_at + (u32)((part * F::ST + into) * F::STAGE);
-        bool some = false;
-        Page page[F::GROUPS];
+    // scores of 32 keys: k is their rows in LDS, `scales` theirs
+    auto scores = [&](const char *k, const char *scales) INLINE {
+        v16f s = {};
+        if constexpr (NARROW) {
 #pragma unroll
-        for (int g = 0; g < F::GROUPS; ++g) page[g] = page_of(j + 16 * g), some |= page[g].valid < 16;
-#pragma unroll
-        for (int l = 0; l < 2 * F::GROUPS * F::LOADS / WM; ++l) {
-            const int n = l * WM + wm, which = n / (F::GROUPS * F::LOADS), g = n / F::LOADS % F::GROUPS, i = n % F::LOADS;
-            i64 number = page[0].page;
-            int first = page[0].row, valid = page[0].valid;
-#pragma unroll
-            for (int o = 1; o < F::GROUPS; ++o)
-                if (g == o) number = page[o].page, first = page[o].row, valid = page[o].valid;
-            const i64 page_apart = which ? A.cache.half[1].page : A.cache.half[0].page, row_apart = which ? A.cache.half[1].row : A.cache.half[0].row;
-            const char *base = (which ? values : keys) + number * page_apart + first * row_apart;
-            const int row = i * F::PER_LOAD + lane / UNITS, unit = lane % UNITS ^ order<UNITS>(row);
-            const u32 off = (u32)row * (u32)row_apart + (u32)unit * 16;
-            const u32 place = (u32)(which * F::HALF + g * 16 * ROW + i * 1024);
-            if (valid == 16 && full_units == UNITS) {
-                fetch_to_lds(at + place, off, base);
-            } else {
-                if (row < valid && unit < full_units) fetch_to_lds(at + place, off, base);
-                else *(v4u *)(stage + place + lane * 16) = v4u{0, 0, 0, 0};
+            for (int st = 0; st < DP / 16; st += 2) {
+                const v4u w = *(const v4u *)(k + key_at[st / 2]);
+                s = multiply<DT>(widen(v2u{w.x, w.y}), q[st], s);
+                s = multiply<DT>(widen(v2u{w.z, w.w}), q[st + 1], s);
             }
+        } else {
+#pragma unroll
+            for (int st = 0; st < DP / 16; ++st) s = multiply<DT>(*(const v4u *)(k + key_at[st]), q[st], s);
         }
         if constexpr (F::I8) {
-            // lanes 0 .. 31 the scales of 32 keys, the others of as many values
 #pragma unroll
-            for (int kb = 0; kb < F::KBS; ++kb) {
-                const bool second = lane & 16;
-                const i64 number = second ? page[2 * kb + 1].page : page[2 * kb].page;
-                const int first = second ? page[2 * kb + 1].row : page[2 * kb].row, valid = second ? page[2 * kb + 1].valid : page[2 * kb].valid;
-                const float *base = half ? value_scales : key_scales;
-                const i64 apart = half ? A.cache.half[1].scale_page : A.cache.half[0].scale_page;
-                const u32 place = 2 * F::HALF + kb * 256;
-                if ((lane & 15) < valid) fetch_words_to_lds(at + place, base + number * apart + first + (lane & 15));
-                else *(float *)(stage + place + lane * 4) = 0.0f;
+            for (int g = 0; g < 4; ++g) {
+                const v4f f = *(const v4f *)(scales + (8 * g + 4 * half) * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[4 * g + i] *= f[i];
             }
         }
-        partial = (partial & ~(1u << into)) | (u32)some << into;
+        return s;
     };
 
-    v16f o[NB][DP / 32];
-    float most[NB], relative[NB], sum[NB];     // largest score so far (or up to LATE behind), times c: what the sums are relative to
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        most[nb] = -INFINITY, relative[nb] = -INFINITY, sum[nb] = 0;
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db) o[nb][db] = v16f{};
-    }
+    // V^T of 32 columns and 16 keys, in the order of the registers: four from 4 half on, four from 8 + 4 half on
+    auto columns = [&](const char *v, int db, int st) INLINE {
+        if constexpr (NARROW) {
+            const v2u w = read_columns8(v + value_at[db][0] + st * 16 * ROW);
+            return v4u{w.x, w.y, 0, 0};
+        } else {
+            const v2u one = read_columns16(v + value_at[db][0] + st * 16 * ROW), two = read_columns16(v + value_at[db][1] + st * 16 * ROW);
+            return v4u{one.x, one.y, two.x, two.y};
+        }
+    };
 
-    // 32 keys from j on, in the stage's block kb; the low and the high sixteen have so many
-    auto block = [&](const char *stage, int kb, int j, int low, int high, auto masked) {
-        constexpr bool MASKED = decltype(masked)::value;
-        u32 window[NB];
-        if constexpr (MASKED) {
-            const u32 there = (low >= 16 ? 0xFFFFu : (1u << low) - 1) | (high >= 16 ? 0xFFFFu : (1u << high) - 1) << 16;
-            bool any = false;
+    // masked scores are none; the sums are kept relative to about the largest
+    auto settle = [&](v16f &s, bool masked, u32 window) INLINE {
+        if (masked) {
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                u32 w = ~0u;
-                if (limit[nb] >= 0) {
-                    if (!tree) {
-                        const int left = limit[nb] - j;
-                        w = left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
-                    } else {
-                        const int node = j - context;
-                        const u32 *bits = masks + limit[nb];
-                        if (node <= -32) w = ~0u;
-                        else if (node < 0) w = bits[0] << -node | ((1u << -node) - 1);
-                        else if (node < MAX_NODES) w = (u32)(((u64)bits[(node >> 5) + 1] << 32 | bits[node >> 5]) >> (node & 31));
-                        else w = 0;
-                    }
-                }
-                window[nb] = w & there;
-                any |= window[nb] != 0;
-            }
-            if (!__any(any)) return;
+            for (int r = 0; r < 16; ++r) s[r] = window >> bit_of(r) & 1 ? s[r] : -INFINITY;
         }
-        const char *k = stage + kb * 32 * ROW, *v = stage + F::HALF + kb * 32 * ROW;
-        v16f s[NB];
+        float top = s[0];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) s[nb] = v16f{};
-        {
-            const int row = lane & 31;
-            const char *mine = k + row * ROW;
-            const int o_ = order<UNITS>(row & 15);
-            if constexpr (F::I8) {
+        for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+        top = most_of_halves(top);
+        if (__any(top * A.c > relative + LATE)) {
+            asm volatile("");                  // a branch: the compiler would multiply by one, each time
+            const float now = fmaxf(most, top), then = now * A.c;
+            const float by = relative == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(relative - then);
+            most = now, relative = then, sum *= by;
 #pragma unroll
-                for (int st = 0; st < DP / 16; st += 2) {
-                    const v4u w = *(const v4u *)(mine + ((st + half) ^ o_) * 16);
-                    const v4u lo = widen(v2u{w.x, w.y}), hi = widen(v2u{w.z, w.w});
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) s[nb] = multiply<DT>(lo, q[nb][st], s[nb]);
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) s[nb] = multiply<DT>(hi, q[nb][st + 1], s[nb]);
-                }
-                v4f scale[4];
-#pragma unroll
-                for (int g = 0; g < 4; ++g) scale[g] = *(const v4f *)(stage + 2 * F::HALF + kb * 256 + (8 * g + 4 * half) * 4);
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[nb][r] *= scale[r / 4][r % 4];
-            } else {
-#pragma unroll
-                for (int st = 0; st < DP / 16; ++st) {
-                    const v4u w = *(const v4u *)(mine + ((2 * st + half) ^ o_) * 16);
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) s[nb] = multiply<DT>(w, q[nb][st], s[nb]);
-                }
-            }
+            for (int db = 0; db < DP / 32; ++db) o[db] *= by;
         }
-        v4u p[NB][2];
-        v4f value_scale[4];
+    };
+    // the exponentials of scores, as the second operand of the product with V^T
+    auto weights = [&](const v16f &s, const char *scales, v4u (&p)[2]) INLINE {
+        const float base = relative == -INFINITY ? 0.0f : relative;
+        float e[16], add = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], A.c, -base));
+            add += e[r];
+        }
+        sum += add;
         if constexpr (F::I8) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) value_scale[g] = *(const v4f *)(stage + 2 * F::HALF + kb * 256 + 128 + (8 * g + 4 * half) * 4);
+            for (int g = 0; g < 4; ++g) {
+                const v4f f = *(const v4f *)(scales + (8 * g + 4 * half) * 4);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) e[4 * g + i] = s[4 * g + i] == -INFINITY ? 0.0f : e[4 * g + i] * f[i];       // a scale in a masked place may be a NaN
+            }
         }
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-            if constexpr (MASKED) {
+        for (int i = 0; i < 8; ++i) p[i / 4][i % 4] = pack<DT>(e[2 * i], e[2 * i + 1]);
+    };
+
+    // 0 times an infinity or a NaN in a masked place would be a NaN.  Where keys are masked such values are left out of the products, and seen once more behind
+    // the pass, for the rows that attend to them.  (Those of 8-bit integers are in the scales.)
+    constexpr u32 INF = DT == VI_BF16 ? 0x7F80u : 0x7C00u;
+    bool wild = false;
+    auto tame = [&](v4u &w) INLINE {
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (!(window[nb] >> (8 * (r / 4) + 4 * half + r % 4) & 1)) s[nb][r] = -INFINITY;
-            }
-            float top = s[nb][0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) top = fmaxf(top, s[nb][r]);
-            top = most_of_halves(top);
-            if (__any(top * A.c > relative[nb] + LATE)) {
-                const float now = fmaxf(most[nb], top), then = now * A.c;
-                const float by = relative[nb] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(relative[nb] - then);
-                most[nb] = now, relative[nb] = then, sum[nb] *= by;
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db) o[nb][db] *= by;
-            }
-            const float base = relative[nb] == -INFINITY ? 0.0f : relative[nb];
-            float e[16], add = 0;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                e[r] = __builtin_amdgcn_exp2f(fmaf(s[nb][r], A.c, -base));
-                add += e[r];
-            }
-            sum[nb] += add;
-            if constexpr (F::I8) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    e[r] *= value_scale[r / 4][r % 4];
-                    if (MASKED && !(window[nb] >> (8 * (r / 4) + 4 * half + r % 4) & 1)) e[r] = 0;     // its scale may be a NaN
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[nb][i / 4][i % 4] = pack<DT>(e[2 * i], e[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) {
+            const bool low = (w[i] & INF) == INF, high = (w[i] & INF << 16) == INF << 16;
+            w[i] = high ? w[i] & 0xFFFFu : w[i];
+            w[i] = low ? w[i] & 0xFFFF0000u : w[i];
+            wild = wild || low || high;
         }
-        // V^T, keys in the order of the registers: four from 4 half on, four from 8 + 4 half on
-        const int in = lane & 15, right = lane >> 4 & 1;
-        auto columns = [&](int db, int st) {
-            v2u two[2];
+    };
+    auto add_values = [&](const char *v, const v4u (&p)[2], bool masked) INLINE {
+        v4u w[DP / 32][2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int row = 8 * i + 4 * half + (in >> 2), unit = (4 * db + 2 * right + (in >> 1 & 1)) ^ order<UNITS>(row);
-                two[i] = read_columns16(v + (16 * st + row) * ROW + unit * 16 + (in & 1) * 8);
-            }
-            return v4u{two[0].x, two[0].y, two[1].x, two[1].y};
-        };
-        // 0 times an infinity or a NaN in a masked place would be a NaN: where there are any they are left out of the products, and what they
-        // make of the sums is put in behind, by which kinds of them a row attends to
-        constexpr u32 INF = DT == VI_BF16 ? 0x7F80u : 0x7C00u, ONE = DT == VI_BF16 ? 0x3F80u : 0x3C00u;
-        auto is_wild = [&](u32 b) { return (b & INF) == INF; };
-        bool wild = false;
-        if constexpr (MASKED && !F::I8) {
-#pragma unroll 1
-            for (int u = half; u < UNITS; u += 2) {
-                const v4u w = *(const v4u *)(v + (lane & 31) * ROW + u * 16);
+        for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) wild |= is_wild(w[i]) || is_wild(w[i] >> 16);
+            for (int st = 0; st < 2; ++st) w[db][st] = columns(v, db, st);
+        if constexpr (!F::I8) {
+            if (masked) {
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) tame(w[db][st]);
             }
-            wild = __any(wild);
         }
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                v4u w;
-                if constexpr (F::I8) {
-                    const int row = (in >> 3) * 8 + 4 * half + (in >> 1 & 3), unit = (2 * db + right) ^ order<UNITS>(row);
-                    w = widen(read_columns8(v + (16 * st + row) * ROW + unit * 16 + (in & 1) * 8));
-                } else {
-                    w = columns(db, st);
-                    if (MASKED && wild)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] &= (is_wild(w[i] & 0xFFFFu) ? 0 : 0xFFFFu) | (is_wild(w[i] >> 16) ? 0 : 0xFFFF0000u);
-                }
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) o[nb][db] = multiply<DT>(w, p[nb][st], o[nb][db]);
+                if constexpr (NARROW) o[db] = multiply<DT>(widen(v2u{w[db][st].x, w[db][st].y}), p[st], o[db]);
+                else o[db] = multiply<DT>(w[db][st], p[st], o[db]);
             }
-        if constexpr (MASKED && !F::I8) {
-            if (!wild) return;
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                v4u counts[2];                 // ones at the keys that the row attends to
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const u32 bits = window[nb] >> (8 * (2 * i / 4) + 4 * half + 2 * i % 4);
-                    counts[i / 4][i % 4] = (bits & 1 ? ONE : 0) | (bits & 2 ? ONE : 0) << 16;
-                }
-#pragma unroll
-                for (int db = 0; db < DP / 32; ++db) {
-                    const v4u w[2] = {columns(db, 0), columns(db, 1)};
-                    v16f more = {};
-#pragma unroll
-                    for (int kind = 0; kind < 3; ++kind) {             // +inf, -inf, NaN: inf - inf is a NaN too
-                        v16f n = {};
-#pragma unroll
-                        for (int st = 0; st < 2; ++st) {
-                            auto one = [&](u32 b) { return (kind == 0 ? b == INF : kind == 1 ? b == (INF | 0x8000u) : (b & 0x7FFFu) > INF) ? ONE : 0; };
-                            v4u ones;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) ones[i] = one(w[st][i] & 0xFFFFu) | one(w[st][i] >> 16) << 16;
-                            n = multiply<DT>(ones, counts[st], n);
-                        }
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (n[r] > 0) more[r] += kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __uint_as_float(0x7FC00000u);
-                    }
-                    o[nb][db] += more;
-                }
-            }
-        }
     };
 
+    if constexpr (WM == 1) {
+        // A wavefront's own keys: each half of its stage is asked for anew as soon as it has been used, under the work on the other half.
+        Pages now = {}, next = {};
+        bool now_whole = false;
+        if (stages) {
+            now = look_up(0);
+            now_whole = whole(now, stage_key(0));
+            fetch(0, place_of(0, 0), stage_key(0), now, now_whole);
+            fetch(1, place_of(1, 0), stage_key(0), now, now_whole);
+        }
+        if (stages > 1) next = look_up(1);
+        const char *k = lds + part * F::STAGE, *v = k + F::HALF;
 #pragma unroll 1
-    for (int it = 0; it < min(F::ST - 1, stages); ++it) fetch(it);
-#pragma unroll 1
-    for (int it = 0; it < stages; ++it) {
-        // this stage's loads have arrived; those of the ones behind it may be on their way, where each has all its loads
-        const u32 behind = partial & ~(1u << it % F::ST) & ~(1u << (it + F::ST - 1) % F::ST);
-        if (F::ST == 2 || behind || it + F::ST - 2 >= stages) arrive<0>();
-        else arrive<(F::ST - 2) * F::MINE>();
-        if (WM > 1) meet_group();
-        else meet_wave();
-        if (it + F::ST - 1 < stages) fetch(it + F::ST - 1);
-        const char *stage = lds + (part * F::ST + it % F::ST) * F::STAGE;
-#pragma unroll 1
-        for (int kb = 0; kb < F::KBS; ++kb) {
+        for (int it = 0; it < stages; ++it) {
+            const int j = stage_key(it);
+            const bool more = it + 1 < stages, next_whole = more && whole(next, stage_key(it + 1)), needed = j < wave_end;
+            if (now_whole) arrive<LOADS_OF_HALF>();
+            else arrive<0>();
+            meet_wave();
+            v16f s = {};
+            if (needed) s = scores(k, k + F::KEYS * ROW);
+            if (more) {
+                read();
+                meet_wave();
+                fetch(0, place_of(0, 0), stage_key(it + 1), next, next_whole);
+            }
+            const int low = now_whole ? 16 : valid_of(now.number[0], j), high = now_whole ? 16 : valid_of(number_of(now, 1), j + 16);
+            const bool masked = low < 16 || high < 16 || j + 32 > wave_free;
+            if (next_whole) arrive<LOADS_OF_HALF>();
+            else arrive<0>();
+            meet_wave();
+            if (needed) {
+                v4u p[2];
+                settle(s, masked, masked ? window_of(j, low, high) : ~0u);
+                weights(s, v + F::KEYS * ROW, p);
+                add_values(v, p, masked);
+            }
+            if (more) {
+                read();
+                meet_wave();
+                fetch(1, place_of(1, 0), stage_key(it + 1), next, next_whole);
+                now = next, now_whole = next_whole;
+                if (it + 2 < stages) next = look_up(it + 2);
+            }
+        }
+    } else {
+        // Keys that WM wavefronts share, a stage of 64 in two steps of 32.  The scores of a step's keys are taken in the step before, under the exponentials there:
+        // the second step of a stage is the last that reads the stage's values and the first that reads the next one's keys, so that the values of stage
+        // it + 1 are asked for in the first step of stage it, and the keys of stage it + 2 in the second; both have two steps to come.
+        auto key_rows = [&](int it, int kb) INLINE { return lds + place_of(0, it % 2) + kb * 32 * ROW; };
+        auto key_scales = [&](int it, int kb) INLINE { return lds + place_of(0, it % 2) + F::KEYS * ROW + kb * 128; };
+        // 8-bit integers are widened on their way, from registers; a thread has units of sixteen columns
+        constexpr int EIGHTS = DP / 16, MINE8 = F::KEYS * EIGHTS / (64 * WM);
+        const int unit8 = wm * 64 + lane;
+        struct Raw {
+            v4u w[MINE8];
+            float scale;
+        };
+        auto load_wide = [&](int h, int it, const Pages &p) INLINE {
+            Raw r;
+            const int j = stage_key(it);
+            auto address = [&](int key, int *valid) INLINE {
+                int number = number_of(p, 0);
+#pragma unroll
+                for (int g = 1; g < F::GROUPS; ++g) number = key >> 4 == g ? number_of(p, g) : number;
+                *valid = valid_of(number, j + (key & ~15)) > (key & 15) ? number : -1;
+            };
+#pragma unroll
+            for (int l = 0; l < MINE8; ++l) {
+                const int n = l * 64 * WM + unit8, key = n / EIGHTS, u = n % EIGHTS;
+                int number;
+                address(key, &number);
+                r.w[l] = v4u{0, 0, 0, 0};
+                if (number >= 0 && u * 16 < A.cache.dim) r.w[l] = *(const v4u *)(from[h] + (u64)(u32)number * page_apart[h] + (u32)((j + key) & row_mask) * row_apart[h] + u * 16);
+            }
+            r.scale = 0;
+            if (unit8 < F::KEYS) {
+                int number;
+                address(unit8, &number);
+                if (number >= 0) r.scale = scales_from[h][number * A.cache.half[h].scale_page + ((j + unit8) & row_mask)];
+            }
+            return r;
+        };
+        auto store_wide = [&](int h, int it, const Raw &r) INLINE {
+            char *to = lds + place_of(h, it % 2);
+#pragma unroll
+            for (int l = 0; l < MINE8; ++l) {
+                const int n = l * 64 * WM + unit8, key = n / EIGHTS, u = n % EIGHTS, o_ = order<UNITS>(key & 15);
+                *(v4u *)(to + key * ROW + ((2 * u) ^ o_) * 16) = widen(v2u{r.w[l].x, r.w[l].y});
+                *(v4u *)(to + key * ROW + ((2 * u + 1) ^ o_) * 16) = widen(v2u{r.w[l].z, r.w[l].w});
+            }
+            if (unit8 < F::KEYS) *(float *)(to + F::KEYS * ROW + unit8 * 4) = r.scale;
+        };
+        Raw raw_keys = {}, raw_values = {};
+        v16f s = {};
+        Pages next = {}, behind = {};          // of stages it + 1 and it + 2
+        bool all = false, next_all = false;    // whether stages it and it + 1 are whole
+        if (stages) {
+            const Pages now = look_up(0);
+            all = whole(now, stage_key(0));
+            if (stages > 1) next = look_up(1);
+            next_all = stages > 1 && whole(next, stage_key(1));
+            if (stages > 2) behind = look_up(2);
+            if constexpr (F::WIDE) {
+                store_wide(0, 0, load_wide(0, 0, now));
+                store_wide(1, 0, load_wide(1, 0, now));
+                if (stages > 1) store_wide(0, 1, load_wide(0, 1, next)), raw_values = load_wide(1, 1, next);
+                if (stages > 2) raw_keys = load_wide(0, 2, behind);
+                read();
+            } else {
+                fetch(0, place_of(0, 0), stage_key(0), now, all);
+                fetch(1, place_of(1, 0), stage_key(0), now, all);
+                if (stages > 1) fetch(0, place_of(0, 1), stage_key(1), next, next_all);
+                arrive<0>();
+            }
+            meet_group();
+            s = scores(key_rows(0, 0), key_scales(0, 0));
+        }
+        auto step = [&](int it, int kb, const char *k, const char *scales) INLINE {
             const int j = stage_key(it) + 32 * kb;
-            if (j >= wave_end) break;
-            const int low = page_of(j).valid, high = page_of(j + 16).valid;
-            if (low == 16 && high == 16 && j + 32 <= wave_free) block(stage, kb, j, low, high, std::false_type());
-            else block(stage, kb, j, low, high, std::true_type());
+            if (j >= wave_end) return;
+            int low = 16, high = 16;
+            if (!all) {
+                const Pages p = look_up(it);
+                low = valid_of(number_of(p, 2 * kb), j), high = valid_of(number_of(p, 2 * kb + 1), j + 16);
+            }
+            const bool masked = low < 16 || high < 16 || j + 32 > wave_free;
+            settle(s, masked, masked ? window_of(j, low, high) : ~0u);
+            const v16f ahead = scores(k, scales);      // behind the last stage: of what lies there, and not used
+            v4u p[2];
+            weights(s, lds + place_of(1, it % 2) + F::KEYS * ROW + kb * 128, p);
+            add_values(lds + place_of(1, it % 2) + kb * 32 * ROW, p, masked);
+            s = ahead;
+        };
+        auto arrived = [&]() INLINE {          // all but what was asked for in the step before, which is of stage it + 1
+            if constexpr (F::WIDE) {
+                read();
+            } else {
+                if (next_all) arrive<LOADS_OF_HALF>();
+                else arrive<0>();
+            }
+            meet_group();
+        };
+#pragma unroll 1
+        for (int it = 0; it < stages; ++it) {
+            arrived();
+            if (!F::WIDE && it + 1 < stages) fetch(1, place_of(1, (it + 1) % 2), stage_key(it + 1), next, next_all);
+            step(it, 0, key_rows(it, 1), key_scales(it, 1));
+            if constexpr (F::WIDE) {
+                if (it + 1 < stages) store_wide(1, it + 1, raw_values);
+                if (it + 2 < stages) raw_values = load_wide(1, it + 2, behind);
+            }
+            arrived();
+            const bool behind_all = it + 2 < stages && whole(behind, stage_key(it + 2));
+            if (!F::WIDE && it + 2 < stages) fetch(0, place_of(0, it % 2), stage_key(it + 2), behind, behind_all);
+            next = behind;
+            if (it + 3 < stages) behind = look_up(it + 3);
+            step(it, 1, key_rows(it + 1, 0), key_scales(it + 1, 0));
+            if constexpr (F::WIDE) {
+                if (it + 2 < stages) store_wide(0, it + 2, raw_keys);
+                if (it + 3 < stages) raw_keys = load_wide(0, it + 3, behind);
+            }
+            all = next_all, next_all = behind_all;
+        }
+    }
+
+    // ---- the values that were left out, of the keys that some row of the wavefront does not attend to, by those that do
+    if constexpr (!F::I8) {
+        if (__any(wild)) {
+#pragma unroll 1
+            for (int j = first_key; j < min(first_key + stages * WK * F::KEYS, wave_end); ++j) {
+                const int number = pages[j >> A.cache.shift], block = j & ~31;
+                if (block + 32 <= min(wave_free, end) && valid_of(pages[block >> A.cache.shift], block) == 16 && valid_of(pages[(block + 16) >> A.cache.shift], block + 16) == 16) continue;
+                if (WK > 1 && (block - first_key) / F::KEYS % WK != part) continue;
+                if (valid_of(number, j & ~15) <= (j & 15)) continue;
+                if (!there || !(window_of(j, 16, 16) & 1)) continue;
+                const T *x = (const T *)(from[1] + (u64)(u32)number * page_apart[1] + (u32)(j & row_mask) * row_apart[1]);
+#pragma unroll
+                for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int col = 32 * db + bit_of(r);
+                        const float f = col < A.cache.dim ? (float)x[col] : 0.0f;
+                        if (!(fabsf(f) < INFINITY)) o[db][r] += f;
+                    }
+            }
         }
     }
 
     // ---- the WK groups' sums as one, and out
     arrive<0>();
     __syncthreads();
-    float *buf = (float *)lds, *of_waves = buf + F::WAVES * NB * 32 * F::PITCH, *of_rows = of_waves + F::WAVES * NB * 32 * 2;
-    float factor[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum[nb]), __float_as_uint(sum[nb]), false, false);
-        sum[nb] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-        if (half == 0) {
-            of_waves[((wave * NB + nb) * 32 + lane) * 2] = relative[nb];
-            of_waves[((wave * NB + nb) * 32 + lane) * 2 + 1] = sum[nb];
-        }
+    float *buf = (float *)lds, *of_waves = buf + F::WAVES * 32 * F::PITCH, *of_rows = of_waves + F::WAVES * 32 * 2;
+    {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
+        sum = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        if (half == 0) of_waves[(wave * 32 + lane) * 2] = relative, of_waves[(wave * 32 + lane) * 2 + 1] = sum;
     }
     __syncthreads();
+    float top = -INFINITY, total = 0;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        float top = -INFINITY, total = 0;
+    for (int w = 0; w < WK; ++w) top = fmaxf(top, of_waves[((w * WM + wm) * 32 + (lane & 31)) * 2]);
+    const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-        for (int w = 0; w < WK; ++w) top = fmaxf(top, of_waves[(((w * WM + wm) * NB + nb) * 32 + (lane & 31)) * 2]);
-        const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int w = 0; w < WK; ++w) {
-            const float *x = of_waves + (((w * WM + wm) * NB + nb) * 32 + (lane & 31)) * 2;
-            total += __builtin_amdgcn_exp2f(x[0] - base) * x[1];
-        }
-        factor[nb] = __builtin_amdgcn_exp2f(relative[nb] - base);
-        if (part == 0 && half == 0) {
-            of_rows[((wm * NB + nb) * 32 + lane) * 2] = top;
-            of_rows[((wm * NB + nb) * 32 + lane) * 2 + 1] = total;
-        }
+    for (int w = 0; w < WK; ++w) {
+        const float *x = of_waves + ((w * WM + wm) * 32 + (lane & 31)) * 2;
+        total += __builtin_amdgcn_exp2f(x[0] - base) * x[1];
     }
+    const float factor = __builtin_amdgcn_exp2f(relative - base);
+    if (part == 0 && half == 0) of_rows[(wm * 32 + lane) * 2] = top, of_rows[(wm * 32 + lane) * 2 + 1] = total;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) {
         if (db) __syncthreads();
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const v4f x = {o[nb][db][4 * g] * factor[nb], o[nb][db][4 * g + 1] * factor[nb], o[nb][db][4 * g + 2] * factor[nb], o[nb][db][4 * g + 3] * factor[nb]};
-                *(v4f *)(buf + ((wave * NB + nb) * 32 + (lane & 31)) * F::PITCH + 8 * g + 4 * half) = x;
-            }
+        for (int g = 0; g < 4; ++g) {
+            const v4f x = {o[db][4 * g] * factor, o[db][4 * g + 1] * factor, o[db][4 * g + 2] * factor, o[db][4 * g + 3] * factor};
+            *(v4f *)(buf + (wave * 32 + (lane & 31)) * F::PITCH + 8 * g + 4 * half) = x;
+        }
         __syncthreads();
         for (int i = threadIdx.x; i < F::ROWS * 8; i += F::THREADS) {
-            const int r = i / 8, col = 32 * db + i % 8 * 4, row = t.first + r, tok = token(row), g = row - tok * A.group;
-            if (tok >= t.n || col >= A.cache.dim) continue;
+            const int r = i / 8, col = 32 * db + i % 8 * 4, its = t.first + r, of = token(its);
+            if (of >= t.n || col >= A.cache.dim) continue;
             v4f x = *(const v4f *)(buf + r * F::PITCH + i % 8 * 4);
 #pragma unroll
             for (int w = 1; w < WK; ++w) x += *(const v4f *)(buf + (w * F::ROWS + r) * F::PITCH + i % 8 * 4);
-            if (A.splits > 1) {
+            if (parts > 1) {
                 *(v4f *)(A.part + (slot * F::ROWS + r) * DP + col) = x;
             } else {
-                const float total = of_rows[r * 2 + 1], per = total == 0.0f ? 0.0f : 1.0f / total;
+                const float all = of_rows[r * 2 + 1], per = all == 0.0f ? 0.0f : 1.0f / all;
                 const v2u two = {pack<DT>(x.x * per, x.y * per), pack<DT>(x.z * per, x.w * per)};
-                store_any((T *)A.out + (t.s0 + tok) * A.out_token + (head * A.group + g) * A.out_head + col, two);
+                store_any((T *)A.out + ((i64)t.s0 + of) * A.out_token + (head * A.group + its - of * A.group) * A.out_head + col, two);
             }
         }
     }
-    if (A.splits > 1)
+    if (parts > 1)
         for (int r = threadIdx.x; r < F::ROWS; r += F::THREADS) {
             A.most[(slot * F::ROWS + r) * 2] = of_rows[r * 2];
             A.most[(slot * F::ROWS + r) * 2 + 1] = of_rows[r * 2 + 1];
@@ -580,42 +734,39 @@ __global__ __launch_bounds__(JOIN) void k_join(Args A) {
     Tile t;
     if (!find_tile<ROWS>(A, tile, &t)) return;
     const i64 slot = ((i64)tile * heads + head) * A.splits;
+    const int parts = parts_of(A, t.end);
+    if (parts <= 1) return;                    // the only one is done
     for (int i = (int)blockIdx.y * JOIN + (int)threadIdx.x; i < ROWS * (DP / 4); i += (int)gridDim.y * JOIN) {
         const int r = i / (DP / 4), col = i % (DP / 4) * 4, row = t.first + r, tok = (int)((u32)row / (u32)A.group), g = row - tok * A.group;
         if (tok >= t.n || col >= A.cache.dim) continue;
         const float *most = A.most + (slot * ROWS + r) * 2, *part = A.part + (slot * ROWS + r) * DP + col;
         float top = -INFINITY, total = 0;
-        for (int s = 0; s < A.splits; ++s) top = fmaxf(top, most[(i64)s * ROWS * 2]);
+        for (int s = 0; s < parts; ++s) top = fmaxf(top, most[(i64)s * ROWS * 2]);
         const float base = top == -INFINITY ? 0.0f : top;
         v4f x = {0, 0, 0, 0};
 #pragma unroll 4
-        for (int s = 0; s < A.splits; ++s) {
+        for (int s = 0; s < parts; ++s) {
             const float its = most[(i64)s * ROWS * 2], of = most[(i64)s * ROWS * 2 + 1], by = __builtin_amdgcn_exp2f(its - base);
-            if (its == -INFINITY && of == 0.0f) continue;              // no keys: nothing was written
             total += by * of;
             x += by * *(const v4f *)(part + (i64)s * ROWS * DP);
         }
         const float per = total == 0.0f ? 0.0f : 1.0f / total;
         const v2u two = {pack<DT>(x.x * per, x.y * per), pack<DT>(x.z * per, x.w * per)};
-        store_any((T *)A.out + (t.s0 + tok) * A.out_token + (head * A.group + g) * A.out_head + col, two);
+        store_any((T *)A.out + ((i64)t.s0 + tok) * A.out_token + (head * A.group + g) * A.out_head + col, two);
     }
 }
 
 // ---- forms --------------------------------------------------------------------------------------------------------
 // Up to 32 rows of a sequence: four wavefronts (two where columns are many) with keys of their own; up to 64: the same, two products of each operand of
 // keys or values; more: four wavefronts' rows share the keys.
-constexpr int key_groups(bool i8, int dp) { return dp > 128 && !i8 ? 2 : 4; }
-constexpr int stages_of(bool i8, int dp) { return dp <= 128 && (i8 || dp == 64) ? 4 : 2; }
 template <int DT, bool I8, int DP>
-struct Few : Form<DT, I8, DP, 1, 1, key_groups(I8, DP), 1, stages_of(I8, DP), 1> {};
+struct Few : Form<DT, I8, DP, 1, 4, (DP > 128 ? 1 : 2)> {};
 template <int DT, bool I8, int DP>
-struct Some : Form<DT, I8, DP, 2, 1, key_groups(I8, DP), 1, stages_of(I8, DP), 1> {};
-template <int DT, bool I8, int DP>
-struct Many : Form<DT, I8, DP, 1, 4, 1, (DP > 128 ? 1 : 2), 2, (DP > 128 ? 1 : 2)> {};
+struct Many : Form<DT, I8, DP, 4, 1, (DP > 128 ? 1 : 2)> {};
 
-enum { FEW, SOME, MANY };
+enum { FEW, MANY };
 struct Plan {
-    int form, rows, dp, tiles, splits;
+    int form, rows, dp, tiles, splits, per_split;
     size_t ws_bytes;
 };
 constexpr int CUS = 256;                       // of a whole card; on a part of one the choice of splits costs time, nothing else
@@ -624,17 +775,23 @@ Plan make_plan(int cache_dtype, i64 dim, i64 cache_heads, i64 n, i64 heads, i64 
     Plan L = {};
     const i64 group = heads / cache_heads, rows = (n * group + sequences - 1) / sequences;           // of a sequence, on an average
     L.dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
-    L.form = rows <= 32 ? FEW : rows <= 64 && L.dp <= 128 ? SOME : MANY;
-    L.rows = L.form == FEW ? 32 : L.form == SOME ? 64 : 128;
-    const i64 tiles = n * group / L.rows + sequences, busy = (n * group + L.rows - 1) / L.rows > sequences ? (n * group + L.rows - 1) / L.rows : sequences;
+    // A tile of 128 rows reads its keys once, but its wavefronts wait for each other: 64 sequences of 64 rows over 4096 entries take 239 us as two tiles of
+    // 32, 308 as one of 64 whose wavefronts share the keys; 16 of 100 rows 91 us as four tiles, 82 as one of 128, but over 8-bit integers, which are
+    // widened on a longer way there, 98 and 103.
+    L.form = rows <= (cache_dtype == VI_I8 ? 128 : 64) ? FEW : MANY;
+    L.rows = L.form == FEW ? 32 : 128;
+    const i64 tiles = n * group / L.rows + sequences, full = (n * group + L.rows - 1) / L.rows, busy = full > sequences ? full : sequences;
     L.tiles = (int)(tiles < MAX_BLOCKS ? tiles : MAX_BLOCKS);
-    // as many parts of the keys as make two workgroups a CU, of 512 keys at least
-    i64 splits = 2 * CUS / (busy * cache_heads), most = longest / 512;
-    splits = splits < most ? splits : most;
-    splits = splits < 64 ? splits : 64;
-    L.splits = (int)(splits > 1 ? splits : 1);
+    // The keys are cut into parts of one size where there are few tiles: two workgroups a CU, as many as there is room for (a sequence of 32768 entries,
+    // 8 heads: 54 us, 64 with four a CU), or four where sequences alone make two, for their lengths differ (attend_batch's 64 of 500 to 8192: 224 us, 237 uncut).  A
+    // part has 128 keys at least, a round of a workgroup's wavefronts, and 512 where there are many.
+    const i64 all = busy * cache_heads, wanted = (all < 2 * CUS ? 2 : 4) * CUS, parts = wanted / all, round = 128, least = all >= CUS ? 4 * round : round;
+    i64 keys = parts > 1 ? (longest + parts - 1) / parts : longest;
+    keys = keys < least ? least : keys;
+    keys = longest > keys * MAX_PARTS ? (longest + MAX_PARTS - 1) / MAX_PARTS : keys;
+    L.per_split = (int)((keys + round - 1) / round * round);
+    L.splits = (int)(longest > L.per_split ? (longest + L.per_split - 1) / L.per_split : 1);
     if (L.splits > 1) L.ws_bytes = (size_t)(tiles * cache_heads * L.splits * L.rows) * (L.dp + 2) * 4 + vi::WS_SLACK;
-    (void)cache_dtype;
     return L;
 }
 
@@ -650,8 +807,6 @@ void launch(const Args &A, hipStream_t s) {
 template <int DT, bool I8, int DP>
 void launch_form(int form, const Args &A, hipStream_t s) {
     if (form == FEW) return launch<Few<DT, I8, DP>>(A, s);
-    if constexpr (DP <= 128)
-        if (form == SOME) return launch<Some<DT, I8, DP>>(A, s);
     launch<Many<DT, I8, DP>>(A, s);
 }
 template <int DT, bool I8>
@@ -692,7 +847,7 @@ extern "C" int vi_attend_cache(const vi_cache *cache, const vi_batch *batch, int
     if (cache->heads * (i64)L.tiles * L.splits > MAX_BLOCKS) return vi::fail(VI_EINVAL, "%s: %lld tokens of %lld sequences", who, (long long)n, (long long)sequences);
     if (ws_bytes < L.ws_bytes || (L.ws_bytes && !ws)) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, L.ws_bytes);
     A.q = q, A.out = out, A.q_token = q_token, A.q_head = q_head, A.out_token = out_token, A.out_head = out_head, A.n = n, A.parents = parents;
-    A.heads = (int)heads, A.group = (int)(heads / cache->heads), A.tiles = L.tiles, A.splits = L.splits, A.clear = clear != 0, A.c = scale * 1.44269504f;
+    A.heads = (int)heads, A.group = (int)(heads / cache->heads), A.tiles = L.tiles, A.splits = L.splits, A.per_split = L.per_split, A.clear = clear != 0, A.c = scale * 1.44269504f;
     if (L.splits > 1) {
         A.part = (float *)vi::align16(ws);
         A.most = A.part + (i64)L.tiles * cache->heads * L.splits * L.rows * L.dp;

@@ -65,7 +65,9 @@ inline int take(const char *who, const vi_cache *c, const vi_batch *b, Cache *to
         const int64_t *s = h ? c->value_strides : c->key_strides, *e = h ? c->value_scale_strides : c->key_scale_strides;
         const uintptr_t at = (uintptr_t)(h ? c->values : c->keys);
         if ((at | s[0] * size | s[1] * size | s[2] * size) & 15) return vi::fail(VI_EINVAL, "%s: a cache whose entries do not start at multiples of 16 bytes", who);
-        if (s[0] < 0 || s[1] < 0 || s[2] < 0 || s[2] > (1 << 24)) return vi::fail(VI_EINVAL, "%s: a cache of entries %lld apart", who, (long long)s[2]);
+        // an entry's place in its page is taken in 32 bits
+        if (s[0] < 0 || s[1] < 0 || s[2] < 0 || s[2] > (1 << 20) || s[0] * size >= (1ll << 32))
+            return vi::fail(VI_EINVAL, "%s: a cache of pages %lld, entries %lld apart", who, (long long)s[0], (long long)s[2]);
         to->half[h] = {(char *)at, h ? c->value_scales : c->key_scales, s[0] * size, s[1] * size, s[2] * size, e[0], e[1]};
     }
     to->pages = c->pages, to->heads = c->heads, to->shift = vi::ilog2(c->page_size), to->mask = (int)c->page_size - 1;
