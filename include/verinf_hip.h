@@ -466,7 +466,7 @@ int vi_attend_cache(const vi_cache *cache, const vi_batch *batch, int dtype, con
  * uniforms[root] sum(R); where nothing is left of R, R = p; -1 where a row has a NaN or +inf or only -inf (no draft below it is accepted).
  * counts (sequences): accepted drafts; nodes (sequences, depth): their numbers, -1 behind; out (sequences, depth + 1): their tokens, the one behind, -1.
  * ws: vi_verify_drafts_workspace_bytes() bytes of device scratch. */
-size_t vi_verify_drafts_workspace_bytes(int dtype, int64_t n, int64_t v, int drafted);
+size_t vi_verify_drafts_workspace_bytes(int dtype, int64_t n, int64_t v, int64_t sequences, int drafted);
 int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_t v, int64_t ld, const void *draft, int64_t ld_draft, const int64_t *tokens,
                      const int32_t *starts, int64_t sequences, const int32_t *parents, const double *uniforms, double temperature, int64_t depth,
                      int64_t *counts, int64_t *nodes, int64_t *out, void *ws, size_t ws_bytes, void *stream);

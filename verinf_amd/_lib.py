@@ -181,7 +181,7 @@ def lib():
     L.vi_attend_cache_workspace_bytes.argtypes = [c_int, i64, i64, i64, i64, i64, i64]
     L.vi_attend_cache.argtypes = [cache, batch, c_int, vp, i64, i64, i64, i64, vp, c_float, i64, c_int, vp, i64, i64, vp, sz, vp]
     L.vi_verify_drafts_workspace_bytes.restype = sz
-    L.vi_verify_drafts_workspace_bytes.argtypes = [c_int, i64, i64, c_int]
+    L.vi_verify_drafts_workspace_bytes.argtypes = [c_int, i64, i64, i64, c_int]
     L.vi_verify_drafts.argtypes = [c_int, vp, i64, i64, i64, vp, i64, vp, vp, i64, vp, vp, c_double, i64, vp, vp, vp, vp, sz, vp]
     L.vi_keep_drafts.argtypes = [cache, batch, vp, i64, vp, vp, vp]
     for name in ("vi_rotate_heads", "vi_append_tokens", "vi_attend_cache", "vi_verify_drafts", "vi_keep_drafts"):

@@ -10,10 +10,11 @@
 // the refused tokens and is otherwise p.
 //
 // Whole numbers come of it, decided by comparisons next to borders, of which the last token's have as many as there are tokens: all in 64
-// bits, exponentials too (the series of 2^f to the 12th power, 2e-16).
+// bits, exponentials too (the series of 2^f to the 11th power, 6e-15).
 //
-// Two launches: largest entry and sum of every row, in slices (k_stats), then a workgroup a sequence for the walk (k_walk).  What bounds them: reading the
-// logits, and 17 operations in 64 bits an exponential beside it.
+// All rows' largest entries and sums, in slices (k_stats), and the sums behind a first refusal, for nodes with other children (k_first), are taken by the whole
+// chip; a workgroup a sequence walks (k_walk), with a pass over two rows for each further refusal; the whole chip adds up what is left behind the paths
+// (k_left), and a workgroup a sequence looks for the token (k_pick).  What bounds them: reading the logits, and 18 operations in 64 bits an exponential beside it.
 #include "cache.hpp"
 
 namespace {
@@ -25,7 +26,6 @@ constexpr i64 MAX_V = 1 << 20;
 constexpr i64 MAX_BLOCKS = 1 << 23;            // of a launch, which has less than 2^32 threads
 constexpr int MAX_NODES = 1024, MAX_DEPTH = 256;
 constexpr int EIGHT = 8;                       // neighbouring entries of a thread
-constexpr int MAX_SEGMENTS = (int)(MAX_V / (64 * EIGHT));               // of a row: a wavefront's entries
 
 struct Part {                                  // of a slice: its largest entry (NaN: it has a NaN or +inf), sum of 2^((x - most) c)
     double z;
@@ -35,17 +35,31 @@ struct Row {                                   // of a row: the most c that its 
     double mc, per_z;
 };
 
-// 2^t, 0 from -1100 on
-__device__ __forceinline__ double exp2_64(double t) {
-    t = fmax(t, -1100.0);
-    const double n = rint(t), f = t - n;
-    constexpr double C[] = {2.5678435993488206e-11, 4.4455382718708116e-10, 7.0549116208011233e-9,  1.0178086009239700e-7, 1.3215486790144310e-6,
-                            1.5252733804059841e-5,  1.5403530393381610e-4,  1.3333558146428443e-3, 9.6181291076284772e-3, 5.5504108664821580e-2,
-                            2.4022650695910071e-1,  6.9314718055994531e-1,  1.0};
-    double p = C[0];
+// 2^t of N numbers side by side (one alone waits for itself at each step), t up to 0 or hardly above, 2^-1000 from there on: the whole part by an addition
+// whose result has units of one, and into the exponent
+template <int N>
+__device__ __forceinline__ void exp2_64(double (&t)[N]) {
+    constexpr double C[] = {4.4455382718708116e-10, 7.0549116208011233e-9,  1.0178086009239700e-7, 1.3215486790144310e-6, 1.5252733804059841e-5, 1.5403530393381610e-4,
+                            1.3333558146428443e-3,  9.6181291076284772e-3,  5.5504108664821580e-2, 2.4022650695910071e-1, 6.9314718055994531e-1, 1.0};
+    double m[N], f[N], p[N];
 #pragma unroll
-    for (int i = 1; i < 13; ++i) p = fma(p, f, C[i]);
-    return ldexp(p, (int)n);
+    for (int e = 0; e < N; ++e) {
+        t[e] = fmax(t[e], -1000.0);
+        m[e] = t[e] + 6755399441055744.0;
+        f[e] = t[e] - (m[e] - 6755399441055744.0);
+        p[e] = C[0];
+    }
+#pragma unroll
+    for (int i = 1; i < 12; ++i)
+#pragma unroll
+        for (int e = 0; e < N; ++e) p[e] = fma(p[e], f[e], C[i]);
+#pragma unroll
+    for (int e = 0; e < N; ++e) t[e] = __builtin_bit_cast(double, __builtin_bit_cast(u64, p[e]) + (__builtin_bit_cast(u64, m[e]) << 52));
+}
+__device__ __forceinline__ double exp2_64(double t) {
+    double one[1] = {t};
+    exp2_64(one);
+    return one[0];
 }
 
 template <int DT>
@@ -69,17 +83,62 @@ __device__ __forceinline__ Entries<DT> eight(const typename type<DT>::t *x, i64 
     return r;
 }
 
-struct Stats {
+// e^(x - most) of eight entries, in 64 bits
+template <int DT>
+__device__ __forceinline__ void exponentials(const Entries<DT> &v, double c, double mc, double (&r)[EIGHT]) {
+#pragma unroll
+    for (int h = 0; h < EIGHT; h += 4) {
+        double t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = fma((double)entry<DT>(v, h + e), c, -mc);
+        exp2_64(t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r[h + e] = t[e];
+    }
+}
+
+struct Job {
     const void *x[2];                          // the target's logits, the draft's
     i64 ld[2], n, v;
-    int slices;
+    int slices, firsts, sequences, depth, drafted;
     double c;                                  // log2(e) / temperature
     Part *parts;                               // [2 n][slices]
+    double *first;                             // [n][firsts]: the sum of max(p - q, 0) of a slice
+    Row *rows;                                 // [2 n]
+    struct End *ends;                          // [sequences]
+    double *segments;                          // [sequences][segments of a row]
+    const i64 *tokens;
+    const int *starts, *parents;
+    const double *uniforms;
+    i64 *counts, *nodes, *out;
 };
+
+// How many children the node of a row has, two at most, by a wavefront that asks for one row
+__device__ __forceinline__ int children(const Job &A, i64 row) {
+    int found = -1;
+    i64 s0 = 0, s1 = 0;
+    for (int first = 0; first < A.sequences; first += 64) {
+        const int b = min(first + (int)(threadIdx.x & 63), A.sequences - 1);
+        const i64 start = A.starts[b], next = A.starts[b + 1];
+        const int count = __popcll(__ballot(first + (int)(threadIdx.x & 63) < A.sequences && start <= row));
+        if (count == 0) break;
+        found = first + count - 1;
+        s0 = __shfl((int)start, count - 1), s1 = __shfl((int)next, count - 1);
+    }
+    s0 = max(s0, (i64)0), s1 = min(s1, A.n);
+    if (found < 0 || row >= s1) return 0;
+    if (!A.parents) return row + 1 < s1;
+    int count = 0;
+    for (i64 j = row + 1; j < min(s1, s0 + MAX_NODES) && count < 2; j += 64) {
+        const i64 i = j + (threadIdx.x & 63);
+        count += __popcll(__ballot(i < min(s1, s0 + MAX_NODES) && s0 + A.parents[min(i, s1 - 1)] == row));
+    }
+    return min(count, 2);
+}
 
 // R times eight entries a thread
 template <int DT, int R>
-__global__ __launch_bounds__(BLOCK) void k_stats(Stats A) {
+__global__ __launch_bounds__(BLOCK) void k_stats(Job A) {
     typedef typename type<DT>::t T;
     __shared__ float most_of[BLOCK / 64];
     __shared__ double sum_of[BLOCK / 64];
@@ -87,6 +146,7 @@ __global__ __launch_bounds__(BLOCK) void k_stats(Stats A) {
     const int slice = (int)(blockIdx.x % A.slices), which = row >= A.n, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
     const T *x = (const T *)A.x[which] + (row - (which ? A.n : 0)) * A.ld[which];
     const i64 first = (i64)slice * (BLOCK * EIGHT * R);
+    if (which && children(A, row - A.n) == 0) return;                  // nobody asks
     Entries<DT> v[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) v[r] = eight<DT>(x, first + (r * BLOCK + (int)threadIdx.x) * EIGHT, A.v);
@@ -110,9 +170,12 @@ __global__ __launch_bounds__(BLOCK) void k_stats(Stats A) {
     if (most > -INFINITY && most < INFINITY) {
         const double mc = (double)most * A.c;
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int r = 0; r < R; ++r) {
+            double t[EIGHT];
+            exponentials<DT>(v[r], A.c, mc, t);
 #pragma unroll
-            for (int e = 0; e < EIGHT; ++e) z += exp2_64(fma((double)entry<DT>(v[r], e), A.c, -mc));
+            for (int e = 0; e < EIGHT; ++e) z += t[e];
+        }
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) z += __shfl_xor(z, d);
@@ -121,25 +184,34 @@ __global__ __launch_bounds__(BLOCK) void k_stats(Stats A) {
     if (threadIdx.x == 0) A.parts[blockIdx.x] = {(sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]), most == INFINITY ? __uint_as_float(0x7FC00000u) : most, 0.0f};
 }
 
-struct Walk {
-    const void *x[2];
-    i64 ld[2], n, v;
-    int slices, sequences, depth, drafted;
-    double c;
-    const Part *parts;
-    Row *rows;                                 // [2 n]
-    const i64 *tokens;
-    const int *starts, *parents;
-    const double *uniforms;
-    i64 *counts, *nodes, *out;
+struct End {                                   // where a path ends: its node's row (-1: no sequence), its number, what is left of its probabilities
+    double a;
+    i64 row;
+    int node, refused, count, pad;
 };
+struct Tree {                                  // -1: none, also of nodes that cannot be accepted
+    int parent[MAX_NODES], token[MAX_NODES];
+};
+// a sequence's nodes
+template <int THREADS>
+__device__ __forceinline__ int take_tree(const Job &A, int b, Tree &tree, i64 *first) {
+    const i64 s0 = max((i64)0, min((i64)A.starts[b], A.n)), s1 = max(s0, min((i64)A.starts[b + 1], A.n));
+    const int nodes = (int)min(s1 - s0, (i64)MAX_NODES);
+    for (int i = threadIdx.x; i < nodes; i += THREADS) {
+        const int parent = i ? A.parents ? A.parents[s0 + i] : i - 1 : -1;
+        const i64 token = A.tokens[s0 + i];
+        const bool fine = parent >= 0 && parent < i && token >= 0 && token < A.v;
+        tree.parent[i] = fine ? parent : -1;
+        tree.token[i] = fine ? (int)token : -1;
+    }
+    *first = s0;
+    return nodes;
+}
 
 struct Shared {
+    Tree tree;
     double have[MAX_NODES], said[MAX_NODES], u[MAX_NODES];             // p and q of a node's token behind its parent
-    int parent[MAX_NODES], token[MAX_NODES];                           // -1: none
-    double segment[MAX_SEGMENTS];
-    double total, rest;
-    int found;
+    double sums[WALK / 64];
 };
 
 // the sum of the wavefront's values up to this lane's
@@ -165,23 +237,25 @@ struct Left {
     Row p, q;
     double a, c;
     i64 v;
-    const Shared *sh;
+    const Tree *tree;
     int nodes, cur;                            // the refused are the children of cur (-1: none are)
 
     __device__ __forceinline__ void eight_at(i64 at, double (&r)[EIGHT]) const {
         const Entries<DT> e = eight<DT>(x, at, v);
+        exponentials<DT>(e, c, p.mc, r);
 #pragma unroll
-        for (int i = 0; i < EIGHT; ++i) r[i] = exp2_64(fma((double)entry<DT>(e, i), c, -p.mc)) * p.per_z;
+        for (int i = 0; i < EIGHT; ++i) r[i] = entry<DT>(e, i) > -INFINITY ? r[i] * p.per_z : 0.0;
         if (a > 0) {
-            const Entries<DT> f = eight<DT>(y, at, v);
             const double per = a * q.per_z;
+            double o[EIGHT];
+            exponentials<DT>(eight<DT>(y, at, v), c, q.mc, o);
 #pragma unroll
-            for (int i = 0; i < EIGHT; ++i) r[i] = fmax(r[i] - exp2_64(fma((double)entry<DT>(f, i), c, -q.mc)) * per, 0.0);
+            for (int i = 0; i < EIGHT; ++i) r[i] = fmax(r[i] - o[i] * per, 0.0);
         }
         if (cur >= 0) {
             for (int j = 1; j < nodes; ++j) {
-                const i64 place = sh->token[j] - at;
-                if (sh->parent[j] == cur && place >= 0 && place < EIGHT) {
+                const i64 place = tree->token[j] - at;
+                if (tree->parent[j] == cur && place >= 0 && place < EIGHT) {
 #pragma unroll
                     for (int i = 0; i < EIGHT; ++i)
                         if (place == i) r[i] = 0;
@@ -191,40 +265,28 @@ struct Left {
     }
 };
 
-// the sum of what is left, and of each segment of 64 times eight entries; for all threads
+__device__ __forceinline__ int segments_of(i64 v) { return (int)((v + 64 * EIGHT - 1) / (64 * EIGHT)); }
+// the sum of a segment, 64 times eight entries, by a wavefront
 template <int DT>
-__device__ double sum_left(Shared &sh, const Left<DT> &left) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64, segments = (int)((left.v + 64 * EIGHT - 1) / (64 * EIGHT));
-    __syncthreads();
-    for (int s = wave; s < segments; s += WALK / 64) {
-        double r[EIGHT], sum = 0;
-        left.eight_at((i64)(s * 64 + lane) * EIGHT, r);
+__device__ __forceinline__ double sum_segment(const Left<DT> &left, int segment) {
+    double r[EIGHT], sum = 0;
+    left.eight_at((i64)(segment * 64 + (int)(threadIdx.x & 63)) * EIGHT, r);
 #pragma unroll
-        for (int i = 0; i < EIGHT; ++i) sum += r[i];
+    for (int i = 0; i < EIGHT; ++i) sum += r[i];
 #pragma unroll
-        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-        if (lane == 0) sh.segment[s] = sum;
-    }
-    __syncthreads();
-    if (wave == 0) {
-        double sum = 0;
-        const int each = (segments + 63) / 64;
-        for (int s = lane * each; s < min(segments, (lane + 1) * each); ++s) sum += sh.segment[s];
-#pragma unroll
-        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-        if (lane == 0) sh.total = sum;
-    }
-    __syncthreads();
-    return sh.total;
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    return sum;
 }
 
-// the smallest j with R(0) + ... + R(j) > threshold, behind sum_left; by the first wavefront
+// the smallest j with R(0) + ... + R(j) > u sum(R); by a wavefront, from the sums of the segments
 template <int DT>
-__device__ int find_left(const Shared &sh, const Left<DT> &left, double threshold) {
-    const int lane = threadIdx.x & 63, segments = (int)((left.v + 64 * EIGHT - 1) / (64 * EIGHT)), each = (segments + 63) / 64;
+__device__ int find_left(const double *segment_sums, const Left<DT> &left, double u, double *total) {
+    const int lane = threadIdx.x & 63, segments = segments_of(left.v), each = (segments + 63) / 64;
     double own = 0;
-    for (int s = lane * each; s < min(segments, (lane + 1) * each); ++s) own += sh.segment[s];
+    for (int s = lane * each; s < min(segments, (lane + 1) * each); ++s) own += segment_sums[s];
     double sum = sum_up_to(own);
+    *total = __shfl(sum, 63);
+    const double threshold = u * *total;
     int at = first_above(sum, own, threshold);
     if (at < 0) return -1;
     double before = __shfl(sum, max(at - 1, 0));
@@ -232,11 +294,12 @@ __device__ int find_left(const Shared &sh, const Left<DT> &left, double threshol
     int segment = -1;
     double base = 0;                           // what lies in front of the segment
     for (int s = at * each; s < min(segments, (at + 1) * each); ++s) {               // the same for all lanes
-        if (sh.segment[s] > 0) {
+        const double here = segment_sums[s];
+        if (here > 0) {
             segment = s, base = before;
-            if (before + sh.segment[s] > threshold) break;
+            if (before + here > threshold) break;
         }
-        before += sh.segment[s];
+        before += here;
     }
     if (segment < 0) return -1;
     double r[EIGHT];
@@ -277,13 +340,40 @@ __device__ __forceinline__ Row join(const Part *parts, int slices, double c) {
     return {mc, 1.0 / z};
 }
 
+// The sum behind a first refusal, max(p - q, 0), where another child is tried behind it.
 template <int DT>
-__global__ __launch_bounds__(WALK) void k_walk(Walk A) {
+__global__ __launch_bounds__(BLOCK) void k_first(Job A) {
+    typedef typename type<DT>::t T;
+    __shared__ double sum_of[BLOCK / 64];
+    const i64 row = blockIdx.x / A.firsts;
+    const int slice = (int)(blockIdx.x % A.firsts), lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    if (children(A, row) < 2) return;
+    const Row p = join(A.parts + row * A.slices, A.slices, A.c), q = join(A.parts + (A.n + row) * A.slices, A.slices, A.c);
+    const T *x = (const T *)A.x[0] + row * A.ld[0], *y = (const T *)A.x[1] + row * A.ld[1];
+    double sum = 0;
+#pragma unroll 1
+    for (i64 at = ((i64)slice * BLOCK + threadIdx.x) * EIGHT; at < A.v; at += (i64)A.firsts * (BLOCK * EIGHT)) {
+        const Entries<DT> e = eight<DT>(x, at, A.v), f = eight<DT>(y, at, A.v);
+        double t[EIGHT], o[EIGHT];
+        exponentials<DT>(e, A.c, p.mc, t);
+        exponentials<DT>(f, A.c, q.mc, o);
+#pragma unroll
+        for (int i = 0; i < EIGHT; ++i) sum += fmax(t[i] * p.per_z - o[i] * q.per_z, 0.0);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) sum_of[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) A.first[blockIdx.x] = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
+}
+
+template <int DT>
+__global__ __launch_bounds__(WALK) void k_walk(Job A) {
     typedef typename type<DT>::t T;
     __shared__ Shared sh;
     const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t / 64;
-    const i64 s0 = max((i64)0, min((i64)A.starts[b], A.n)), s1 = max(s0, min((i64)A.starts[b + 1], A.n));
-    const int nodes = (int)min(s1 - s0, (i64)MAX_NODES);
+    i64 s0;
+    const int nodes = take_tree<WALK>(A, b, sh.tree, &s0);
     for (int d = t; d < A.depth; d += WALK) A.nodes[(i64)b * A.depth + d] = -1;
     for (int d = t; d <= A.depth; d += WALK) A.out[(i64)b * (A.depth + 1) + d] = -1;
     for (int r = wave; r < nodes * (A.drafted ? 2 : 1); r += WALK / 64) {
@@ -293,14 +383,10 @@ __global__ __launch_bounds__(WALK) void k_walk(Walk A) {
     }
     __syncthreads();
     for (int i = t; i < nodes; i += WALK) {
-        const int parent = i ? A.parents ? A.parents[s0 + i] : i - 1 : -1;
-        const i64 token = A.tokens[s0 + i];
-        const bool fine = parent >= 0 && parent < i && token >= 0 && token < A.v;
-        sh.parent[i] = fine ? parent : -1;
-        sh.token[i] = fine ? (int)token : -1;
+        const int parent = sh.tree.parent[i], token = sh.tree.token[i];
         sh.u[i] = A.uniforms[s0 + i];
         sh.have[i] = sh.said[i] = 0;
-        if (fine) {
+        if (parent >= 0) {
             auto of = [&](int which) {
                 const Row r = A.rows[(which ? A.n : 0) + s0 + parent];
                 return r.per_z == 0 ? 0.0 : exp2_64(fma((double)(float)((const T *)A.x[which])[(s0 + parent) * A.ld[which] + token], A.c, -r.mc)) * r.per_z;
@@ -312,56 +398,108 @@ __global__ __launch_bounds__(WALK) void k_walk(Walk A) {
     __syncthreads();
     // from here on all threads do the same
     Left<DT> left = {};
-    left.c = A.c, left.v = A.v, left.sh = &sh, left.nodes = nodes;
-    int cur = 0, count = 0;
+    left.c = A.c, left.v = A.v, left.tree = &sh.tree, left.nodes = nodes;
+    int cur = 0, count = 0, refusals = 0;
     auto stand_at = [&](int node) {
-        cur = node, left.a = 0, left.cur = -1;
+        cur = node, left.a = 0, left.cur = -1, refusals = 0;
         if (node < nodes) {
             left.x = (const T *)A.x[0] + (s0 + node) * A.ld[0], left.p = A.rows[s0 + node];
             if (A.drafted) left.y = (const T *)A.x[1] + (s0 + node) * A.ld[1], left.q = A.rows[A.n + s0 + node];
         }
     };
     stand_at(0);
-    double w = 1;                              // the sum of what is left; below zero: not known
+    double w = 1;                              // the sum of what is left
     for (int i = 1; i < nodes; ++i) {
-        if (sh.parent[i] != cur || count == A.depth || left.p.per_z == 0 || (A.drafted && left.q.per_z == 0)) continue;
+        if (sh.tree.parent[i] != cur || count == A.depth || left.p.per_z == 0 || (A.drafted && left.q.per_z == 0)) continue;
         double have = sh.have[i];
         if (!A.drafted) {
             for (int j = 1; j < i; ++j)
-                if (sh.parent[j] == cur && sh.token[j] == sh.token[i]) have = 0;       // refused before
-        } else if (left.a > 0) {
-            if (w < 0) w = sum_left(sh, left);
+                if (sh.tree.parent[j] == cur && sh.tree.token[j] == sh.tree.token[i]) have = 0;        // refused before
+        } else if (refusals) {
+            if (refusals == 1) {
+                w = 0;
+                for (int k = 0; k < A.firsts; ++k) w += A.first[(s0 + cur) * A.firsts + k];
+            } else {
+                w = 0;
+                for (int k = wave; k < segments_of(A.v); k += WALK / 64) w += sum_segment(left, k);
+                __syncthreads();
+                if (lane == 0) sh.sums[wave] = w;
+                __syncthreads();
+                w = 0;
+                for (int k = 0; k < WALK / 64; ++k) w += sh.sums[k];
+            }
             have = fmax(have - left.a * sh.said[i], 0.0);
         }
         if (sh.u[i] * sh.said[i] * w < have) {
             if (t == 0) {
                 A.nodes[(i64)b * A.depth + count] = i;
-                A.out[(i64)b * (A.depth + 1) + count] = sh.token[i];
+                A.out[(i64)b * (A.depth + 1) + count] = sh.tree.token[i];
             }
             ++count;
             stand_at(i);
             w = 1;
         } else if (A.drafted) {
             left.a += w;
-            w = -1;
+            ++refusals;
         } else {
             w -= have;
             left.cur = cur;
         }
     }
-    int last = -1;
-    if (nodes > 0 && left.p.per_z != 0) {
-        double sum = sum_left(sh, left);
-        if (!(sum > 0)) {
-            left.a = 0, left.cur = -1;
-            sum = sum_left(sh, left);
-        }
-        if (wave == 0) last = find_left(sh, left, sh.u[0] * sum);
-    }
     if (t == 0) {
         A.counts[b] = count;
-        A.out[(i64)b * (A.depth + 1) + count] = last;
+        A.ends[b] = {left.a, nodes > 0 && left.p.per_z != 0 ? s0 + cur : -1, cur, left.cur >= 0, count, 0};
     }
+}
+
+// what is left at the end of a sequence's path
+template <int DT, int THREADS>
+__device__ __forceinline__ Left<DT> left_at(const Job &A, int b, const End &end, Tree &tree) {
+    typedef typename type<DT>::t T;
+    Left<DT> left = {};
+    left.c = A.c, left.v = A.v, left.tree = &tree, left.a = end.a, left.cur = end.refused ? end.node : -1;
+    if (end.refused) {
+        i64 s0;
+        left.nodes = take_tree<THREADS>(A, b, tree, &s0);
+        __syncthreads();
+    }
+    left.x = (const T *)A.x[0] + end.row * A.ld[0], left.p = A.rows[end.row];
+    if (A.drafted) left.y = (const T *)A.x[1] + end.row * A.ld[1], left.q = A.rows[A.n + end.row];
+    return left;
+}
+
+template <int DT>
+__global__ __launch_bounds__(BLOCK) void k_left(Job A) {
+    __shared__ Tree tree;
+    const int groups = (segments_of(A.v) + BLOCK / 64 - 1) / (BLOCK / 64), b = (int)(blockIdx.x / groups), segment = (int)(blockIdx.x % groups) * (BLOCK / 64) + (int)threadIdx.x / 64;
+    const End end = A.ends[b];
+    if (end.row < 0) return;
+    const Left<DT> left = left_at<DT, BLOCK>(A, b, end, tree);
+    if (segment >= segments_of(A.v)) return;
+    const double sum = sum_segment(left, segment);
+    if ((threadIdx.x & 63) == 0) A.segments[(i64)b * segments_of(A.v) + segment] = sum;
+}
+
+template <int DT>
+__global__ __launch_bounds__(64) void k_pick(Job A) {
+    __shared__ Tree tree;
+    const int b = blockIdx.x;
+    const End end = A.ends[b];
+    if (end.row < 0) return;                   // -1 is there
+    Left<DT> left = left_at<DT, 64>(A, b, end, tree);
+    double *segments = A.segments + (i64)b * segments_of(A.v), total;
+    const double u = A.uniforms[max((i64)0, (i64)A.starts[b])];
+    int last = find_left(segments, left, u, &total);
+    if (!(total > 0)) {                        // nothing: of the target's probabilities
+        left.a = 0, left.cur = -1;
+        for (int s = 0; s < segments_of(A.v); ++s) {
+            const double sum = sum_segment(left, s);
+            if (threadIdx.x == 0) segments[s] = sum;
+        }
+        __syncthreads();
+        last = find_left(segments, left, u, &total);
+    }
+    if (threadIdx.x == 0) A.out[(i64)b * (A.depth + 1) + end.count] = last;
 }
 
 // eight entries a thread once where there are few, up to four times
@@ -372,6 +510,8 @@ int rounds(int64_t v, int64_t rows) {
     }
     return 8;
 }
+// slices of a sum behind a first refusal: sixteen at most, for its rows are few
+i64 firsts_of(int64_t v) { return v <= 16 * BLOCK * EIGHT ? (v + BLOCK * EIGHT - 1) / (BLOCK * EIGHT) : 16; }
 i64 slices_of(int64_t v, int r) { return (v + BLOCK * EIGHT * r - 1) / (BLOCK * EIGHT * r); }
 // the largest rows that eight times eight entries a thread and 64 slices hold
 static_assert(MAX_V <= (i64)BLOCK * EIGHT * 8 * 64, "rows of too many slices");
@@ -449,10 +589,11 @@ __global__ __launch_bounds__(BLOCK) void k_keep(Keep A) {
 
 }  // namespace
 
-extern "C" size_t vi_verify_drafts_workspace_bytes(int dtype, int64_t n, int64_t v, int drafted) {
-    if (!is_float(dtype) || n <= 0 || n > MAX_BLOCKS || v <= 0 || v > MAX_V) return 0;
-    const i64 rows = drafted ? 2 * n : n;
-    return (size_t)(2 * n) * sizeof(Row) + (size_t)(rows * slices_of(v, rounds(v, rows))) * sizeof(Part) + vi::WS_SLACK;
+extern "C" size_t vi_verify_drafts_workspace_bytes(int dtype, int64_t n, int64_t v, int64_t sequences, int drafted) {
+    if (!is_float(dtype) || n < 0 || n > MAX_BLOCKS || v <= 0 || v > MAX_V || sequences < 0 || sequences > 0xFFFFFF) return 0;
+    const i64 rows = drafted ? 2 * n : n, slices = slices_of(v, rounds(v, rows));
+    return (size_t)(2 * n) * sizeof(Row) + (size_t)(rows * slices) * sizeof(Part) + (size_t)sequences * (sizeof(End) + 8 * ((v + 64 * EIGHT - 1) / (64 * EIGHT))) +
+           (drafted ? (size_t)(n * firsts_of(v)) * 8 : 0) + vi::WS_SLACK;
 }
 
 extern "C" int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_t v, int64_t ld, const void *draft, int64_t ld_draft, const int64_t *tokens,
@@ -467,38 +608,49 @@ extern "C" int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_
     if (!(temperature >= 1e-3 && temperature <= 1e3)) return vi::fail(VI_EINVAL, "%s: temperature %g", who, temperature);
     if (sequences == 0) return VI_OK;
     if (!starts || !counts || !out || (depth && !nodes) || (n && (!logits || !tokens || !uniforms))) return vi::fail(VI_EINVAL, "%s: null pointer", who);
-    const size_t need = vi_verify_drafts_workspace_bytes(dtype, n, v, draft != nullptr);
-    if (ws_bytes < need || (need && !ws)) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, need);
-    const i64 rows = draft ? 2 * n : n;
+    const i64 rows = draft ? 2 * n : n, segments = (v + 64 * EIGHT - 1) / (64 * EIGHT), groups = (segments + BLOCK / 64 - 1) / (BLOCK / 64);
     const int r = rounds(v, rows);
-    if (rows * slices_of(v, r) > MAX_BLOCKS) return vi::fail(VI_EINVAL, "%s: %lld rows of %lld logits", who, (long long)n, (long long)v);
+    if (rows * slices_of(v, r) > MAX_BLOCKS || sequences * groups > MAX_BLOCKS || n * firsts_of(v) > MAX_BLOCKS)
+        return vi::fail(VI_EINVAL, "%s: %lld rows of %lld logits, %lld sequences", who, (long long)n, (long long)v, (long long)sequences);
+    const size_t need = vi_verify_drafts_workspace_bytes(dtype, n, v, sequences, draft != nullptr);
+    if (ws_bytes < need || !ws) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, need);
     const hipStream_t s = (hipStream_t)stream;
-    Walk W = {};
-    W.rows = (Row *)vi::align16(ws);
-    Part *parts = (Part *)(W.rows + 2 * n);
-    W.x[0] = logits, W.x[1] = draft, W.ld[0] = ld, W.ld[1] = ld_draft, W.n = n, W.v = v, W.slices = (int)slices_of(v, r), W.sequences = (int)sequences;
-    W.depth = (int)depth, W.drafted = draft != nullptr, W.c = 1.4426950408889634 / temperature, W.parts = parts, W.tokens = tokens, W.starts = starts;
-    W.parents = parents, W.uniforms = uniforms, W.counts = counts, W.nodes = nodes, W.out = out;
-    const Stats A = {{logits, draft}, {ld, ld_draft}, n, v, W.slices, W.c, parts};
-    const dim3 grid((unsigned)(rows * W.slices));
-#define STATS(DT, R) hipLaunchKernelGGL((k_stats<DT, R>), grid, dim3(BLOCK), 0, s, A)
-#define GO(DT)                                                                                      \
+    Job J = {};
+    J.x[0] = logits, J.x[1] = draft, J.ld[0] = ld, J.ld[1] = ld_draft, J.n = n, J.v = v, J.slices = (int)slices_of(v, r), J.firsts = (int)firsts_of(v), J.sequences = (int)sequences;
+    J.depth = (int)depth, J.drafted = draft != nullptr, J.c = 1.4426950408889634 / temperature, J.tokens = tokens, J.starts = starts, J.parents = parents;
+    J.uniforms = uniforms, J.counts = counts, J.nodes = nodes, J.out = out;
+    J.rows = (Row *)vi::align16(ws);
+    J.parts = (Part *)(J.rows + 2 * n);
+    J.ends = (End *)(J.parts + rows * J.slices);
+    J.segments = (double *)(J.ends + sequences);
+    J.first = J.segments + sequences * segments;
+    const dim3 of_rows((unsigned)(rows * J.slices)), of_nodes((unsigned)(n * J.firsts)), of_groups((unsigned)(sequences * groups)), of_sequences((unsigned)sequences);
+#define ROWS(K, GRID)                                                                               \
     do {                                                                                            \
-        if (n) {                                                                                    \
-            if (r == 1) STATS(DT, 1);                                                               \
-            else if (r == 2) STATS(DT, 2);                                                          \
-            else if (r == 4) STATS(DT, 4);                                                          \
-            else STATS(DT, 8);                                                                      \
-            VI_LAUNCH_CHECK(who);                                                                   \
-        }                                                                                           \
-        hipLaunchKernelGGL(k_walk<DT>, dim3((unsigned)sequences), dim3(WALK), 0, s, W);             \
+        if (r == 1) hipLaunchKernelGGL((K<DT, 1>), GRID, dim3(BLOCK), 0, s, J);                     \
+        else if (r == 2) hipLaunchKernelGGL((K<DT, 2>), GRID, dim3(BLOCK), 0, s, J);                \
+        else if (r == 4) hipLaunchKernelGGL((K<DT, 4>), GRID, dim3(BLOCK), 0, s, J);                \
+        else hipLaunchKernelGGL((K<DT, 8>), GRID, dim3(BLOCK), 0, s, J);                            \
+        VI_LAUNCH_CHECK(who);                                                                       \
+    } while (0)
+#define GO(TYPE)                                                                                    \
+    do {                                                                                            \
+        constexpr int DT = TYPE;                                                                    \
+        if (n) ROWS(k_stats, of_rows);                                                              \
+        if (n && draft && parents) hipLaunchKernelGGL(k_first<DT>, of_nodes, dim3(BLOCK), 0, s, J); \
+        VI_LAUNCH_CHECK(who);                                                                       \
+        hipLaunchKernelGGL(k_walk<DT>, of_sequences, dim3(WALK), 0, s, J);                          \
+        VI_LAUNCH_CHECK(who);                                                                       \
+        hipLaunchKernelGGL(k_left<DT>, of_groups, dim3(BLOCK), 0, s, J);                            \
+        VI_LAUNCH_CHECK(who);                                                                       \
+        hipLaunchKernelGGL(k_pick<DT>, of_sequences, dim3(64), 0, s, J);                            \
+        VI_LAUNCH_CHECK(who);                                                                       \
     } while (0)
     if (dtype == VI_F32) GO(VI_F32);
     if (dtype == VI_BF16) GO(VI_BF16);
     if (dtype == VI_F16) GO(VI_F16);
 #undef GO
-#undef STATS
-    VI_LAUNCH_CHECK(who);
+#undef ROWS
     return VI_OK;
 }
 

@@ -341,7 +341,9 @@ extern "C" int vi_append_tokens(const vi_cache *cache, const vi_batch *batch, in
     if (!k || !v) return vi::fail(VI_EINVAL, "%s: null pointer", who);
     A.x[0] = k, A.x[1] = v, A.token[0] = k_token, A.token[1] = v_token, A.head[0] = k_head, A.head[1] = v_head, A.n = n, A.positions = positions;
     A.turn = {steps, steps ? (int)rotated : 0, interleaved != 0, amplitude};
-    A.tokens = (int)(2 * cache->heads >= GROUPS ? 1 : GROUPS / (2 * cache->heads));
+    // a group of lanes has a head at least; where there are many tokens four to a workgroup, whose threads then have an angle each (4096 tokens into 8 heads
+    // of 8 bits: 11 us, 18 with one)
+    A.tokens = (int)(2 * cache->heads >= GROUPS ? (n >= 2048 ? 4 : 1) : GROUPS / (2 * cache->heads));
     const dim3 grid((unsigned)((n + A.tokens - 1) / A.tokens));
     const hipStream_t s = (hipStream_t)stream;
 #define FROM(DT)                                                            \

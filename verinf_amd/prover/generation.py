@@ -319,7 +319,7 @@ def verify_drafts(logits, tokens, starts, parents, uniforms, depth, draft_logits
     L = _lib.lib()
     with _lib.on_device(dev):
         sp = _lib.stream_ptr()
-        need = _lib.workspace_bytes("verify_drafts", kind, n, v, int(draft is not None))
+        need = _lib.workspace_bytes("verify_drafts", kind, n, v, sequences, int(draft is not None))
         with _lib.stream_lock(sp):
             ws = _lib.workspace(need, "drafts", sp)
             _lib.check(L.vi_verify_drafts(kind, logits.data_ptr(), n, v, ld, draft, ld_draft, ids, at, sequences, above, u, temperature, depth, counts.data_ptr(),
