@@ -417,7 +417,8 @@ int vi_token_logprobs(int dtype, const void *logits, int64_t m, int64_t v, int64
 /* ---- answering with a cache and drafted tokens (no counterpart in the reference) -------------------------------------
  * A paged cache of keys and values: entry (page, head, row) is `dim` neighbouring numbers of type VI_BF16, VI_F16, or VI_I8 with a
  * float32 scale each; strides are in elements, between pages, heads and rows (those of the scales: pages and heads, rows adjacent).
- * dim is a multiple of 16 up to 256, page_size a power of two from 16 to 1024, entries start at multiples of 16 bytes. */
+ * dim is a multiple of 16 up to 256, page_size a power of two from 16 to 1024; entries start at multiples of 16 bytes, pages less than 4 GiB and rows at most
+ * 2^20 elements apart.  A sequence has at most 2^30 entries. */
 #define VI_I8 5
 typedef struct vi_cache {
     void *keys, *values;

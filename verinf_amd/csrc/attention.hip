@@ -32,6 +32,7 @@ typedef float v16f __attribute__((ext_vector_type(16)));
 constexpr int MAX_NODES = 256;                 // of a tree
 constexpr int MASK_WORDS = MAX_NODES / 32 + 1;
 constexpr i64 MAX_BLOCKS = 1 << 22;            // of a launch, which has less than 2^32 threads
+constexpr i64 MAX_HEADS = 1 << 30;             // of all tokens together
 constexpr i64 MAX_PARTS = 128;                 // of a sequence's keys
 constexpr int CLEARING = 64;                   // workgroups that look for rows of no sequence
 constexpr float LATE = 8.0f;                   // powers of two that scores may exceed what they are relative to
@@ -153,7 +154,7 @@ __device__ __forceinline__ bool find_tile(const Args &A, int tile, Tile *t) {
     for (int first = 0; first < A.batch.sequences; first += 64) {
         const int b = min(first + (int)(threadIdx.x & 63), A.batch.sequences - 1);
         const i64 here = max((i64)0, min((i64)A.batch.starts[b], A.n)), next = max((i64)0, min((i64)A.batch.starts[b + 1], A.n));
-        const int its = A.batch.lengths[b];
+        const int its = max(A.batch.lengths[b], 0);
         const int count = __popcll(__ballot(first + (int)(threadIdx.x & 63) < A.batch.sequences && here * A.group / ROWS + b <= tile));
         if (count == 0) break;                 // starts rises
         found = first + count - 1;
@@ -178,7 +179,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     constexpr int DT = F::DT, DP = F::DP, WM = F::WM, WK = F::WK, ROW = F::ROW, UNITS = F::UNITS;
     constexpr bool NARROW = F::I8 && !F::WIDE;                         // 8-bit integers in LDS
     typedef typename type<DT>::t T;
-    __shared__ alignas(16) char lds[F::LDS];
+    __shared__ char lds[F::LDS] __attribute__((aligned(16)));
     __shared__ u32 masks[F::MASKS * MASK_WORDS];
     __shared__ int above[MAX_NODES];
     const int lane = threadIdx.x & 63, half = lane >> 5, wave = same((int)threadIdx.x >> 6), wm = WM == 1 ? 0 : WK == 1 ? wave : wave % WM, part = WK == 1 ? 0 : WM == 1 ? wave : wave / WM;
@@ -226,7 +227,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     u32 page_apart[2], row_apart[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        from[h] = A.cache.half[h].at + head * A.cache.half[h].head, scales_from[h] = A.cache.half[h].scales + head * A.cache.half[h].scale_head;
+        from[h] = A.cache.half[h].at + head * A.cache.half[h].head, scales_from[h] = F::I8 ? A.cache.half[h].scales + head * A.cache.half[h].scale_head : nullptr;
         page_apart[h] = (u32)A.cache.half[h].page, row_apart[h] = (u32)A.cache.half[h].row;
     }
     const int full_units = A.cache.dim * (F::I8 ? 1 : 2) / 16, row_mask = A.cache.mask;
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     // the rows' ancestors among the new tokens, a bit each
     if (tree) {
         const int first = token(t.first), last = min(t.n - 1, token(t.first + F::ROWS - 1));
-        for (int i = threadIdx.x; i < t.n; i += F::THREADS) above[i] = A.parents ? A.parents[t.s0 + i] : -1;
+        for (int i = threadIdx.x; i < t.n; i += F::THREADS) above[i] = A.parents[t.s0 + i];
         __syncthreads();
         for (int i = first + (int)threadIdx.x; i <= last; i += F::THREADS) {
             u32 *bits = masks + (i - first) * MASK_WORDS;
@@ -654,21 +655,25 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     if constexpr (!F::I8) {
         if (__any(wild)) {
 #pragma unroll 1
-            for (int j = first_key; j < min(first_key + stages * WK * F::KEYS, wave_end); ++j) {
-                const int number = pages[j >> A.cache.shift], block = j & ~31;
-                if (block + 32 <= min(wave_free, end) && valid_of(pages[block >> A.cache.shift], block) == 16 && valid_of(pages[(block + 16) >> A.cache.shift], block + 16) == 16) continue;
-                if (WK > 1 && (block - first_key) / F::KEYS % WK != part) continue;
-                if (valid_of(number, j & ~15) <= (j & 15)) continue;
-                if (!there || !(window_of(j, 16, 16) & 1)) continue;
-                const T *x = (const T *)(from[1] + (u64)(u32)number * page_apart[1] + (u32)(j & row_mask) * row_apart[1]);
+            for (int i = 0; i < stages * (F::KEYS / 32); ++i) {
+                const int it = i / (F::KEYS / 32), j = stage_key(it) + i % (F::KEYS / 32) * 32;
+                if (j >= wave_end) break;
+                const int one = pages[j >> A.cache.shift], two = pages[min(j + 16, end - 1) >> A.cache.shift], low = valid_of(one, j), high = valid_of(two, j + 16);
+                if (low == 16 && high == 16 && j + 32 <= wave_free) continue;
+                const u32 window = there ? window_of(j, low, high) : 0;
+#pragma unroll 1
+                for (int k = 0; k < 32; ++k) {
+                    if (!(window >> k & 1)) continue;
+                    const T *x = (const T *)(from[1] + (u64)(u32)(k < 16 ? one : two) * page_apart[1] + (u32)((j + k) & row_mask) * row_apart[1]);
 #pragma unroll
-                for (int db = 0; db < DP / 32; ++db)
+                    for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int col = 32 * db + bit_of(r);
-                        const float f = col < A.cache.dim ? (float)x[col] : 0.0f;
-                        if (!(fabsf(f) < INFINITY)) o[db][r] += f;
-                    }
+                        for (int r = 0; r < 16; ++r) {
+                            const int col = 32 * db + bit_of(r);
+                            const float f = col < A.cache.dim ? (float)x[col] : 0.0f;
+                            if (!(fabsf(f) < INFINITY)) o[db][r] += f;
+                        }
+                }
             }
         }
     }
@@ -818,7 +823,7 @@ void launch_columns(const Plan &L, const Args &A, hipStream_t s) {
 
 bool sizes_fine(int dtype, i64 dim, i64 cache_heads, i64 n, i64 heads, i64 sequences, i64 longest) {
     return (dtype == VI_BF16 || dtype == VI_F16 || dtype == VI_I8) && dim >= 16 && dim <= 256 && cache_heads >= 1 && cache_heads <= 0xFFFF && n > 0 && heads >= cache_heads &&
-           heads % cache_heads == 0 && heads <= 0xFFFF && n <= 0x7FFFFFFF / heads && sequences > 0 && sequences <= 0xFFFFFF && longest >= 0;
+           heads % cache_heads == 0 && heads <= 0xFFFF && n <= MAX_HEADS / heads && sequences > 0 && sequences <= 0xFFFFFF && longest >= 0;
 }
 
 }  // namespace
@@ -834,7 +839,7 @@ extern "C" int vi_attend_cache(const vi_cache *cache, const vi_batch *batch, int
     Args A = {};
     if (const int rc = take(who, cache, batch, &A.cache, &A.batch)) return rc;
     if (dtype != (cache->dtype == VI_F16 ? VI_F16 : VI_BF16)) return vi::fail(VI_EINVAL, "%s: queries of dtype %d over a cache of dtype %lld", who, dtype, (long long)cache->dtype);
-    if (n < 0 || heads < 1 || heads > 0xFFFF || heads % cache->heads || n > 0x7FFFFFFF / heads)
+    if (n < 0 || heads < 1 || heads > 0xFFFF || heads % cache->heads || n > MAX_HEADS / heads)
         return vi::fail(VI_EINVAL, "%s: %lld tokens of %lld heads over a cache of %lld", who, (long long)n, (long long)heads, (long long)cache->heads);
     if (!(scale > 0 && scale < 1e30f)) return vi::fail(VI_EINVAL, "%s: a scale of %g", who, (double)scale);
     if (longest < 0) return vi::fail(VI_EINVAL, "%s: no sequence longer than %lld", who, (long long)longest);

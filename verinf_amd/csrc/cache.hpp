@@ -56,7 +56,7 @@ inline int take(const char *who, const vi_cache *c, const vi_batch *b, Cache *to
     if (c->page_size < 16 || c->page_size > 1024 || !vi::is_pow2(c->page_size))
         return vi::fail(VI_EINVAL, "%s: pages of %lld entries (powers of two from 16 to 1024)", who, (long long)c->page_size);
     if (c->pages < 0 || c->pages > 0x7FFFFFFF || c->heads < 1 || c->heads > 0xFFFF) return vi::fail(VI_EINVAL, "%s: %lld pages of %lld heads", who, (long long)c->pages, (long long)c->heads);
-    if (b->sequences < 0 || b->sequences > 0xFFFFFF || b->width < 0 || b->width > 0x7FFFFFFF / 1024 || (b->sequences > 1 && b->stride < b->width))
+    if (b->sequences < 0 || b->sequences > 0xFFFFFF || b->width < 0 || b->width > (1 << 30) / c->page_size || (b->sequences > 1 && b->stride < b->width))
         return vi::fail(VI_EINVAL, "%s: %lld sequences of %lld pages", who, (long long)b->sequences, (long long)b->width);
     if (!b->starts || (b->sequences && (!b->lengths || (b->width && !b->pages)))) return vi::fail(VI_EINVAL, "%s: null pointer", who);
     if (c->pages && (!c->keys || !c->values || (c->dtype == VI_I8 && (!c->key_scales || !c->value_scales)))) return vi::fail(VI_EINVAL, "%s: null pointer", who);
