@@ -10,11 +10,15 @@
 // the refused tokens and is otherwise p.
 //
 // Whole numbers come of it, decided by comparisons next to borders, of which the last token's have as many as there are tokens: all in 64
-// bits, exponentials too (the series of 2^f to the 11th power, 6e-15).
+// bits, exponentials too (1.6e-13 off).
 //
 // All rows' largest entries and sums, in slices (k_stats), and the sums behind a first refusal, for nodes with other children (k_first), are taken by the whole
 // chip; a workgroup a sequence walks (k_walk), with a pass over two rows for each further refusal; the whole chip adds up what is left behind the paths
-// (k_left), and a workgroup a sequence looks for the token (k_pick).  What bounds them: reading the logits, and 18 operations in 64 bits an exponential beside it.
+// (k_left), and a workgroup a sequence looks for the token (k_pick).
+//
+// What bounds them: some 15 instructions an exponential, eleven of them in 64 bits, which issue every 5 cycles.  64 trees of 16 nodes, 32000 bf16 logits of both models:
+// 126 us (46 all rows' sums, 30 first refusals, 55 the walk of the sequence with the most refusals, 10 us each, 11 the last tokens; 25 to read them); with the 11
+// powers of a series on [-1/2, 1/2] in place of table and 4 powers 149.  One chain of five nodes, f32: 15 us, the latency of four launches.
 #include "cache.hpp"
 
 namespace {
@@ -26,40 +30,53 @@ constexpr i64 MAX_V = 1 << 20;
 constexpr i64 MAX_BLOCKS = 1 << 23;            // of a launch, which has less than 2^32 threads
 constexpr int MAX_NODES = 1024, MAX_DEPTH = 256;
 constexpr int EIGHT = 8;                       // neighbouring entries of a thread
+constexpr double MARGIN = 64;                  // bits
 
-struct Part {                                  // of a slice: its largest entry (NaN: it has a NaN or +inf), sum of 2^((x - most) c)
+struct Part {                                  // of a slice: an entry of its largest (NaN: it has a NaN or +inf), sum of 2^((x - most) c / 32)
     double z;
     float most, pad;
 };
-struct Row {                                   // of a row: the most c that its sum is relative to; 1 / sum, 0 where it has none
+struct Row {                                   // of a row: the most c that its sum is relative to; 1 / sum, 0 where it has none (or NaN, +inf among its entries)
     double mc, per_z;
 };
 
-// 2^t of N numbers side by side (one alone waits for itself at each step), t up to 0 or hardly above, 2^-1000 from there on: the whole part by an addition
-// whose result has units of one, and into the exponent
+// 2^(t / 32) of N numbers side by side (one alone waits for itself at each step), t up to 0 or hardly above, 2^-1000 below 32 times that: the whole part by an
+// addition whose result has units of one, its last five bits from a table, the others into the exponent, the rest by a polynomial (over Chebyshev's nodes, 1.6e-13).
+// The table has 256 bytes, a pair of banks to each entry; the exponent comes into the entry by adding the whole part as it is, 15 bits up in the upper half, from
+// where the entry has lost its own number before.
+constexpr int STEPS = 32;
+__device__ const double TABLE[STEPS] = {0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0, 0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0,
+                                      0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0, 0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+                                      0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0, 0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0,
+                                      0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0, 0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+                                      0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0, 0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0,
+                                      0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+__device__ __forceinline__ void take_table(double *table) {        // a barrier has to follow
+    if (threadIdx.x < STEPS) table[threadIdx.x] = __builtin_bit_cast(double, __builtin_bit_cast(u64, TABLE[threadIdx.x]) - ((u64)threadIdx.x << 47));
+}
 template <int N>
-__device__ __forceinline__ void exp2_64(double (&t)[N]) {
-    constexpr double C[] = {4.4455382718708116e-10, 7.0549116208011233e-9,  1.0178086009239700e-7, 1.3215486790144310e-6, 1.5252733804059841e-5, 1.5403530393381610e-4,
-                            1.3333558146428443e-3,  9.6181291076284772e-3,  5.5504108664821580e-2, 2.4022650695910071e-1, 6.9314718055994531e-1, 1.0};
-    double m[N], f[N], p[N];
+__device__ __forceinline__ void exp2_64(const double *table, double (&t)[N], double (&scale)[N]) {         // times scale
+    constexpr double C[] = {9.172598566029335e-09, 1.6938609067364198e-06, 0.00023459619820112603, 0.021660849392187844, 1.0};
+    double m[N], f[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-        t[e] = fmax(t[e], -1000.0);
+        t[e] = fmax(t[e], -1000.0 * STEPS);
         m[e] = t[e] + 6755399441055744.0;
         f[e] = t[e] - (m[e] - 6755399441055744.0);
-        p[e] = C[0];
+        const u32 k = (u32)__builtin_bit_cast(u64, m[e]);
+        const u64 entry = __builtin_bit_cast(u64, table[k % STEPS]);
+        scale[e] = __builtin_bit_cast(double, (u64)((u32)(entry >> 32) + (k << 15)) << 32 | (u32)entry);
+        t[e] = C[0];
     }
 #pragma unroll
-    for (int i = 1; i < 12; ++i)
+    for (int i = 1; i < 5; ++i)
 #pragma unroll
-        for (int e = 0; e < N; ++e) p[e] = fma(p[e], f[e], C[i]);
-#pragma unroll
-    for (int e = 0; e < N; ++e) t[e] = __builtin_bit_cast(double, __builtin_bit_cast(u64, p[e]) + (__builtin_bit_cast(u64, m[e]) << 52));
+        for (int e = 0; e < N; ++e) t[e] = fma(t[e], f[e], C[i]);
 }
-__device__ __forceinline__ double exp2_64(double t) {
-    double one[1] = {t};
-    exp2_64(one);
-    return one[0];
+__device__ __forceinline__ double exp2_64(const double *table, double t) {
+    double one[1] = {t}, scale[1];
+    exp2_64(table, one, scale);
+    return one[0] * scale[0];
 }
 
 template <int DT>
@@ -82,26 +99,37 @@ __device__ __forceinline__ Entries<DT> eight(const typename type<DT>::t *x, i64 
     __builtin_memcpy(&r, e, sizeof(r));
     return r;
 }
-
-// e^(x - most) of eight entries, in 64 bits
+// the eight from `at` on where there are eight, anything otherwise: asked for ahead of their use
 template <int DT>
-__device__ __forceinline__ void exponentials(const Entries<DT> &v, double c, double mc, double (&r)[EIGHT]) {
+__device__ __forceinline__ Entries<DT> first_eight(const typename type<DT>::t *x, i64 at, i64 end) {
+    Entries<DT> r = {};
+    if (at + EIGHT <= end) r = load_any<Entries<DT>>(x + at);
+    return r;
+}
+
+// e^(x - most) of eight entries, in 64 bits: t times scale, to(i, t, scale)
+template <int DT, class To>
+__device__ __forceinline__ void exponentials(const double *table, const Entries<DT> &v, double c, double mc, To to) {
 #pragma unroll
     for (int h = 0; h < EIGHT; h += 4) {
-        double t[4];
+        double t[4], scale[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = fma((double)entry<DT>(v, h + e), c, -mc);
-        exp2_64(t);
+        exp2_64(table, t, scale);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[h + e] = t[e];
+        for (int e = 0; e < 4; ++e) to(h + e, t[e], scale[e]);
     }
+}
+template <int DT>
+__device__ __forceinline__ void exponentials(const double *table, const Entries<DT> &v, double c, double mc, double (&r)[EIGHT]) {
+    exponentials<DT>(table, v, c, mc, [&](int i, double t, double scale) __attribute__((always_inline)) { r[i] = t * scale; });
 }
 
 struct Job {
     const void *x[2];                          // the target's logits, the draft's
     i64 ld[2], n, v;
-    int slices, firsts, sequences, depth, drafted;
-    double c;                                  // log2(e) / temperature
+    int slices, per_slice, firsts, sequences, depth, drafted;
+    double c;                                  // 32 log2(e) / temperature
     Part *parts;                               // [2 n][slices]
     double *first;                             // [n][firsts]: the sum of max(p - q, 0) of a slice
     Row *rows;                                 // [2 n]
@@ -136,47 +164,54 @@ __device__ __forceinline__ int children(const Job &A, i64 row) {
     return min(count, 2);
 }
 
-// R times eight entries a thread
-template <int DT, int R>
+// The sum of a slice.  A thread's is relative to the largest of the first entries that it has seen, or of later ones where they are 2^MARGIN times those.
+template <int DT>
 __global__ __launch_bounds__(BLOCK) void k_stats(Job A) {
     typedef typename type<DT>::t T;
     __shared__ float most_of[BLOCK / 64];
-    __shared__ double sum_of[BLOCK / 64];
+    __shared__ double sum_of[BLOCK / 64], table[STEPS];
     const i64 row = blockIdx.x / A.slices;
     const int slice = (int)(blockIdx.x % A.slices), which = row >= A.n, lane = threadIdx.x & 63, wave = threadIdx.x / 64;
     const T *x = (const T *)A.x[which] + (row - (which ? A.n : 0)) * A.ld[which];
-    const i64 first = (i64)slice * (BLOCK * EIGHT * R);
+    const i64 end = min(A.v, (i64)(slice + 1) * A.per_slice);
+    i64 at = (i64)slice * A.per_slice + (int)threadIdx.x * EIGHT;
+    Entries<DT> v = first_eight<DT>(x, at, end);
     if (which && children(A, row - A.n) == 0) return;                  // nobody asks
-    Entries<DT> v[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) v[r] = eight<DT>(x, first + (r * BLOCK + (int)threadIdx.x) * EIGHT, A.v);
-    float most = -INFINITY;
+    take_table(table);
+    __syncthreads();
+    const float margin = (float)(MARGIN * STEPS / A.c);
+    float most = -INFINITY, bound = -INFINITY;
+    double z = 0, mc = 0;
     bool bad = false;
+    auto add = [&](const Entries<DT> &e) __attribute__((always_inline)) {
+        float here = entry<DT>(e, 0);
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int e = 0; e < EIGHT; ++e) {
-            const float f = entry<DT>(v[r], e);
-            most = fmaxf(most, f);
-            bad |= !(f < INFINITY);
+        for (int i = 1; i < EIGHT; ++i) here = __builtin_elementwise_maximum(here, entry<DT>(e, i));           // NaN where there is one
+        bad |= !(here < INFINITY);
+        if (here > bound && !bad) {
+            const double next = (double)here * A.c;
+            z = z > 0 ? z * exp2_64(table, mc - next) : 0.0;
+            most = here, bound = here + margin, mc = next;
         }
+        if (most > -INFINITY) {
+            exponentials<DT>(table, e, A.c, mc, [&](int, double t, double scale) __attribute__((always_inline)) { z = fma(t, scale, z); });
+        }
+    };
+    while (at + EIGHT <= end) {
+        const i64 next = at + BLOCK * EIGHT;
+        const Entries<DT> ahead = first_eight<DT>(x, next, end);
+        add(v);
+        v = ahead, at = next;
+    }
+    if (at < end) add(eight<DT>(x, at, end));
     if (bad) most = INFINITY;
+    const float own = most;
 #pragma unroll
     for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
     if (lane == 0) most_of[wave] = most;
     __syncthreads();
     most = fmaxf(fmaxf(most_of[0], most_of[1]), fmaxf(most_of[2], most_of[3]));
-    double z = 0;
-    if (most > -INFINITY && most < INFINITY) {
-        const double mc = (double)most * A.c;
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            double t[EIGHT];
-            exponentials<DT>(v[r], A.c, mc, t);
-#pragma unroll
-            for (int e = 0; e < EIGHT; ++e) z += t[e];
-        }
-    }
+    z = own > -INFINITY && most < INFINITY ? z * exp2_64(table, mc - (double)most * A.c) : 0.0;
 #pragma unroll
     for (int d = 32; d; d >>= 1) z += __shfl_xor(z, d);
     if (lane == 0) sum_of[wave] = z;
@@ -211,7 +246,7 @@ __device__ __forceinline__ int take_tree(const Job &A, int b, Tree &tree, i64 *f
 struct Shared {
     Tree tree;
     double have[MAX_NODES], said[MAX_NODES], u[MAX_NODES];             // p and q of a node's token behind its parent
-    double sums[WALK / 64];
+    double sums[WALK / 64], table[STEPS];
 };
 
 // the sum of the wavefront's values up to this lane's
@@ -238,17 +273,20 @@ struct Left {
     double a, c;
     i64 v;
     const Tree *tree;
+    const double *table;
     int nodes, cur;                            // the refused are the children of cur (-1: none are)
 
     __device__ __forceinline__ void eight_at(i64 at, double (&r)[EIGHT]) const {
-        const Entries<DT> e = eight<DT>(x, at, v);
-        exponentials<DT>(e, c, p.mc, r);
+        of(at, eight<DT>(x, at, v), a > 0 ? eight<DT>(y, at, v) : Entries<DT>{}, r);
+    }
+    __device__ __forceinline__ void of(i64 at, const Entries<DT> &e, const Entries<DT> &f, double (&r)[EIGHT]) const {
+        exponentials<DT>(table, e, c, p.mc, r);
 #pragma unroll
         for (int i = 0; i < EIGHT; ++i) r[i] = entry<DT>(e, i) > -INFINITY ? r[i] * p.per_z : 0.0;
         if (a > 0) {
             const double per = a * q.per_z;
             double o[EIGHT];
-            exponentials<DT>(eight<DT>(y, at, v), c, q.mc, o);
+            exponentials<DT>(table, f, c, q.mc, o);
 #pragma unroll
             for (int i = 0; i < EIGHT; ++i) r[i] = fmax(r[i] - o[i] * per, 0.0);
         }
@@ -273,6 +311,30 @@ __device__ __forceinline__ double sum_segment(const Left<DT> &left, int segment)
     left.eight_at((i64)(segment * 64 + (int)(threadIdx.x & 63)) * EIGHT, r);
 #pragma unroll
     for (int i = 0; i < EIGHT; ++i) sum += r[i];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    return sum;
+}
+
+// a thread's of the sum of a row that WALK threads add up, and its wavefront's
+template <int DT>
+__device__ __forceinline__ double sum_own(const Left<DT> &left) {
+    i64 at = (i64)threadIdx.x * EIGHT;
+    Entries<DT> e = first_eight<DT>(left.x, at, left.v), f = first_eight<DT>(left.y, at, left.v);
+    double r[EIGHT], sum = 0;
+    while (at + EIGHT <= left.v) {
+        const i64 next = at + WALK * EIGHT;
+        const Entries<DT> e_ahead = first_eight<DT>(left.x, next, left.v), f_ahead = first_eight<DT>(left.y, next, left.v);
+        left.of(at, e, f, r);
+#pragma unroll
+        for (int i = 0; i < EIGHT; ++i) sum += r[i];
+        e = e_ahead, f = f_ahead, at = next;
+    }
+    if (at < left.v) {
+        left.eight_at(at, r);
+#pragma unroll
+        for (int i = 0; i < EIGHT; ++i) sum += r[i];
+    }
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     return sum;
@@ -324,7 +386,7 @@ __device__ int find_left(const double *segment_sums, const Left<DT> &left, doubl
 }
 
 // The largest entry and the sum of a row of its slices', by a wavefront
-__device__ __forceinline__ Row join(const Part *parts, int slices, double c) {
+__device__ __forceinline__ Row join(const double *table, const Part *parts, int slices, double c) {
     const int lane = threadIdx.x & 63;
     Part p = {0.0, -INFINITY, 0.0f};
     if (lane < slices) p = parts[lane];
@@ -334,7 +396,7 @@ __device__ __forceinline__ Row join(const Part *parts, int slices, double c) {
     for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
     if (bad || !(most > -INFINITY)) return {0.0, 0.0};
     const double mc = (double)most * c;
-    double z = p.most > -INFINITY ? p.z * exp2_64((double)p.most * c - mc) : 0.0;
+    double z = p.most > -INFINITY ? p.z * exp2_64(table, (double)p.most * c - mc) : 0.0;
 #pragma unroll
     for (int d = 32; d; d >>= 1) z += __shfl_xor(z, d);
     return {mc, 1.0 / z};
@@ -344,22 +406,31 @@ __device__ __forceinline__ Row join(const Part *parts, int slices, double c) {
 template <int DT>
 __global__ __launch_bounds__(BLOCK) void k_first(Job A) {
     typedef typename type<DT>::t T;
-    __shared__ double sum_of[BLOCK / 64];
+    __shared__ double sum_of[BLOCK / 64], table[STEPS];
     const i64 row = blockIdx.x / A.firsts;
     const int slice = (int)(blockIdx.x % A.firsts), lane = threadIdx.x & 63, wave = threadIdx.x / 64;
-    if (children(A, row) < 2) return;
-    const Row p = join(A.parts + row * A.slices, A.slices, A.c), q = join(A.parts + (A.n + row) * A.slices, A.slices, A.c);
     const T *x = (const T *)A.x[0] + row * A.ld[0], *y = (const T *)A.x[1] + row * A.ld[1];
+    i64 at = ((i64)slice * BLOCK + threadIdx.x) * EIGHT;
+    if (children(A, row) < 2) return;
+    Entries<DT> e = first_eight<DT>(x, at, A.v), f = first_eight<DT>(y, at, A.v);
+    take_table(table);
+    __syncthreads();
+    const Row p = join(table, A.parts + row * A.slices, A.slices, A.c), q = join(table, A.parts + (A.n + row) * A.slices, A.slices, A.c);
     double sum = 0;
-#pragma unroll 1
-    for (i64 at = ((i64)slice * BLOCK + threadIdx.x) * EIGHT; at < A.v; at += (i64)A.firsts * (BLOCK * EIGHT)) {
-        const Entries<DT> e = eight<DT>(x, at, A.v), f = eight<DT>(y, at, A.v);
+    auto add = [&](const Entries<DT> &e, const Entries<DT> &f) __attribute__((always_inline)) {
         double t[EIGHT], o[EIGHT];
-        exponentials<DT>(e, A.c, p.mc, t);
-        exponentials<DT>(f, A.c, q.mc, o);
+        exponentials<DT>(table, e, A.c, p.mc, t);
+        exponentials<DT>(table, f, A.c, q.mc, o);
 #pragma unroll
         for (int i = 0; i < EIGHT; ++i) sum += fmax(t[i] * p.per_z - o[i] * q.per_z, 0.0);
+    };
+    while (at + EIGHT <= A.v) {
+        const i64 next = at + (i64)A.firsts * (BLOCK * EIGHT);
+        const Entries<DT> e_ahead = first_eight<DT>(x, next, A.v), f_ahead = first_eight<DT>(y, next, A.v);
+        add(e, f);
+        e = e_ahead, f = f_ahead, at = next;
     }
+    if (at < A.v) add(eight<DT>(x, at, A.v), eight<DT>(y, at, A.v));
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     if (lane == 0) sum_of[wave] = sum;
@@ -374,11 +445,13 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
     const int b = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t / 64;
     i64 s0;
     const int nodes = take_tree<WALK>(A, b, sh.tree, &s0);
+    take_table(sh.table);
+    __syncthreads();
     for (int d = t; d < A.depth; d += WALK) A.nodes[(i64)b * A.depth + d] = -1;
     for (int d = t; d <= A.depth; d += WALK) A.out[(i64)b * (A.depth + 1) + d] = -1;
     for (int r = wave; r < nodes * (A.drafted ? 2 : 1); r += WALK / 64) {
         const i64 row = r < nodes ? s0 + r : A.n + s0 + r - nodes;
-        const Row joined = join(A.parts + row * A.slices, A.slices, A.c);
+        const Row joined = join(sh.table, A.parts + row * A.slices, A.slices, A.c);
         if (lane == 0) A.rows[row] = joined;
     }
     __syncthreads();
@@ -389,7 +462,7 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
         if (parent >= 0) {
             auto of = [&](int which) {
                 const Row r = A.rows[(which ? A.n : 0) + s0 + parent];
-                return r.per_z == 0 ? 0.0 : exp2_64(fma((double)(float)((const T *)A.x[which])[(s0 + parent) * A.ld[which] + token], A.c, -r.mc)) * r.per_z;
+                return r.per_z == 0 ? 0.0 : exp2_64(sh.table, fma((double)(float)((const T *)A.x[which])[(s0 + parent) * A.ld[which] + token], A.c, -r.mc)) * r.per_z;
             };
             sh.have[i] = of(0);
             sh.said[i] = A.drafted ? of(1) : 1.0;
@@ -398,7 +471,7 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
     __syncthreads();
     // from here on all threads do the same
     Left<DT> left = {};
-    left.c = A.c, left.v = A.v, left.tree = &sh.tree, left.nodes = nodes;
+    left.c = A.c, left.v = A.v, left.tree = &sh.tree, left.table = sh.table, left.nodes = nodes;
     int cur = 0, count = 0, refusals = 0;
     auto stand_at = [&](int node) {
         cur = node, left.a = 0, left.cur = -1, refusals = 0;
@@ -420,8 +493,7 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
                 w = 0;
                 for (int k = 0; k < A.firsts; ++k) w += A.first[(s0 + cur) * A.firsts + k];
             } else {
-                w = 0;
-                for (int k = wave; k < segments_of(A.v); k += WALK / 64) w += sum_segment(left, k);
+                w = sum_own(left);
                 __syncthreads();
                 if (lane == 0) sh.sums[wave] = w;
                 __syncthreads();
@@ -454,15 +526,16 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
 
 // what is left at the end of a sequence's path
 template <int DT, int THREADS>
-__device__ __forceinline__ Left<DT> left_at(const Job &A, int b, const End &end, Tree &tree) {
+__device__ __forceinline__ Left<DT> left_at(const Job &A, int b, const End &end, Tree &tree, double *table) {
     typedef typename type<DT>::t T;
     Left<DT> left = {};
-    left.c = A.c, left.v = A.v, left.tree = &tree, left.a = end.a, left.cur = end.refused ? end.node : -1;
+    left.c = A.c, left.v = A.v, left.tree = &tree, left.table = table, left.a = end.a, left.cur = end.refused ? end.node : -1;
+    take_table(table);
     if (end.refused) {
         i64 s0;
         left.nodes = take_tree<THREADS>(A, b, tree, &s0);
-        __syncthreads();
     }
+    __syncthreads();
     left.x = (const T *)A.x[0] + end.row * A.ld[0], left.p = A.rows[end.row];
     if (A.drafted) left.y = (const T *)A.x[1] + end.row * A.ld[1], left.q = A.rows[A.n + end.row];
     return left;
@@ -471,10 +544,11 @@ __device__ __forceinline__ Left<DT> left_at(const Job &A, int b, const End &end,
 template <int DT>
 __global__ __launch_bounds__(BLOCK) void k_left(Job A) {
     __shared__ Tree tree;
+    __shared__ double table[STEPS];
     const int groups = (segments_of(A.v) + BLOCK / 64 - 1) / (BLOCK / 64), b = (int)(blockIdx.x / groups), segment = (int)(blockIdx.x % groups) * (BLOCK / 64) + (int)threadIdx.x / 64;
     const End end = A.ends[b];
     if (end.row < 0) return;
-    const Left<DT> left = left_at<DT, BLOCK>(A, b, end, tree);
+    const Left<DT> left = left_at<DT, BLOCK>(A, b, end, tree, table);
     if (segment >= segments_of(A.v)) return;
     const double sum = sum_segment(left, segment);
     if ((threadIdx.x & 63) == 0) A.segments[(i64)b * segments_of(A.v) + segment] = sum;
@@ -483,10 +557,11 @@ __global__ __launch_bounds__(BLOCK) void k_left(Job A) {
 template <int DT>
 __global__ __launch_bounds__(64) void k_pick(Job A) {
     __shared__ Tree tree;
+    __shared__ double table[STEPS];
     const int b = blockIdx.x;
     const End end = A.ends[b];
     if (end.row < 0) return;                   // -1 is there
-    Left<DT> left = left_at<DT, 64>(A, b, end, tree);
+    Left<DT> left = left_at<DT, 64>(A, b, end, tree, table);
     double *segments = A.segments + (i64)b * segments_of(A.v), total;
     const double u = A.uniforms[max((i64)0, (i64)A.starts[b])];
     int last = find_left(segments, left, u, &total);
@@ -502,19 +577,14 @@ __global__ __launch_bounds__(64) void k_pick(Job A) {
     if (threadIdx.x == 0) A.out[(i64)b * (A.depth + 1) + end.count] = last;
 }
 
-// eight entries a thread once where there are few, up to four times
-int rounds(int64_t v, int64_t rows) {
-    for (int r = 1; r < 8; r *= 2) {
-        const i64 slices = (v + BLOCK * EIGHT * r - 1) / (BLOCK * EIGHT * r);
-        if (slices <= 64 && slices * rows <= 4096) return r;
-    }
-    return 8;
+// Entries of a slice of a row: as many as leave 8192 workgroups, 2048 at least, and 64 slices at most
+i64 per_slice_of(int64_t v, int64_t rows) {
+    const i64 at_once = BLOCK * EIGHT, all = (v + at_once - 1) / at_once, slices = min(min(all, (i64)64), max((i64)1, 8192 / max(rows, (i64)1)));
+    return (all + slices - 1) / slices * at_once;
 }
-// slices of a sum behind a first refusal: sixteen at most, for its rows are few
-i64 firsts_of(int64_t v) { return v <= 16 * BLOCK * EIGHT ? (v + BLOCK * EIGHT - 1) / (BLOCK * EIGHT) : 16; }
-i64 slices_of(int64_t v, int r) { return (v + BLOCK * EIGHT * r - 1) / (BLOCK * EIGHT * r); }
-// the largest rows that eight times eight entries a thread and 64 slices hold
-static_assert(MAX_V <= (i64)BLOCK * EIGHT * 8 * 64, "rows of too many slices");
+i64 slices_of(int64_t v, int64_t rows) { return (v + per_slice_of(v, rows) - 1) / per_slice_of(v, rows); }
+// slices of a sum behind a first refusal: its rows are some of the nodes'
+i64 firsts_of(int64_t v, int64_t n) { return min((v + BLOCK * EIGHT - 1) / (BLOCK * EIGHT), max((i64)4, min((i64)16, 4096 / max(n, (i64)1)))); }
 
 // ---- the path's entries -------------------------------------------------------------------------------------------
 struct Keep {
@@ -591,9 +661,9 @@ __global__ __launch_bounds__(BLOCK) void k_keep(Keep A) {
 
 extern "C" size_t vi_verify_drafts_workspace_bytes(int dtype, int64_t n, int64_t v, int64_t sequences, int drafted) {
     if (!is_float(dtype) || n < 0 || n > MAX_BLOCKS || v <= 0 || v > MAX_V || sequences < 0 || sequences > 0xFFFFFF) return 0;
-    const i64 rows = drafted ? 2 * n : n, slices = slices_of(v, rounds(v, rows));
+    const i64 rows = drafted ? 2 * n : n, slices = slices_of(v, rows);
     return (size_t)(2 * n) * sizeof(Row) + (size_t)(rows * slices) * sizeof(Part) + (size_t)sequences * (sizeof(End) + 8 * ((v + 64 * EIGHT - 1) / (64 * EIGHT))) +
-           (drafted ? (size_t)(n * firsts_of(v)) * 8 : 0) + vi::WS_SLACK;
+           (drafted ? (size_t)(n * firsts_of(v, n)) * 8 : 0) + vi::WS_SLACK;
 }
 
 extern "C" int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_t v, int64_t ld, const void *draft, int64_t ld_draft, const int64_t *tokens,
@@ -609,15 +679,14 @@ extern "C" int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_
     if (sequences == 0) return VI_OK;
     if (!starts || !counts || !out || (depth && !nodes) || (n && (!logits || !tokens || !uniforms))) return vi::fail(VI_EINVAL, "%s: null pointer", who);
     const i64 rows = draft ? 2 * n : n, segments = (v + 64 * EIGHT - 1) / (64 * EIGHT), groups = (segments + BLOCK / 64 - 1) / (BLOCK / 64);
-    const int r = rounds(v, rows);
-    if (rows * slices_of(v, r) > MAX_BLOCKS || sequences * groups > MAX_BLOCKS || n * firsts_of(v) > MAX_BLOCKS)
+    if (rows * slices_of(v, rows) > MAX_BLOCKS || sequences * groups > MAX_BLOCKS || n * firsts_of(v, n) > MAX_BLOCKS)
         return vi::fail(VI_EINVAL, "%s: %lld rows of %lld logits, %lld sequences", who, (long long)n, (long long)v, (long long)sequences);
     const size_t need = vi_verify_drafts_workspace_bytes(dtype, n, v, sequences, draft != nullptr);
     if (ws_bytes < need || !ws) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, need);
     const hipStream_t s = (hipStream_t)stream;
     Job J = {};
-    J.x[0] = logits, J.x[1] = draft, J.ld[0] = ld, J.ld[1] = ld_draft, J.n = n, J.v = v, J.slices = (int)slices_of(v, r), J.firsts = (int)firsts_of(v), J.sequences = (int)sequences;
-    J.depth = (int)depth, J.drafted = draft != nullptr, J.c = 1.4426950408889634 / temperature, J.tokens = tokens, J.starts = starts, J.parents = parents;
+    J.x[0] = logits, J.x[1] = draft, J.ld[0] = ld, J.ld[1] = ld_draft, J.n = n, J.v = v, J.slices = (int)slices_of(v, rows), J.per_slice = (int)per_slice_of(v, rows), J.firsts = (int)firsts_of(v, n), J.sequences = (int)sequences;
+    J.depth = (int)depth, J.drafted = draft != nullptr, J.c = STEPS * 1.4426950408889634 / temperature, J.tokens = tokens, J.starts = starts, J.parents = parents;
     J.uniforms = uniforms, J.counts = counts, J.nodes = nodes, J.out = out;
     J.rows = (Row *)vi::align16(ws);
     J.parts = (Part *)(J.rows + 2 * n);
@@ -625,18 +694,11 @@ extern "C" int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_
     J.segments = (double *)(J.ends + sequences);
     J.first = J.segments + sequences * segments;
     const dim3 of_rows((unsigned)(rows * J.slices)), of_nodes((unsigned)(n * J.firsts)), of_groups((unsigned)(sequences * groups)), of_sequences((unsigned)sequences);
-#define ROWS(K, GRID)                                                                               \
-    do {                                                                                            \
-        if (r == 1) hipLaunchKernelGGL((K<DT, 1>), GRID, dim3(BLOCK), 0, s, J);                     \
-        else if (r == 2) hipLaunchKernelGGL((K<DT, 2>), GRID, dim3(BLOCK), 0, s, J);                \
-        else if (r == 4) hipLaunchKernelGGL((K<DT, 4>), GRID, dim3(BLOCK), 0, s, J);                \
-        else hipLaunchKernelGGL((K<DT, 8>), GRID, dim3(BLOCK), 0, s, J);                            \
-        VI_LAUNCH_CHECK(who);                                                                       \
-    } while (0)
 #define GO(TYPE)                                                                                    \
     do {                                                                                            \
         constexpr int DT = TYPE;                                                                    \
-        if (n) ROWS(k_stats, of_rows);                                                              \
+        if (n) hipLaunchKernelGGL(k_stats<DT>, of_rows, dim3(BLOCK), 0, s, J);                      \
+        VI_LAUNCH_CHECK(who);                                                                       \
         if (n && draft && parents) hipLaunchKernelGGL(k_first<DT>, of_nodes, dim3(BLOCK), 0, s, J); \
         VI_LAUNCH_CHECK(who);                                                                       \
         hipLaunchKernelGGL(k_walk<DT>, of_sequences, dim3(WALK), 0, s, J);                          \
@@ -650,7 +712,6 @@ extern "C" int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_
     if (dtype == VI_BF16) GO(VI_BF16);
     if (dtype == VI_F16) GO(VI_F16);
 #undef GO
-#undef ROWS
     return VI_OK;
 }
 
