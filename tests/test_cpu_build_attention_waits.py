@@ -25,11 +25,11 @@ def test_loads_to_lds_wait_for_their_address_and_place(tmp_path):
             op = s.split()[0]
             if op in seen:
                 seen[op] += 1
-                assert instructions[i - 1].startswith("s_nop") and re.match(r"s_mov_b32 m0, s\d+$", instructions[i - 2]), (name, instructions[i - 3:i + 1])
+                assert instructions[i - 1].startswith("s_nop") and re.match(r"s_mov_b32 m0, (s\d+|vcc_lo|vcc_hi)$", instructions[i - 2]), (name, instructions[i - 3:i + 1])
                 if op == "global_load_lds_dwordx4":
                     base = registers(s.rsplit(", ", 1)[1])
                     assert base and wait_states_before(instructions, i, base) >= WAIT_STATES, (name, instructions[i - 6:i + 1])
             else:
-                assert not re.search(r"\bm0\b", s) or re.match(r"s_mov_b32 m0, s\d+$", s), (name, s)
+                assert not re.search(r"\bm0\b", s) or re.match(r"s_mov_b32 m0, (s\d+|vcc_lo|vcc_hi)$", s), (name, s)
             assert not s.startswith("scratch_"), (name, s)             # waits that count loads have none of the compiler's between
     assert seen["global_load_lds_dwordx4"] > 200 and seen["global_load_lds_dword"] >= 12

@@ -94,5 +94,5 @@ def test_a_wait_for_fewer_loads_is_found(tmp_path, mistake):
 
 
 def test_loads_over_what_is_still_read_are_found(tmp_path):
-    mistake = ("fetch(0, place_of(0, it % 2), stage_key(it + 2), behind, behind_all);", "fetch(0, place_of(0, (it + 1) % 2), stage_key(it + 2), behind, behind_all);")
+    mistake = ("fetch(0, place_of(0, own), stage_key(it + 2), behind, behind_all);", "fetch(0, place_of(0, other), stage_key(it + 2), behind, behind_all);")
     assert run(_build("attention", str(tmp_path), mistake), "attend").returncode != 0

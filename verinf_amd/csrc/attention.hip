@@ -13,7 +13,12 @@
 // meet all banks: unit u (16 bytes) of a row lies at u ^ order(row).  WM wavefronts share a stage; WK such groups take every WK-th stage and are added at the end.  Where
 // there are few tiles the keys are cut between workgroups too, and k_join adds what they leave.
 //
-// Roundings: P to the type of the queries (as V has), relative to a largest score that may be up to 2^8 behind; all sums in 32 bits.
+// Roundings: P to the type of the queries (as V has), to fp16 for 8-bit integers, relative to a largest score that may be up to 2^8 behind; all sums in 32 bits.
+//
+// What bounds it (bf16, 8 heads of 128 columns for 32, where nothing else is said): 64 sequences of 4096 entries and a token each 198 us, 5.4 TB/s, as a large copy
+// (118 us over 8-bit integers, 4.7); 4096 tokens of a prompt, 32 heads of the cache, fp16, 198 us, 694 TFLOP/s, where the matrix units are busy for a third of the time and
+// the exponentials and their like, 125 instructions to each 16 products, for half of it (180 us, 766 TFLOP/s, with four heads to one of the cache; 236 over 8-bit
+// integers); a token over 1000 entries 13 us, the latency of two launches.
 #include <type_traits>
 
 #include "cache.hpp"
@@ -37,21 +42,21 @@ constexpr i64 MAX_PARTS = 128;                 // of a sequence's keys
 constexpr int CLEARING = 64;                   // workgroups that look for rows of no sequence
 constexpr float LATE = 8.0f;                   // powers of two that scores may exceed what they are relative to
 
-// DT: of queries and outputs; I8: the cache has 8-bit integers; DP: columns, at least the cache's; OCC: workgroups of a CU
+// DT: of queries and outputs; I8: the cache has 8-bit integers, whose products are taken in fp16; DP: columns, at least the cache's; OCC: workgroups of a CU
 template <int DT_, bool I8_, int DP_, int WM_, int WK_, int OCC_>
 struct Form {
-    static constexpr int DT = DT_, DP = DP_, WM = WM_, WK = WK_, ST = WM > 1 ? 2 : 1;
-    static constexpr bool I8 = I8_, WIDE = I8 && WM > 1;               // WIDE: 8-bit integers lie in LDS as 16-bit numbers
+    static constexpr int DT = DT_, CT = I8_ ? VI_F16 : DT_, DP = DP_, WM = WM_, WK = WK_, ST = WM > 1 ? 2 : 1;
+    static constexpr bool I8 = I8_;
     static constexpr int WAVES = WM * WK, THREADS = 64 * WAVES, ROWS = 32 * WM, OCC = OCC_ * WAVES / 4 > 0 ? OCC_ * WAVES / 4 : 1;           // wavefronts of a SIMD
     static constexpr int KEYS = WM > 1 ? 64 : 32, GROUPS = KEYS / 16;  // of a stage; sixteen keys are of one page
-    static constexpr int ROW = DP * (I8 && !WIDE ? 1 : 2), UNITS = ROW / 16, PER_LOAD = 64 / UNITS, LOADS = 16 / PER_LOAD;       // bytes, units; rows of a load, loads of a group
+    static constexpr int ROW = DP * (I8 ? 1 : 2), UNITS = ROW / 16, PER_LOAD = 64 / UNITS, LOADS = 16 / PER_LOAD;       // bytes, units; rows of a load, loads of a group
     static constexpr int SCALES = I8 ? KEYS * 4 : 0, HALF = KEYS * ROW + SCALES, STAGE = 2 * HALF;
     static constexpr int MINE = GROUPS * LOADS / WM, KINDS = LOADS > WM ? LOADS / WM : 1;              // loads of a wavefront in half a stage, different ones of a group
     static constexpr int PITCH = 36;           // floats between rows of 32 on their way out
     static constexpr int OUT = WAVES * 32 * PITCH * 4 + WAVES * 32 * 8 + ROWS * 8;
     static constexpr int LDS = WK * ST * STAGE > OUT ? WK * ST * STAGE : OUT;
     static constexpr int MASKS = ROWS < MAX_NODES ? ROWS : MAX_NODES;
-    static_assert(WIDE || (GROUPS * LOADS % WM == 0 && (LOADS % WM == 0 || WM % LOADS == 0)), "loads of a stage");
+    static_assert(GROUPS * LOADS % WM == 0 && (LOADS % WM == 0 || WM % LOADS == 0) && (WM == 1 ? GROUPS == 2 : GROUPS == WM), "loads of a stage");
 };
 
 struct Args {
@@ -117,15 +122,26 @@ __device__ __forceinline__ u32 pack(float a, float b) {
     typedef typename type<DT>::t v2t __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(u32, __builtin_convertvector((v2f{a, b}), v2t));
 }
-// eight 8-bit integers as bfloat16: exact
+// Eight 8-bit integers, + 128 and so 0 to 255, as the fp16 numbers that these are as they lie: 2^-24 of them, below the smallest normal number, which the matrix
+// instructions take as it is.  Of each four the first and third come first, then the other two (in two_of's order).
+constexpr float OF_BYTES = 0x1p24f, MIDDLE = 128.0f;
 __device__ __forceinline__ v4u widen(v2u w) {
     v4u r;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const u32 s = w[i / 2] >> (16 * (i & 1));
-        r[i] = pack<VI_BF16>((float)(signed char)s, (float)(signed char)(s >> 8));
+    for (int i = 0; i < 2; ++i) {
+        const u32 u = w[i] ^ 0x80808080u;
+        r[2 * i] = u & 0x00FF00FFu, r[2 * i + 1] = __builtin_amdgcn_perm(u, u, 0x0C030C01u);
     }
     return r;
+}
+
+__device__ __forceinline__ int two_of(int i) { return i / 2 * 4 + i % 2; }            // the first of word i
+__device__ __forceinline__ float element_of(v4u w, int i) { return (float)__builtin_bit_cast(_Float16, (unsigned short)(w[i / 2] >> (16 * (i & 1)))); }
+// the sum of both halves of a word and c
+__device__ __forceinline__ float add_two(u32 w, float c) {
+    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+    const v2h ones = {(_Float16)1.0f, (_Float16)1.0f};
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), ones, c, false);
 }
 
 template <int DT>
@@ -139,6 +155,10 @@ __device__ __forceinline__ v16f multiply(v4u a, v4u b, v16f c) {
 __device__ __forceinline__ float most_of_halves(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_of_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 __device__ __forceinline__ int same(int v) { return (int)__builtin_amdgcn_readfirstlane((u32)v); }
 
@@ -176,8 +196,8 @@ __device__ __forceinline__ int parts_of(const Args &A, int end) { return max(1, 
 // ---- the pass over the keys ---------------------------------------------------------------------------------------
 template <class F>
 __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
-    constexpr int DT = F::DT, DP = F::DP, WM = F::WM, WK = F::WK, ROW = F::ROW, UNITS = F::UNITS;
-    constexpr bool NARROW = F::I8 && !F::WIDE;                         // 8-bit integers in LDS
+    constexpr int DT = F::DT, CT = F::CT, DP = F::DP, WM = F::WM, WK = F::WK, ROW = F::ROW, UNITS = F::UNITS;
+    constexpr bool NARROW = F::I8;             // 8-bit integers in LDS
     typedef typename type<DT>::t T;
     __shared__ char lds[F::LDS] __attribute__((aligned(16)));
     __shared__ u32 masks[F::MASKS * MASK_WORDS];
@@ -214,10 +234,35 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
         const T *x = (const T *)A.q + ((i64)t.s0 + (there ? tok : 0)) * A.q_token + (head * A.group + (there ? row - tok * A.group : 0)) * A.q_head;
 #pragma unroll
         for (int st = 0; st < DP / 16; ++st) {
-            const int chunk = F::I8 && !F::WIDE ? 4 * (st / 2) + 2 * half + st % 2 : 2 * st + half;
+            const int chunk = NARROW ? 4 * (st / 2) + 2 * half + st % 2 : 2 * st + half;
             q[st] = v4u{0, 0, 0, 0};
             if (there && chunk * 8 < A.cache.dim) q[st] = load_any<v4u>(x + chunk * 8);
         }
+    }
+    // For 8-bit integers a row's queries are fp16, their largest brought to 2^14 by a power of two, which goes into what its scores are multiplied by: exact, but for
+    // numbers 2^28 times smaller than the largest.  What the integers are more than themselves is taken off from the start.
+    float c = A.c, start = 0;
+    if constexpr (F::I8) {
+        auto number = [](const v4u &w, int i) INLINE { return __uint_as_float(i & 1 ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16); };          // bfloat16
+        float largest = 0;
+#pragma unroll
+        for (int st = 0; st < DP / 16; ++st)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(number(q[st], i)));
+        const u32 exponent = __float_as_uint(most_of_halves(largest)) >> 23, e = exponent == 255 ? 141 : max(exponent, 15u);
+        const float by = __uint_as_float((268 - e) << 23);
+        c *= __uint_as_float((e - 14) << 23);
+        c *= OF_BYTES;
+#pragma unroll
+        for (int st = 0; st < DP / 16; ++st) {
+            v4u r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = pack<CT>(number(q[st], two_of(i)) * by, number(q[st], two_of(i) + 2) * by);
+            q[st] = r;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) start += element_of(r, i);
+        }
+        start = sum_of_halves(start) * (-MIDDLE / OF_BYTES);
     }
 
     // ---- stages
@@ -297,10 +342,14 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
                 else *(v4u *)(lds + (at - lds_at) + lane * 16) = v4u{0, 0, 0, 0};
             }
         }
-        if constexpr (F::I8 && !F::WIDE) {
-            const int one = number_of(p, 0), two = number_of(p, 1), jj = j + (lane & 16), number = lane & 16 ? two : one;
-            const u32 at = place + F::KEYS * ROW;
-            if (lane < 32) {
+        if constexpr (F::I8) {                 // a scale a lane: a wavefront alone has the stage's 32, four have sixteen each
+            constexpr int SCALES = F::KEYS / WM;
+            const int g = WM == 1 ? lane >> 4 & 1 : wm, jj = j + 16 * g;
+            int number = number_of(p, 0);
+#pragma unroll
+            for (int o = 1; o < F::GROUPS; ++o) number = g == o ? number_of(p, o) : number;
+            const u32 at = place + F::KEYS * ROW + (WM == 1 ? 0 : wm * 64);
+            if (lane < SCALES) {
                 if ((lane & 15) < valid_of(number, jj)) fetch_words_to_lds(lds_at + at, scales_from[h] + number * A.cache.half[h].scale_page + (jj & row_mask) + (lane & 15));
                 else *(float *)(lds + at + lane * 4) = 0.0f;
             }
@@ -332,7 +381,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     v16f o[DP / 32];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) o[db] = v16f{};
-    float most = -INFINITY, relative = -INFINITY, sum = 0;             // largest score so far (or up to LATE behind), times c: what the sums are relative to
+    float most = -INFINITY, relative = -INFINITY, sum = 0, weighed = 0;             // largest score so far (or up to LATE behind), times c: what the sums are relative to
 
     // which of the 32 keys from j on the lane's row attends to; the low and the high sixteen have so many
     auto window_of = [&](int j, int low, int high) INLINE {
@@ -372,19 +421,31 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             for (int i = 0; i < (NARROW ? 1 : 2); ++i) asm volatile("" : "+v"(value_at[db][i]));
     }
 
-    // scores of 32 keys: k is their rows in LDS, `scales` theirs
-    auto scores = [&](const char *k, const char *scales) INLINE {
+    v16f starts;                               // kept in registers like those
+#pragma unroll
+    for (int r = 0; r < 16; ++r) starts[r] = start;
+    if constexpr (F::I8) asm volatile("" : "+v"(starts));
+    // Scores of 32 keys: k is their rows in LDS, `scales` theirs.  `beside(st)` is done between the products, two of the keys' units ahead of which are on their
+    // way.
+    auto scores_beside = [&](const char *k, const char *scales, auto beside) INLINE {
+        constexpr int READS = DP / 16 / (NARROW ? 2 : 1);
         v16f s = {};
-        if constexpr (NARROW) {
+        if constexpr (NARROW) s = starts;
+        v4u w[READS];
 #pragma unroll
-            for (int st = 0; st < DP / 16; st += 2) {
-                const v4u w = *(const v4u *)(k + key_at[st / 2]);
-                s = multiply<DT>(widen(v2u{w.x, w.y}), q[st], s);
-                s = multiply<DT>(widen(v2u{w.z, w.w}), q[st + 1], s);
+        for (int i = 0; i < 2; ++i) w[i] = *(const v4u *)(k + key_at[i]);
+#pragma unroll
+        for (int i = 0; i < READS; ++i) {
+            if (i + 2 < READS) w[i + 2] = *(const v4u *)(k + key_at[i + 2]);
+            if constexpr (NARROW) {
+                s = multiply<CT>(widen(v2u{w[i].x, w[i].y}), q[2 * i], s);
+                beside(2 * i);
+                s = multiply<CT>(widen(v2u{w[i].z, w[i].w}), q[2 * i + 1], s);
+                beside(2 * i + 1);
+            } else {
+                s = multiply<CT>(w[i], q[i], s);
+                beside(i);
             }
-        } else {
-#pragma unroll
-            for (int st = 0; st < DP / 16; ++st) s = multiply<DT>(*(const v4u *)(k + key_at[st]), q[st], s);
         }
         if constexpr (F::I8) {
 #pragma unroll
@@ -396,6 +457,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
         }
         return s;
     };
+    auto scores = [&](const char *k, const char *scales) INLINE { return scores_beside(k, scales, [](int) INLINE {}); };
 
     // V^T of 32 columns and 16 keys, in the order of the registers: four from 4 half on, four from 8 + 4 half on
     auto columns = [&](const char *v, int db, int st) INLINE {
@@ -418,35 +480,87 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
 #pragma unroll
         for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
         top = most_of_halves(top);
-        if (__any(top * A.c > relative + LATE)) {
+        if (__any(top * c > relative + LATE)) {
             asm volatile("");                  // a branch: the compiler would multiply by one, each time
-            const float now = fmaxf(most, top), then = now * A.c;
+            const float now = fmaxf(most, top), then = now * c;
             const float by = relative == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(relative - then);
-            most = now, relative = then, sum *= by;
+            most = now, relative = then, sum *= by, weighed *= by;
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db) o[db] *= by;
         }
     };
-    // the exponentials of scores, as the second operand of the product with V^T
-    auto weights = [&](const v16f &s, const char *scales, v4u (&p)[2]) INLINE {
-        const float base = relative == -INFINITY ? 0.0f : relative;
-        float e[16], add = 0;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            e[r] = __builtin_amdgcn_exp2f(fmaf(s[r], A.c, -base));
-            add += e[r];
-        }
-        sum += add;
+    // The exponentials of scores, as the second operand of the product with V^T.  Those that values' scales are multiplied into go by a power of two, a row's, that
+    // keeps scales below 2^6 and so products in fp16's range: the largest there are, or have been (LATE's 2^8 times 2^6).
+    float gain = 0x1p100f;
+    struct Scales {
+        float of[F::I8 ? 16 : 1];
+    };
+    auto scales_of = [&](const v16f &s, const char *scales, bool masked) INLINE {
+        Scales f = {};
         if constexpr (F::I8) {
+            float top = 0;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const v4f f = *(const v4f *)(scales + (8 * g + 4 * half) * 4);
+                const v4f four = *(const v4f *)(scales + (8 * g + 4 * half) * 4);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) e[4 * g + i] = s[4 * g + i] == -INFINITY ? 0.0f : e[4 * g + i] * f[i];       // a scale in a masked place may be a NaN
+                for (int i = 0; i < 4; ++i) f.of[4 * g + i] = four[i];
+            }
+            if (masked) {                      // a scale in a masked place may be anything
+                asm volatile("");
+#pragma unroll
+                for (int r = 0; r < 16; ++r) f.of[r] = s[r] == -INFINITY ? 0.0f : f.of[r];
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f.of[r]));
+            if (__any(top * gain > 64.0f)) {
+                asm volatile("");
+                float finite = 0;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) finite = fmaxf(finite, fabsf(f.of[r]) < INFINITY ? fabsf(f.of[r]) : 0.0f);
+                finite = most_of_halves(finite);
+                if (finite * gain > 64.0f) {
+                    const float now = __uint_as_float(max(254u - (__float_as_uint(finite) >> 23), 1u) << 23), by = now / gain;
+                    gain = now, weighed *= by;
+#pragma unroll
+                    for (int db = 0; db < DP / 32; ++db) o[db] *= by;
+                }
             }
         }
+        return f;
+    };
+    // word i of the operand
+    auto weigh = [&](const v16f &s, const Scales &f, float base, int i, v4u (&p)[2]) INLINE {
+        const int one = F::I8 ? i / 4 * 8 + two_of(i % 4) : 2 * i, two = F::I8 ? one + 2 : one + 1;
+        float a = __builtin_amdgcn_exp2f(fmaf(s[one], c, -base)), b = __builtin_amdgcn_exp2f(fmaf(s[two], c, -base));
+        sum += a + b;
+        if constexpr (F::I8) a = a * gain * f.of[one], b = b * gain * f.of[two];
+        const u32 w = pack<CT>(a, b);
+        p[i / 4][i % 4] = w;
+        if constexpr (F::I8) weighed = add_two(w, weighed);            // as rounded: what the integers are more than themselves goes by it
+    };
+    auto weights = [&](const v16f &s, const char *scales, bool masked, v4u (&p)[2]) INLINE {
+        const Scales f = scales_of(s, scales, masked);
+        const float base = relative == -INFINITY ? 0.0f : relative;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) p[i / 4][i % 4] = pack<DT>(e[2 * i], e[2 * i + 1]);
+        for (int i = 0; i < 8; ++i) weigh(s, f, base, i, p);
+    };
+    // The same with the next keys' scores beside them, product after product between the exponentials: in an order of its own, for the compiler would take the
+    // products one after the other, each of which waits for the one before (4096 tokens of a prompt 206 us so, 201 in this order).
+    auto weights_and_scores = [&](const v16f &s, const char *scales, bool masked, v4u (&p)[2], const char *k, const char *key_scales) INLINE {
+        const Scales f = scales_of(s, scales, masked);
+        const float base = relative == -INFINITY ? 0.0f : relative;
+        constexpr int PRODUCTS = DP / 16;
+        __builtin_amdgcn_sched_barrier(0);
+        return scores_beside(k, key_scales, [&](int st) INLINE {
+#pragma unroll
+            for (int i = st * 8 / PRODUCTS; i < (st + 1) * 8 / PRODUCTS; ++i) {
+                weigh(s, f, base, i, p);
+                u32 here = p[i / 4][i % 4];
+                asm volatile("" : "+v"(here)); // not behind the branches that follow
+                p[i / 4][i % 4] = here;
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
     };
 
     // 0 times an infinity or a NaN in a masked place would be a NaN.  Where keys are masked such values are left out of the products, and seen once more behind
@@ -480,8 +594,8 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
         for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                if constexpr (NARROW) o[db] = multiply<DT>(widen(v2u{w[db][st].x, w[db][st].y}), p[st], o[db]);
-                else o[db] = multiply<DT>(w[db][st], p[st], o[db]);
+                if constexpr (NARROW) o[db] = multiply<CT>(widen(v2u{w[db][st].x, w[db][st].y}), p[st], o[db]);
+                else o[db] = multiply<CT>(w[db][st], p[st], o[db]);
             }
     };
 
@@ -504,7 +618,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             if (now_whole) arrive<LOADS_OF_HALF>();
             else arrive<0>();
             meet_wave();
-            v16f s = {};
+            v16f s;                            // of keys that are needed
             if (needed) s = scores(k, k + F::KEYS * ROW);
             if (more) {
                 read();
@@ -519,7 +633,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             if (needed) {
                 v4u p[2];
                 settle(s, masked, masked ? window_of(j, low, high) : ~0u);
-                weights(s, v + F::KEYS * ROW, p);
+                weights(s, v + F::KEYS * ROW, masked, p);
                 add_values(v, p, masked);
             }
             if (more) {
@@ -534,51 +648,8 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
         // Keys that WM wavefronts share, a stage of 64 in two steps of 32.  The scores of a step's keys are taken in the step before, under the exponentials there:
         // the second step of a stage is the last that reads the stage's values and the first that reads the next one's keys, so that the values of stage
         // it + 1 are asked for in the first step of stage it, and the keys of stage it + 2 in the second; both have two steps to come.
-        auto key_rows = [&](int it, int kb) INLINE { return lds + place_of(0, it % 2) + kb * 32 * ROW; };
-        auto key_scales = [&](int it, int kb) INLINE { return lds + place_of(0, it % 2) + F::KEYS * ROW + kb * 128; };
-        // 8-bit integers are widened on their way, from registers; a thread has units of sixteen columns
-        constexpr int EIGHTS = DP / 16, MINE8 = F::KEYS * EIGHTS / (64 * WM);
-        const int unit8 = wm * 64 + lane;
-        struct Raw {
-            v4u w[MINE8];
-            float scale;
-        };
-        auto load_wide = [&](int h, int it, const Pages &p) INLINE {
-            Raw r;
-            const int j = stage_key(it);
-            auto address = [&](int key, int *valid) INLINE {
-                int number = number_of(p, 0);
-#pragma unroll
-                for (int g = 1; g < F::GROUPS; ++g) number = key >> 4 == g ? number_of(p, g) : number;
-                *valid = valid_of(number, j + (key & ~15)) > (key & 15) ? number : -1;
-            };
-#pragma unroll
-            for (int l = 0; l < MINE8; ++l) {
-                const int n = l * 64 * WM + unit8, key = n / EIGHTS, u = n % EIGHTS;
-                int number;
-                address(key, &number);
-                r.w[l] = v4u{0, 0, 0, 0};
-                if (number >= 0 && u * 16 < A.cache.dim) r.w[l] = *(const v4u *)(from[h] + (u64)(u32)number * page_apart[h] + (u32)((j + key) & row_mask) * row_apart[h] + u * 16);
-            }
-            r.scale = 0;
-            if (unit8 < F::KEYS) {
-                int number;
-                address(unit8, &number);
-                if (number >= 0) r.scale = scales_from[h][number * A.cache.half[h].scale_page + ((j + unit8) & row_mask)];
-            }
-            return r;
-        };
-        auto store_wide = [&](int h, int it, const Raw &r) INLINE {
-            char *to = lds + place_of(h, it % 2);
-#pragma unroll
-            for (int l = 0; l < MINE8; ++l) {
-                const int n = l * 64 * WM + unit8, key = n / EIGHTS, u = n % EIGHTS, o_ = order<UNITS>(key & 15);
-                *(v4u *)(to + key * ROW + ((2 * u) ^ o_) * 16) = widen(v2u{r.w[l].x, r.w[l].y});
-                *(v4u *)(to + key * ROW + ((2 * u + 1) ^ o_) * 16) = widen(v2u{r.w[l].z, r.w[l].w});
-            }
-            if (unit8 < F::KEYS) *(float *)(to + F::KEYS * ROW + unit8 * 4) = r.scale;
-        };
-        Raw raw_keys = {}, raw_values = {};
+        auto key_rows = [&](int slot, int kb) INLINE { return lds + place_of(0, slot) + kb * 32 * ROW; };
+        auto key_scales = [&](int slot, int kb) INLINE { return lds + place_of(0, slot) + F::KEYS * ROW + kb * 128; };
         v16f s = {};
         Pages next = {}, behind = {};          // of stages it + 1 and it + 2
         bool all = false, next_all = false;    // whether stages it and it + 1 are whole
@@ -588,22 +659,14 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             if (stages > 1) next = look_up(1);
             next_all = stages > 1 && whole(next, stage_key(1));
             if (stages > 2) behind = look_up(2);
-            if constexpr (F::WIDE) {
-                store_wide(0, 0, load_wide(0, 0, now));
-                store_wide(1, 0, load_wide(1, 0, now));
-                if (stages > 1) store_wide(0, 1, load_wide(0, 1, next)), raw_values = load_wide(1, 1, next);
-                if (stages > 2) raw_keys = load_wide(0, 2, behind);
-                read();
-            } else {
-                fetch(0, place_of(0, 0), stage_key(0), now, all);
-                fetch(1, place_of(1, 0), stage_key(0), now, all);
-                if (stages > 1) fetch(0, place_of(0, 1), stage_key(1), next, next_all);
-                arrive<0>();
-            }
+            fetch(0, place_of(0, 0), stage_key(0), now, all);
+            fetch(1, place_of(1, 0), stage_key(0), now, all);
+            if (stages > 1) fetch(0, place_of(0, 1), stage_key(1), next, next_all);
+            arrive<0>();
             meet_group();
             s = scores(key_rows(0, 0), key_scales(0, 0));
         }
-        auto step = [&](int it, int kb, const char *k, const char *scales) INLINE {
+        auto step = [&](int it, auto slot, int kb, const char *k, const char *scales) INLINE {
             const int j = stage_key(it) + 32 * kb;
             if (j >= wave_end) return;
             int low = 16, high = 16;
@@ -613,41 +676,34 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             }
             const bool masked = low < 16 || high < 16 || j + 32 > wave_free;
             settle(s, masked, masked ? window_of(j, low, high) : ~0u);
-            const v16f ahead = scores(k, scales);      // behind the last stage: of what lies there, and not used
             v4u p[2];
-            weights(s, lds + place_of(1, it % 2) + F::KEYS * ROW + kb * 128, p);
-            add_values(lds + place_of(1, it % 2) + kb * 32 * ROW, p, masked);
+            const v16f ahead = weights_and_scores(s, lds + place_of(1, decltype(slot)::value) + F::KEYS * ROW + kb * 128, masked, p, k, scales);      // behind the last stage: of what lies there, and not used
+            add_values(lds + place_of(1, decltype(slot)::value) + kb * 32 * ROW, p, masked);
             s = ahead;
         };
         auto arrived = [&]() INLINE {          // all but what was asked for in the step before, which is of stage it + 1
-            if constexpr (F::WIDE) {
-                read();
-            } else {
-                if (next_all) arrive<LOADS_OF_HALF>();
-                else arrive<0>();
-            }
+            if (next_all) arrive<LOADS_OF_HALF>();
+            else arrive<0>();
             meet_group();
         };
-#pragma unroll 1
-        for (int it = 0; it < stages; ++it) {
+        // `slot` is it % 2 and known, so that places in LDS are in the instructions (201 us with it % 2 in registers, 198)
+        auto stage = [&](int it, auto slot) INLINE {
+            constexpr int own = decltype(slot)::value, other = 1 - own;
             arrived();
-            if (!F::WIDE && it + 1 < stages) fetch(1, place_of(1, (it + 1) % 2), stage_key(it + 1), next, next_all);
-            step(it, 0, key_rows(it, 1), key_scales(it, 1));
-            if constexpr (F::WIDE) {
-                if (it + 1 < stages) store_wide(1, it + 1, raw_values);
-                if (it + 2 < stages) raw_values = load_wide(1, it + 2, behind);
-            }
+            if (it + 1 < stages) fetch(1, place_of(1, other), stage_key(it + 1), next, next_all);
+            step(it, slot, 0, key_rows(own, 1), key_scales(own, 1));
             arrived();
             const bool behind_all = it + 2 < stages && whole(behind, stage_key(it + 2));
-            if (!F::WIDE && it + 2 < stages) fetch(0, place_of(0, it % 2), stage_key(it + 2), behind, behind_all);
+            if (it + 2 < stages) fetch(0, place_of(0, own), stage_key(it + 2), behind, behind_all);
             next = behind;
             if (it + 3 < stages) behind = look_up(it + 3);
-            step(it, 1, key_rows(it + 1, 0), key_scales(it + 1, 0));
-            if constexpr (F::WIDE) {
-                if (it + 2 < stages) store_wide(0, it + 2, raw_keys);
-                if (it + 3 < stages) raw_keys = load_wide(0, it + 3, behind);
-            }
+            step(it, slot, 1, key_rows(other, 0), key_scales(other, 0));
             all = next_all, next_all = behind_all;
+        };
+#pragma unroll 1
+        for (int it = 0; it < stages; it += 2) {
+            stage(it, std::integral_constant<int, 0>());
+            if (it + 1 < stages) stage(it + 1, std::integral_constant<int, 1>());
         }
     }
 
@@ -683,8 +739,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     __syncthreads();
     float *buf = (float *)lds, *of_waves = buf + F::WAVES * 32 * F::PITCH, *of_rows = of_waves + F::WAVES * 32 * 2;
     {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(sum), __float_as_uint(sum), false, false);
-        sum = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+        sum = sum_of_halves(sum);
         if (half == 0) of_waves[(wave * 32 + lane) * 2] = relative, of_waves[(wave * 32 + lane) * 2 + 1] = sum;
     }
     __syncthreads();
@@ -697,7 +752,14 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
         const float *x = of_waves + ((w * WM + wm) * 32 + (lane & 31)) * 2;
         total += __builtin_amdgcn_exp2f(x[0] - base) * x[1];
     }
-    const float factor = __builtin_amdgcn_exp2f(relative - base);
+    const float factor = __builtin_amdgcn_exp2f(relative - base) * (F::I8 ? 1.0f / gain : 1.0f);
+    if constexpr (F::I8) {
+        const float more = sum_of_halves(weighed) * -MIDDLE;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[db][r] = fmaf(o[db][r], OF_BYTES, more);
+    }
     if (part == 0 && half == 0) of_rows[(wm * 32 + lane) * 2] = top, of_rows[(wm * 32 + lane) * 2 + 1] = total;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) {
@@ -762,8 +824,7 @@ __global__ __launch_bounds__(JOIN) void k_join(Args A) {
 }
 
 // ---- forms --------------------------------------------------------------------------------------------------------
-// Up to 32 rows of a sequence: four wavefronts (two where columns are many) with keys of their own; up to 64: the same, two products of each operand of
-// keys or values; more: four wavefronts' rows share the keys.
+// Few rows of a sequence: four wavefronts with keys of their own.  Many: four wavefronts' rows share the keys.
 template <int DT, bool I8, int DP>
 struct Few : Form<DT, I8, DP, 1, 4, (DP > 128 ? 1 : 2)> {};
 template <int DT, bool I8, int DP>
@@ -781,14 +842,14 @@ Plan make_plan(int cache_dtype, i64 dim, i64 cache_heads, i64 n, i64 heads, i64 
     const i64 group = heads / cache_heads, rows = (n * group + sequences - 1) / sequences;           // of a sequence, on an average
     L.dp = dim <= 64 ? 64 : dim <= 128 ? 128 : 256;
     // A tile of 128 rows reads its keys once, but its wavefronts wait for each other: 64 sequences of 64 rows over 4096 entries take 239 us as two tiles of
-    // 32, 308 as one of 64 whose wavefronts share the keys; 16 of 100 rows 91 us as four tiles, 82 as one of 128, but over 8-bit integers, which are
-    // widened on a longer way there, 98 and 103.
+    // 32, 308 as one of 64 whose wavefronts share the keys; 16 of 100 rows 91 us as four tiles, 82 as one of 128, but over 8-bit integers, of which
+    // there are half the bytes to read, 87 and 92.
     L.form = rows <= (cache_dtype == VI_I8 ? 128 : 64) ? FEW : MANY;
     L.rows = L.form == FEW ? 32 : 128;
     const i64 tiles = n * group / L.rows + sequences, full = (n * group + L.rows - 1) / L.rows, busy = full > sequences ? full : sequences;
     L.tiles = (int)(tiles < MAX_BLOCKS ? tiles : MAX_BLOCKS);
     // The keys are cut into parts of one size where there are few tiles: two workgroups a CU, as many as there is room for (a sequence of 32768 entries,
-    // 8 heads: 54 us, 64 with four a CU), or four where sequences alone make two, for their lengths differ (attend_batch's 64 of 500 to 8192: 224 us, 237 uncut).  A
+    // 8 heads: 54 us, 64 with four a CU), or four where sequences alone make two, for their lengths differ (64 of 500 to 8192: 224 us, 237 uncut).  A
     // part has 128 keys at least, a round of a workgroup's wavefronts, and 512 where there are many.
     const i64 all = busy * cache_heads, wanted = (all < 2 * CUS ? 2 : 4) * CUS, parts = wanted / all, round = 128, least = all >= CUS ? 4 * round : round;
     i64 keys = parts > 1 ? (longest + parts - 1) / parts : longest;
