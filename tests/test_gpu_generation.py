@@ -447,6 +447,43 @@ def test_attention_writes_where_it_should():
     assert torch.equal(gen.attend_cache(wide, m.cache, m.batch), want)
 
 
+@pytest.mark.parametrize("new", [[3, 1], [40, 70]])
+@pytest.mark.parametrize("low,high", [(-110, -90), (-60, 60), (60, 90), (-2, 2)])
+def test_value_scales_of_any_size(new, low, high):
+    """Scales that differ by 2^(high - low) from entry to entry, some of them 0; a token does not see those behind it, however large."""
+    m = Made(torch.int8, [300, 20], new, 2, 128, 16)
+    g = seeded(low, high)
+    power = torch.randint(low, high + 1, m.cache.value_scales.shape, generator=g)
+    scales = torch.ldexp(torch.rand(power.shape, generator=g) + 1, power)
+    scales[torch.rand(power.shape, generator=g) < 0.1] = 0.0
+    m.cache.value_scales.copy_(scales)
+    q = normal((m.n, 4, 128), g, torch.bfloat16)
+    got, (want, size, far) = gen.attend_cache(q, m.cache, m.batch, scale=0.3).cpu().double(), attend64(m, q, 2, scale=0.3)
+    # Where a column's values of the largest weights are 0 or small, `size` is small beside what these weights are rounded with.  The weights p f are fp16, the largest of
+    # a row 1 or more: each is 2^-12 of itself off, or 2^-25 of the largest where that is more, times values up to 128.  Their sums in 32 bits, a rounding a product of
+    # 16 keys and eight for those of partial sums, are of values up to 256: with W the sum of the weights, count 2^-25 128 W + (count / 16 + 8) 2^-24 256 W.
+    m.cache.values.fill_(1)
+    whole, count = attend64(m, q, 2, scale=0.3)[0], 300 + new[0]
+    r = ROUND[torch.bfloat16]
+    off = (r + 4 * far + 2.0 ** -20) * size + (count * 2.0 ** -18 + (count / 16 + 8) * 2.0 ** -16) * whole + LEAST[torch.bfloat16]
+    assert ((got - want).abs() <= off + r * (want.abs() + off)).all()
+
+
+@pytest.mark.parametrize("power", [-120, -30, 30, 110])
+def test_queries_of_any_size(power):
+    """Rows whose queries differ in size, with scales of keys that bring their scores back."""
+    m = Made(torch.int8, [100], [40], 1, 96, 16)
+    q = normal((40, 2, 96), seeded(power), torch.bfloat16)
+    q[::3] *= 2.0 ** -20
+    far = torch.ldexp(q.double(), torch.tensor(power).cuda()).to(torch.bfloat16)
+    q = torch.ldexp(far.double(), torch.tensor(-power).cuda()).to(torch.bfloat16)      # without the digits that bfloat16 has not down there
+    want = gen.attend_cache(q, m.cache, m.batch)
+    m.cache.key_scales.copy_(torch.ldexp(m.cache.key_scales, torch.tensor(-power).cuda()))
+    got = gen.attend_cache(far, m.cache, m.batch)
+    assert torch.equal(got[1::3], want[1::3]) and torch.equal(got[2::3], want[2::3])
+    assert ((got - want).abs().float() <= 2.0 ** -8 * 2 * 4).all()     # two roundings of values up to 4; the small queries may have lost digits
+
+
 def test_large_scores():
     """Scores up to 10^4, one far above the rest, and equal ones."""
     m = Made(torch.bfloat16, [700], [1], 1, 128, 16)
@@ -489,7 +526,8 @@ def verify64(logits, tokens, starts, parents, u, depth, draft, temperature):
         def p_of(x, i):
             z = x[s0 + i].double() / temperature
             good = (z < math.inf).all() and (z > -math.inf).any()
-            return torch.softmax(z, dim=0) if good else None
+            e = torch.exp(z - z.max())             # torch.softmax on the GPU has no probabilities below 2^-126
+            return e / e.sum() if good else None
 
         path, p = [0], p_of(logits, 0)
         first = p
@@ -592,6 +630,20 @@ def test_drafts_that_are_hard_to_verify():
         check_drafts(logits, tokens, starts, parents, u, d, 4)
     check_drafts(logits, tokens, [0, 0, 6, 6, 40, 72], parents, u, draft, 3)           # sequences of nothing, and of other lengths
     check_drafts(logits, tokens, [5, 9], parents, u, draft, 3)                         # rows of no sequence
+
+
+def test_rows_that_rise_and_fall():
+    """Logits over many powers of two, in an order in which the largest come last, first or anywhere, in long rows."""
+    for v in (5000, 200001):
+        up = torch.linspace(-300, 300, v)
+        logits = torch.stack((up, up.flip(0), up[torch.randperm(v, generator=seeded(v))], up * 0.01))
+        draft = logits + torch.randn(4, v, generator=seeded(v, 1))
+        draft[1, :v // 2] = -math.inf
+        u = torch.rand(4, generator=seeded(v, 2), dtype=torch.float64)
+        for tokens in ([0, v - 1, 0, 5], [0, 3, int(logits[2].argmax()), 7]):
+            for d in (draft, None):
+                check_drafts(logits, tokens, [0, 4], [-1, 0, 0, 0], u, d, 3)
+                check_drafts(logits, tokens, [0, 4], [-1, 0, 1, 2], u, d, 3, temperature=30.0)
 
 
 def test_a_refused_token_of_everything():

@@ -40,6 +40,7 @@ constexpr i64 MAX_BLOCKS = 1 << 22;            // of a launch, which has less th
 constexpr i64 MAX_HEADS = 1 << 30;             // of all tokens together
 constexpr i64 MAX_PARTS = 128;                 // of a sequence's keys
 constexpr int CLEARING = 64;                   // workgroups that look for rows of no sequence
+constexpr float MAX_GAIN = 0x1p126f;
 constexpr float LATE = 8.0f;                   // powers of two that scores may exceed what they are relative to
 
 // DT: of queries and outputs; I8: the cache has 8-bit integers, whose products are taken in fp16; DP: columns, at least the cache's; OCC: workgroups of a CU
@@ -251,8 +252,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(number(q[st], i)));
         const u32 exponent = __float_as_uint(most_of_halves(largest)) >> 23, e = exponent == 255 ? 141 : max(exponent, 15u);
         const float by = __uint_as_float((268 - e) << 23);
-        c *= __uint_as_float((e - 14) << 23);
-        c *= OF_BYTES;
+        c = c * OF_BYTES * __uint_as_float((e - 14) << 23);            // in this order a normal number
 #pragma unroll
         for (int st = 0; st < DP / 16; ++st) {
             v4u r;
@@ -381,7 +381,9 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     v16f o[DP / 32];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) o[db] = v16f{};
-    float most = -INFINITY, relative = -INFINITY, sum = 0, weighed = 0;             // largest score so far (or up to LATE behind), times c: what the sums are relative to
+    // For 8-bit integers, exponentials times scales are multiplied by `gain` to be in fp16's range: a power of two at first, 2^14 at most of the largest so far.
+    float gain = MAX_GAIN, weighed = 0;
+    float most = -INFINITY, relative = -INFINITY, sum = 0;             // largest score so far (or up to LATE behind), times c: what the sums are relative to
 
     // which of the 32 keys from j on the lane's row attends to; the low and the high sixteen have so many
     auto window_of = [&](int j, int low, int high) INLINE {
@@ -484,41 +486,63 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             asm volatile("");                  // a branch: the compiler would multiply by one, each time
             const float now = fmaxf(most, top), then = now * c;
             const float by = relative == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(relative - then);
-            most = now, relative = then, sum *= by, weighed *= by;
+            most = now, relative = then, sum *= by;
+            float less = by;                   // of the products' sums: where they have a power of their own that follows
+            if constexpr (F::I8) {
+                const float more = fminf(gain / by, MAX_GAIN);
+                less = more < MAX_GAIN ? 1.0f : by * (more / gain);
+                gain = more, weighed *= less;
+            }
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db) o[db] *= by;
+            for (int db = 0; db < DP / 32; ++db) o[db] *= less;
         }
     };
-    // The exponentials of scores, as the second operand of the product with V^T.  Those that values' scales are multiplied into go by a power of two, a row's, that
-    // keeps scales below 2^6 and so products in fp16's range: the largest there are, or have been (LATE's 2^8 times 2^6).
-    float gain = 0x1p100f;
-    struct Scales {
-        float of[F::I8 ? 16 : 1];
+    // The exponentials of scores, as the second operand of the product with V^T.
+    struct Weights {
+        float of[16];
     };
+    // values' scales; in a masked place there may be anything
     auto scales_of = [&](const v16f &s, const char *scales, bool masked) INLINE {
-        Scales f = {};
+        Weights f = {};
         if constexpr (F::I8) {
-            float top = 0;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const v4f four = *(const v4f *)(scales + (8 * g + 4 * half) * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) f.of[4 * g + i] = four[i];
             }
-            if (masked) {                      // a scale in a masked place may be anything
+            if (masked) {
                 asm volatile("");
 #pragma unroll
                 for (int r = 0; r < 16; ++r) f.of[r] = s[r] == -INFINITY ? 0.0f : f.of[r];
             }
+        }
+        return f;
+    };
+    // two exponentials, times their scales; the pair goes into word i of the operand
+    auto weigh = [&](const v16f &s, Weights &f, float base, int i) INLINE {
+        const int one = F::I8 ? i / 4 * 8 + two_of(i % 4) : 2 * i, two = F::I8 ? one + 2 : one + 1;
+        const float a = __builtin_amdgcn_exp2f(fmaf(s[one], c, -base)), b = __builtin_amdgcn_exp2f(fmaf(s[two], c, -base));
+        sum += a + b;
+        f.of[one] = F::I8 ? a * f.of[one] : a, f.of[two] = F::I8 ? b * f.of[two] : b;
+    };
+    auto word_of = [&](const Weights &f, int i) INLINE {
+        const int one = F::I8 ? i / 4 * 8 + two_of(i % 4) : 2 * i, two = F::I8 ? one + 2 : one + 1;
+        return F::I8 ? pack<CT>(f.of[one] * gain, f.of[two] * gain) : pack<CT>(f.of[one], f.of[two]);
+    };
+    // For 8-bit integers: in fp16's range, and what the integers are more than themselves goes by them as rounded
+    auto words_of = [&](const Weights &f, v4u (&p)[2]) INLINE {
+        if constexpr (F::I8) {
+            float top = 0;
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(f.of[r]));
-            if (__any(top * gain > 64.0f)) {
+            if (__any(top * gain > 0x1p14f)) {
                 asm volatile("");
                 float finite = 0;
 #pragma unroll
                 for (int r = 0; r < 16; ++r) finite = fmaxf(finite, fabsf(f.of[r]) < INFINITY ? fabsf(f.of[r]) : 0.0f);
                 finite = most_of_halves(finite);
-                if (finite * gain > 64.0f) {
+                if (finite * gain > 0x1p14f) {
                     const float now = __uint_as_float(max(254u - (__float_as_uint(finite) >> 23), 1u) << 23), by = now / gain;
                     gain = now, weighed *= by;
 #pragma unroll
@@ -526,41 +550,40 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
                 }
             }
         }
-        return f;
-    };
-    // word i of the operand
-    auto weigh = [&](const v16f &s, const Scales &f, float base, int i, v4u (&p)[2]) INLINE {
-        const int one = F::I8 ? i / 4 * 8 + two_of(i % 4) : 2 * i, two = F::I8 ? one + 2 : one + 1;
-        float a = __builtin_amdgcn_exp2f(fmaf(s[one], c, -base)), b = __builtin_amdgcn_exp2f(fmaf(s[two], c, -base));
-        sum += a + b;
-        if constexpr (F::I8) a = a * gain * f.of[one], b = b * gain * f.of[two];
-        const u32 w = pack<CT>(a, b);
-        p[i / 4][i % 4] = w;
-        if constexpr (F::I8) weighed = add_two(w, weighed);            // as rounded: what the integers are more than themselves goes by it
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            p[i / 4][i % 4] = word_of(f, i);
+            if constexpr (F::I8) weighed = add_two(p[i / 4][i % 4], weighed);
+        }
     };
     auto weights = [&](const v16f &s, const char *scales, bool masked, v4u (&p)[2]) INLINE {
-        const Scales f = scales_of(s, scales, masked);
+        Weights f = scales_of(s, scales, masked);
         const float base = relative == -INFINITY ? 0.0f : relative;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) weigh(s, f, base, i, p);
+        for (int i = 0; i < 8; ++i) weigh(s, f, base, i);
+        words_of(f, p);
     };
     // The same with the next keys' scores beside them, product after product between the exponentials: in an order of its own, for the compiler would take the
     // products one after the other, each of which waits for the one before (4096 tokens of a prompt 206 us so, 201 in this order).
     auto weights_and_scores = [&](const v16f &s, const char *scales, bool masked, v4u (&p)[2], const char *k, const char *key_scales) INLINE {
-        const Scales f = scales_of(s, scales, masked);
+        Weights f = scales_of(s, scales, masked);
         const float base = relative == -INFINITY ? 0.0f : relative;
         constexpr int PRODUCTS = DP / 16;
         __builtin_amdgcn_sched_barrier(0);
-        return scores_beside(k, key_scales, [&](int st) INLINE {
+        const v16f ahead = scores_beside(k, key_scales, [&](int st) INLINE {
 #pragma unroll
             for (int i = st * 8 / PRODUCTS; i < (st + 1) * 8 / PRODUCTS; ++i) {
-                weigh(s, f, base, i, p);
-                u32 here = p[i / 4][i % 4];
-                asm volatile("" : "+v"(here)); // not behind the branches that follow
-                p[i / 4][i % 4] = here;
+                weigh(s, f, base, i);
+                if constexpr (!F::I8) {
+                    u32 here = word_of(f, i);
+                    asm volatile("" : "+v"(here));                     // not behind the branches that follow
+                    p[i / 4][i % 4] = here;
+                }
             }
             __builtin_amdgcn_sched_barrier(0);
         });
+        if constexpr (F::I8) words_of(f, p);
+        return ahead;
     };
 
     // 0 times an infinity or a NaN in a masked place would be a NaN.  Where keys are masked such values are left out of the products, and seen once more behind
