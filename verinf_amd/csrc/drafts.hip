@@ -587,6 +587,8 @@ i64 slices_of(int64_t v, int64_t rows) { return (v + per_slice_of(v, rows) - 1) 
 i64 firsts_of(int64_t v, int64_t n) { return min((v + BLOCK * EIGHT - 1) / (BLOCK * EIGHT), max((i64)4, min((i64)16, 4096 / max(n, (i64)1)))); }
 
 // ---- the path's entries -------------------------------------------------------------------------------------------
+// A thread moves one place of all entries of a path.  64 paths of up to eight entries in 256 heads of 128 columns and 8 bits: 14 us, of which reading and writing the rows,
+// 128 bytes each in pages of their own, would be 7; a path in 8 heads 4.7: a load behind the other, of numbers, page and entry.
 struct Keep {
     Cache cache;
     Batch batch;
