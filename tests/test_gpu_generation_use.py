@@ -299,3 +299,21 @@ def test_functions_refuse():
     refused("nodes must", gen.keep_drafts, m.cache, m.batch, i64(2, 3), i64(1))
     refused("counts has", gen.keep_drafts, m.cache, m.batch, i64(1, 3), i64(2))
     refused("depth", gen.keep_drafts, m.cache, m.batch, i64(1, 257), i64(1))
+
+
+def test_what_a_call_has_checked_cannot_be_changed():
+    """A batch's other lengths would be read from where the first ones lay."""
+    m = Made(torch.int8, [10], [3], 2, 64, 16)
+    for thing, names in ((m.batch, ("starts", "lengths", "pages")), (m.cache, ("keys", "values", "key_scales", "value_scales")), (gen.rotary_plan(64), ("steps", "rotated"))):
+        for name in names:
+            with pytest.raises(AttributeError, match="cannot be changed"):
+                setattr(thing, name, getattr(thing, name))
+            with pytest.raises(AttributeError):
+                delattr(thing, name)
+    with pytest.raises(RuntimeError, match="steps"):
+        gen.RotaryPlan(gen.rotary_plan(32).steps, 64, False, 1.0)
+    # what the tensors hold is read anew
+    q = normal((3, 4, 64), seeded(1), torch.bfloat16)
+    first = gen.attend_cache(q, m.cache, m.batch)
+    m.batch.lengths.fill_(5)
+    assert not torch.equal(gen.attend_cache(q, m.cache, m.batch), first)

@@ -58,12 +58,28 @@ def _overlaps(t):
     return False
 
 
-class RotaryPlan:
-    """Frequencies as whole numbers of 2^-64 turns a position, so that the angle of any position is exact."""
+class _Fixed:
+    """What is checked once and goes into every call as it is: made anew where it is to be another."""
+    __slots__ = ()
+
+    def _fix(self, **values):
+        for name, value in values.items():
+            object.__setattr__(self, name, value)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{type(self).__name__}.{name} cannot be changed: make another {type(self).__name__}")
+
+    __delattr__ = lambda self, name: self.__setattr__(name, None)              # noqa: E731
+
+
+class RotaryPlan(_Fixed):
+    """Frequencies as whole numbers of 2^-64 turns a position, so that the angle of any position is exact.  Cannot be changed."""
     __slots__ = ("steps", "rotated", "interleaved", "amplitude")
 
     def __init__(self, steps, rotated, interleaved, amplitude):
-        self.steps, self.rotated, self.interleaved, self.amplitude = steps, rotated, interleaved, amplitude
+        if steps.dtype != torch.int64 or steps.dim() != 1 or not steps.is_contiguous() or 2 * steps.shape[0] != rotated:
+            raise RuntimeError(f"a plan of {tuple(steps.shape)} steps for {rotated} columns")
+        self._fix(steps=steps, rotated=int(rotated), interleaved=bool(interleaved), amplitude=float(amplitude))
 
 
 def rotary_plan(dim, base=10000.0, interleaved=False, scaling=None, device="cuda"):
@@ -136,10 +152,10 @@ def rotate_heads(x, positions, plan, out=None):
     return out
 
 
-class Cache:
+class Cache(_Fixed):
     """A paged cache: keys and values (pages, heads, page_size, dim) bfloat16, float16 or int8, int8 with key_scales and value_scales
-    (pages, heads, page_size) float32.  Columns have unit stride, the rest any, so that views do: entries start at multiples of 16 bytes.
-    page_size a power of two from 16 to 1024, dim a multiple of 16 up to 256."""
+    (pages, heads, page_size) float32, of which an infinite one counts as NaN.  Columns have unit stride, the rest any, so that views do: entries start at multiples of 16 bytes.
+    page_size a power of two from 16 to 1024, dim a multiple of 16 up to 256.  Cannot be changed but in what its tensors hold: they are not resized."""
     __slots__ = ("keys", "values", "key_scales", "value_scales", "device", "_args")
 
     def __init__(self, keys, values, key_scales=None, value_scales=None):
@@ -168,10 +184,10 @@ class Cache:
                 raise RuntimeError(f"{name} go with a cache of int8")
             else:
                 scale_strides.append((ctypes.c_int64 * 2)())
-        self.keys, self.values, self.key_scales, self.value_scales, self.device = keys, values, key_scales, value_scales, dev
-        self._args = _lib.CacheArgs(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr() if scaled else None, value_scales.data_ptr() if scaled else None,
-                                    (ctypes.c_int64 * 3)(*keys.stride()[:3]), (ctypes.c_int64 * 3)(*values.stride()[:3]), *scale_strides,
-                                    pages, heads, size, dim, _KINDS[keys.dtype])
+        args = _lib.CacheArgs(keys.data_ptr(), values.data_ptr(), key_scales.data_ptr() if scaled else None, value_scales.data_ptr() if scaled else None,
+                              (ctypes.c_int64 * 3)(*keys.stride()[:3]), (ctypes.c_int64 * 3)(*values.stride()[:3]), *scale_strides,
+                              pages, heads, size, dim, _KINDS[keys.dtype])
+        self._fix(keys=keys, values=values, key_scales=key_scales, value_scales=value_scales, device=dev, _args=args)
 
 
 def new_cache(pages, heads, page_size, dim, dtype=torch.bfloat16, device="cuda"):
@@ -185,13 +201,13 @@ def new_cache(pages, heads, page_size, dim, dtype=torch.bfloat16, device="cuda")
     return Cache(both[:, 0], both[:, 1], scales[:, 0], scales[:, 1])
 
 
-class Batch:
+class Batch(_Fixed):
     """Which rows of the new tokens' tensors belong to which sequence, and where its entries lie: starts (sequences + 1,), rising,
     lengths (sequences,), the entries of a sequence with the new tokens', and pages (sequences, most pages), all int32.
 
     Entry j of a sequence lies in row j % page_size of page pages[b, j // page_size]; the new tokens' are its last.  Rows of no sequence are
     left alone.  A page outside the cache holds nothing: it is not written, what it should hold is masked.  Two sequences may share pages that
-    neither of them writes."""
+    neither of them writes.  Cannot be changed but in what its tensors hold, which every call reads anew: they are not resized."""
     __slots__ = ("starts", "lengths", "pages", "device", "_args")
 
     def __init__(self, starts, lengths, pages):
@@ -202,9 +218,9 @@ class Batch:
         stride = pages.stride(0) if sequences > 1 else width
         if sequences > 1 and width and stride < width:
             raise RuntimeError("pages has rows that overlap")
-        self.starts, self.lengths, self.pages, self.device = starts, lengths, pages, dev
-        self._args = _lib.BatchArgs(_vector(starts, "starts", sequences + 1, torch.int32, dev), _vector(lengths, "lengths", sequences, torch.int32, dev),
-                                    pages.data_ptr(), sequences, width, max(stride, width))
+        args = _lib.BatchArgs(_vector(starts, "starts", sequences + 1, torch.int32, dev), _vector(lengths, "lengths", sequences, torch.int32, dev),
+                              pages.data_ptr(), sequences, width, max(stride, width))
+        self._fix(starts=starts, lengths=lengths, pages=pages, device=dev, _args=args)
 
 
 def _both(cache, batch, who):
