@@ -76,8 +76,7 @@ def test_heads_are_turned(dtype, n, heads, d, dim, interleaved, far, scaling):
     positions = torch.randint(0, far, (n,), generator=g)
     positions[-1] = far - 1
     if dim == 0:
-        plan = gen.rotary_plan(2)
-        plan.rotated = 0
+        plan = gen.RotaryPlan(gen.rotary_plan(2).steps[:0], 0, False, 1.0)
         got, want, off = gen.rotate_heads(x, positions.cuda(), plan), x.cpu().double(), 0.0
     else:
         plan = gen.rotary_plan(dim, interleaved=interleaved, scaling=scaling)
