@@ -283,6 +283,21 @@ def drafts(so):
                 for b, (c, nodes, out) in enumerate(walk(decode(logits, kind), tokens, starts, pa, u, depth, decode(draft, kind) if drafted else None, t)):
                     assert rc[b] == c and rn[b].tolist() == nodes and ro[b].tolist() == out, (b, rc[b], c, rn[b], nodes, ro[b], out)
 
+    # one sibling refused after the other: more entries left than the lists of them hold, and fewer
+    for kind, v, n in ((0, 36000, 5), (2, 3000, 9)):
+        print("siblings", kind, v, flush=True)
+        rng = np.random.default_rng(v)
+        logits, draft = (encode(rng.standard_normal((n, v)) * 3, kind) for _ in range(2))
+        likelier = np.argsort(decode(logits, kind)[0] - decode(draft, kind)[0])          # by the draft model, and so refused
+        tokens, starts, parents, u = likelier[:n].astype(np.int64), np.array([0, n], np.int32), np.array([-1] + [0] * (n - 1), np.int32), rng.random(n)
+        tokens[-1] = likelier[-1]
+        rc, rn, ro = np.zeros(1, np.int64), np.zeros((1, 2), np.int64), np.zeros((1, 3), np.int64)
+        need = L.vi_verify_drafts_workspace_bytes(kind, n, v, 1, 1)
+        ws = np.full(need + 8, 0xA5, dtype=np.uint8)[8:]
+        assert L.vi_verify_drafts(kind, ptr(logits), n, v, v, ptr(draft), v, ptr(tokens), ptr(starts), 1, ptr(parents), ptr(u), 1.0, 2, ptr(rc), ptr(rn), ptr(ro), ptr(ws), need, None) == 0
+        (c, nodes, out), = walk(decode(logits, kind), tokens, starts, parents, u, 2, decode(draft, kind), 1.0)
+        assert c == 1 and rc[0] == c and rn[0].tolist() == nodes and ro[0].tolist() == out, (rc, c, rn, nodes, ro, out)
+
 
 def keep(so):
     L = ctypes.CDLL(so)

@@ -611,6 +611,23 @@ def test_many_siblings_are_refused_one_after_the_other():
     assert len(accepted) == 2 and all(0 in a and 1 in a for a in accepted)
 
 
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("v", [5000, 33000, 150001])
+def test_refusals_leave_less_and_less(dtype, v):
+    """Siblings that the draft model thinks likelier than the target does are refused; what is left of long rows does not fit into one place."""
+    g = seeded(v)
+    logits, draft = ((torch.randn(20, v, generator=g) * 3).to(dtype) for _ in range(2))
+    tokens, parents = [], []
+    for s0 in (0, 10):
+        likelier = (torch.softmax(logits[s0].double(), 0) / torch.softmax(draft[s0].double(), 0)).argsort()
+        tokens += likelier[:5].tolist() + likelier[v // 2 - 2:v // 2 + 2].tolist() + [int(likelier[-1])]
+        parents += [-1] + [0] * 9
+    u = torch.rand(20, generator=g, dtype=torch.float64) * 0.5 + 0.5
+    check_drafts(logits, tokens, [0, 10, 20], parents, u, draft, 4)
+    u[9] = u[19] = 1.0 - 2.0 ** -53            # the last ones refused as well, it may be: the token from what is left
+    check_drafts(logits, tokens, [0, 10, 20], parents, u, draft, 4, temperature=0.7)
+
+
 def test_drafts_that_are_hard_to_verify():
     inf_, v = math.inf, 70
     logits, tokens, starts, parents, u, draft = draft_case(12, 6, v, torch.float32, True, 3)
