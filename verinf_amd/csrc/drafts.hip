@@ -128,7 +128,7 @@ __device__ __forceinline__ void exponentials(const double *table, const Entries<
 struct Job {
     const void *x[2];                          // the target's logits, the draft's
     i64 ld[2], n, v;
-    int slices, per_slice, firsts, sequences, depth, drafted;
+    int slices, per_slice, firsts, sequences, apart, depth, drafted;           // apart: nodes of a sequence, on an average
     double c;                                  // 32 log2(e) / temperature
     Part *parts;                               // [2 n][slices]
     double *first;                             // [n][firsts]: the sum of max(p - q, 0) of a slice
@@ -407,8 +407,11 @@ template <int DT>
 __global__ __launch_bounds__(BLOCK) void k_first(Job A) {
     typedef typename type<DT>::t T;
     __shared__ double sum_of[BLOCK / 64], table[STEPS];
-    const i64 row = blockIdx.x / A.firsts;
-    const int slice = (int)(blockIdx.x % A.firsts), lane = threadIdx.x & 63, wave = threadIdx.x / 64;
+    // neighbours in the launch are nodes of one number in different trees, as far as these are alike: first nodes have more children, and what has to be done lies evenly
+    const int turn = blockIdx.x / A.firsts, slice = (int)(blockIdx.x % A.firsts);
+    const i64 row = (i64)(turn % A.sequences) * A.apart + turn / A.sequences;
+    if (row >= A.n) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / 64;
     const T *x = (const T *)A.x[0] + row * A.ld[0], *y = (const T *)A.x[1] + row * A.ld[1];
     i64 at = ((i64)slice * BLOCK + threadIdx.x) * EIGHT;
     if (children(A, row) < 2) return;
@@ -435,7 +438,7 @@ __global__ __launch_bounds__(BLOCK) void k_first(Job A) {
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     if (lane == 0) sum_of[wave] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) A.first[blockIdx.x] = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
+    if (threadIdx.x == 0) A.first[row * A.firsts + slice] = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
 }
 
 template <int DT>
@@ -681,21 +684,21 @@ extern "C" int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_
     if (sequences == 0) return VI_OK;
     if (!starts || !counts || !out || (depth && !nodes) || (n && (!logits || !tokens || !uniforms))) return vi::fail(VI_EINVAL, "%s: null pointer", who);
     const i64 rows = draft ? 2 * n : n, segments = (v + 64 * EIGHT - 1) / (64 * EIGHT), groups = (segments + BLOCK / 64 - 1) / (BLOCK / 64);
-    if (rows * slices_of(v, rows) > MAX_BLOCKS || sequences * groups > MAX_BLOCKS || n * firsts_of(v, n) > MAX_BLOCKS)
+    if (rows * slices_of(v, rows) > MAX_BLOCKS || sequences * groups > MAX_BLOCKS || (n + sequences) * firsts_of(v, n) > MAX_BLOCKS)
         return vi::fail(VI_EINVAL, "%s: %lld rows of %lld logits, %lld sequences", who, (long long)n, (long long)v, (long long)sequences);
     const size_t need = vi_verify_drafts_workspace_bytes(dtype, n, v, sequences, draft != nullptr);
     if (ws_bytes < need || !ws) return vi::fail(VI_ENOMEM, "%s: workspace %zu < %zu bytes", who, ws_bytes, need);
     const hipStream_t s = (hipStream_t)stream;
     Job J = {};
     J.x[0] = logits, J.x[1] = draft, J.ld[0] = ld, J.ld[1] = ld_draft, J.n = n, J.v = v, J.slices = (int)slices_of(v, rows), J.per_slice = (int)per_slice_of(v, rows), J.firsts = (int)firsts_of(v, n), J.sequences = (int)sequences;
-    J.depth = (int)depth, J.drafted = draft != nullptr, J.c = STEPS * 1.4426950408889634 / temperature, J.tokens = tokens, J.starts = starts, J.parents = parents;
+    J.apart = (int)((n + sequences - 1) / sequences), J.depth = (int)depth, J.drafted = draft != nullptr, J.c = STEPS * 1.4426950408889634 / temperature, J.tokens = tokens, J.starts = starts, J.parents = parents;
     J.uniforms = uniforms, J.counts = counts, J.nodes = nodes, J.out = out;
     J.rows = (Row *)vi::align16(ws);
     J.parts = (Part *)(J.rows + 2 * n);
     J.ends = (End *)(J.parts + rows * J.slices);
     J.segments = (double *)(J.ends + sequences);
     J.first = J.segments + sequences * segments;
-    const dim3 of_rows((unsigned)(rows * J.slices)), of_nodes((unsigned)(n * J.firsts)), of_groups((unsigned)(sequences * groups)), of_sequences((unsigned)sequences);
+    const dim3 of_rows((unsigned)(rows * J.slices)), of_nodes((unsigned)((i64)J.apart * sequences * J.firsts)), of_groups((unsigned)(sequences * groups)), of_sequences((unsigned)sequences);
 #define GO(TYPE)                                                                                    \
     do {                                                                                            \
         constexpr int DT = TYPE;                                                                    \
