@@ -17,8 +17,8 @@
 // (k_left), and a workgroup a sequence looks for the token (k_pick).
 //
 // What bounds them: some 15 instructions an exponential, eleven of them in 64 bits, which issue every 5 cycles.  64 trees of 16 nodes, 32000 bf16 logits of both models:
-// 126 us (46 all rows' sums, 30 first refusals, 55 the walk of the sequence with the most refusals, 10 us each, 11 the last tokens; 25 to read them); with the 11
-// powers of a series on [-1/2, 1/2] in place of table and 4 powers 149.  One chain of five nodes, f32: 15 us, the latency of four launches.
+// 114 us (45 all rows' sums, 23 first refusals, 52 the walk of the sequence with the most refusals, 9 us each, 11 the last tokens; 25 to read them); with the 11
+// powers of a series on [-1/2, 1/2] in place of table and 4 powers 149 in place of 126.  One chain of five nodes, f32: 15 us, the latency of four launches.
 #include "cache.hpp"
 
 namespace {
@@ -123,6 +123,14 @@ __device__ __forceinline__ void exponentials(const double *table, const Entries<
 template <int DT>
 __device__ __forceinline__ void exponentials(const double *table, const Entries<DT> &v, double c, double mc, double (&r)[EIGHT]) {
     exponentials<DT>(table, v, c, mc, [&](int i, double t, double scale) __attribute__((always_inline)) { r[i] = t * scale; });
+}
+
+// The sum of max(e^(x - most) - ratio e^(y - most), 0) of eight entries of two rows.  (Where x is -inf that is 2^-1000 instead of nothing.)
+template <int DT>
+__device__ __forceinline__ void add_left(const double *table, const Entries<DT> &e, const Entries<DT> &f, double c, double p_mc, double q_mc, double ratio, double &sum) {
+    double o[EIGHT];
+    exponentials<DT>(table, f, c, q_mc, [&](int i, double t, double scale) __attribute__((always_inline)) { o[i] = t * (scale * ratio); });
+    exponentials<DT>(table, e, c, p_mc, [&](int i, double t, double scale) __attribute__((always_inline)) { sum += fmax(fma(t, scale, -o[i]), 0.0); });
 }
 
 struct Job {
@@ -316,28 +324,24 @@ __device__ __forceinline__ double sum_segment(const Left<DT> &left, int segment)
     return sum;
 }
 
-// a thread's of the sum of a row that WALK threads add up, and its wavefront's
+// a wavefront's of what WALK threads add up of a row, with the draft's
 template <int DT>
 __device__ __forceinline__ double sum_own(const Left<DT> &left) {
     i64 at = (i64)threadIdx.x * EIGHT;
     Entries<DT> e = first_eight<DT>(left.x, at, left.v), f = first_eight<DT>(left.y, at, left.v);
-    double r[EIGHT], sum = 0;
+    double sum = 0;
+    const double ratio = left.a * left.q.per_z / left.p.per_z;
+    auto add = [&](const Entries<DT> &e, const Entries<DT> &f) __attribute__((always_inline)) { add_left<DT>(left.table, e, f, left.c, left.p.mc, left.q.mc, ratio, sum); };
     while (at + EIGHT <= left.v) {
         const i64 next = at + WALK * EIGHT;
         const Entries<DT> e_ahead = first_eight<DT>(left.x, next, left.v), f_ahead = first_eight<DT>(left.y, next, left.v);
-        left.of(at, e, f, r);
-#pragma unroll
-        for (int i = 0; i < EIGHT; ++i) sum += r[i];
+        add(e, f);
         e = e_ahead, f = f_ahead, at = next;
     }
-    if (at < left.v) {
-        left.eight_at(at, r);
-#pragma unroll
-        for (int i = 0; i < EIGHT; ++i) sum += r[i];
-    }
+    if (at < left.v) add(eight<DT>(left.x, at, left.v), eight<DT>(left.y, at, left.v));
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-    return sum;
+    return sum * left.p.per_z;
 }
 
 // the smallest j with R(0) + ... + R(j) > u sum(R); by a wavefront, from the sums of the segments
@@ -407,7 +411,8 @@ template <int DT>
 __global__ __launch_bounds__(BLOCK) void k_first(Job A) {
     typedef typename type<DT>::t T;
     __shared__ double sum_of[BLOCK / 64], table[STEPS];
-    // neighbours in the launch are nodes of one number in different trees, as far as these are alike: first nodes have more children, and what has to be done lies evenly
+    // neighbours in the launch are nodes of one number in different trees, as far as these are alike: first nodes have more children, and what has to be done lies evenly (64 trees of 16: 23 us, 30 in
+    // the order of the rows)
     const int turn = blockIdx.x / A.firsts, slice = (int)(blockIdx.x % A.firsts);
     const i64 row = (i64)(turn % A.sequences) * A.apart + turn / A.sequences;
     if (row >= A.n) return;
@@ -420,13 +425,8 @@ __global__ __launch_bounds__(BLOCK) void k_first(Job A) {
     __syncthreads();
     const Row p = join(table, A.parts + row * A.slices, A.slices, A.c), q = join(table, A.parts + (A.n + row) * A.slices, A.slices, A.c);
     double sum = 0;
-    auto add = [&](const Entries<DT> &e, const Entries<DT> &f) __attribute__((always_inline)) {
-        double t[EIGHT], o[EIGHT];
-        exponentials<DT>(table, e, A.c, p.mc, t);
-        exponentials<DT>(table, f, A.c, q.mc, o);
-#pragma unroll
-        for (int i = 0; i < EIGHT; ++i) sum += fmax(t[i] * p.per_z - o[i] * q.per_z, 0.0);
-    };
+    const double ratio = q.per_z / p.per_z;
+    auto add = [&](const Entries<DT> &e, const Entries<DT> &f) __attribute__((always_inline)) { add_left<DT>(table, e, f, A.c, p.mc, q.mc, ratio, sum); };
     while (at + EIGHT <= A.v) {
         const i64 next = at + (i64)A.firsts * (BLOCK * EIGHT);
         const Entries<DT> e_ahead = first_eight<DT>(x, next, A.v), f_ahead = first_eight<DT>(y, next, A.v);
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(BLOCK) void k_first(Job A) {
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     if (lane == 0) sum_of[wave] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) A.first[row * A.firsts + slice] = (sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3]);
+    if (threadIdx.x == 0) A.first[row * A.firsts + slice] = ((sum_of[0] + sum_of[1]) + (sum_of[2] + sum_of[3])) * p.per_z;
 }
 
 template <int DT>
