@@ -18,7 +18,7 @@
 // What bounds it (bf16, 8 heads of 128 columns for 32, where nothing else is said): 64 sequences of 4096 entries and a token each 198 us, 5.4 TB/s, as a large copy
 // (118 us over 8-bit integers, 4.7); 4096 tokens of a prompt, 32 heads of the cache, fp16, 198 us, 694 TFLOP/s, where the matrix units are busy for a third of the time and
 // the exponentials and their like, 125 instructions to each 16 products, for half of it (180 us, 766 TFLOP/s, with four heads to one of the cache; 236 over 8-bit
-// integers); a token over 1000 entries 13 us, the latency of two launches.
+// integers); a token over 1000 entries 12.5 us, the latency of two launches.
 #include <type_traits>
 
 #include "cache.hpp"
@@ -815,34 +815,55 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
         }
 }
 
-// What the workgroups of a tile have left, as one.
-constexpr int JOIN = 256;
-template <int DT, int DP, int ROWS>
+// What the workgroups of a tile have left, as one.  A thread has four columns of a row and every GROUPS-th part: all of them where parts are few, so that a workgroup
+// has several rows, else as many groups as a row leaves room for (64 parts of a token over 32768 entries, 8 heads: 20 us by one thread, 6 by eight).
+constexpr int JOIN = 256, FEW_PARTS = 8;
+template <int DT, int DP, int ROWS, bool MANY_PARTS>
 __global__ __launch_bounds__(JOIN) void k_join(Args A) {
     typedef typename type<DT>::t T;
+    constexpr int COLS = DP / 4, GROUPS = MANY_PARTS ? JOIN / COLS : 1, AT_ONCE = JOIN / COLS / GROUPS, MOST = MANY_PARTS ? (int)MAX_PARTS : FEW_PARTS;
+    __shared__ float of_parts[AT_ONCE * MOST][2];
+    __shared__ v4f of_groups[MANY_PARTS ? JOIN : 1];
     const int heads = (int)A.cache.heads, head = (int)blockIdx.x % heads, tile = (int)blockIdx.x / heads;
+    const int col = (int)threadIdx.x % COLS * 4, group = (int)threadIdx.x / COLS % GROUPS, own = (int)threadIdx.x / COLS / GROUPS;
     Tile t;
     if (!find_tile<ROWS>(A, tile, &t)) return;
     const i64 slot = ((i64)tile * heads + head) * A.splits;
-    const int parts = parts_of(A, t.end);
+    const int parts = parts_of(A, t.end), rows = min(ROWS, t.n * A.group - t.first);
     if (parts <= 1) return;                    // the only one is done
-    for (int i = (int)blockIdx.y * JOIN + (int)threadIdx.x; i < ROWS * (DP / 4); i += (int)gridDim.y * JOIN) {
-        const int r = i / (DP / 4), col = i % (DP / 4) * 4, row = t.first + r, tok = (int)((u32)row / (u32)A.group), g = row - tok * A.group;
-        if (tok >= t.n || col >= A.cache.dim) continue;
-        const float *most = A.most + (slot * ROWS + r) * 2, *part = A.part + (slot * ROWS + r) * DP + col;
-        float top = -INFINITY, total = 0;
-        for (int s = 0; s < parts; ++s) top = fmaxf(top, most[(i64)s * ROWS * 2]);
-        const float base = top == -INFINITY ? 0.0f : top;
-        v4f x = {0, 0, 0, 0};
-#pragma unroll 4
-        for (int s = 0; s < parts; ++s) {
-            const float its = most[(i64)s * ROWS * 2], of = most[(i64)s * ROWS * 2 + 1], by = __builtin_amdgcn_exp2f(its - base);
-            total += by * of;
-            x += by * *(const v4f *)(part + (i64)s * ROWS * DP);
+    for (int first = (int)blockIdx.y * AT_ONCE; first < rows; first += (int)gridDim.y * AT_ONCE) {
+        for (int i = threadIdx.x; i < AT_ONCE * parts; i += JOIN) {
+            const int r = first + i / parts, s = i % parts;
+            if (r < rows) __builtin_memcpy(of_parts[i], A.most + ((slot + s) * ROWS + r) * 2, 8);
         }
-        const float per = total == 0.0f ? 0.0f : 1.0f / total;
-        const v2u two = {pack<DT>(x.x * per, x.y * per), pack<DT>(x.z * per, x.w * per)};
-        store_any((T *)A.out + ((i64)t.s0 + tok) * A.out_token + (head * A.group + g) * A.out_head + col, two);
+        __syncthreads();
+        const int r = first + own, row = t.first + r, tok = (int)((u32)row / (u32)A.group), g = row - tok * A.group;
+        const bool there = r < rows && col < A.cache.dim;
+        float total = 0;
+        v4f x = {0, 0, 0, 0};
+        if (there) {
+            const float(*its)[2] = of_parts + own * parts, *part = A.part + (slot * ROWS + r) * DP + col;
+            float top = -INFINITY;
+            for (int s = 0; s < parts; ++s) top = fmaxf(top, its[s][0]);
+            const float base = top == -INFINITY ? 0.0f : top;
+            for (int s = 0; s < parts; ++s) total += __builtin_amdgcn_exp2f(its[s][0] - base) * its[s][1];
+#pragma unroll 8
+            for (int s = group; s < parts; s += GROUPS) x += __builtin_amdgcn_exp2f(its[s][0] - base) * *(const v4f *)(part + (i64)s * ROWS * DP);
+        }
+        if constexpr (MANY_PARTS) {
+            of_groups[threadIdx.x] = x;
+            __syncthreads();
+            if (group == 0) {
+#pragma unroll
+                for (int k = 1; k < GROUPS; ++k) x += of_groups[threadIdx.x + k * COLS];
+            }
+        }
+        if (there && group == 0) {
+            const float per = total == 0.0f ? 0.0f : 1.0f / total;
+            const v2u two = {pack<DT>(x.x * per, x.y * per), pack<DT>(x.z * per, x.w * per)};
+            store_any((T *)A.out + ((i64)t.s0 + tok) * A.out_token + (head * A.group + g) * A.out_head + col, two);
+        }
+        __syncthreads();                       // before the next rows' parts
     }
 }
 
@@ -872,7 +893,7 @@ Plan make_plan(int cache_dtype, i64 dim, i64 cache_heads, i64 n, i64 heads, i64 
     const i64 tiles = n * group / L.rows + sequences, full = (n * group + L.rows - 1) / L.rows, busy = full > sequences ? full : sequences;
     L.tiles = (int)(tiles < MAX_BLOCKS ? tiles : MAX_BLOCKS);
     // The keys are cut into parts of one size where there are few tiles: two workgroups a CU, as many as there is room for (a sequence of 32768 entries,
-    // 8 heads: 54 us, 64 with four a CU), or four where sequences alone make two, for their lengths differ (64 of 500 to 8192: 224 us, 237 uncut).  A
+    // 8 heads: 38 us, 41 with four a CU; 16 trees of 25 78 and 90, 96 with one a CU), or four where sequences alone make two, for their lengths differ (64 of 500 to 8192: 224 us, 237 uncut).  A
     // part has 128 keys at least, a round of a workgroup's wavefronts, and 512 where there are many.
     const i64 all = busy * cache_heads, wanted = (all < 2 * CUS ? 2 : 4) * CUS, parts = wanted / all, round = 128, least = all >= CUS ? 4 * round : round;
     i64 keys = parts > 1 ? (longest + parts - 1) / parts : longest;
@@ -889,8 +910,11 @@ void launch(const Args &A, hipStream_t s) {
     const i64 heads = A.cache.heads;
     hipLaunchKernelGGL(k_attend<F>, dim3((unsigned)(heads * A.tiles * A.splits)), dim3(F::THREADS), 0, s, A);
     if (A.splits > 1) {
-        const int blocks = F::ROWS * (F::DP / 4) / JOIN;
-        hipLaunchKernelGGL((k_join<F::DT, F::DP, F::ROWS>), dim3((unsigned)(heads * A.tiles), (unsigned)(heads * A.tiles < 2 * CUS ? blocks : 1)), dim3(JOIN), 0, s, A);
+        const bool many = A.splits > FEW_PARTS;
+        const i64 tiles = heads * A.tiles, rows = many ? 1 : JOIN / (F::DP / 4);
+        const dim3 grid((unsigned)tiles, (unsigned)(tiles < 2 * CUS ? F::ROWS / rows : 1));
+        if (many) hipLaunchKernelGGL((k_join<F::DT, F::DP, F::ROWS, true>), grid, dim3(JOIN), 0, s, A);
+        else hipLaunchKernelGGL((k_join<F::DT, F::DP, F::ROWS, false>), grid, dim3(JOIN), 0, s, A);
     }
 }
 template <int DT, bool I8, int DP>
