@@ -351,6 +351,17 @@ def test_attention_over_the_cache(cached, before, new, heads, group, dim, page):
 
 
 @pytest.mark.parametrize("cached", CACHED)
+@pytest.mark.parametrize("dim", [48, 64, 128, 208, 256])
+@pytest.mark.parametrize("new,group", [([1, 3], 2), ([100, 1], 1)])
+def test_attention_in_many_parts(cached, dim, new, group):
+    """Few heads over long sequences, cut as the longest that there may be says, which may be wrong."""
+    m = Made(cached, [5000, 1100], new, 1, dim, 64)
+    q = normal((m.n, group, dim), seeded(dim, group), torch.float16 if cached == torch.float16 else torch.bfloat16)
+    for longest in (None, 0, 700, 1 << 30):
+        check_attention(m, q, group, longest=longest)
+
+
+@pytest.mark.parametrize("cached", CACHED)
 @pytest.mark.parametrize("before,new,heads,group,dim,page", [([100], [17], 2, 3, 96, 16), ([3, 2000], [25, 9], 2, 4, 128, 128), ([0, 37, 5], [33, 1, 64], 3, 1, 64, 16),
                                                              ([15, 700], [256, 100], 1, 2, 128, 16), ([40, 0], [100, 300], 2, 1, 128, 32), ([9], [20], 1, 8, 256, 16)])
 def test_attention_of_trees(cached, before, new, heads, group, dim, page):
