@@ -1,0 +1,27 @@
+"""Attention over the cache and drafts on the CPU at the ends of numbers' ranges: cpu_build/simt_generation_edges.py over the builds of test_cpu_build_generation.py."""
+import os
+import subprocess
+import sys
+
+import pytest
+
+from test_cpu_build_generation import _build
+from test_cpu_build_inference import DIR, _runtime
+
+pytestmark = pytest.mark.skipif(not _runtime(), reason="no clang with AddressSanitizer")
+
+
+@pytest.fixture(scope="module")
+def built(tmp_path_factory):
+    made, folder = {}, str(tmp_path_factory.mktemp("simt_edges"))
+    return lambda unit: made[unit] if unit in made else made.setdefault(unit, _build(unit, folder))
+
+
+def check(built, unit, what):
+    env = dict(os.environ, LD_PRELOAD=_runtime(), ASAN_OPTIONS="detect_leaks=0,verify_asan_link_order=0", OPENBLAS_NUM_THREADS="1")
+    res = subprocess.run([sys.executable, os.path.join(DIR, "simt_generation_edges.py"), what, built(unit)], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True, env=env, timeout=900)
+    assert res.returncode == 0 and res.stdout.strip().endswith("OK"), res.stdout[-4000:]
+
+
+def test_keys_far_above_those_before_them(built):
+    check(built, "attention", "late_keys")

@@ -489,8 +489,9 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             most = now, relative = then, sum *= by;
             float less = by;                   // of the products' sums: where they have a power of their own that follows
             if constexpr (F::I8) {
+                // MAX_GAIN / gain may be beyond 32 bits where `by` is nothing; what both come to is 1 at most
                 const float more = fminf(gain / by, MAX_GAIN);
-                less = more < MAX_GAIN ? 1.0f : by * (more / gain);
+                less = more < MAX_GAIN ? 1.0f : by * 0x1p63f / gain * (MAX_GAIN * 0x1p-63f);
                 gain = more, weighed *= less;
             }
 #pragma unroll
