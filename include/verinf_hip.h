@@ -464,7 +464,7 @@ int vi_attend_cache(const vi_cache *cache, const vi_batch *batch, int dtype, con
  * starts[b + 1] - 1: a root and drafts, in an order in which parents[node], a number in the sequence, is lower than the node's own; row `node` of
  * logits (n, v), v <= 2^20, is what the target says behind it.  From the root on, a node's children are tried in their order: with R = p, child c is accepted
  * where uniforms[c] q(tokens[c]) sum(R) < R(tokens[c]), q = softmax(draft / temperature) of the node's row; behind a refused one R = max(R / sum(R) - q, 0).  Without
- * draft logits q = 1 and R loses the entry.  A sequence's first 1024 nodes are tried.  Once none is accepted, or `depth` <= 256 are, the token behind the path is the smallest j with R(0) + ... + R(j) >
+ * draft logits q = 1 and R loses the entry.  Probabilities below 2^-1022 of a row's largest are 0.  A sequence's first 1024 nodes are tried.  Once none is accepted, or `depth` <= 256 are, the token behind the path is the smallest j with R(0) + ... + R(j) >
  * uniforms[root] sum(R); where nothing is left of R, R = p; -1 where a row has a NaN or +inf or only -inf (no draft below it is accepted).
  * counts (sequences): accepted drafts; nodes (sequences, depth): their numbers, -1 behind; out (sequences, depth + 1): their tokens, the one behind, -1.
  * ws: vi_verify_drafts_workspace_bytes() bytes of device scratch. */

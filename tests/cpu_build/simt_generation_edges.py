@@ -5,8 +5,8 @@ import math
 import sys
 
 import numpy as np
-from simt_generation_checks import F32, I8, I64, INT, ROUND, VP, Made
-from simt_inference_checks import decode, encode, ptr
+from simt_generation_checks import F32, F64, I8, I64, INT, ROUND, SZ, VP, Made, walk
+from simt_inference_checks import LOWEST, decode, encode, ptr
 
 
 def attention(so):
@@ -68,6 +68,83 @@ def late_keys(so):
                     got = attended(L, m, q, form, splits, per, 1.0)[0, 0]
                     bad = ~(np.abs(got - want) <= off + ROUND[1] * (np.abs(want) + off))
                     assert not bad.any(), ("late", value_scale, ahead, late, form, splits, int(bad.sum()), got[:3], want[:3])
+
+
+# ---- drafts -------------------------------------------------------------------------------------------------------
+def drafts(so):
+    L = ctypes.CDLL(so)
+    L.vi_verify_drafts_workspace_bytes.restype = SZ
+    L.vi_verify_drafts_workspace_bytes.argtypes = [INT, I64, I64, I64, INT]
+    L.vi_verify_drafts.argtypes = [INT, VP, I64, I64, I64, VP, I64, VP, VP, I64, VP, VP, F64, I64, VP, VP, VP, VP, SZ, VP]
+    return L
+
+
+def verified(L, kind, logits, draft, tokens, parents, u, depth, t=1.0):
+    """One sequence; what comes out, and what walk() says."""
+    n, v = logits.shape
+    tokens, parents, u = np.array(tokens, np.int64), np.array(parents, np.int32), np.array(u, np.float64)
+    starts = np.array([0, n], np.int32)
+    count, nodes, out = np.zeros(1, np.int64), np.full((1, depth), 9, np.int64), np.full((1, depth + 1), 9, np.int64)
+    need = L.vi_verify_drafts_workspace_bytes(kind, n, v, 1, int(draft is not None))
+    ws = np.full(need + 8, 0xA5, dtype=np.uint8)[8:]
+    assert L.vi_verify_drafts(kind, ptr(logits), n, v, v, ptr(draft), v, ptr(tokens), ptr(starts), 1, ptr(parents), ptr(u), t, depth, ptr(count), ptr(nodes), ptr(out), ptr(ws), need, None) == 0
+    (c, wn, wo), = walk(decode(logits, kind), tokens, starts, parents, u, depth, None if draft is None else decode(draft, kind), t)
+    return (int(count[0]), nodes[0].tolist(), out[0].tolist()), (c, wn, wo)
+
+
+ALMOST_ONE = 1.0 - 2.0 ** -53
+
+
+def masked_drafts(so):
+    """Drafts whose token the target, the draft model or both mask, with -inf or far down, behind refusals of others or of none."""
+    L = drafts(so)
+    for kind in (0, 1, 2):
+        for v in (50, 2100):
+            rng = np.random.default_rng(v + kind)
+            for mask in (-np.inf, -1e9, LOWEST[kind]):
+                logits, draft = (rng.standard_normal((5, v)).astype(np.float32) * 3 for _ in range(2))
+                likelier = np.argsort(logits[0] - draft[0])            # by the draft model, and so refused by numbers close to one
+                masked = int(likelier[v // 2])
+                for where in ("target", "draft", "both"):
+                    x, y = logits.copy(), draft.copy()
+                    if where != "draft":
+                        x[0, masked] = mask
+                    if where != "target":
+                        y[0, masked] = mask
+                    x, y = encode(x, kind), encode(y, kind)
+                    for refused in (0, 1, 2):
+                        for u in (0.0, 0.3, ALMOST_ONE):
+                            for root in (0.0, 0.6):
+                                tokens = [0] + likelier[:refused].tolist() + [masked] + [int(likelier[-1])] * (3 - refused)
+                                numbers = [root] + [ALMOST_ONE] * refused + [u] + [0.5] * (3 - refused)
+                                for given in (None, y):
+                                    got, want = verified(L, kind, x, given, tokens, [-1] + [0] * 4, numbers, 2)
+                                    assert got == want, (kind, v, mask, where, refused, u, root, given is not None, got, want)
+
+
+def first_tokens(so):
+    """The token of a root's number zero is the first that has a probability, and where nothing is left behind refusals, too."""
+    L = drafts(so)
+    for kind in (0, 1, 2):
+        for v in (40, 1100, 9000):
+            for mask in (-np.inf, -1e9, LOWEST[kind]):
+                rng = np.random.default_rng(v)
+                x = rng.standard_normal((3, v)).astype(np.float32)
+                x[:, :v // 2] = mask
+                x[:, v - 3:] = mask
+                x = encode(x, kind)
+                for given in (None, x):
+                    for u in (0.0, 0.5, ALMOST_ONE):
+                        # p - p is nothing, where p / sum(p) - p in 64 bits may leave 1e-17: of p itself, which refused tokens without a probability change as little without a draft model
+                        args = [0, 1, 2], [-1, 0, 0], [u, ALMOST_ONE, ALMOST_ONE], 2
+                        got, want = verified(L, kind, x, given, *args)[0], verified(L, kind, x, None, *args)[1]
+                        assert got == want, (kind, v, mask, u, given is not None, got, want)
+                one = np.full((2, v), mask, np.float32)        # all of it refused
+                one[:, v // 2] = 1.0
+                one = encode(one, kind)
+                for given in (None, one):
+                    got, _ = verified(L, kind, one, given, [0, v // 2], [-1, 0], [0.0, 1.0], 1)
+                    assert got == (0, [-1], [v // 2, -1]), (kind, v, mask, given is not None, got)
 
 
 if __name__ == "__main__":

@@ -25,3 +25,11 @@ def check(built, unit, what):
 
 def test_keys_far_above_those_before_them(built):
     check(built, "attention", "late_keys")
+
+
+def test_drafts_of_masked_tokens(built):
+    check(built, "drafts", "masked_drafts")
+
+
+def test_first_tokens_that_have_a_probability(built):
+    check(built, "drafts", "first_tokens")

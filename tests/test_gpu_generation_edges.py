@@ -1,10 +1,12 @@
 """Attention over the cache and drafts at the ends of numbers' ranges, against 64 bits."""
+import math
+
 import pytest
 
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
-from test_gpu_generation import ROUND, Made  # noqa: E402
+from test_gpu_generation import FLOATS, ROUND, Made, check_drafts, seeded  # noqa: E402
 from verinf_amd.prover import generation as gen  # noqa: E402
 
 
@@ -26,7 +28,7 @@ def seen64(m, scores, tokens):
     """What each of the tokens sees: probabilities (tokens, entries) and values (entries, dim)."""
     count = len(scores)
     seen = torch.ones(tokens, count, dtype=torch.bool).tril(count - tokens)
-    return torch.softmax(torch.where(seen, scores.double(), float("-inf")), dim=1), m.held(0, "values", count)[:, 0]
+    return torch.softmax(torch.where(seen, scores.double(), -math.inf), dim=1), m.held(0, "values", count)[:, 0]
 
 
 @pytest.mark.parametrize("tokens", [1, 100])
@@ -48,3 +50,55 @@ def test_keys_far_above_those_before_them(tokens, count, value_scale):
             for longest in (None, 0):
                 got = gen.attend_cache(q, m.cache, m.batch, scale=1.0, longest=longest)[:, 0].cpu().double()
                 assert ((got - want).abs() <= off + r * (want.abs() + off)).all(), (ahead, late, longest)
+
+
+# ---- drafts -------------------------------------------------------------------------------------------------------
+ALMOST_ONE = 1.0 - 2.0 ** -53
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("v", [50, 33000])
+@pytest.mark.parametrize("mask", [-math.inf, -1e9, None])
+def test_drafts_of_masked_tokens(dtype, v, mask):
+    """Tokens that the target, the draft model or both mask, with -inf or far down, behind refusals of others or of none: a sequence for each."""
+    g = seeded(v, 41)
+    mask = torch.finfo(dtype).min if mask is None else mask
+    first = [(torch.randn(v, generator=g) * 3) for _ in range(2)]
+    likelier = (first[0] - first[1]).argsort().tolist()                # by the draft model, and so refused by numbers close to one
+    masked = likelier[v // 2]
+    logits, draft, tokens, parents, u = [], [], [], [], []
+    for where in ("target", "draft", "both"):
+        for refused in (0, 1, 2):
+            for number in (0.0, 0.3, ALMOST_ONE):
+                for root in (0.0, 0.6):
+                    x, y = (torch.randn(5, v, generator=g) * 3 for _ in range(2))
+                    x[0], y[0] = first
+                    if where != "draft":
+                        x[0, masked] = mask
+                    if where != "target":
+                        y[0, masked] = mask
+                    logits.append(x.to(dtype)), draft.append(y.to(dtype))
+                    tokens += [0] + likelier[:refused] + [masked] + [likelier[-1]] * (3 - refused)
+                    parents += [-1] + [0] * 4
+                    u += [root] + [ALMOST_ONE] * refused + [number] + [0.5] * (3 - refused)
+    starts = list(range(0, len(tokens) + 1, 5))
+    for given in (torch.cat(draft), None):
+        check_drafts(torch.cat(logits), tokens, starts, parents, torch.tensor(u, dtype=torch.float64), given, 2)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("v", [40, 9000, 40001])
+@pytest.mark.parametrize("mask", [-math.inf, -1e9, None])
+def test_first_tokens_that_have_a_probability(dtype, v, mask):
+    """The token of a root's number zero is the first that has a probability, and where nothing is left behind refusals, too."""
+    mask = torch.finfo(dtype).min if mask is None else mask
+    x = torch.randn(3, v, generator=seeded(v, 42))
+    x[:, :v // 2] = mask
+    x[:, v - 3:] = mask
+    x = x.to(dtype)
+    for root in (0.0, 0.5, ALMOST_ONE):
+        u = torch.tensor([root, ALMOST_ONE, ALMOST_ONE], dtype=torch.float64)
+        check_drafts(x, [0, 1, 2], [0, 3], [-1, 0, 0], u, None, 2)
+        args = x.cuda(), torch.tensor([0, 1, 2]).cuda(), torch.tensor([0, 3], dtype=torch.int32).cuda(), torch.tensor([-1, 0, 0], dtype=torch.int32).cuda(), u.cuda(), 2
+        # p - p is nothing: of p itself, which refused tokens without a probability change as little without a draft model
+        assert all(torch.equal(a, b) for a, b in zip(gen.verify_drafts(*args, draft_logits=args[0]), gen.verify_drafts(*args)))

@@ -40,11 +40,12 @@ struct Row {                                   // of a row: the most c that its 
     double mc, per_z;
 };
 
-// 2^(t / 32) of N numbers side by side (one alone waits for itself at each step), t up to 0 or hardly above, 2^-1000 below 32 times that: the whole part by an
+// 2^(t / 32) of N numbers side by side (one alone waits for itself at each step), t up to 0 or hardly above, LEAST (2^-1022) below 32 times that: the whole part by an
 // addition whose result has units of one, its last five bits from a table, the others into the exponent, the rest by a polynomial (over Chebyshev's nodes, 1.6e-13).
 // The table has 256 bytes, a pair of banks to each entry; the exponent comes into the entry by adding the whole part as it is, 15 bits up in the upper half, from
 // where the entry has lost its own number before.
 constexpr int STEPS = 32;
+constexpr double LEAST = 0x1p-1022;            // where it stands for anything down to nothing: of a masked entry, say
 __device__ const double TABLE[STEPS] = {0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0, 0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0,
                                       0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0, 0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
                                       0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0, 0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0,
@@ -60,7 +61,7 @@ __device__ __forceinline__ void exp2_64(const double *table, double (&t)[N], dou
     double m[N], f[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-        t[e] = fmax(t[e], -1000.0 * STEPS);
+        t[e] = fmax(t[e], -1022.0 * STEPS);
         m[e] = t[e] + 6755399441055744.0;
         f[e] = t[e] - (m[e] - 6755399441055744.0);
         const u32 k = (u32)__builtin_bit_cast(u64, m[e]);
@@ -78,6 +79,8 @@ __device__ __forceinline__ double exp2_64(const double *table, double t) {
     exp2_64(table, one, scale);
     return one[0] * scale[0];
 }
+// an entry's part of its row's sum as a probability: none where it is LEAST
+__device__ __forceinline__ double probability(double part, double per_z) { return part > LEAST ? part * per_z : 0.0; }
 
 template <int DT>
 struct Entries {                               // as they come
@@ -125,7 +128,8 @@ __device__ __forceinline__ void exponentials(const double *table, const Entries<
     exponentials<DT>(table, v, c, mc, [&](int i, double t, double scale) __attribute__((always_inline)) { r[i] = t * scale; });
 }
 
-// The sum of max(e^(x - most) - ratio e^(y - most), 0) of eight entries of two rows.  (Where x is -inf that is 2^-1000 instead of nothing.)
+// The sum of max(e^(x - most) - ratio e^(y - most), 0) of eight entries of two rows.  (LEAST in the place of nothing: too
+// little to change what comes of a sum.)
 template <int DT>
 __device__ __forceinline__ void add_left(const double *table, const Entries<DT> &e, const Entries<DT> &f, double c, double p_mc, double q_mc, double ratio, double &sum) {
     double o[EIGHT];
@@ -290,7 +294,7 @@ struct Left {
     __device__ __forceinline__ void of(i64 at, const Entries<DT> &e, const Entries<DT> &f, double (&r)[EIGHT]) const {
         exponentials<DT>(table, e, c, p.mc, r);
 #pragma unroll
-        for (int i = 0; i < EIGHT; ++i) r[i] = entry<DT>(e, i) > -INFINITY ? r[i] * p.per_z : 0.0;
+        for (int i = 0; i < EIGHT; ++i) r[i] = probability(r[i], p.per_z);
         if (a > 0) {
             const double per = a * q.per_z;
             double o[EIGHT];
@@ -465,7 +469,8 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
         if (parent >= 0) {
             auto of = [&](int which) {
                 const Row r = A.rows[(which ? A.n : 0) + s0 + parent];
-                return r.per_z == 0 ? 0.0 : exp2_64(sh.table, fma((double)(float)((const T *)A.x[which])[(s0 + parent) * A.ld[which] + token], A.c, -r.mc)) * r.per_z;
+                if (r.per_z == 0) return 0.0;
+                return probability(exp2_64(sh.table, fma((double)(float)((const T *)A.x[which])[(s0 + parent) * A.ld[which] + token], A.c, -r.mc)), r.per_z);
             };
             sh.have[i] = of(0);
             sh.said[i] = A.drafted ? of(1) : 1.0;

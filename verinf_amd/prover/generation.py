@@ -304,7 +304,8 @@ def verify_drafts(logits, tokens, starts, parents, uniforms, depth, draft_logits
 
     Returns (counts (sequences,), nodes (sequences, depth), out (sequences, depth + 1)), int64: accepted drafts, their numbers in the sequence, -1
     behind; their tokens, the one that follows, -1 behind.  All in 64 bits.  A row with a NaN or +inf, or only -inf, has no probabilities: no draft
-    below it is accepted, and the token that follows it is -1.  Drafts whose token is outside [0, v) or whose parent is none are refused; v is at most
+    below it is accepted, and the token that follows it is -1.  An entry less than 2^-1022 of its row's largest has none either (-inf, or masked far down): it
+    is neither accepted nor the token that follows, and as the draft's counts as never drawn.  Drafts whose token is outside [0, v) or whose parent is none are refused; v is at most
     2^20, and a sequence's first 1024 nodes are tried."""
     n, v, ld = _matrix(logits, "logits", _FLOATS)
     dev = logits.device
