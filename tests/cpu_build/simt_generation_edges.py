@@ -147,6 +147,27 @@ def first_tokens(so):
                     assert got == (0, [-1], [v // 2, -1]), (kind, v, mask, given is not None, got)
 
 
+def far_logits(so):
+    """Rows all of whose entries are the type's lowest, or as large, or near to each other and far from nothing."""
+    L = drafts(so)
+    for kind in (0, 1, 2):
+        for v in (7, 1300):
+            rng = np.random.default_rng(v)
+            for far in (LOWEST[kind], LOWEST[kind] / 2, -LOWEST[kind], 3e4, -1.7e4, 1e6, -1e12, 1e20):
+                if kind == 2 and abs(far) > 65504:
+                    continue
+                for near in (False, True):
+                    x = np.full((4, v), far, np.float32)
+                    if near:                   # neighbouring numbers of the type, or equal ones
+                        x *= (1 - rng.integers(0, 3, x.shape) * {0: 2.0 ** -23, 1: 2.0 ** -7, 2: 2.0 ** -10}[kind]).astype(np.float32)
+                    x = encode(x, kind)
+                    y = encode(rng.standard_normal((4, v)), kind)
+                    for t in (1.0, 0.7, 0.3, 1e-3, 1e3, 17.0):
+                        for given in (None, y):
+                            got, want = verified(L, kind, x, given, [0] + rng.integers(0, v, 3).tolist(), [-1, 0, 0, 1], rng.random(4), 2, t)
+                            assert got == want, (kind, v, far, near, t, given is not None, got, want)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[1]](sys.argv[2])
     print("OK")

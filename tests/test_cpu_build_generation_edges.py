@@ -33,3 +33,7 @@ def test_drafts_of_masked_tokens(built):
 
 def test_first_tokens_that_have_a_probability(built):
     check(built, "drafts", "first_tokens")
+
+
+def test_logits_far_from_nothing(built):
+    check(built, "drafts", "far_logits")

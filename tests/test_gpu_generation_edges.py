@@ -102,3 +102,21 @@ def test_first_tokens_that_have_a_probability(dtype, v, mask):
         args = x.cuda(), torch.tensor([0, 1, 2]).cuda(), torch.tensor([0, 3], dtype=torch.int32).cuda(), torch.tensor([-1, 0, 0], dtype=torch.int32).cuda(), u.cuda(), 2
         # p - p is nothing: of p itself, which refused tokens without a probability change as little without a draft model
         assert all(torch.equal(a, b) for a, b in zip(gen.verify_drafts(*args, draft_logits=args[0]), gen.verify_drafts(*args)))
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("v", [7, 40000])
+def test_logits_far_from_nothing(dtype, v):
+    """Rows all of whose entries are the type's lowest, or as large, or near to each other and far from nothing."""
+    g = seeded(v, 43)
+    lowest = torch.finfo(dtype).min
+    for far in (lowest, lowest / 2, -lowest, 3e4, 1e6, -1e12, 1e20):
+        if abs(far) > -lowest:
+            continue
+        for near in (0, 3):                    # equal, or neighbouring numbers of the type
+            x = (far * (1 - torch.randint(0, max(near, 1), (4, v), generator=g) * torch.finfo(dtype).eps).double()).to(dtype)
+            y = torch.randn(4, v, generator=g).to(dtype)
+            for t in (1.0, 0.7, 1e-3, 1e3):
+                tokens, u = [0] + torch.randint(0, v, (3,), generator=g).tolist(), torch.rand(4, generator=g, dtype=torch.float64)
+                for given in (None, y):
+                    check_drafts(x, tokens, [0, 4], [-1, 0, 0, 1], u, given, 2, t)

@@ -36,16 +36,21 @@ struct Part {                                  // of a slice: an entry of its la
     double z;
     float most, pad;
 };
-struct Row {                                   // of a row: the most c that its sum is relative to; 1 / sum, 0 where it has none (or NaN, +inf among its entries)
-    double mc, per_z;
+struct Row {                                   // of a row: the largest, which its sum is relative to; 1 / sum, 0 where it has none (or NaN, +inf among its entries)
+    double most, per_z;
 };
 
-// 2^(t / 32) of N numbers side by side (one alone waits for itself at each step), t up to 0 or hardly above, LEAST (2^-1022) below 32 times that: the whole part by an
+// 2^(d c / 32) of N numbers side by side (one alone waits for itself at each step), d c up to 0 or hardly above, less than LEAST from where it would be that: the whole part by an
 // addition whose result has units of one, its last five bits from a table, the others into the exponent, the rest by a polynomial (over Chebyshev's nodes, 1.6e-13).
+// d is a difference of entries, taken before the product: c times an entry of 10^38 has no digits that c times another could be taken from.
 // The table has 256 bytes, a pair of banks to each entry; the exponent comes into the entry by adding the whole part as it is, 15 bits up in the upper half, from
 // where the entry has lost its own number before.
 constexpr int STEPS = 32;
-constexpr double LEAST = 0x1p-1022;            // where it stands for anything down to nothing: of a masked entry, say
+constexpr double LEAST = 0x1p-1022;            // what is below it stands for anything down to nothing: of a masked entry, say
+constexpr double DEEPEST = -1022.25 * STEPS;   // of d c: a quarter of a power of two below LEAST, so that no rounding of it is above
+struct Scale {                                 // of a launch: 32 log2(e) / temperature, DEEPEST / c
+    double c, deepest;
+};
 __device__ const double TABLE[STEPS] = {0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0, 0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0,
                                       0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0, 0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
                                       0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0, 0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0,
@@ -56,27 +61,27 @@ __device__ __forceinline__ void take_table(double *table) {        // a barrier 
     if (threadIdx.x < STEPS) table[threadIdx.x] = __builtin_bit_cast(double, __builtin_bit_cast(u64, TABLE[threadIdx.x]) - ((u64)threadIdx.x << 47));
 }
 template <int N>
-__device__ __forceinline__ void exp2_64(const double *table, double (&t)[N], double (&scale)[N]) {         // times scale
+__device__ __forceinline__ void exp2_64(const double *table, const Scale &S, double (&d)[N], double (&scale)[N]) {         // times scale
     constexpr double C[] = {9.172598566029335e-09, 1.6938609067364198e-06, 0.00023459619820112603, 0.021660849392187844, 1.0};
     double m[N], f[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-        t[e] = fmax(t[e], -1022.0 * STEPS);
-        m[e] = t[e] + 6755399441055744.0;
-        f[e] = t[e] - (m[e] - 6755399441055744.0);
+        d[e] = fmax(d[e], S.deepest);
+        m[e] = fma(d[e], S.c, 6755399441055744.0);
+        f[e] = fma(d[e], S.c, -(m[e] - 6755399441055744.0));
         const u32 k = (u32)__builtin_bit_cast(u64, m[e]);
         const u64 entry = __builtin_bit_cast(u64, table[k % STEPS]);
         scale[e] = __builtin_bit_cast(double, (u64)((u32)(entry >> 32) + (k << 15)) << 32 | (u32)entry);
-        t[e] = C[0];
+        d[e] = C[0];
     }
 #pragma unroll
     for (int i = 1; i < 5; ++i)
 #pragma unroll
-        for (int e = 0; e < N; ++e) t[e] = fma(t[e], f[e], C[i]);
+        for (int e = 0; e < N; ++e) d[e] = fma(d[e], f[e], C[i]);
 }
-__device__ __forceinline__ double exp2_64(const double *table, double t) {
-    double one[1] = {t}, scale[1];
-    exp2_64(table, one, scale);
+__device__ __forceinline__ double exp2_64(const double *table, const Scale &S, double d) {
+    double one[1] = {d}, scale[1];
+    exp2_64(table, S, one, scale);
     return one[0] * scale[0];
 }
 // an entry's part of its row's sum as a probability: none where it is LEAST
@@ -112,36 +117,36 @@ __device__ __forceinline__ Entries<DT> first_eight(const typename type<DT>::t *x
 
 // e^(x - most) of eight entries, in 64 bits: t times scale, to(i, t, scale)
 template <int DT, class To>
-__device__ __forceinline__ void exponentials(const double *table, const Entries<DT> &v, double c, double mc, To to) {
+__device__ __forceinline__ void exponentials(const double *table, const Scale &S, const Entries<DT> &v, double most, To to) {
 #pragma unroll
     for (int h = 0; h < EIGHT; h += 4) {
         double t[4], scale[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = fma((double)entry<DT>(v, h + e), c, -mc);
-        exp2_64(table, t, scale);
+        for (int e = 0; e < 4; ++e) t[e] = (double)entry<DT>(v, h + e) - most;
+        exp2_64(table, S, t, scale);
 #pragma unroll
         for (int e = 0; e < 4; ++e) to(h + e, t[e], scale[e]);
     }
 }
 template <int DT>
-__device__ __forceinline__ void exponentials(const double *table, const Entries<DT> &v, double c, double mc, double (&r)[EIGHT]) {
-    exponentials<DT>(table, v, c, mc, [&](int i, double t, double scale) __attribute__((always_inline)) { r[i] = t * scale; });
+__device__ __forceinline__ void exponentials(const double *table, const Scale &S, const Entries<DT> &v, double most, double (&r)[EIGHT]) {
+    exponentials<DT>(table, S, v, most, [&](int i, double t, double scale) __attribute__((always_inline)) { r[i] = t * scale; });
 }
 
 // The sum of max(e^(x - most) - ratio e^(y - most), 0) of eight entries of two rows.  (LEAST in the place of nothing: too
 // little to change what comes of a sum.)
 template <int DT>
-__device__ __forceinline__ void add_left(const double *table, const Entries<DT> &e, const Entries<DT> &f, double c, double p_mc, double q_mc, double ratio, double &sum) {
+__device__ __forceinline__ void add_left(const double *table, const Scale &S, const Entries<DT> &e, const Entries<DT> &f, double p_most, double q_most, double ratio, double &sum) {
     double o[EIGHT];
-    exponentials<DT>(table, f, c, q_mc, [&](int i, double t, double scale) __attribute__((always_inline)) { o[i] = t * (scale * ratio); });
-    exponentials<DT>(table, e, c, p_mc, [&](int i, double t, double scale) __attribute__((always_inline)) { sum += fmax(fma(t, scale, -o[i]), 0.0); });
+    exponentials<DT>(table, S, f, q_most, [&](int i, double t, double scale) __attribute__((always_inline)) { o[i] = t * (scale * ratio); });
+    exponentials<DT>(table, S, e, p_most, [&](int i, double t, double scale) __attribute__((always_inline)) { sum += fmax(fma(t, scale, -o[i]), 0.0); });
 }
 
 struct Job {
     const void *x[2];                          // the target's logits, the draft's
     i64 ld[2], n, v;
     int slices, per_slice, firsts, sequences, apart, depth, drafted;           // apart: nodes of a sequence, on an average
-    double c;                                  // 32 log2(e) / temperature
+    Scale scale;
     Part *parts;                               // [2 n][slices]
     double *first;                             // [n][firsts]: the sum of max(p - q, 0) of a slice
     Row *rows;                                 // [2 n]
@@ -191,9 +196,9 @@ __global__ __launch_bounds__(BLOCK) void k_stats(Job A) {
     if (which && children(A, row - A.n) == 0) return;                  // nobody asks
     take_table(table);
     __syncthreads();
-    const float margin = (float)(MARGIN * STEPS / A.c);
+    const float margin = (float)(MARGIN * STEPS / A.scale.c);
     float most = -INFINITY, bound = -INFINITY;
-    double z = 0, mc = 0;
+    double z = 0, from = 0;
     bool bad = false;
     auto add = [&](const Entries<DT> &e) __attribute__((always_inline)) {
         float here = entry<DT>(e, 0);
@@ -201,12 +206,11 @@ __global__ __launch_bounds__(BLOCK) void k_stats(Job A) {
         for (int i = 1; i < EIGHT; ++i) here = __builtin_elementwise_maximum(here, entry<DT>(e, i));           // NaN where there is one
         bad |= !(here < INFINITY);
         if (here > bound && !bad) {
-            const double next = (double)here * A.c;
-            z = z > 0 ? z * exp2_64(table, mc - next) : 0.0;
-            most = here, bound = here + margin, mc = next;
+            z = z > 0 ? z * exp2_64(table, A.scale, from - (double)here) : 0.0;
+            most = here, bound = here + margin, from = (double)here;
         }
         if (most > -INFINITY) {
-            exponentials<DT>(table, e, A.c, mc, [&](int, double t, double scale) __attribute__((always_inline)) { z = fma(t, scale, z); });
+            exponentials<DT>(table, A.scale, e, from, [&](int, double t, double scale) __attribute__((always_inline)) { z = fma(t, scale, z); });
         }
     };
     while (at + EIGHT <= end) {
@@ -223,7 +227,7 @@ __global__ __launch_bounds__(BLOCK) void k_stats(Job A) {
     if (lane == 0) most_of[wave] = most;
     __syncthreads();
     most = fmaxf(fmaxf(most_of[0], most_of[1]), fmaxf(most_of[2], most_of[3]));
-    z = own > -INFINITY && most < INFINITY ? z * exp2_64(table, mc - (double)most * A.c) : 0.0;
+    z = own > -INFINITY && most < INFINITY ? z * exp2_64(table, A.scale, from - (double)most) : 0.0;
 #pragma unroll
     for (int d = 32; d; d >>= 1) z += __shfl_xor(z, d);
     if (lane == 0) sum_of[wave] = z;
@@ -282,7 +286,8 @@ template <int DT>
 struct Left {
     const typename type<DT>::t *x, *y;
     Row p, q;
-    double a, c;
+    double a;
+    Scale scale;
     i64 v;
     const Tree *tree;
     const double *table;
@@ -292,13 +297,13 @@ struct Left {
         of(at, eight<DT>(x, at, v), a > 0 ? eight<DT>(y, at, v) : Entries<DT>{}, r);
     }
     __device__ __forceinline__ void of(i64 at, const Entries<DT> &e, const Entries<DT> &f, double (&r)[EIGHT]) const {
-        exponentials<DT>(table, e, c, p.mc, r);
+        exponentials<DT>(table, scale, e, p.most, r);
 #pragma unroll
         for (int i = 0; i < EIGHT; ++i) r[i] = probability(r[i], p.per_z);
         if (a > 0) {
             const double per = a * q.per_z;
             double o[EIGHT];
-            exponentials<DT>(table, f, c, q.mc, o);
+            exponentials<DT>(table, scale, f, q.most, o);
 #pragma unroll
             for (int i = 0; i < EIGHT; ++i) r[i] = fmax(r[i] - o[i] * per, 0.0);
         }
@@ -335,7 +340,7 @@ __device__ __forceinline__ double sum_own(const Left<DT> &left) {
     Entries<DT> e = first_eight<DT>(left.x, at, left.v), f = first_eight<DT>(left.y, at, left.v);
     double sum = 0;
     const double ratio = left.a * left.q.per_z / left.p.per_z;
-    auto add = [&](const Entries<DT> &e, const Entries<DT> &f) __attribute__((always_inline)) { add_left<DT>(left.table, e, f, left.c, left.p.mc, left.q.mc, ratio, sum); };
+    auto add = [&](const Entries<DT> &e, const Entries<DT> &f) __attribute__((always_inline)) { add_left<DT>(left.table, left.scale, e, f, left.p.most, left.q.most, ratio, sum); };
     while (at + EIGHT <= left.v) {
         const i64 next = at + WALK * EIGHT;
         const Entries<DT> e_ahead = first_eight<DT>(left.x, next, left.v), f_ahead = first_eight<DT>(left.y, next, left.v);
@@ -394,7 +399,7 @@ __device__ int find_left(const double *segment_sums, const Left<DT> &left, doubl
 }
 
 // The largest entry and the sum of a row of its slices', by a wavefront
-__device__ __forceinline__ Row join(const double *table, const Part *parts, int slices, double c) {
+__device__ __forceinline__ Row join(const double *table, const Scale &S, const Part *parts, int slices) {
     const int lane = threadIdx.x & 63;
     Part p = {0.0, -INFINITY, 0.0f};
     if (lane < slices) p = parts[lane];
@@ -403,11 +408,10 @@ __device__ __forceinline__ Row join(const double *table, const Part *parts, int 
 #pragma unroll
     for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
     if (bad || !(most > -INFINITY)) return {0.0, 0.0};
-    const double mc = (double)most * c;
-    double z = p.most > -INFINITY ? p.z * exp2_64(table, (double)p.most * c - mc) : 0.0;
+    double z = p.most > -INFINITY ? p.z * exp2_64(table, S, (double)p.most - (double)most) : 0.0;
 #pragma unroll
     for (int d = 32; d; d >>= 1) z += __shfl_xor(z, d);
-    return {mc, 1.0 / z};
+    return {(double)most, 1.0 / z};
 }
 
 // The sum behind a first refusal, max(p - q, 0), where another child is tried behind it.
@@ -427,10 +431,10 @@ __global__ __launch_bounds__(BLOCK) void k_first(Job A) {
     Entries<DT> e = first_eight<DT>(x, at, A.v), f = first_eight<DT>(y, at, A.v);
     take_table(table);
     __syncthreads();
-    const Row p = join(table, A.parts + row * A.slices, A.slices, A.c), q = join(table, A.parts + (A.n + row) * A.slices, A.slices, A.c);
+    const Row p = join(table, A.scale, A.parts + row * A.slices, A.slices), q = join(table, A.scale, A.parts + (A.n + row) * A.slices, A.slices);
     double sum = 0;
     const double ratio = q.per_z / p.per_z;
-    auto add = [&](const Entries<DT> &e, const Entries<DT> &f) __attribute__((always_inline)) { add_left<DT>(table, e, f, A.c, p.mc, q.mc, ratio, sum); };
+    auto add = [&](const Entries<DT> &e, const Entries<DT> &f) __attribute__((always_inline)) { add_left<DT>(table, A.scale, e, f, p.most, q.most, ratio, sum); };
     while (at + EIGHT <= A.v) {
         const i64 next = at + (i64)A.firsts * (BLOCK * EIGHT);
         const Entries<DT> e_ahead = first_eight<DT>(x, next, A.v), f_ahead = first_eight<DT>(y, next, A.v);
@@ -458,7 +462,7 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
     for (int d = t; d <= A.depth; d += WALK) A.out[(i64)b * (A.depth + 1) + d] = -1;
     for (int r = wave; r < nodes * (A.drafted ? 2 : 1); r += WALK / 64) {
         const i64 row = r < nodes ? s0 + r : A.n + s0 + r - nodes;
-        const Row joined = join(sh.table, A.parts + row * A.slices, A.slices, A.c);
+        const Row joined = join(sh.table, A.scale, A.parts + row * A.slices, A.slices);
         if (lane == 0) A.rows[row] = joined;
     }
     __syncthreads();
@@ -470,7 +474,7 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
             auto of = [&](int which) {
                 const Row r = A.rows[(which ? A.n : 0) + s0 + parent];
                 if (r.per_z == 0) return 0.0;
-                return probability(exp2_64(sh.table, fma((double)(float)((const T *)A.x[which])[(s0 + parent) * A.ld[which] + token], A.c, -r.mc)), r.per_z);
+                return probability(exp2_64(sh.table, A.scale, (double)(float)((const T *)A.x[which])[(s0 + parent) * A.ld[which] + token] - r.most), r.per_z);
             };
             sh.have[i] = of(0);
             sh.said[i] = A.drafted ? of(1) : 1.0;
@@ -479,7 +483,7 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
     __syncthreads();
     // from here on all threads do the same
     Left<DT> left = {};
-    left.c = A.c, left.v = A.v, left.tree = &sh.tree, left.table = sh.table, left.nodes = nodes;
+    left.scale = A.scale, left.v = A.v, left.tree = &sh.tree, left.table = sh.table, left.nodes = nodes;
     int cur = 0, count = 0, refusals = 0;
     auto stand_at = [&](int node) {
         cur = node, left.a = 0, left.cur = -1, refusals = 0;
@@ -537,7 +541,7 @@ template <int DT, int THREADS>
 __device__ __forceinline__ Left<DT> left_at(const Job &A, int b, const End &end, Tree &tree, double *table) {
     typedef typename type<DT>::t T;
     Left<DT> left = {};
-    left.c = A.c, left.v = A.v, left.tree = &tree, left.table = table, left.a = end.a, left.cur = end.refused ? end.node : -1;
+    left.scale = A.scale, left.v = A.v, left.tree = &tree, left.table = table, left.a = end.a, left.cur = end.refused ? end.node : -1;
     take_table(table);
     if (end.refused) {
         i64 s0;
@@ -696,7 +700,7 @@ extern "C" int vi_verify_drafts(int dtype, const void *logits, int64_t n, int64_
     const hipStream_t s = (hipStream_t)stream;
     Job J = {};
     J.x[0] = logits, J.x[1] = draft, J.ld[0] = ld, J.ld[1] = ld_draft, J.n = n, J.v = v, J.slices = (int)slices_of(v, rows), J.per_slice = (int)per_slice_of(v, rows), J.firsts = (int)firsts_of(v, n), J.sequences = (int)sequences;
-    J.apart = (int)((n + sequences - 1) / sequences), J.depth = (int)depth, J.drafted = draft != nullptr, J.c = STEPS * 1.4426950408889634 / temperature, J.tokens = tokens, J.starts = starts, J.parents = parents;
+    J.apart = (int)((n + sequences - 1) / sequences), J.depth = (int)depth, J.drafted = draft != nullptr, J.scale.c = STEPS * 1.4426950408889634 / temperature, J.scale.deepest = DEEPEST / J.scale.c, J.tokens = tokens, J.starts = starts, J.parents = parents;
     J.uniforms = uniforms, J.counts = counts, J.nodes = nodes, J.out = out;
     J.rows = (Row *)vi::align16(ws);
     J.parts = (Part *)(J.rows + 2 * n);
