@@ -168,6 +168,28 @@ def far_logits(so):
                             assert got == want, (kind, v, far, near, t, given is not None, got, want)
 
 
+def few_tokens_left(so):
+    """Without a draft model, refusals that leave little or one token, or nothing: what is left is summed, not taken for what the refused ones lack to one."""
+    L = drafts(so)
+    for kind in (0, 1, 2):
+        for v in (3, 60, 1500):
+            for allowed in (2, 3, 5):
+                for seed in range(6):
+                    rng = np.random.default_rng(seed)
+                    allowed = min(allowed, v)
+                    x = np.full((allowed + 3, v), -np.inf, np.float32)
+                    tokens = rng.permutation(v)[:allowed]
+                    # one after the other 10 to 40 nats apart, or near each other
+                    x[0, tokens] = rng.standard_normal(allowed) if seed < 3 else -rng.uniform(5, 45, allowed).cumsum().astype(np.float32) / (1 if allowed < 5 else 3)
+                    x[1:, 0] = 0
+                    x = encode(x, kind)
+                    for u in ([ALMOST_ONE] * (allowed - 1) + [0.5], [ALMOST_ONE] * allowed, [ALMOST_ONE] * (allowed - 1) + [0.999]):
+                        # the same token twice; in the end the one that is left, again, and any
+                        children = tokens.tolist()[:-1] + [int(tokens[0]), int(tokens[-1])] + [int(tokens[-1])]
+                        got, want = verified(L, kind, x, None, [0] + children, [-1] + [0] * (allowed + 2), [0.4] + u[:-1] + [0.7, u[-1], 0.0], 2)
+                        assert got == want, (kind, v, allowed, seed, u, got, want)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[1]](sys.argv[2])
     print("OK")

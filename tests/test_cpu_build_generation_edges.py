@@ -37,3 +37,7 @@ def test_first_tokens_that_have_a_probability(built):
 
 def test_logits_far_from_nothing(built):
     check(built, "drafts", "far_logits")
+
+
+def test_few_tokens_left(built):
+    check(built, "drafts", "few_tokens_left")

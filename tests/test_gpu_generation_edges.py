@@ -120,3 +120,24 @@ def test_logits_far_from_nothing(dtype, v):
                 tokens, u = [0] + torch.randint(0, v, (3,), generator=g).tolist(), torch.rand(4, generator=g, dtype=torch.float64)
                 for given in (None, y):
                     check_drafts(x, tokens, [0, 4], [-1, 0, 0, 1], u, given, 2, t)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("v,allowed", [(3, 2), (60, 3), (60, 5), (33000, 2), (33000, 3)])
+def test_few_tokens_left(dtype, v, allowed):
+    """Without a draft model, refusals that leave little, one token or nothing: what is left is summed, not taken for what the refused ones lack to one."""
+    g = seeded(v, allowed, 44)
+    logits, tokens, u, parents = [], [], [], []
+    for seed in range(10):
+        for numbers in ([ALMOST_ONE] * (allowed - 1) + [0.5], [ALMOST_ONE] * allowed, [ALMOST_ONE] * (allowed - 1) + [0.999]):
+            x = torch.full((allowed + 3, v), -math.inf)
+            few = torch.randperm(v, generator=g)[:allowed]
+            # near each other, or one after the other 5 to 40 nats apart
+            x[0, few] = torch.randn(allowed, generator=g) if seed < 5 else -(torch.rand(allowed, generator=g) * 35 + 5).cumsum(0) / (1 if allowed < 5 else 3)
+            x[1:, 0] = 0
+            few = few.tolist()
+            logits.append(x.to(dtype))
+            tokens += [0] + few[:-1] + [few[0], few[-1], few[-1]]      # the same token twice; in the end the one that is left, and again
+            u += [0.4] + numbers[:-1] + [0.7, numbers[-1], 0.0]
+            parents += [-1] + [0] * (allowed + 2)
+    check_drafts(torch.cat(logits), tokens, list(range(0, len(tokens) + 1, allowed + 3)), parents, torch.tensor(u, dtype=torch.float64), None, 2)

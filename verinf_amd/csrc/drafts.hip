@@ -31,6 +31,7 @@ constexpr i64 MAX_BLOCKS = 1 << 23;            // of a launch, which has less th
 constexpr int MAX_NODES = 1024, MAX_DEPTH = 256;
 constexpr int EIGHT = 8;                       // neighbouring entries of a thread
 constexpr double MARGIN = 64;                  // bits
+constexpr double CLOSE = 0x1p-40;              // sums of up to 2^20 probabilities, 4096 a thread, are 2^-41 off at most
 
 struct Part {                                  // of a slice: an entry of its largest (NaN: it has a NaN or +inf), sum of 2^((x - most) c / 32)
     double z;
@@ -493,6 +494,14 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
         }
     };
     stand_at(0);
+    auto sum_of_waves = [&](double own) {
+        __syncthreads();
+        if (lane == 0) sh.sums[wave] = own;
+        __syncthreads();
+        double sum = 0;
+        for (int k = 0; k < WALK / 64; ++k) sum += sh.sums[k];
+        return sum;
+    };
     double w = 1;                              // the sum of what is left
     for (int i = 1; i < nodes; ++i) {
         if (sh.tree.parent[i] != cur || count == A.depth || left.p.per_z == 0 || (A.drafted && left.q.per_z == 0)) continue;
@@ -500,17 +509,19 @@ __global__ __launch_bounds__(WALK) void k_walk(Job A) {
         if (!A.drafted) {
             for (int j = 1; j < i; ++j)
                 if (sh.tree.parent[j] == cur && sh.tree.token[j] == sh.tree.token[i]) have = 0;        // refused before
+            // w is one without the refused, whose sum is CLOSE to right: summed anew where that might decide
+            if (left.cur >= 0 && have > 0 && fabs(sh.u[i] * w - have) <= CLOSE) {
+                left.nodes = i;
+                w = 0;
+                for (int s = wave; s < segments_of(A.v); s += WALK / 64) w += sum_segment(left, s);
+                w = sum_of_waves(w);
+            }
         } else if (refusals) {
             if (refusals == 1) {
                 w = 0;
                 for (int k = 0; k < A.firsts; ++k) w += A.first[(s0 + cur) * A.firsts + k];
             } else {
-                w = sum_own(left);
-                __syncthreads();
-                if (lane == 0) sh.sums[wave] = w;
-                __syncthreads();
-                w = 0;
-                for (int k = 0; k < WALK / 64; ++k) w += sh.sums[k];
+                w = sum_of_waves(sum_own(left));
             }
             have = fmax(have - left.a * sh.said[i], 0.0);
         }
