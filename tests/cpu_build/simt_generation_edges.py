@@ -70,6 +70,41 @@ def late_keys(so):
                     assert not bad.any(), ("late", value_scale, ahead, late, form, splits, int(bad.sum()), got[:3], want[:3])
 
 
+def small_weights(so, kinds):
+    """A key far ahead whose value is nothing, and what all the others' weights come to: wherever it is, in keys of one part and of several."""
+    L = attention(so)
+    for kind in kinds:
+        given = 2 if kind == 2 else 1
+        for count, value in ((1024, 1.0), (301, 1000.0), (1024, 0.01)):
+            for ahead in (10.0, 15.0, 18.5, 20.5, 22.5, 25.1):
+                for strong in (0, 40, count // 2, count - 1):
+                    key_scale, value_scale = np.float32(0.15), np.float32(value / 100)
+                    number = round(ahead * math.log(2) / 0.15) if kind == I8 else ahead * math.log(2)
+                    scores = np.zeros(count)
+                    scores[strong] = number
+                    m, q = one_token(kind, scores, key_scale=key_scale)
+                    m.data[1][:] = 100 if kind == I8 else encode(np.array([value]), kind)[0]
+                    if kind == I8:
+                        m.scales[1][:] = value_scale
+                    p_, r_ = m.place(0, strong)
+                    m.data[1][p_, :, r_] = 0
+                    exact = float(number * np.float64(key_scale)) if kind == I8 else float(decode(encode(np.array([number]), kind), kind)[0])
+                    v = float(100 * np.float64(value_scale)) if kind == I8 else float(decode(encode(np.array([value]), kind), kind)[0])
+                    others = (count - 1) * math.exp(-exact)
+                    want = v * others / (1 + others)
+                    # Weights are rounded to 16 bits, the other ones all alike: half a step of them, or fp16's 2^-25 where the largest is 2^7; scores and exponentials 2^-20; the result.
+                    weight = math.exp(-exact)
+                    rounding = ROUND[1 if kind == 1 else 2] * weight + (0 if kind == 1 else 2.0 ** -32)
+                    off = want * (rounding / weight + 2.0 ** -20 * (1 + exact)) + (2.0 ** -25 if kind == 2 else 0)
+                    for form, splits, per in FORMS:
+                        got = attended(L, m, q, form, splits, per, 1.0)[0, 0]
+                        assert (np.abs(got - want) <= off + ROUND[given] * (want + off)).all(), (kind, count, value, ahead, strong, form, splits, got[0], want, off)
+
+
+def small_weights_16(so):
+    small_weights(so, (1, 2))
+
+
 # ---- drafts -------------------------------------------------------------------------------------------------------
 def drafts(so):
     L = ctypes.CDLL(so)

@@ -27,6 +27,10 @@ def test_keys_far_above_those_before_them(built):
     check(built, "attention", "late_keys")
 
 
+def test_weights_that_are_small_together(built):
+    check(built, "attention", "small_weights_16")
+
+
 def test_drafts_of_masked_tokens(built):
     check(built, "drafts", "masked_drafts")
 

@@ -52,6 +52,35 @@ def test_keys_far_above_those_before_them(tokens, count, value_scale):
                 assert ((got - want).abs() <= off + r * (want.abs() + off)).all(), (ahead, late, longest)
 
 
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [1, 100])
+@pytest.mark.parametrize("count,value", [(1024, 1.0), (301, 1000.0), (6000, 0.01)])
+def test_weights_that_are_small_together(kind, tokens, count, value):
+    """A key far ahead whose value is nothing, and what all the others' weights come to: wherever it is, in keys of one part and of several."""
+    key_scale, value_scale = (0.15, value / 100) if kind == torch.int8 else (1.0, value)
+    for ahead in (10.0, 15.0, 18.5, 20.5, 22.5, 25.1):
+        for strong in (0, 40, count // 2, count - tokens):
+            scores = torch.zeros(count)
+            scores[strong] = round(ahead * math.log(2) / key_scale) if kind == torch.int8 else ahead * math.log(2)
+            m, q, page, row = with_scores(kind, scores, tokens)
+            m.cache.values.fill_(100 if kind == torch.int8 else value)
+            m.cache.values[page[strong], 0, row[strong]] = 0
+            if kind == torch.int8:
+                m.cache.key_scales.fill_(key_scale)
+                m.cache.value_scales.fill_(value_scale)
+            exact = m.held(0, "keys", count)[strong, 0, 0]             # ahead by so much
+            weight, v = torch.exp(-exact), m.held(0, "values", count)[(strong + 1) % count, 0, 0]
+            others = (torch.arange(count - tokens, count) * weight)[:, None]
+            want = v * others / (1 + others)
+            # Weights are rounded to 16 bits, the other ones all alike: half a step of them, or fp16's 2^-25 where the largest is 2^7; scores and exponentials 2^-20; the result.
+            bf16 = kind == torch.bfloat16
+            rounding = ROUND[kind if bf16 else torch.float16] * weight + (0 if bf16 else 2.0 ** -32)
+            off = want * (rounding / weight + 2.0 ** -20 * (1 + exact)) + (2.0 ** -25 if kind == torch.float16 else 0)
+            for longest in (None, 0):
+                got = gen.attend_cache(q, m.cache, m.batch, scale=1.0, longest=longest)
+                assert ((got[:, 0].cpu().double() - want).abs() <= off + ROUND[got.dtype] * (want + off)).all(), (ahead, strong, longest)
+
+
 # ---- drafts -------------------------------------------------------------------------------------------------------
 ALMOST_ONE = 1.0 - 2.0 ** -53
 

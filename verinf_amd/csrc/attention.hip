@@ -13,7 +13,8 @@
 // meet all banks: unit u (16 bytes) of a row lies at u ^ order(row).  WM wavefronts share a stage; WK such groups take every WK-th stage and are added at the end.  Where
 // there are few tiles the keys are cut between workgroups too, and k_join adds what they leave.
 //
-// Roundings: P to the type of the queries (as V has), to fp16 for 8-bit integers, relative to a largest score that may be up to 2^8 behind; all sums in 32 bits.
+// Roundings: P to the type of the queries (as V has), to fp16 for 8-bit integers, relative to a largest score that may be up to 2^8 behind, fp16 with 2^7 of what it has room for
+// above that; all sums in 32 bits.
 //
 // What bounds it (bf16, 8 heads of 128 columns for 32, where nothing else is said): 64 sequences of 4096 entries and a token each 198 us, 5.4 TB/s, as a large copy
 // (118 us over 8-bit integers, 4.7); 4096 tokens of a prompt, 32 heads of the cache, fp16, 198 us, 694 TFLOP/s, where the matrix units are busy for a third of the time and
@@ -53,6 +54,8 @@ struct Form {
     static constexpr int ROW = DP * (I8 ? 1 : 2), UNITS = ROW / 16, PER_LOAD = 64 / UNITS, LOADS = 16 / PER_LOAD;       // bytes, units; rows of a load, loads of a group
     static constexpr int SCALES = I8 ? KEYS * 4 : 0, HALF = KEYS * ROW + SCALES, STAGE = 2 * HALF;
     static constexpr int MINE = GROUPS * LOADS / WM, KINDS = LOADS > WM ? LOADS / WM : 1;              // loads of a wavefront in half a stage, different ones of a group
+    // fp16's weights are 2^RAISED times as large, sums with them: up to 2^15, so that those 2^-21 of the largest still have all digits, and 2^-32 of it is half a step
+    static constexpr float RAISED = DT_ == VI_F16 && !I8_ ? 7.0f : 0.0f;
     static constexpr int PITCH = 36;           // floats between rows of 32 on their way out
     static constexpr int OUT = WAVES * 32 * PITCH * 4 + WAVES * 32 * 8 + ROWS * 8;
     static constexpr int LDS = WK * ST * STAGE > OUT ? WK * ST * STAGE : OUT;
@@ -498,6 +501,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             for (int db = 0; db < DP / 32; ++db) o[db] *= less;
         }
     };
+    auto base_of = [&](float relative) INLINE { return relative == -INFINITY ? 0.0f : relative - F::RAISED; };
     // The exponentials of scores, as the second operand of the product with V^T.
     struct Weights {
         float of[16];
@@ -559,7 +563,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     };
     auto weights = [&](const v16f &s, const char *scales, bool masked, v4u (&p)[2]) INLINE {
         Weights f = scales_of(s, scales, masked);
-        const float base = relative == -INFINITY ? 0.0f : relative;
+        const float base = base_of(relative);
 #pragma unroll
         for (int i = 0; i < 8; ++i) weigh(s, f, base, i);
         words_of(f, p);
@@ -568,7 +572,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     // products one after the other, each of which waits for the one before (4096 tokens of a prompt 206 us so, 201 in this order).
     auto weights_and_scores = [&](const v16f &s, const char *scales, bool masked, v4u (&p)[2], const char *k, const char *key_scales) INLINE {
         Weights f = scales_of(s, scales, masked);
-        const float base = relative == -INFINITY ? 0.0f : relative;
+        const float base = base_of(relative);
         constexpr int PRODUCTS = DP / 16;
         __builtin_amdgcn_sched_barrier(0);
         const v16f ahead = scores_beside(k, key_scales, [&](int st) INLINE {
