@@ -80,6 +80,7 @@ template <class V>
 float simt_dot2(V a, V b, float c) { return (float)a[0] * (float)b[0] + (float)a[1] * (float)b[1] + c; }
 #define __builtin_amdgcn_sched_barrier(mask)
 #define __builtin_amdgcn_fdot2(a, b, c, clamp) simt_dot2(a, b, c)
+#define __builtin_amdgcn_fdot2_f32_bf16(a, b, c, clamp) simt_dot2(a, b, c)
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, x, y, z) simt::mfma_32x32x16(a, b, c)
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, x, y, z) simt::mfma_32x32x16(a, b, c)
 #define __builtin_amdgcn_ds_read_tr16_b64_v4i16(p) simt::transposed<v4s, short, 4>(p)

@@ -105,6 +105,23 @@ def small_weights_16(so):
     small_weights(so, (1, 2))
 
 
+def values_alike(so):
+    """Values all alike come out as they are, whatever 16 bits make of their weights: of late keys that count for nearly all, too."""
+    L = attention(so)
+    for kind in (1, 2):
+        for count in (60, 300):
+            for dim in (64, 128):
+                rng = np.random.default_rng(count + dim)
+                late = [np.where(np.arange(count) == at, x, np.where(np.arange(count) == 0, 0.0, -30.0)) for x in (4.55, 4.9, 5.0, 5.5) for at in (29, 40, 129) if at < count]
+                for scores in (rng.standard_normal(count), rng.standard_normal(count) * 4, np.linspace(0, 5, count), *late):
+                    m, q = one_token(kind, scores, dim)
+                    v = encode(rng.standard_normal(dim), kind)
+                    m.data[1][:] = v
+                    for form, splits, per in FORMS:
+                        got = attended(L, m, q, form, splits, per, 1.0)[0, 0]
+                        assert np.array_equal(got, decode(v, kind).astype(np.float64)), (kind, count, dim, form, splits)
+
+
 # ---- drafts -------------------------------------------------------------------------------------------------------
 def drafts(so):
     L = ctypes.CDLL(so)

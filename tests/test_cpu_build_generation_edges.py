@@ -31,6 +31,10 @@ def test_weights_that_are_small_together(built):
     check(built, "attention", "small_weights_16")
 
 
+def test_values_all_alike(built):
+    check(built, "attention", "values_alike")
+
+
 def test_drafts_of_masked_tokens(built):
     check(built, "drafts", "masked_drafts")
 

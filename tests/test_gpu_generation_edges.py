@@ -81,6 +81,24 @@ def test_weights_that_are_small_together(kind, tokens, count, value):
                 assert ((got[:, 0].cpu().double() - want).abs() <= off + ROUND[got.dtype] * (want + off)).all(), (ahead, strong, longest)
 
 
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [48, 64, 128, 256])
+@pytest.mark.parametrize("tokens", [1, 100])
+def test_values_all_alike_come_out_as_they_are(kind, dim, tokens):
+    """What is added up of weights is what is multiplied: sums are 2^-20 off, which does not move a number of 16 bits."""
+    g = seeded(dim, tokens, 45)
+    for count in (230, 4000):
+        # one late key that counts for nearly all, its weight relative to the first
+        late = [torch.tensor([0.0] + [-30.0] * (at - 1) + [x] + [-30.0] * (count - at - 1)) for x in (4.55, 4.9, 5.0, 5.5) for at in (29, 129)]
+        for scores in (torch.randn(count, generator=g), torch.randn(count, generator=g) * 4, torch.linspace(0, 5, count), *late):
+            m, q, page, row = with_scores(kind, scores, tokens, dim)
+            v = torch.randn(dim, generator=g).to(kind).cuda()
+            m.cache.values[:] = v
+            for longest in (None, 0):
+                got = gen.attend_cache(q, m.cache, m.batch, scale=1.0, longest=longest)
+                assert torch.equal(got, v.expand_as(got)), (count, longest)
+
+
 # ---- drafts -------------------------------------------------------------------------------------------------------
 ALMOST_ONE = 1.0 - 2.0 ** -53
 

@@ -14,7 +14,8 @@
 // there are few tiles the keys are cut between workgroups too, and k_join adds what they leave.
 //
 // Roundings: P to the type of the queries (as V has), to fp16 for 8-bit integers, relative to a largest score that may be up to 2^8 behind, fp16 with 2^7 of what it has room for
-// above that; all sums in 32 bits.
+// above that; their sum is of them as rounded, but over 8-bit integers, where it is of the exponentials; all sums in 32 bits.  The matrix instructions take 16 bits, and P as a sum of
+// two such numbers would be half as many products again; with one, a bf16 result is up to 1.4 times as far from 64 bits as its own rounding takes it.
 //
 // What bounds it (bf16, 8 heads of 128 columns for 32, where nothing else is said): 64 sequences of 4096 entries and a token each 198 us, 5.4 TB/s, as a large copy
 // (118 us over 8-bit integers, 4.7); 4096 tokens of a prompt, 32 heads of the cache, fp16, 198 us, 694 TFLOP/s, where the matrix units are busy for a third of the time and
@@ -142,10 +143,12 @@ __device__ __forceinline__ v4u widen(v2u w) {
 __device__ __forceinline__ int two_of(int i) { return i / 2 * 4 + i % 2; }            // the first of word i
 __device__ __forceinline__ float element_of(v4u w, int i) { return (float)__builtin_bit_cast(_Float16, (unsigned short)(w[i / 2] >> (16 * (i & 1)))); }
 // the sum of both halves of a word and c
+template <int DT>
 __device__ __forceinline__ float add_two(u32 w, float c) {
-    typedef _Float16 v2h __attribute__((ext_vector_type(2)));
-    const v2h ones = {(_Float16)1.0f, (_Float16)1.0f};
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, w), ones, c, false);
+    typedef typename type<DT>::t v2t __attribute__((ext_vector_type(2)));
+    const v2t ones = {(typename type<DT>::t)1.0f, (typename type<DT>::t)1.0f}, two = __builtin_bit_cast(v2t, w);
+    if constexpr (DT == VI_BF16) return __builtin_amdgcn_fdot2_f32_bf16(two, ones, c, false);
+    else return __builtin_amdgcn_fdot2(two, ones, c, false);
 }
 
 template <int DT>
@@ -386,7 +389,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     for (int db = 0; db < DP / 32; ++db) o[db] = v16f{};
     // For 8-bit integers, exponentials times scales are multiplied by `gain` to be in fp16's range: a power of two at first, 2^14 at most of the largest so far.
     float gain = MAX_GAIN, weighed = 0;
-    float most = -INFINITY, relative = -INFINITY, sum = 0;             // largest score so far (or up to LATE behind), times c: what the sums are relative to
+    float most = -INFINITY, relative = -INFINITY, sum = 0, sum_odd = 0;             // largest score so far (or up to LATE behind), times c: what the sums are relative to
 
     // which of the 32 keys from j on the lane's row attends to; the low and the high sixteen have so many
     auto window_of = [&](int j, int low, int high) INLINE {
@@ -489,7 +492,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             asm volatile("");                  // a branch: the compiler would multiply by one, each time
             const float now = fmaxf(most, top), then = now * c;
             const float by = relative == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(relative - then);
-            most = now, relative = then, sum *= by;
+            most = now, relative = then, sum *= by, sum_odd *= by;
             float less = by;                   // of the products' sums: where they have a power of their own that follows
             if constexpr (F::I8) {
                 // MAX_GAIN / gain may be beyond 32 bits where `by` is nothing; what both come to is 1 at most
@@ -528,12 +531,16 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     auto weigh = [&](const v16f &s, Weights &f, float base, int i) INLINE {
         const int one = F::I8 ? i / 4 * 8 + two_of(i % 4) : 2 * i, two = F::I8 ? one + 2 : one + 1;
         const float a = __builtin_amdgcn_exp2f(fmaf(s[one], c, -base)), b = __builtin_amdgcn_exp2f(fmaf(s[two], c, -base));
-        sum += a + b;
+        if (F::I8) sum += a + b;               // others as rounded (word_of)
         f.of[one] = F::I8 ? a * f.of[one] : a, f.of[two] = F::I8 ? b * f.of[two] : b;
     };
+    // The sum is of what is multiplied, rounded, so that values all alike come out as they are (a prompt of 4096, four heads to one of the cache, 180 us, 176 with the sum of the exponentials
+    // themselves, which was 0.3 per cent off beside one late key); in two, for an addition waits for the one before.  For 8-bit integers it cannot be, for their weights have scales in them.
     auto word_of = [&](const Weights &f, int i) INLINE {
         const int one = F::I8 ? i / 4 * 8 + two_of(i % 4) : 2 * i, two = F::I8 ? one + 2 : one + 1;
-        return F::I8 ? pack<CT>(f.of[one] * gain, f.of[two] * gain) : pack<CT>(f.of[one], f.of[two]);
+        const u32 word = F::I8 ? pack<CT>(f.of[one] * gain, f.of[two] * gain) : pack<CT>(f.of[one], f.of[two]);
+        if constexpr (!F::I8) (i & 1 ? sum_odd : sum) = add_two<CT>(word, i & 1 ? sum_odd : sum);
+        return word;
     };
     // For 8-bit integers: in fp16's range, and what the integers are more than themselves goes by them as rounded
     auto words_of = [&](const Weights &f, v4u (&p)[2]) INLINE {
@@ -558,7 +565,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             p[i / 4][i % 4] = word_of(f, i);
-            if constexpr (F::I8) weighed = add_two(p[i / 4][i % 4], weighed);
+            if constexpr (F::I8) weighed = add_two<CT>(p[i / 4][i % 4], weighed);
         }
     };
     auto weights = [&](const v16f &s, const char *scales, bool masked, v4u (&p)[2]) INLINE {
@@ -767,7 +774,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
     __syncthreads();
     float *buf = (float *)lds, *of_waves = buf + F::WAVES * 32 * F::PITCH, *of_rows = of_waves + F::WAVES * 32 * 2;
     {
-        sum = sum_of_halves(sum);
+        sum = sum_of_halves(sum + sum_odd);
         if (half == 0) of_waves[(wave * 32 + lane) * 2] = relative, of_waves[(wave * 32 + lane) * 2 + 1] = sum;
     }
     __syncthreads();
