@@ -122,6 +122,26 @@ def values_alike(so):
                         assert np.array_equal(got, decode(v, kind).astype(np.float64)), (kind, count, dim, form, splits)
 
 
+def small_scales(so):
+    """Queries and scales so small that all scores are nothing: each key counts alike, and none that is hidden."""
+    L = attention(so)
+    for kind in (1, 2, I8):
+        for scale in (1e-10, 1e-30, 1e-45):
+            for size in (0.0, 1e-30, 1.0):
+                for count in (40, 300):
+                    m = Made(kind, [count - 3], [3], 1, 64, 64)
+                    q = encode(np.full((3, 1, 64), size), 2 if kind == 2 else 1)
+                    v = np.stack([m.held(1, 0, j)[0] for j in range(count)])
+                    for form, splits, per in FORMS:
+                        got = attended(L, m, q, form, splits, per, scale)[:, 0]
+                        for i in range(3):
+                            seen = v[:count - 2 + i]
+                            want, size_ = seen.mean(0), np.abs(seen).mean(0)
+                            # weights all alike are right, but times scales over integers, where they are fp16 and 32-bit sums of values up to 256; the result
+                            off = 2.0 ** -20 * size_ + (2.0 ** -11 * size_ + (count / 16 + 8) * 2.0 ** -24 * 256 * 0.03 if kind == I8 else 0) + (2.0 ** -25 if kind == 2 else 0)
+                            assert (np.abs(got[i] - want) <= off + ROUND[2 if kind == 2 else 1] * (np.abs(want) + off)).all(), (kind, scale, size, count, form, splits, i, got[i][:3], want[:3])
+
+
 # ---- drafts -------------------------------------------------------------------------------------------------------
 def drafts(so):
     L = ctypes.CDLL(so)

@@ -35,6 +35,10 @@ def test_values_all_alike(built):
     check(built, "attention", "values_alike")
 
 
+def test_scores_that_are_all_nothing(built):
+    check(built, "attention", "small_scales")
+
+
 def test_drafts_of_masked_tokens(built):
     check(built, "drafts", "masked_drafts")
 

@@ -6,7 +6,7 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
-from test_gpu_generation import FLOATS, ROUND, Made, check_drafts, seeded  # noqa: E402
+from test_gpu_generation import CACHED, FLOATS, ROUND, Made, check_drafts, seeded  # noqa: E402
 from verinf_amd.prover import generation as gen  # noqa: E402
 
 
@@ -97,6 +97,23 @@ def test_values_all_alike_come_out_as_they_are(kind, dim, tokens):
             for longest in (None, 0):
                 got = gen.attend_cache(q, m.cache, m.batch, scale=1.0, longest=longest)
                 assert torch.equal(got, v.expand_as(got)), (count, longest)
+
+
+@pytest.mark.parametrize("kind", CACHED)
+@pytest.mark.parametrize("scale", [1e-10, 1e-30, 1e-45])
+@pytest.mark.parametrize("tokens", [3, 100])
+def test_scores_that_are_all_nothing(kind, scale, tokens):
+    """Queries and scales so small that all scores are nothing: each key counts alike, and none that is hidden."""
+    for size in (0.0, 1e-30, 1.0):
+        for count in (140, 3000):
+            m = Made(kind, [count - tokens], [tokens], 1, 64, 64)
+            q = torch.full((tokens, 1, 64), size, dtype=torch.float16 if kind == torch.float16 else torch.bfloat16, device="cuda")
+            v, seen = m.held(0, "values", count)[:, 0], torch.arange(count - tokens + 1, count + 1)[:, None]
+            want, size_ = v.cumsum(0)[count - tokens:] / seen, v.abs().cumsum(0)[count - tokens:] / seen
+            # Weights all alike are right, but times scales over integers, where they are fp16 and 32-bit sums of values up to 256; sums; the result.
+            off = 2.0 ** -20 * size_ + (2.0 ** -11 * size_ + (count / 16 + 8) * 2.0 ** -24 * 256 * 0.03 if kind == torch.int8 else 0) + (2.0 ** -25 if kind == torch.float16 else 0)
+            got = gen.attend_cache(q, m.cache, m.batch, scale=scale)
+            assert ((got[:, 0].cpu().double() - want).abs() <= off + ROUND[got.dtype] * (want.abs() + off)).all(), (size, count)
 
 
 # ---- drafts -------------------------------------------------------------------------------------------------------

@@ -258,7 +258,7 @@ __global__ __launch_bounds__(F::THREADS, F::OCC) void k_attend(Args A) {
             for (int i = 0; i < 8; ++i) largest = fmaxf(largest, fabsf(number(q[st], i)));
         const u32 exponent = __float_as_uint(most_of_halves(largest)) >> 23, e = exponent == 255 ? 141 : max(exponent, 15u);
         const float by = __uint_as_float((268 - e) << 23);
-        c = c * OF_BYTES * __uint_as_float((e - 14) << 23);            // in this order a normal number
+        c = fmaxf(c * OF_BYTES * __uint_as_float((e - 14) << 23), 0x1p-126f);      // nothing would make a NaN of a hidden key's -inf; scores that this is much for are nothing either
 #pragma unroll
         for (int st = 0; st < DP / 16; ++st) {
             v4u r;
