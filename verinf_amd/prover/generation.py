@@ -94,13 +94,19 @@ def rotary_plan(dim, base=10000.0, interleaved=False, scaling=None, device="cuda
         raise RuntimeError(f"rotary_plan: {dim} columns (even, up to 256)")
     if not (base > 1 and math.isfinite(base)):
         raise RuntimeError(f"rotary_plan: a base of {base}")
-    kind, factor, *more = scaling or (None, 1.0)
+    try:
+        kind, factor, *more = scaling or (None, 1.0)
+    except (TypeError, ValueError):
+        raise RuntimeError(f"rotary_plan: no scaling {scaling!r}") from None
     if kind not in (None, "linear", "base", "parts") or (kind == "parts") != (len(more) in (1, 3)) or (kind != "parts" and more):
         raise RuntimeError(f"rotary_plan: no scaling {scaling!r}")
     if not (factor >= 1 and math.isfinite(factor)):
         raise RuntimeError(f"rotary_plan: a factor of {factor}")
     half = dim // 2
     if kind == "base" and half > 1:
+        # base factor^(half / (half - 1)), which is beyond what a power gives where it is infinite
+        if math.log(base) + math.log(factor) * half / (half - 1) >= 709.0:
+            raise RuntimeError(f"rotary_plan: a base of {base} and a factor of {factor}")
         base = base * factor ** (half / (half - 1))
     radians = [base ** (-i / half) for i in range(half)]
     amplitude = 1.0
