@@ -262,6 +262,21 @@ def few_tokens_left(so):
                         assert got == want, (kind, v, allowed, seed, u, got, want)
 
 
+def next_to_the_border(so):
+    """Drafts whose number is 3 10^-14 of it above or below p / q.  Entries are at most 32 below their row's largest: differences of them are 32 2^-53 off, their exponentials
+    4 10^-16, sums and quotients 10 2^-53 - of p and q together 10^-14."""
+    L = drafts(so)
+    for kind in (0, 1, 2):
+        rng = np.random.default_rng(kind)
+        x, y = (encode(np.clip(rng.standard_normal((2, 300)) * 3, -16, 16), kind) for _ in range(2))
+        p, q = (np.exp(z - z.max()) for z in (decode(x[0], kind).astype(np.longdouble), decode(y[0], kind).astype(np.longdouble)))
+        share = (p / p.sum()) / (q / q.sum())
+        for token in np.argsort(share)[:40].tolist():
+            for above in (0, 1):
+                (count, _, _), _ = verified(L, kind, x, y, [0, token], [-1, 0], [0.5, float(share[token] * (1 + (2 * above - 1) * np.longdouble(3e-14)))], 1)
+                assert count == 1 - above, (kind, token, above)
+
+
 if __name__ == "__main__":
     globals()[sys.argv[1]](sys.argv[2])
     print("OK")

@@ -53,3 +53,7 @@ def test_logits_far_from_nothing(built):
 
 def test_few_tokens_left(built):
     check(built, "drafts", "few_tokens_left")
+
+
+def test_numbers_next_to_the_border(built):
+    check(built, "drafts", "next_to_the_border")

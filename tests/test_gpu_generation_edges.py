@@ -205,3 +205,22 @@ def test_few_tokens_left(dtype, v, allowed):
             u += [0.4] + numbers[:-1] + [0.7, numbers[-1], 0.0]
             parents += [-1] + [0] * (allowed + 2)
     check_drafts(torch.cat(logits), tokens, list(range(0, len(tokens) + 1, allowed + 3)), parents, torch.tensor(u, dtype=torch.float64), None, 2)
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("v", [300, 20000])
+def test_numbers_next_to_the_border(dtype, v):
+    """Drafts whose number is 3 10^-14 of it above or below p / q.  Entries are at most 32 below their row's largest: differences of them, times log2(e), are 32 2^-53 off, their
+    exponentials 4 10^-16, sums and quotients 10 2^-53 - of p and q together 10^-14."""
+    g = seeded(v, 46)
+    n = 300
+    logits, draft = ((torch.randn(2 * n, v, generator=g) * 3).clamp(-16, 16).to(dtype) for _ in range(2))
+    p, q = (torch.softmax(x[::2].double(), dim=1) for x in (logits, draft))
+    x = (q / p).topk(20, dim=1).indices.gather(1, torch.randint(0, 20, (n, 1), generator=g))
+    share = (p.gather(1, x) / q.gather(1, x))[:, 0]
+    above = torch.arange(n) % 2
+    u = torch.stack((torch.full((n,), 0.5, dtype=torch.float64), share * (1 + (2 * above - 1).double() * 3e-14)), dim=1)
+    assert (u < 1).all()
+    tokens = torch.stack((torch.zeros_like(x[:, 0]), x[:, 0]), dim=1)
+    counts, _, _ = gen.verify_drafts(logits.cuda(), tokens.flatten().cuda(), (torch.arange(n + 1) * 2).int().cuda(), None, u.flatten().cuda(), 1, draft_logits=draft.cuda())
+    assert torch.equal(counts.cpu(), 1 - above)

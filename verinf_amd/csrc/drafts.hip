@@ -10,13 +10,13 @@
 // the refused tokens and is otherwise p.
 //
 // Whole numbers come of it, decided by comparisons next to borders, of which the last token's have as many as there are tokens: all in 64
-// bits, exponentials too (1.6e-13 off).
+// bits, exponentials too (4e-16 off).
 //
 // All rows' largest entries and sums, in slices (k_stats), and the sums behind a first refusal, for nodes with other children (k_first), are taken by the whole
 // chip; a workgroup a sequence walks (k_walk), with a pass over two rows for each further refusal; the whole chip adds up what is left behind the paths
 // (k_left), and a workgroup a sequence looks for the token (k_pick).
 //
-// What bounds them: some 15 instructions an exponential, eleven of them in 64 bits, which issue every 5 cycles.  64 trees of 16 nodes, 32000 bf16 logits of both models:
+// What bounds them: some 16 instructions an exponential, twelve of them in 64 bits, which issue every 5 cycles.  64 trees of 16 nodes, 32000 bf16 logits of both models:
 // 114 us (45 all rows' sums, 23 first refusals, 52 the walk of the sequence with the most refusals, 9 us each, 11 the last tokens; 25 to read them); with the 11
 // powers of a series on [-1/2, 1/2] in place of table and 4 powers 149 in place of 126.  One chain of five nodes, f32: 15 us, the latency of four launches.
 #include "cache.hpp"
@@ -42,7 +42,7 @@ struct Row {                                   // of a row: the largest, which i
 };
 
 // 2^(d c / 32) of N numbers side by side (one alone waits for itself at each step), d c up to 0 or hardly above, less than LEAST from where it would be that: the whole part by an
-// addition whose result has units of one, its last five bits from a table, the others into the exponent, the rest by a polynomial (over Chebyshev's nodes, 1.6e-13).
+// addition whose result has units of one, its last five bits from a table, the others into the exponent, the rest by a polynomial (over Chebyshev's nodes, 1.4e-16).
 // d is a difference of entries, taken before the product: c times an entry of 10^38 has no digits that c times another could be taken from.
 // The table has 256 bytes, a pair of banks to each entry; the exponent comes into the entry by adding the whole part as it is, 15 bits up in the upper half, from
 // where the entry has lost its own number before.
@@ -63,7 +63,7 @@ __device__ __forceinline__ void take_table(double *table) {        // a barrier 
 }
 template <int N>
 __device__ __forceinline__ void exp2_64(const double *table, const Scale &S, double (&d)[N], double (&scale)[N]) {         // times scale
-    constexpr double C[] = {9.172598566029335e-09, 1.6938609067364198e-06, 0.00023459619820112603, 0.021660849392187844, 1.0};
+    constexpr double C[] = {3.9737238568525983e-11, 9.172607532092245e-09, 1.6938509724285119e-06, 0.0002345961981994449, 0.021660849392498290, 1.0};
     double m[N], f[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -76,7 +76,7 @@ __device__ __forceinline__ void exp2_64(const double *table, const Scale &S, dou
         d[e] = C[0];
     }
 #pragma unroll
-    for (int i = 1; i < 5; ++i)
+    for (int i = 1; i < 6; ++i)
 #pragma unroll
         for (int e = 0; e < N; ++e) d[e] = fma(d[e], f[e], C[i]);
 }
