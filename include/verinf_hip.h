@@ -451,7 +451,7 @@ int vi_append_tokens(const vi_cache *cache, const vi_batch *batch, int dtype, co
 
 /* out = softmax(scale q k^T) v over the cache's entries, for q (n, heads, dim): heads / cache->heads heads of q share one of the cache's.  New token i of
  * a sequence attends to all entries before the new ones' and, of those, to 0 .. i (parents NULL), or to itself and its ancestors: parents[row] is its parent's
- * number in its sequence, lower than its own, anything else makes it a root.  A sequence of more than 256 new tokens is taken for a chain.  A token that
+ * number in its sequence, lower than its own, anything else makes it a root.  A sequence of more than 256 new tokens is taken for a chain, whatever parents says.  A token that
  * attends to nothing gets zeros.  dtype VI_BF16 or VI_F16 as the cache's; VI_BF16 for a cache of VI_I8, then of queries below
  * 2^100.  clear: rows of no sequence become zero.  longest:
  * no sequence is longer (a hint: how the work is cut).  ws: vi_attend_cache_workspace_bytes() bytes of device scratch. */

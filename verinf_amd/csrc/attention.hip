@@ -17,10 +17,13 @@
 // above that; their sum is of them as rounded, but over 8-bit integers, where it is of the exponentials; all sums in 32 bits.  The matrix instructions take 16 bits, and P as a sum of
 // two such numbers would be half as many products again; with one, a bf16 result is up to 1.4 times as far from 64 bits as its own rounding takes it.
 //
-// What bounds it (bf16, 8 heads of 128 columns for 32, where nothing else is said): 64 sequences of 4096 entries and a token each 198 us, 5.4 TB/s, as a large copy
-// (118 us over 8-bit integers, 4.7); 4096 tokens of a prompt, 32 heads of the cache, fp16, 198 us, 694 TFLOP/s, where the matrix units are busy for a third of the time and
-// the exponentials and their like, 125 instructions to each 16 products, for half of it (180 us, 766 TFLOP/s, with four heads to one of the cache; 236 over 8-bit
-// integers); a token over 1000 entries 12.5 us, the latency of two launches.
+// What bounds it (bf16, 8 heads of 128 columns for 32, where nothing else is said): 64 sequences of 4096 entries and a token each 202 us, 5.3 TB/s, as a large copy
+// (118 to 124 us over 8-bit integers, 4.5 to 4.7); 4096 tokens of a prompt, 32 heads of the cache, fp16, 193 to 202 us, 680 to 712 TFLOP/s, where the matrix units are busy for a third of the time and
+// the exponentials and their like, some 120 instructions to each 16 products, for half of it (180 us, 765 TFLOP/s, with four heads to one of the cache; 238 over 8-bit
+// integers); a token over 1000 entries 12.5 us, over 128, of which a wavefront has one stage, 8.8 in one launch: loads behind each other, of sequence, page and keys.
+//
+// Columns that are none of 64, 128 or 256 leave units empty, which are zeros in LDS, written anew with each stage, whose loads are waited for at once: 64 tokens over 4096 entries of 80, 96 and
+// 112 columns 143, 161 and 185 us, 4.7 to 5.1 TB/s, of 8-bit integers 124 to 138, 2.9 to 3.5; 4096 tokens of a prompt 231 to 233 us, of 128 columns 178 to 180.
 #include <type_traits>
 
 #include "cache.hpp"

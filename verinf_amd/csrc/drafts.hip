@@ -17,8 +17,10 @@
 // (k_left), and a workgroup a sequence looks for the token (k_pick).
 //
 // What bounds them: some 16 instructions an exponential, twelve of them in 64 bits, which issue every 5 cycles.  64 trees of 16 nodes, 32000 bf16 logits of both models:
-// 114 us (45 all rows' sums, 23 first refusals, 52 the walk of the sequence with the most refusals, 9 us each, 11 the last tokens; 25 to read them); with the 11
-// powers of a series on [-1/2, 1/2] in place of table and 4 powers 149 in place of 126.  One chain of five nodes, f32: 15 us, the latency of four launches.
+// 116 us over three sets of inputs, 108 to 118 by the sequence with the most refusals, 9 us each.  The parts of a set that takes 131: 46 all rows' sums, 24 first refusals, 54 the walk,
+// 11 the last tokens.  Half of the sums are of rows that nobody asks for, leaves of the trees; without them and the walks' waiting 9 us would read what is needed.  With
+// the 11 powers of a series on [-1/2, 1/2] in the place of the table and few powers, 149 where four powers took 126; the fifth is 3 % of the whole.  One chain of five nodes, f32: 16 us, the
+// latency of four launches.
 #include "cache.hpp"
 
 namespace {

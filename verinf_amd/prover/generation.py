@@ -261,8 +261,8 @@ def attend_cache(q, cache, batch, parents=None, scale=None, longest=None, out=No
 
     bfloat16 or float16 as the cache's (bfloat16 over int8); groups of heads / cache heads share one of the cache's; scale: dim^-0.5.  A new token
     attends to what its sequence had before and to the new tokens up to itself; with parents (n,) int32, in the place of those to its ancestors: a
-    token's parent as a number in its sequence, below its own (-1: none).  A sequence with more than 256 new tokens is taken for a chain.  A token
-    that attends to nothing gets zeros.  longest: no sequence has more entries (it decides how the work is cut, nothing else).  out: where to; a new
+    token's parent as a number in its sequence, below its own (-1: none).  A sequence with more than 256 new tokens is taken for a chain,
+    whatever parents says of it.  A token that attends to nothing gets zeros.  Over int8 queries are below 2^100.  longest: no sequence has more entries (it decides how the work is cut, nothing else).  out: where to; a new
     tensor by default, whose rows of no sequence are zero."""
     dev = _both(cache, batch, "attend_cache")
     a = cache._args
@@ -312,7 +312,7 @@ def verify_drafts(logits, tokens, starts, parents, uniforms, depth, draft_logits
     behind; their tokens, the one that follows, -1 behind.  All in 64 bits.  A row with a NaN or +inf, or only -inf, has no probabilities: no draft
     below it is accepted, and the token that follows it is -1.  An entry less than 2^-1022 of its row's largest has none either (-inf, or masked far down): it
     is neither accepted nor the token that follows, and as the draft's counts as never drawn.  Drafts whose token is outside [0, v) or whose parent is none are refused; v is at most
-    2^20, and a sequence's first 1024 nodes are tried."""
+    2^20, and a sequence's first 1024 nodes are tried (attend_cache has trees of 256 at most)."""
     n, v, ld = _matrix(logits, "logits", _FLOATS)
     dev = logits.device
     ids = _vector(tokens, "tokens", n, torch.int64, dev)
